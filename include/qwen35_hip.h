@@ -354,6 +354,114 @@ int qhip_launch_mul_mat_ragged(const void *d_w, const void *d_xq_packed, float *
                                int cols, const int *d_offsets, int nseq, int total_tokens,
                                int ttype, void *stream);
 
+/* ---- key/value cache in 8 bits --------------------------------------------------
+ * The cache of one attention layer: the keys and values of all sequences in
+ * blocks of `block_size` tokens, int8 codes with one f32 scale for each block
+ * and head (value = code * scale).  No reference counterpart (the reference
+ * keeps its cache in f32, on the CPU or in the CUDA backend).  A serving step
+ * calls qhip_launch_kv_tables once, then for each layer qhip_launch_kv_append
+ * and qhip_launch_kv_attention.  All arrays are device memory; none of these
+ * calls allocates, waits or keeps anything.
+ *
+ *   k, v              int8 [num_blocks][kv_heads][block_size][head_dim], 16-byte aligned
+ *   k_scale, v_scale  f32  [num_blocks][kv_heads]
+ *   block_size        16, 32, 64, 128 or 256; 0 < num_blocks * block_size < 2^31
+ *   head_dim          64, 128 or 256 (others: QHIP_DECLINE)
+ *
+ * Element types of keys, values, queries and outputs are GGUF type ids. */
+#define QHIP_TT_F32 0
+#define QHIP_TT_F16 1
+#define QHIP_TT_BF16 30
+typedef struct qhip_kv_cache {
+  void *k;
+  void *v;
+  float *k_scale;
+  float *v_scale;
+  int num_blocks;
+  int block_size;
+  int kv_heads;
+  int head_dim;
+} qhip_kv_cache;
+
+/* Block tables and slot maps from the lengths of a step's requests.  Sequence
+ * i < nseq has d_cached[i] tokens in the cache and brings d_new[i] (either may
+ * be 0; negative counts as 0); its blocks are d_table[i * table_width ...], of
+ * which the first ceil(cached / block_size) are there.  Sequences take the
+ * further blocks that they need from d_free[0 .. nfree) in order, from entry
+ * d_taken[0] (NULL = 0) on.  Written:
+ *   d_table     the new entries only (-1 past the end of the free list)
+ *   d_offsets   [nseq + 1] prefix sums of d_new: the packed tokens' order
+ *   d_kv_lens   [nseq] cached + new
+ *   d_slots     [tokens] block * block_size + place in the block of each packed
+ *               token; -1 where no block was left or the row of the table is too
+ *               short, and for tokens at or past the sum of d_new (a batch that
+ *               is padded to `tokens`)
+ *   d_positions [tokens] (nullable) each token's place in its sequence, 0 for padding
+ *   d_taken_out the free-list entries taken, these included: more than nfree
+ *               says that blocks were short
+ * Outputs must not overlap inputs, d_table apart. */
+int qhip_launch_kv_tables(const int *d_cached, const int *d_new, int nseq, const int *d_free, int nfree,
+                          const int *d_taken, int block_size, int *d_table, int table_width, int tokens,
+                          int *d_offsets, int *d_kv_lens, int *d_slots, int *d_positions, int *d_taken_out,
+                          void *stream);
+
+/* Writes new tokens' keys and values into their slots.  Token t, head h has
+ * head_dim contiguous elements of `type` at d_k + t * k_token_stride + h *
+ * k_head_stride (strides in elements; d_v alike).  d_slots[t] outside the pool
+ * (-1) skips the token, whose values are not read.  Tokens of one block must be
+ * adjacent and in slot order, as qhip_launch_kv_tables lays them out.  For each
+ * block and head that gets tokens
+ *   scale = max(old scale, max |x| / 127), without the old one where the first
+ *   new token is the block's first;
+ *   codes of the tokens before it: round(code * (old / scale));
+ *   new codes: round(x * (1 / scale)), each an f32 operation, ties to even.
+ * A NaN among the new values makes the scale NaN, an infinity makes it
+ * infinite: the block's head then reads as NaN until the block is begun anew. */
+int qhip_launch_kv_append(const qhip_kv_cache *cache, int type, const void *d_k, long k_token_stride,
+                          long k_head_stride, const void *d_v, long v_token_stride, long v_head_stride,
+                          const int *d_slots, int tokens, void *stream);
+
+/* The values of `nblocks` whole blocks, code * scale: d_k_out and d_v_out are
+ * [nblocks][kv_heads][block_size][head_dim] of `type`, 16-byte aligned (either
+ * may be NULL).  A block id outside the pool gives NaN. */
+int qhip_launch_kv_read(const qhip_kv_cache *cache, const int *d_blocks, int nblocks, int type, void *d_k_out,
+                        void *d_v_out, void *stream);
+
+/* A step's sequences as qhip_launch_kv_tables leaves them.  max_new, max_kv:
+ * no sequence has more new tokens, or more tokens in all. */
+typedef struct qhip_kv_batch {
+  const int *offsets; /* [nseq + 1] packed tokens of sequence i: [offsets[i], offsets[i + 1]) */
+  const int *kv_lens; /* [nseq] its tokens in the cache, the new ones included */
+  const int *table;   /* [nseq][table_width] its blocks */
+  int nseq;
+  int tokens; /* packed tokens in all */
+  int max_new;
+  int max_kv;
+  int table_width;
+} qhip_kv_batch;
+
+/* Attention of each packed token's q_heads query heads over its own sequence's
+ * cached keys and values; query head h reads key head h / (q_heads / kv_heads).
+ *   s_j = softmax_scale * q . k_j over the visible j, out = sum softmax(s)_j v_j,
+ *   lse = log(sum exp(s_j))
+ * The n-th of a sequence's new tokens is its token p = kv_len - new + n; causal
+ * (0 or 1): it sees j <= p, and with window > 0 only j > p - window.  A row that
+ * sees nothing gets out = 0 and lse = -infinity.  A visible token whose table
+ * entry names no block of the pool makes its rows NaN.  d_q, d_out: head_dim
+ * contiguous elements of `type` at token * token_stride + head * head_stride
+ * (elements); d_lse (nullable): f32 [tokens][q_heads].  Rows of tokens at or
+ * past offsets[nseq] are not written.
+ * d_work (nullable): qhip_kv_attention_work_bytes of the same batch, 16-byte
+ * aligned, its first 32 KiB zero before the first launch and zero again after
+ * every launch; with it the keys of long sequences are cut over workgroups and
+ * joined in order (the same results on every run), without it they are not cut.
+ * Launches that share a d_work must not overlap. */
+long qhip_kv_attention_work_bytes(const qhip_kv_cache *cache, const qhip_kv_batch *batch, int q_heads);
+int qhip_launch_kv_attention(const qhip_kv_cache *cache, const qhip_kv_batch *batch, int type, const void *d_q,
+                             long q_token_stride, long q_head_stride, int q_heads, float softmax_scale,
+                             int causal, int window, void *d_out, long out_token_stride, long out_head_stride,
+                             float *d_lse, void *d_work, long work_bytes, void *stream);
+
 /* ---- parity export -----------------------------------------------------------
  * Exact per-block integers through the same unit decode as the GEMV kernels:
  * ints[(t*rows + r)*nints + i], nints = cols/block_elems, except the formats

@@ -20,6 +20,16 @@ class QhipLinear(ctypes.Structure):
                 ("row_bytes", c_long)]
 
 
+class QhipKvCache(ctypes.Structure):
+    _fields_ = [("k", c_void_p), ("v", c_void_p), ("k_scale", c_void_p), ("v_scale", c_void_p),
+                ("num_blocks", c_int), ("block_size", c_int), ("kv_heads", c_int), ("head_dim", c_int)]
+
+
+class QhipKvBatch(ctypes.Structure):
+    _fields_ = [("offsets", c_void_p), ("kv_lens", c_void_p), ("table", c_void_p), ("nseq", c_int), ("tokens", c_int),
+                ("max_new", c_int), ("max_kv", c_int), ("table_width", c_int)]
+
+
 class QhipProfEntry(ctypes.Structure):
     _fields_ = [("slot", c_int), ("ttype", c_int), ("rows", c_int), ("cols", c_int), ("tokens", c_int),
                 ("calls", ctypes.c_longlong), ("device_us", ctypes.c_double), ("bytes", ctypes.c_double),
@@ -85,6 +95,16 @@ SIGNATURES = {
     "qhip_ragged_offsets": (c_int, [c_int_p, c_int, c_int_p]),
     "qhip_launch_mul_mat_ragged": (c_int, [c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p,
                                            c_int, c_int, c_int, c_void_p]),
+    "qhip_launch_kv_tables": (c_int, [c_void_p, c_void_p, c_int, c_void_p, c_int, c_void_p, c_int, c_void_p, c_int,
+                                      c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]),
+    "qhip_launch_kv_append": (c_int, [ctypes.POINTER(QhipKvCache), c_int, c_void_p, c_long, c_long, c_void_p, c_long,
+                                      c_long, c_void_p, c_int, c_void_p]),
+    "qhip_launch_kv_read": (c_int, [ctypes.POINTER(QhipKvCache), c_void_p, c_int, c_int, c_void_p, c_void_p,
+                                    c_void_p]),
+    "qhip_kv_attention_work_bytes": (c_long, [ctypes.POINTER(QhipKvCache), ctypes.POINTER(QhipKvBatch), c_int]),
+    "qhip_launch_kv_attention": (c_int, [ctypes.POINTER(QhipKvCache), ctypes.POINTER(QhipKvBatch), c_int, c_void_p,
+                                         c_long, c_long, c_int, ctypes.c_float, c_int, c_int, c_void_p, c_long, c_long,
+                                         c_void_p, c_void_p, c_long, c_void_p]),
     "qhip_launch_block_ints": (c_int, [c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int,
                                        c_void_p]),
     "qhip_backend_create": (c_void_p, [c_int, c_int_p]),

@@ -9,7 +9,7 @@ import ctypes
 
 import torch
 
-from ._lib import QhipLinear, QhipProfEntry, check, load
+from ._lib import QhipKvBatch, QhipKvCache, QhipLinear, QhipProfEntry, check, load
 
 _GEOM = {8: (32, 34), 20: (32, 18), 12: (256, 144), 14: (256, 210), 13: (256, 176), 11: (256, 110),
          10: (256, 84), 23: (256, 136), 2: (32, 18), 3: (32, 20), 18: (256, 98), 21: (256, 110)}
@@ -294,6 +294,134 @@ def mul_mat_ragged(ttype: int, w: torch.Tensor, xq: torch.Tensor, off_d: torch.T
     check("mul_mat_ragged", load().qhip_launch_mul_mat_ragged(
         _p(w), _p(xq), _p(out), rows, cols, _p(off_d), nseq, total, ttype, _stream()))
     return out[:total]
+
+
+# ---- key/value cache in 8 bits ---------------------------------------------------------
+
+_KV_TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 30}
+
+
+def _ints(name: str, t: torch.Tensor, dims: int = 1) -> int:
+    if t.dtype != torch.int32 or t.dim() != dims or not t.is_cuda or not t.is_contiguous():
+        raise ValueError(f"{name}: a contiguous int32 GPU tensor of {dims} dimension(s)")
+    return t.data_ptr()
+
+
+def _kv_rows(name: str, t: torch.Tensor, dim: int) -> int:
+    """The GGUF type id of token rows [tokens, heads, dim] whose last dimension is contiguous."""
+    if t.dim() != 3 or t.shape[2] != dim or t.stride(2) != 1 or not t.is_cuda or t.dtype not in _KV_TYPES:
+        raise ValueError(f"{name}: a GPU tensor [tokens, heads, {dim}] of f32, f16 or bf16 with contiguous heads")
+    return _KV_TYPES[t.dtype]
+
+
+class KvCache:
+    """One layer's keys and values: int8 [blocks, kv_heads, block_size, head_dim] with f32 scales [blocks, kv_heads]."""
+
+    def __init__(self, k: torch.Tensor, v: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor):
+        for t in (k, v):
+            if t.dtype != torch.int8 or t.dim() != 4 or t.shape != k.shape or not t.is_cuda or not t.is_contiguous():
+                raise ValueError("k, v: contiguous int8 GPU tensors [blocks, kv_heads, block_size, head_dim]")
+        for t in (k_scale, v_scale):
+            if t.dtype != torch.float32 or t.shape != k.shape[:2] or not t.is_cuda or not t.is_contiguous():
+                raise ValueError("k_scale, v_scale: contiguous f32 GPU tensors [blocks, kv_heads]")
+        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        self.num_blocks, self.kv_heads, self.block_size, self.head_dim = k.shape
+        self._c = QhipKvCache(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), self.num_blocks,
+                              self.block_size, self.kv_heads, self.head_dim)
+        self._ref = ctypes.byref(self._c)
+
+    @classmethod
+    def empty(cls, num_blocks: int, kv_heads: int, block_size: int, head_dim: int, device="cuda") -> "KvCache":
+        shape = (num_blocks, kv_heads, block_size, head_dim)
+        return cls(torch.zeros(shape, dtype=torch.int8, device=device), torch.zeros(shape, dtype=torch.int8, device=device),
+                   torch.zeros(shape[:2], device=device), torch.zeros(shape[:2], device=device))
+
+
+class KvStep:
+    """What kv_tables writes for a step of `nseq` sequences and `tokens` packed tokens."""
+
+    def __init__(self, nseq: int, tokens: int, device="cuda"):
+        def ints(n):
+            return torch.empty(n, dtype=torch.int32, device=device)
+
+        self.nseq, self.tokens = nseq, tokens
+        self.offsets, self.kv_lens, self.taken = ints(nseq + 1), ints(nseq), ints(1)
+        self.slots, self.positions = ints(tokens), ints(tokens)
+
+
+def kv_tables(cached: torch.Tensor, new: torch.Tensor, free: torch.Tensor, table: torch.Tensor, block_size: int,
+              step: KvStep, taken: torch.Tensor | None = None) -> KvStep:
+    """Blocks and slots for `new` [nseq] tokens behind `cached` [nseq]: the new entries of `table` [nseq, width] come
+    from `free`, from entry `taken` [1] on; `step` receives the rest."""
+    nseq = step.nseq
+    if table.dim() != 2 or len(cached) != nseq or len(new) != nseq or len(table) != nseq:
+        raise ValueError(f"cached, new, table: {nseq} sequences")
+    check("kv_tables", load().qhip_launch_kv_tables(
+        _ints("cached", cached), _ints("new", new), nseq, _ints("free", free), len(free),
+        None if taken is None else _ints("taken", taken), block_size, _ints("table", table, 2), table.shape[1], step.tokens,
+        step.offsets.data_ptr(), step.kv_lens.data_ptr(), step.slots.data_ptr(), step.positions.data_ptr(),
+        step.taken.data_ptr(), _stream()))
+    return step
+
+
+def kv_append(cache: KvCache, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor) -> None:
+    """Write k, v [tokens, kv_heads, head_dim] into `slots` [tokens] (-1: skip); the blocks' scales grow as needed."""
+    tt = _kv_rows("k", k, cache.head_dim)
+    if _kv_rows("v", v, cache.head_dim) != tt or k.shape != v.shape or k.shape[1] != cache.kv_heads or len(slots) != len(k):
+        raise ValueError("k, v: one type, [tokens, kv_heads, head_dim]; slots: [tokens]")
+    check("kv_append", load().qhip_launch_kv_append(
+        cache._ref, tt, k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1),
+        _ints("slots", slots), len(k), _stream()))
+
+
+def kv_read(cache: KvCache, blocks: torch.Tensor, dtype: torch.dtype = torch.float32) -> tuple[torch.Tensor, torch.Tensor]:
+    """The keys and values of whole blocks, [len(blocks), kv_heads, block_size, head_dim] each."""
+    if dtype not in _KV_TYPES:
+        raise ValueError("dtype: f32, f16 or bf16")
+    shape = (len(blocks), cache.kv_heads, cache.block_size, cache.head_dim)
+    k = torch.empty(shape, dtype=dtype, device=blocks.device)
+    v = torch.empty(shape, dtype=dtype, device=blocks.device)
+    check("kv_read", load().qhip_launch_kv_read(cache._ref, _ints("blocks", blocks), len(blocks), _KV_TYPES[dtype],
+                                                k.data_ptr(), v.data_ptr(), _stream()))
+    return k, v
+
+
+def kv_attention_work(cache: KvCache, q_heads: int, nseq: int, tokens: int, max_new: int, max_kv: int) -> torch.Tensor | None:
+    """Zeroed workspace for kv_attention's batches of up to these sizes (None when nothing would be cut)."""
+    b = QhipKvBatch(None, None, None, nseq, tokens, max_new, max_kv, 0)
+    n = load().qhip_kv_attention_work_bytes(cache._ref, ctypes.byref(b), q_heads)
+    if n < 0:
+        raise ValueError(f"bad ({q_heads} query heads, {nseq} sequences, {tokens} tokens)")
+    return torch.zeros(n, dtype=torch.uint8, device=cache.k.device) if n > 0 else None
+
+
+def kv_attention(q: torch.Tensor, cache: KvCache, table: torch.Tensor, offsets: torch.Tensor, kv_lens: torch.Tensor,
+                 max_new: int, max_kv: int, scale: float | None = None, causal: bool = True, window: int = 0,
+                 work: torch.Tensor | None = None, out: torch.Tensor | None = None,
+                 lse: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """Attention of q [tokens, q_heads, head_dim] over the cached tokens of each row's sequence: (out, lse [tokens, q_heads]).
+
+    Sequence i has rows offsets[i] .. offsets[i + 1] and kv_lens[i] cached tokens (its new ones included); no sequence
+    has more than max_new rows or max_kv tokens.  scale: 1 / sqrt(head_dim) by default."""
+    tt, nseq = _kv_rows("q", q, cache.head_dim), len(kv_lens)
+    tokens, heads = q.shape[0], q.shape[1]
+    if len(table) != nseq or len(offsets) != nseq + 1:
+        raise ValueError(f"table: {nseq} rows, offsets: {nseq + 1}")
+    if out is None:
+        out = torch.empty((tokens, heads, cache.head_dim), dtype=q.dtype, device=q.device)
+    elif _kv_rows("out", out, cache.head_dim) != tt or out.shape != q.shape:
+        raise ValueError("out: as q")
+    if lse is None:
+        lse = torch.empty((tokens, heads), dtype=torch.float32, device=q.device)
+    elif lse.dtype != torch.float32 or lse.shape != (tokens, heads) or not lse.is_contiguous() or not lse.is_cuda:
+        raise ValueError("lse: f32 [tokens, q_heads]")
+    b = QhipKvBatch(_ints("offsets", offsets), _ints("kv_lens", kv_lens), _ints("table", table, 2), nseq, tokens, max_new,
+                    max_kv, table.shape[1])
+    check("kv_attention", load().qhip_launch_kv_attention(
+        cache._ref, ctypes.byref(b), tt, q.data_ptr(), q.stride(0), q.stride(1), heads,
+        cache.head_dim ** -0.5 if scale is None else scale, int(causal), window, out.data_ptr(), out.stride(0), out.stride(1),
+        lse.data_ptr(), None if work is None else work.data_ptr(), 0 if work is None else work.numel(), _stream()))
+    return out, lse
 
 
 class Backend:
