@@ -1,8 +1,7 @@
 // kv_attention.hip -- attention over the 8-bit key/value cache.
 //
-// One wave per packed token and query head: 64 keys at a time, a key a lane
-// for the scores, eight or fewer dimensions' sums a lane for the output, with
-// the running maximum and sum of the softmax in f32.
+// Two kernels, each for its own sequences of a batch: those of a few rows, whose
+// cost is reading the codes, and those of many, whose cost is the products.
 #include "kv_internal.hpp"
 #include "qhip_device.hpp"
 #include "qhip_internal.hpp"
@@ -22,9 +21,11 @@ struct KvAttnArgs {
   int causal, window;
   int type, group, few_tokens;  // group: query heads of a key head; sequences of up to few_tokens new tokens are few rows
   bool q_vec, out_vec;          // rows that 16-byte accesses may touch
-  // the cut of long sequences (few rows): off, or items aimed for, least 32-key units of one, bound of a sequence's units
+  // the cut of long sequences: off, or items aimed for, fewest key units of one,
+  // bound of a sequence's units, rows of a chunk's partial results
   bool cut;
-  int few_target, few_min, max_units, few_rows;
+  int target, least, max_units, rows;
+  long slots;  // chunks that the workspace holds
   unsigned* counters;
   float* partial;
 };
@@ -65,8 +66,8 @@ typedef _Float16 h16x2 __attribute__((ext_vector_type(2)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kFewRows = 64;         // most rows of a sequence's key head
-constexpr long kFewCountBytes = 32768;
-constexpr int kFewPairs = kFewCountBytes / 4;  // most (sequence, key head) pairs that are cut
+constexpr long kCountBytes = 32768;
+constexpr int kMaxCut = kCountBytes / 4;  // most row tiles that are cut
 constexpr float kCodeScale = 0x1p9f;  // codes are held as code * 2^-9
 constexpr float kMinusInf = -INFINITY;
 
@@ -144,8 +145,8 @@ __device__ __forceinline__ bool few_item(const KvAttnArgs& a, int lane, FewItem&
     int total = s.units;
     for (int i = 64 + lane; i - lane < a.nseq; i += 64) total += few_seq(a, i).units;
     total = wave_sum(total);
-    // about few_target items in all, none of fewer than few_min units
-    unit = max(a.few_min, (int)(((long)total * a.kv_heads + a.few_target - 1) / a.few_target));
+    // about `target` items in all, none of fewer than `least` units
+    unit = max(a.least, (int)(((long)total * a.kv_heads + a.target - 1) / a.target));
   }
   int items = 0, slots = 0;
   for (int i0 = 0; i0 < a.nseq; i0 += 64) {
@@ -190,39 +191,84 @@ __device__ __forceinline__ void store1(void* out, long at, int type, float v) {
   else if (type == QHIP_TT_F16) ((f16_t*)out)[at] = (f16_t)v;
   else ((bf16_t*)out)[at] = (bf16_t)v;
 }
-// N consecutive values (16-byte stores where vec)
+// N (a power of two) consecutive values, in pieces of up to 16 bytes where vec
+template <typename T, int N>
+__device__ __forceinline__ void store_pieces(T* out, const float* v) {
+  constexpr int P = N * sizeof(T) < 16 ? N : 16 / sizeof(T);
+  typedef T piece __attribute__((ext_vector_type(P)));
+#pragma unroll
+  for (int i = 0; i < N; i += P) {
+    piece x;
+#pragma unroll
+    for (int j = 0; j < P; ++j) x[j] = (T)v[i + j];
+    *(piece*)(out + i) = x;
+  }
+}
 template <int N>
 __device__ __forceinline__ void store_n(void* out, long at, int type, bool vec, const float* v) {
-  if (vec && type == QHIP_TT_F32) {
-#pragma unroll
-    for (int i = 0; i < N; i += 4) *(f32x4*)((float*)out + at + i) = f32x4{v[i], v[i + 1], v[i + 2], v[i + 3]};
-  } else if (vec) {
-#pragma unroll
-    for (int i = 0; i < N; i += 4) {
-      uint64_t w = 0;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const uint16_t b = type == QHIP_TT_F16 ? __builtin_bit_cast(uint16_t, (f16_t)v[i + j])
-                                               : __builtin_bit_cast(uint16_t, (bf16_t)v[i + j]);
-        w |= (uint64_t)b << (16 * j);
-      }
-      *(uint64_t*)((uint16_t*)out + at + i) = w;
-    }
-  } else {
+  if (!vec) {
 #pragma unroll
     for (int i = 0; i < N; ++i) store1(out, at + i, type, v[i]);
+  } else if (type == QHIP_TT_F32) {
+    store_pieces<float, N>((float*)out + at, v);
+  } else if (type == QHIP_TT_F16) {
+    store_pieces<f16_t, N>((f16_t*)out + at, v);
+  } else {
+    store_pieces<bf16_t, N>((bf16_t*)out + at, v);
   }
 }
 
+// power of two of a value scale (a zero or a NaN has none)
+constexpr int kNoScale = -1000;
+__device__ __forceinline__ int scale_exp(float v) { return fabsf(v) > 0.0f ? __builtin_amdgcn_frexp_expf(v) : kNoScale; }
+
 // what e^-(m - M) leaves of a part whose maximum is m (both may be -infinity)
 __device__ __forceinline__ float weight_of(float m, float top) { return m == top ? 1.0f : __builtin_amdgcn_exp2f(m - top); }
+
+// One row of a sequence from its chunks' partial results, D / 64 values a lane:
+// `rows` x D outputs of the chunk's own keys, then each row's m and l, `stride`
+// floats a chunk.  row: of the partial results; seq_row: of the sequence's key head.
+template <int D>
+__device__ __forceinline__ void join_row(const KvAttnArgs& a, const float* parts, long stride, int rows, int row, int chunks,
+                                         int lane, int first_token, int seq_row, int head) {
+  constexpr int W = D / 64;
+  const float* stat = parts + (long)rows * D + 2 * row;
+  float top = kMinusInf;
+  for (int c0 = 0; c0 < chunks; c0 += 64) {
+    float x = c0 + lane < chunks ? sk_load(stat + (c0 + lane) * stride) : kMinusInf;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) x = fmaxf(x, __shfl_xor(x, d, 64));
+    top = fmaxf(top, x);
+  }
+  float acc[W], sum = 0.0f;
+#pragma unroll
+  for (int w = 0; w < W; ++w) acc[w] = 0.0f;
+  for (int c0 = 0; c0 < chunks; c0 += 64) {
+    const int cnt = min(64, chunks - c0);
+    float f = 0.0f;
+    if (lane < cnt) f = weight_of(sk_load(stat + (c0 + lane) * stride), top) * sk_load(stat + (c0 + lane) * stride + 1);
+    for (int i = 0; i < cnt; ++i) {
+      const float fi = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(f), i));
+      const float* x = parts + (c0 + i) * stride + (long)row * D + lane * W;
+      sum += fi;
+#pragma unroll
+      for (int w = 0; w < W; ++w) acc[w] += fi * sk_load(x + w);
+    }
+  }
+  const int tok = seq_row / a.group, t = first_token + tok, qh = head * a.group + (seq_row - tok * a.group);
+  if (t < 0 || t >= a.tokens) return;
+  const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+#pragma unroll
+  for (int w = 0; w < W; ++w) store1(a.out, (long)t * a.out_token + (long)qh * a.out_head + lane * W + w, a.type, acc[w] * inv);
+  if (a.lse && lane == 0) a.lse[(long)t * a.q_heads + qh] = sum == 0.0f ? kMinusInf : (top + __builtin_log2f(sum)) * 0.693147180559945309f;
+}
 
 // SPLIT 2: f32 rows, queries and weights in two f16 parts each
 template <int D, int SPLIT>
 __global__ __launch_bounds__(256, D == 256 ? 2 : D == 128 ? 3 : 4) void k_kv_attention_few(KvAttnArgs a) {
   constexpr int J = D / 64, C = D / 16, W = D / 64;  // 64-dimension pieces, output tiles, dwords of a value load
   __shared__ float s_o[2][C * 4 * 64], s_m[2][64], s_l[2][64];
-  __shared__ int s_e[2];
+  __shared__ int s_e[2][64];
   const int tid = threadIdx.x, lane = tid & 63, r16 = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   FewItem it;
@@ -284,7 +330,7 @@ __global__ __launch_bounds__(256, D == 256 ? 2 : D == 128 ? 3 : 4) void k_kv_att
 #pragma unroll
   for (int c = 0; c < C; ++c) o[c] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
   float m = kMinusInf, l = 0.0f;
-  int ve = -1000;  // the values' power of two: o is in units of 2^(ve - 14) / 2^9
+  int ve = kNoScale;  // power of two of the largest value scale that the row has seen: o is in units of 2^(ve - 14 + 9)
 
   const uint8_t* kc = (const uint8_t*)a.k;
   const uint8_t* vc = (const uint8_t*)a.v;
@@ -305,18 +351,6 @@ __global__ __launch_bounds__(256, D == 256 ? 2 : D == 128 ? 3 : 4) void k_kv_att
       ks = in && finite_bits(__float_as_uint(ks)) ? ks : __builtin_nanf("");
       vs = in && finite_bits(__float_as_uint(vs)) ? vs : __builtin_nanf("");
     }
-    // the largest value scale's power of two (a NaN is never the larger)
-    int e = vs > 0.0f ? __builtin_amdgcn_frexp_expf(vs) : -1000;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) e = max(e, __shfl_xor(e, d, 64));
-    e = max(e, ve);
-    if (e != ve) {
-      const float f = __builtin_ldexpf(1.0f, ve - e);
-#pragma unroll
-      for (int c = 0; c < C; ++c) o[c] *= f;
-      ve = e;
-    }
-    vs = __builtin_ldexpf(vs, 14 - ve);
     const int steps = min(32, (key1 - key0 - 32 * s0 + 32 * parts - 1) / (32 * parts));
 
     kv_u32x4 kr[2][J];
@@ -380,8 +414,8 @@ __global__ __launch_bounds__(256, D == 256 ? 2 : D == 128 ? 3 : 4) void k_kv_att
       if (st + 1 < steps) load_k(st + 1);
       const float c0 = c_row * __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(ks), 2 * st));
       const float c1 = c_row * __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(ks), 2 * st + 1));
-      const float w0 = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(vs), 2 * st));
-      const float w1 = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(vs), 2 * st + 1));
+      const float v0 = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(vs), 2 * st));
+      const float v1 = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(vs), 2 * st + 1));
       float top = kMinusInf;
       const bool edge = key < all_lo || key + 32 > min(all_hi, key1);  // some row does not see some key
 #pragma unroll
@@ -389,25 +423,32 @@ __global__ __launch_bounds__(256, D == 256 ? 2 : D == 128 ? 3 : 4) void k_kv_att
         s[0][r] *= c0;
         s[1][r] *= c1;
       }
+      int e0 = scale_exp(v0), e1 = scale_exp(v1);
       if (edge) {
+        const int end = min(vis_hi, key1);
 #pragma unroll
         for (int tt = 0; tt < 2; ++tt)
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
             const int j = key + 16 * tt + 4 * g + r;
-            if (j < vis_lo || j >= vis_hi || j >= key1) s[tt][r] = kMinusInf;
+            if (j < vis_lo || j >= end) s[tt][r] = kMinusInf;
           }
+        if (key >= end || key + 16 <= vis_lo) e0 = kNoScale;
+        if (key + 16 >= end || key + 32 <= vis_lo) e1 = kNoScale;
       }
+      e0 = max(ve, max(e0, e1));
 #pragma unroll
       for (int r = 0; r < 4; ++r) top = fmaxf(top, fmaxf(s[0][r], s[1][r]));
       top = fmaxf(m, row_max(top));
-      if (__any(top != m)) {
-        const float f = weight_of(m, top);
+      if (__any(top != m || e0 != ve)) {
+        const float f = weight_of(m, top), fo = __builtin_ldexpf(f, ve - e0);
         l *= f;
 #pragma unroll
-        for (int c = 0; c < C; ++c) o[c] *= f;
+        for (int c = 0; c < C; ++c) o[c] *= fo;
         m = top;
+        ve = e0;
       }
+      const float w0 = __builtin_ldexpf(v0, 14 - ve), w1 = __builtin_ldexpf(v1, 14 - ve);
       h16x8 ph, pl;
       float sum = 0.0f;
 #pragma unroll
@@ -459,14 +500,14 @@ __global__ __launch_bounds__(256, D == 256 ? 2 : D == 128 ? 3 : 4) void k_kv_att
         for (int r = 0; r < 4; ++r) s_o[slot][(4 * c + r) * 64 + lane] = o[c][r];
       s_m[slot][lane] = m;
       s_l[slot][lane] = l;
-      if (lane == 0) s_e[slot] = ve;
+      s_e[slot][lane] = ve;
     }
     __syncthreads();
     if (wave < half * tiles) {
       const float m2 = s_m[wave][lane], top = fmaxf(m, m2);
-      const int e = max(ve, s_e[wave]);
+      const int ve2 = s_e[wave][lane], e = max(ve, ve2);
       const float f1 = weight_of(m, top), f2 = weight_of(m2, top);
-      const float g1 = __builtin_ldexpf(f1, ve - e), g2 = __builtin_ldexpf(f2, s_e[wave] - e);
+      const float g1 = __builtin_ldexpf(f1, ve - e), g2 = __builtin_ldexpf(f2, ve2 - e);
 #pragma unroll
       for (int c = 0; c < C; ++c)
 #pragma unroll
@@ -495,7 +536,8 @@ __global__ __launch_bounds__(256, D == 256 ? 2 : D == 128 ? 3 : 4) void k_kv_att
     return;
   }
   // partial results of the chunk: out [rows][D] (of its own keys), then m and l
-  const long stride = (long)a.few_rows * (D + 2);
+  if (it.slot + chunks > a.slots) return;  // offsets or lengths that are none
+  const long stride = (long)a.rows * (D + 2);
   float* parts_at = a.partial + (long)it.slot * stride;
   if (wave < tiles && own_row) {
     float* mine = parts_at + chunk * stride;
@@ -505,108 +547,437 @@ __global__ __launch_bounds__(256, D == 256 ? 2 : D == 128 ? 3 : 4) void k_kv_att
       for (int c = 0; c < C; ++c)
         sk_store(mine + row * D + (4 * g + r) * C + c, __builtin_ldexpf(o[c][r] * norm, ve - 14 + 9));
     if (g == 0) {
-      sk_store(mine + a.few_rows * D + 2 * row, m);
-      sk_store(mine + a.few_rows * D + 2 * row + 1, l);
+      sk_store(mine + a.rows * D + 2 * row, m);
+      sk_store(mine + a.rows * D + 2 * row + 1, l);
     }
   }
   unsigned* count = a.counters + (long)seq * a.kv_heads + head;
   if (!sk_arrive(count, (unsigned)chunks)) return;
   sk_reset(count);
-  // the last workgroup: a wave a row, D / 64 values a lane
-  for (int rw = wave; rw < rows; rw += 4) {
-    float top = kMinusInf;
-    for (int c0 = 0; c0 < chunks; c0 += 64) {
-      float x = c0 + lane < chunks ? sk_load(parts_at + (c0 + lane) * stride + a.few_rows * D + 2 * rw) : kMinusInf;
-#pragma unroll
-      for (int d = 1; d < 64; d <<= 1) x = fmaxf(x, __shfl_xor(x, d, 64));
-      top = fmaxf(top, x);
-    }
-    float acc[W], sum = 0.0f;
-#pragma unroll
-    for (int w = 0; w < W; ++w) acc[w] = 0.0f;
-    for (int c0 = 0; c0 < chunks; c0 += 64) {
-      const int cnt = min(64, chunks - c0);
-      float f = 0.0f;
-      if (lane < cnt) {
-        const float* x = parts_at + (c0 + lane) * stride + a.few_rows * D + 2 * rw;
-        f = weight_of(sk_load(x), top) * sk_load(x + 1);
-      }
-      for (int i = 0; i < cnt; ++i) {
-        const float fi = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(f), i));
-        const float* x = parts_at + (c0 + i) * stride + rw * D + lane * W;
-        sum += fi;
-#pragma unroll
-        for (int w = 0; w < W; ++w) acc[w] += fi * sk_load(x + w);
-      }
-    }
-    const int tk = rw / a.group, tt = a.offsets[seq] + tk, h = head * a.group + (rw - tk * a.group);
-    if (tt < 0 || tt >= a.tokens) continue;
-    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-#pragma unroll
-    for (int w = 0; w < W; ++w) store1(a.out, (long)tt * a.out_token + (long)h * a.out_head + lane * W + w, a.type, acc[w] * inv);
-    if (a.lse && lane == 0) a.lse[(long)tt * a.q_heads + h] = sum == 0.0f ? kMinusInf : (top + __builtin_log2f(sum)) * 0.693147180559945309f;
-  }
+  // the last workgroup: a wave a row
+  for (int rw = wave; rw < rows; rw += 4)
+    join_row<D>(a, parts_at, stride, a.rows, rw, chunks, lane, a.offsets[seq], rw, head);
 }
 
-// ---- every other sequence ------------------------------------------------------------
+// ---- sequences of many rows: key tiles staged in LDS ---------------------------------
+//
+// A workgroup takes kManyRows rows of one key head (row = token * G + head of
+// the group, so that the heads of a group share every key), a wave 32 of them.
+// Per tile of 64 keys the codes are read once from memory, turned into f16 and
+// laid down in LDS as v_mfma_f32_32x32x16_f16 wants them: keys row by row
+// (16-byte pieces of 8 dimensions), values dimension by dimension (16-byte
+// pieces of the 8 keys that a lane's weights belong to), both with the piece
+// index xor-ed so that eight lanes hit eight pieces of a 128-byte row of banks.
+// S^T and O^T as for few rows: lane 32 h + r holds row r; keys 8 i + 4 h ..+3 of
+// a 32-key half are its scores and its half of the weights' operand, and output
+// tile c holds dimensions i D/32 + c.  The next tile's codes are in flight in
+// registers while this one is multiplied.
 
-template <typename T, int D>
-__global__ __launch_bounds__(64) void k_kv_attention(KvAttnArgs a) {
-  constexpr int R = D / 64;
-  __shared__ float s_q[D], s_p[64];
-  __shared__ long s_at[64];
-  const int t = blockIdx.x, h = blockIdx.y, lane = threadIdx.x;
-  int lo = 0, hi = a.nseq;  // the token's sequence
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (a.offsets[mid] <= t) lo = mid; else hi = mid;
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+constexpr int kManyRows = 128;
+constexpr int kManyKeys = 64;
+constexpr int kManyChunks = 16;  // most chunks of a sequence (their weights fit the smallest key tile's LDS)
+
+struct ManySeq {
+  int n, len, tiles, units;  // new tokens (0: not one of these sequences), tokens, row tiles, key tiles to plan for
+};
+__device__ __forceinline__ ManySeq many_seq(const KvAttnArgs& a, int i) {
+  ManySeq s{0, 0, 0, 0};
+  if (i >= a.nseq) return s;
+  const int n = a.offsets[i + 1] - a.offsets[i];
+  if (n <= a.few_tokens || n > a.tokens) return s;
+  s.n = n;
+  s.len = max(a.kv_lens[i], 0);
+  s.tiles = (int)(((long)(min(a.offsets[i + 1], a.tokens) - a.offsets[i]) * a.group + kManyRows - 1) / kManyRows);
+  if (s.tiles <= 0) return ManySeq{0, 0, 0, 0};
+  int keys = s.len;
+  if (a.causal && a.window > 0) keys = (int)min((long)keys, (long)a.window + kManyRows / a.group + 2 * kManyKeys);
+  s.units = min((keys + kManyKeys - 1) / kManyKeys, a.max_units);
+  return s;
+}
+struct ManyItem {
+  int seq, head, tile, chunk, chunks, slot, counter;
+  ManySeq s;
+};
+__device__ __forceinline__ bool many_item(const KvAttnArgs& a, int lane, ManyItem& it) {
+  const int at = blockIdx.x / a.kv_heads;
+  it.head = blockIdx.x - at * a.kv_heads;
+  int unit = 0x7FFFFFFF;
+  ManySeq s = many_seq(a, lane);
+  if (a.cut) {
+    int total = s.tiles * s.units;
+    for (int i = 64 + lane; i - lane < a.nseq; i += 64) {
+      const ManySeq x = many_seq(a, i);
+      total += x.tiles * x.units;
+    }
+    total = wave_sum(total);
+    unit = max(a.least, (int)(((long)total * a.kv_heads + a.target - 1) / a.target));
   }
-  if (t >= a.offsets[a.nseq] || a.offsets[lo + 1] - a.offsets[lo] <= a.few_tokens) return;
-  const int len = a.kv_lens[lo], p = len - a.offsets[lo + 1] + t;
-  const int end = a.causal ? min(p + 1, len) : len;
-  const int begin = a.causal && a.window > 0 ? max(0, p - a.window + 1) : 0;
-  const int kh = h / (a.q_heads / a.kv_heads), mask = (1 << a.shift) - 1;
-  const T* q = (const T*)a.q + (long)t * a.q_token + (long)h * a.q_head;
-  for (int d = lane; d < D; d += 64) s_q[d] = (float)q[d];
-  __syncthreads();
-  float m = -INFINITY, l = 0.0f, acc[R] = {};
-  for (int j0 = begin; j0 < end; j0 += 64) {
-    const int j = j0 + lane;
-    float s = -INFINITY, vs = 0.0f;
-    long at = 0;
-    if (j < end) {
-      const int b = j >> a.shift, id = b < a.width ? a.table[(long)lo * a.width + b] : -1;
+  int items = 0, slots = 0, tiles = 0;
+  for (int i0 = 0; i0 < a.nseq; i0 += 64) {
+    if (i0) s = many_seq(a, i0 + lane);
+    const int c = min(kManyChunks, max(1, (int)(((long)s.units + unit - 1) / unit))), n = s.tiles * c, cut = c > 1 ? n : 0;
+    const int ci = wave_scan(n, lane), cs = wave_scan(cut, lane), ct = wave_scan(s.tiles, lane);
+    const int all = __shfl(ci, 63, 64);
+    if (at < items + all) {
+      const int owner = __builtin_ctzll(__ballot(items + ci > at));
+      it.seq = i0 + owner;
+      it.s = ManySeq{__shfl(s.n, owner, 64), __shfl(s.len, owner, 64), __shfl(s.tiles, owner, 64), 0};
+      it.chunks = __shfl(c, owner, 64);
+      const int local = at - (items + __shfl(ci, owner, 64) - it.s.tiles * it.chunks);
+      const int tile = local / it.chunks;
+      it.chunk = local - tile * it.chunks;
+      it.tile = it.s.tiles - 1 - tile;  // the last rows see the most keys: they begin first
+      it.slot = (slots + __shfl(cs, owner, 64) - (it.s.tiles - tile) * it.chunks) * a.kv_heads + it.head * it.chunks;
+      it.counter = (tiles + __shfl(ct, owner, 64) - it.s.tiles + it.tile) * a.kv_heads + it.head;
+      return true;
+    }
+    items += all;
+    slots += __shfl(cs, 63, 64);
+    tiles += __shfl(ct, 63, 64);
+  }
+  return false;
+}
+
+// the 16-byte piece of a value row that holds piece x of dimension `dim`
+template <int D>
+__device__ __forceinline__ int value_piece(int dim, int x) {
+  if constexpr (D == 64) return x ^ (((dim >> 1) ^ (dim >> 4)) & 7);
+  else return x ^ ((dim / (D / 32)) & 7);
+}
+
+template <int D, int SPLIT>
+__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_kv_attention_many(KvAttnArgs a) {
+  constexpr int S = D / 16, C = D / 32;      // 16-dimension steps, output tiles
+  constexpr int KP = D / 64;                 // 16-byte pieces of a key tile a thread stages
+  constexpr int VW = D == 256 ? 2 : 1;       // dwords of a value row a thread stages (8 keys of 4 VW dimensions)
+  constexpr int VT = 8 * (D / (4 * VW));     // threads that stage values
+  __shared__ __attribute__((aligned(16))) uint8_t s_k[kManyKeys * D * 2], s_v[kManyKeys * D * 2];
+  const int tid = threadIdx.x, lane = tid & 63, r32 = lane & 31, h = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  ManyItem it;
+  if (!many_item(a, lane, it)) return;
+  const int seq = __builtin_amdgcn_readfirstlane(it.seq), n = __builtin_amdgcn_readfirstlane(it.s.n);
+  const int len = __builtin_amdgcn_readfirstlane(it.s.len), head = __builtin_amdgcn_readfirstlane(it.head);
+  const int chunks = __builtin_amdgcn_readfirstlane(it.chunks), chunk = __builtin_amdgcn_readfirstlane(it.chunk);
+  const int row_first = __builtin_amdgcn_readfirstlane(it.tile) * kManyRows;
+  const int rows = (int)min((long)kManyRows, (long)n * a.group - row_first);
+  const int first = len - n;  // place of the sequence's first new token
+  const bool windowed = a.causal && a.window > 0;
+  // the tile's keys, and this chunk's
+  const int tok_a = row_first / a.group, tok_b = (row_first + rows - 1) / a.group;
+  const int lo = windowed ? max(0, first + tok_a - a.window + 1) & ~(kManyKeys - 1) : 0;
+  const int hi = a.causal ? first + tok_b + 1 : len;
+  const int all_tiles = max(0, hi - lo + kManyKeys - 1) / kManyKeys;
+  const int tile0 = (int)((long)all_tiles * chunk / chunks), tile1 = (int)((long)all_tiles * (chunk + 1) / chunks);
+  const int key0 = lo + tile0 * kManyKeys, count = tile1 - tile0;
+
+  // this lane's row, and what the wave's rows see
+  const int wrow = wave * 32, row = wrow + r32;
+  const bool own_row = row < rows;
+  const int tok = own_row ? (row_first + row) / a.group : tok_a, p = first + tok;
+  const int t = a.offsets[seq] + tok, qh = head * a.group + (row_first + row - tok * a.group);
+  const bool live = own_row && t >= 0 && t < a.tokens;
+  const int vis_hi = a.causal ? p + 1 : len, vis_lo = windowed ? p - a.window + 1 : 0;
+  const int wtok_a = (row_first + wrow) / a.group, wtok_b = (row_first + min(wrow + 31, rows - 1)) / a.group;
+  const bool busy = wrow < rows;
+  const int all_hi = a.causal ? first + wtok_a + 1 : len, all_lo = windowed ? first + wtok_b - a.window + 1 : 0;
+  const int any_hi = a.causal ? first + wtok_b + 1 : len, any_lo = windowed ? first + wtok_a - a.window + 1 : 0;
+
+  h16x8 q_hi[S], q_lo[SPLIT == 2 ? S : 1];
+  float c_row;
+  {
+    float top = 0.0f;
+    const long at = (long)t * a.q_token + (long)qh * a.q_head + 8 * h;
+#pragma unroll
+    for (int s = 0; s < S; ++s) {
+      float v[8] = {};
+      if (live) load_q8(a.q, at + 16 * s, a.type, a.q_vec, v);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(v[i]));
+    }
+    const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
+    const int e = 14 - __builtin_amdgcn_frexp_expf(fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1])));
+#pragma unroll
+    for (int s = 0; s < S; ++s) {
+      float v[8] = {};
+      if (live) load_q8(a.q, at + 16 * s, a.type, a.q_vec, v);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float x = __builtin_ldexpf(v[i], e);
+        q_hi[s][i] = (_Float16)x;
+        if constexpr (SPLIT == 2) q_lo[s][i] = (_Float16)(x - (float)q_hi[s][i]);
+      }
+    }
+    c_row = __builtin_ldexpf(a.scale * 1.44269504088896341f * kCodeScale, -e);
+  }
+
+  f32x16 o[C];
+#pragma unroll
+  for (int c = 0; c < C; ++c)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) o[c][i] = 0.0f;
+  float m = kMinusInf, l = 0.0f;
+  int ve = kNoScale;
+
+  // lane i: the 16-key tile i of a round of 16 key tiles
+  struct Info {
+    int id;
+    float ks, vs;
+  };
+  auto load_info = [&](int round) {
+    Info x{0, 0.0f, 0.0f};
+    const int mine = key0 + round * 16 * kManyKeys + 16 * lane;
+    if (mine < hi) {
+      const int b = mine >> a.shift;
+      const int id = b < a.width ? a.table[(long)seq * a.width + b] : -1;
       const bool in = (unsigned)id < (unsigned)a.num_blocks;
-      const long bh = in ? (long)id * a.kv_heads + kh : 0;
-      at = (bh << a.shift | (j & mask)) * D;
-      float dot = 0.0f;
-      for (int d = 0; d < D; ++d) dot = __builtin_fmaf(s_q[d], (float)a.k[at + d], dot);
-      const float ks = in ? a.k_scale[bh] : __builtin_nanf("");
-      s = finite_bits(__float_as_uint(ks)) ? dot * ks * a.scale : __builtin_nanf("");
-      vs = a.v_scale[bh];
-      vs = finite_bits(__float_as_uint(vs)) ? vs : __builtin_nanf("");
+      x.id = in ? id : 0;
+      x.ks = a.k_scale[(long)x.id * a.kv_heads + head];
+      x.vs = a.v_scale[(long)x.id * a.kv_heads + head];
+      x.ks = in && finite_bits(__float_as_uint(x.ks)) ? x.ks : __builtin_nanf("");
+      x.vs = in && finite_bits(__float_as_uint(x.vs)) ? x.vs : __builtin_nanf("");
     }
-    float top = s;
-    for (int d = 1; d < 64; d <<= 1) top = fmaxf(top, __shfl_xor(top, d, 64));
-    const float m1 = fmaxf(m, top), alpha = m == -INFINITY ? 0.0f : expf(m - m1);
-    const float e = j < end ? (s == -INFINITY ? 0.0f : expf(s - m1)) : 0.0f;
-    float sum = e;
-    for (int d = 1; d < 64; d <<= 1) sum += __shfl_xor(sum, d, 64);
-    l = l * alpha + sum;
-    m = m1;
+    return x;
+  };
+  const int mask = (1 << a.shift) - 1;
+  // staging: pieces of keys (D / 16 a key), then 8 keys of 4 VW dimensions of the values
+  const int kkey = tid / (D / 16), kpc = tid % (D / 16);   // first key (a step of 4096 / D further each piece)
+  const int vgrp = tid / (D / (4 * VW)), vdim = (tid % (D / (4 * VW))) * 4 * VW;
+  // group x of the values' eight: keys 32 (x >> 2) + 16 (x >> 1 & 1) + 4 (x & 1) + {0..3, 8..11}
+  const int vkey = 32 * (vgrp >> 2) + 16 * ((vgrp >> 1) & 1) + 4 * (vgrp & 1);
+  kv_u32x4 kr[KP];
+  uint32_t vr[8][VW];
+  auto load_tile = [&](const Info& x, int i) {  // key tile i of the round
+    auto at = [&](int key) {  // byte offset of a key's codes
+      const long id = __shfl(x.id, 4 * i + (key >> 4), 64);
+      return ((id * a.kv_heads + head) << a.shift | ((16 * (4 * i + (key >> 4)) + key0 + (key & 15)) & mask)) * D;
+    };
+#pragma unroll
+    for (int j = 0; j < KP; ++j) kr[j] = *(const kv_u32x4*)((const uint8_t*)a.k + at(kkey + j * (4096 / D)) + 16 * kpc);
+    if (VT == 256 || tid < VT) {
+      const uint8_t* b = (const uint8_t*)a.v + at(vkey) + vdim;  // all eight keys lie in one 16-key tile
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const uint32_t* y = (const uint32_t*)(b + (j < 4 ? j : j + 4) * D);
+        if constexpr (VW == 2) {
+          const kv_u32x2 z = *(const kv_u32x2*)y;
+          vr[j][0] = z[0];
+          vr[j][1] = z[1];
+        } else {
+          vr[j][0] = y[0];
+        }
+      }
+    }
+  };
+  auto store_tile = [&]() {
+#pragma unroll
+    for (int j = 0; j < KP; ++j) {
+      const int key = kkey + j * (4096 / D);
+      const kv_u32x4 x = kr[j] ^ 0x80808080u;
+      uint8_t* row_at = s_k + key * (D * 2);
+      *(h16x8*)(row_at + ((2 * kpc) ^ (key & 7)) * 16) = codes8(x[0], x[1]);
+      *(h16x8*)(row_at + ((2 * kpc + 1) ^ (key & 7)) * 16) = codes8(x[2], x[3]);
+    }
+    if (VT == 256 || tid < VT) {
+#pragma unroll
+      for (int w = 0; w < VW; ++w) {
+        uint32_t x[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] = vr[j][w] ^ 0x80808080u;
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+          h16x2 y[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            y[j] = b == 0 ? codes_of<0>(x[2 * j], x[2 * j + 1]) : b == 1 ? codes_of<1>(x[2 * j], x[2 * j + 1])
+                 : b == 2 ? codes_of<2>(x[2 * j], x[2 * j + 1]) : codes_of<3>(x[2 * j], x[2 * j + 1]);
+          const int dim = vdim + 4 * w + b;
+          *(h16x8*)(s_v + dim * 128 + value_piece<D>(dim, vgrp) * 16) =
+              h16x8{y[0][0], y[0][1], y[1][0], y[1][1], y[2][0], y[2][1], y[3][0], y[3][1]};
+        }
+      }
+    }
+  };
+
+  Info info = load_info(0), next = load_info(1);
+  if (count > 0) load_tile(info, 0);
+  for (int i = 0; i < count; ++i) {
+    const int ri = i & 15;
+    if (ri == 0 && i) {
+      info = next;
+      next = load_info((i >> 4) + 1);
+    }
+    __syncthreads();  // the previous tile has been read
+    store_tile();
     __syncthreads();
-    s_p[lane] = j < end ? e * vs : 0.0f;
-    s_at[lane] = at;
-    __syncthreads();
-    for (int r = 0; r < R; ++r) {
-      float o = acc[r] * alpha;
-      for (int i = 0; i < min(64, end - j0); ++i) o = __builtin_fmaf(s_p[i], (float)a.v[s_at[i] + lane + 64 * r], o);
-      acc[r] = o;
+    if (i + 1 < count) {
+      if (ri == 15) load_tile(next, 0);
+      else load_tile(info, ri + 1);
+    }
+    const int key = key0 + i * kManyKeys;
+#pragma unroll 1
+    for (int mt = 0; mt < 2; ++mt) {
+      const int kt = key + 32 * mt;
+      if (!busy || kt >= any_hi || kt + 32 <= any_lo) continue;  // no row of the wave sees it
+      f32x16 s = {}, sl = {};
+#pragma unroll
+      for (int st = 0; st < S; ++st) {
+        const int kk = 32 * mt + r32;
+        const h16x8 x = *(const h16x8*)(s_k + kk * (D * 2) + ((2 * st + h) ^ (kk & 7)) * 16);
+        s = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, q_hi[st], s, 0, 0, 0);
+        if constexpr (SPLIT == 2) sl = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, q_lo[st], sl, 0, 0, 0);
+      }
+      const int sc = 4 * ri + 2 * mt;
+      const float c0 = c_row * __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(info.ks), sc));
+      const float c1 = c_row * __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(info.ks), sc + 1));
+      const float v0 = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(info.vs), sc));
+      const float v1 = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(info.vs), sc + 1));
+      const bool edge = kt < all_lo || kt + 32 > all_hi;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[r] = (SPLIT == 2 ? s[r] + sl[r] : s[r]) * (r < 8 ? c0 : c1);
+      int e0 = scale_exp(v0), e1 = scale_exp(v1);
+      if (edge) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int j = kt + 8 * (r >> 2) + 4 * h + (r & 3);
+          if (j < vis_lo || j >= vis_hi) s[r] = kMinusInf;
+        }
+        if (kt >= vis_hi || kt + 16 <= vis_lo) e0 = kNoScale;
+        if (kt + 16 >= vis_hi || kt + 32 <= vis_lo) e1 = kNoScale;
+      }
+      e0 = max(ve, max(e0, e1));
+      float top = s[0];
+#pragma unroll
+      for (int r = 1; r < 16; ++r) top = fmaxf(top, s[r]);
+      const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
+      top = fmaxf(m, fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1])));
+      if (__any(top != m || e0 != ve)) {
+        const float f = weight_of(m, top), fo = __builtin_ldexpf(f, ve - e0);
+        l *= f;
+#pragma unroll
+        for (int c = 0; c < C; ++c) o[c] *= fo;
+        m = top;
+        ve = e0;
+      }
+      const float w0 = __builtin_ldexpf(v0, 14 - ve), w1 = __builtin_ldexpf(v1, 14 - ve);
+      h16x8 p_hi[2], p_lo[2];
+      float sum = 0.0f;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        float e = __builtin_amdgcn_exp2f(s[r] - m), x = e * (r < 8 ? w0 : w1);
+        if (edge) {
+          const int j = kt + 8 * (r >> 2) + 4 * h + (r & 3);
+          if (j < vis_lo || j >= vis_hi) e = x = 0.0f;
+        }
+        sum += e;
+        const _Float16 y = (_Float16)x;
+        p_hi[r >> 3][r & 7] = y;
+        if constexpr (SPLIT == 2) p_lo[r >> 3][r & 7] = (_Float16)(x - (float)y);
+      }
+      l += sum;
+#pragma unroll
+      for (int st = 0; st < 2; ++st)
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+          const int dim = r32 * C + c;
+          const h16x8 x = *(const h16x8*)(s_v + dim * 128 + value_piece<D>(dim, 4 * mt + 2 * st + h) * 16);
+          o[c] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, p_hi[st], o[c], 0, 0, 0);
+          if constexpr (SPLIT == 2) o[c] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, p_lo[st], o[c], 0, 0, 0);
+        }
     }
   }
-  T* out = (T*)a.out + (long)t * a.out_token + (long)h * a.out_head;
-  for (int r = 0; r < R; ++r) out[lane + 64 * r] = (T)(end > begin ? acc[r] / l : 0.0f);
-  if (a.lse && lane == 0) a.lse[(long)t * a.q_heads + h] = end > begin ? m + logf(l) : -INFINITY;
+  {
+    const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(l), __float_as_uint(l), false, false);
+    l = __uint_as_float(sw[0]) + __uint_as_float(sw[1]);
+  }
+  const float norm = l == 0.0f ? 0.0f : 1.0f / l;
+  if (chunks == 1) {
+    if (live) {
+      const long at = (long)t * a.out_token + (long)qh * a.out_head;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        float v[C];
+#pragma unroll
+        for (int c = 0; c < C; ++c) v[c] = __builtin_ldexpf(o[c][r] * norm, ve - 14 + 9);
+        store_n<C>(a.out, at + (8 * (r >> 2) + 4 * h + (r & 3)) * C, a.type, a.out_vec, v);
+      }
+      if (a.lse && h == 0) a.lse[(long)t * a.q_heads + qh] = l == 0.0f ? kMinusInf : (m + __builtin_log2f(l)) * 0.693147180559945309f;
+    }
+    return;
+  }
+  if (it.slot + chunks > a.slots || it.counter >= kMaxCut) return;  // offsets or lengths that are none
+  constexpr long kStride = (long)kManyRows * (D + 2);
+  float* parts_at = a.partial + (long)it.slot * kStride;
+  if (own_row) {
+    float* mine = parts_at + chunk * kStride;
+#pragma unroll
+    for (int r = 0; r < 16; ++r)
+#pragma unroll
+      for (int c = 0; c < C; ++c)
+        sk_store(mine + row * D + (8 * (r >> 2) + 4 * h + (r & 3)) * C + c, __builtin_ldexpf(o[c][r] * norm, ve - 14 + 9));
+    if (h == 0) {
+      sk_store(mine + kManyRows * D + 2 * row, m);
+      sk_store(mine + kManyRows * D + 2 * row + 1, l);
+    }
+  }
+  unsigned* counter = a.counters + it.counter;
+  if (!sk_arrive(counter, (unsigned)chunks)) return;
+  sk_reset(counter);
+  // the last workgroup: each row's chunk weights into LDS, then two values a thread
+  float* s_f = (float*)s_k;
+  float* s_inv = (float*)s_v;
+  if (tid < rows) {
+    const float* stat = parts_at + kManyRows * D + 2 * tid;
+    float top = kMinusInf, sum = 0.0f;
+    for (int c = 0; c < chunks; ++c) {
+      const float x = sk_load(stat + c * kStride);
+      s_f[c * kManyRows + tid] = x;
+      top = fmaxf(top, x);
+    }
+    for (int c = 0; c < chunks; ++c) {
+      const float f = weight_of(s_f[c * kManyRows + tid], top) * sk_load(stat + c * kStride + 1);
+      s_f[c * kManyRows + tid] = f;
+      sum += f;
+    }
+    s_inv[tid] = sum == 0.0f ? 0.0f : 1.0f / sum;
+    const int tk = (row_first + tid) / a.group, tt = a.offsets[seq] + tk, qq = head * a.group + (row_first + tid - tk * a.group);
+    if (a.lse && tt >= 0 && tt < a.tokens)
+      a.lse[(long)tt * a.q_heads + qq] = sum == 0.0f ? kMinusInf : (top + __builtin_log2f(sum)) * 0.693147180559945309f;
+  }
+  __syncthreads();
+  constexpr int kFlight = 16;
+  for (int e0 = 0; e0 < rows * (D / 2); e0 += 256 * kFlight) {
+    float acc[kFlight][2] = {};
+    for (int c = 0; c < chunks; ++c) {
+      uint64_t x[kFlight];
+#pragma unroll
+      for (int j = 0; j < kFlight; ++j) {
+        const int e = e0 + 256 * j + tid;
+        x[j] = e < rows * (D / 2) ? __hip_atomic_load((const uint64_t*)(parts_at + c * kStride) + e, __ATOMIC_RELAXED,
+                                                      __HIP_MEMORY_SCOPE_AGENT)
+                                  : 0;
+      }
+#pragma unroll
+      for (int j = 0; j < kFlight; ++j) {
+        const float f = s_f[c * kManyRows + min(e0 + 256 * j + tid, rows * (D / 2) - 1) / (D / 2)];
+        acc[j][0] += f * __uint_as_float((uint32_t)x[j]);
+        acc[j][1] += f * __uint_as_float((uint32_t)(x[j] >> 32));
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < kFlight; ++j) {
+      const int e = e0 + 256 * j + tid;
+      if (e >= rows * (D / 2)) break;
+      const int rw = e / (D / 2), d = 2 * (e % (D / 2));
+      const int tk = (row_first + rw) / a.group, tt = a.offsets[seq] + tk, qq = head * a.group + (row_first + rw - tk * a.group);
+      if (tt < 0 || tt >= a.tokens) continue;
+      const long at = (long)tt * a.out_token + (long)qq * a.out_head + d;
+      store1(a.out, at, a.type, acc[j][0] * s_inv[rw]);
+      store1(a.out, at + 1, a.type, acc[j][1] * s_inv[rw]);
+    }
+  }
 }
 
 template <int SPLIT>
@@ -616,12 +987,11 @@ static void launch_few(const KvAttnArgs& a, int dim, unsigned grid, hipStream_t 
   else hipLaunchKernelGGL((k_kv_attention_few<256, SPLIT>), dim3(grid), dim3(256), 0, s, a);
 }
 
-template <typename T>
-static void launch_attention(const KvAttnArgs& a, int dim, hipStream_t s) {
-  const dim3 grid((unsigned)a.tokens, (unsigned)a.q_heads);
-  if (dim == 64) hipLaunchKernelGGL((k_kv_attention<T, 64>), grid, dim3(64), 0, s, a);
-  else if (dim == 128) hipLaunchKernelGGL((k_kv_attention<T, 128>), grid, dim3(64), 0, s, a);
-  else hipLaunchKernelGGL((k_kv_attention<T, 256>), grid, dim3(64), 0, s, a);
+template <int SPLIT>
+static void launch_many(const KvAttnArgs& a, int dim, unsigned grid, hipStream_t s) {
+  if (dim == 64) hipLaunchKernelGGL((k_kv_attention_many<64, SPLIT>), dim3(grid), dim3(256), 0, s, a);
+  else if (dim == 128) hipLaunchKernelGGL((k_kv_attention_many<128, SPLIT>), dim3(grid), dim3(256), 0, s, a);
+  else hipLaunchKernelGGL((k_kv_attention_many<256, SPLIT>), dim3(grid), dim3(256), 0, s, a);
 }
 
 // 0, hipErrorInvalidValue or QHIP_DECLINE
@@ -633,28 +1003,42 @@ static int check_batch(const qhip_kv_cache* cache, const qhip_kv_batch* b, int q
   return rc;
 }
 
-// How the few-row sequences are cut: items aimed for, and the workspace (0: no cut).
-struct FewPlan {
-  int tokens, rows, max_units, target, least;
-  long grid, work;
+// How one of the two kernels' sequences are cut: grid without and with a cut,
+// key units of the longest sequence, items aimed for, fewest units of one, and
+// the workspace (0: no cut).
+struct AttnPlan {
+  int rows, max_units, target, least;
+  long grid, cut_grid, work;
 };
-static FewPlan few_plan(const qhip_kv_cache* c, const qhip_kv_batch* b, int q_heads) {
-  const int group = q_heads / c->kv_heads;
-  FewPlan p{};
-  p.tokens = kFewRows / group < b->max_new ? kFewRows / group : b->max_new;
-  p.rows = p.tokens * group;
-  p.max_units = (int)(((long)b->max_kv + 31) / 32);
-  p.target = p.rows <= 16 ? 1024 : 512;
-  p.least = 16;
-  const long pairs = (long)b->nseq * c->kv_heads, most = (p.max_units + p.least - 1) / p.least;
-  p.grid = pairs;
-  if (p.tokens > 0 && most > 1 && pairs <= kFewPairs && (long)b->nseq * p.max_units < 0x7FFFFFFFL) {
-    p.grid = pairs * most < p.target + pairs ? pairs * most : p.target + pairs;
-    // sequences that are cut have less than twice target chunks: a chunk holds
-    // at least a target-th of all units
-    const long slots = pairs * most < 2L * p.target ? pairs * most : 2L * p.target;
-    p.work = kFewCountBytes + slots * p.rows * (c->head_dim + 2) * 4;
+// `tiles`: bound of the row tiles over all sequences and key heads; a sequence
+// that is cut has less than twice units / unit chunks, where a chunk's unit is
+// at least a target-th of all units, so the chunks are less than twice target.
+static AttnPlan attn_plan(long tiles, int rows, int units, int target, int least, int dim) {
+  AttnPlan p{rows, units, target, least, tiles, tiles, 0};
+  const long most = (units + least - 1) / least;
+  if (tiles > 0 && most > 1 && tiles <= kMaxCut && tiles * units < 0x7FFFFFFFL) {
+    p.cut_grid = tiles * most < target + tiles ? tiles * most : target + tiles;
+    const long slots = tiles * most < 2L * target ? tiles * most : 2L * target;
+    p.work = kCountBytes + slots * rows * (dim + 2) * 4;
   }
+  return p;
+}
+// most new tokens of a few-row sequence
+static int few_tokens(const qhip_kv_cache* c, const qhip_kv_batch* b, int q_heads) {
+  const int most = kFewRows / (q_heads / c->kv_heads);
+  return most < b->max_new ? most : b->max_new;
+}
+static AttnPlan few_plan(const qhip_kv_cache* c, const qhip_kv_batch* b, int q_heads) {
+  const int rows = few_tokens(c, b, q_heads) * (q_heads / c->kv_heads);
+  const long tiles = rows ? (long)b->nseq * c->kv_heads : 0;
+  return attn_plan(tiles, rows, (int)(((long)b->max_kv + 31) / 32), rows <= 16 ? 1024 : 512, 16, c->head_dim);
+}
+static AttnPlan many_plan(const qhip_kv_cache* c, const qhip_kv_batch* b, int q_heads) {
+  if (b->max_new <= few_tokens(c, b, q_heads)) return AttnPlan{};
+  const long tiles = ((long)b->tokens * (q_heads / c->kv_heads) / kManyRows + b->nseq) * c->kv_heads;
+  const int target = 512;
+  AttnPlan p = attn_plan(tiles, kManyRows, (int)(((long)b->max_kv + kManyKeys - 1) / kManyKeys), target, 8, c->head_dim);
+  if (tiles >= 2 * target) p.work = 0;  // enough workgroups as it is
   return p;
 }
 
@@ -663,7 +1047,9 @@ static FewPlan few_plan(const qhip_kv_cache* c, const qhip_kv_batch* b, int q_he
 using namespace qhip;
 
 extern "C" long qhip_kv_attention_work_bytes(const qhip_kv_cache* cache, const qhip_kv_batch* batch, int q_heads) {
-  return check_batch(cache, batch, q_heads) ? -1 : few_plan(cache, batch, q_heads).work;
+  if (check_batch(cache, batch, q_heads)) return -1;
+  const long few = few_plan(cache, batch, q_heads).work, many = many_plan(cache, batch, q_heads).work;
+  return few > many ? few : many;
 }
 
 extern "C" int qhip_launch_kv_attention(const qhip_kv_cache* cache, const qhip_kv_batch* batch, int type,
@@ -681,26 +1067,32 @@ extern "C" int qhip_launch_kv_attention(const qhip_kv_cache* cache, const qhip_k
     return (int)hipErrorInvalidValue;
   if (rc) return rc;
   if (batch->tokens == 0 || batch->nseq == 0) return 0;
-  const FewPlan plan = few_plan(cache, batch, q_heads);
-  const bool cut = plan.work > 0 && d_work && work_bytes >= plan.work;
-  const int group = q_heads / cache->kv_heads;
-  const KvAttnArgs a{(const int8_t*)cache->k, (const int8_t*)cache->v, cache->k_scale, cache->v_scale, batch->offsets,
-                     batch->kv_lens, batch->table, d_q, d_out, d_lse, q_token_stride, q_head_stride, out_token_stride,
-                     out_head_stride, batch->nseq, batch->tokens, batch->table_width, kv_block_shift(cache->block_size),
-                     cache->num_blocks, cache->kv_heads, q_heads, softmax_scale, causal, window, type, group, plan.tokens,
-                     kv_rows_aligned(d_q, q_token_stride, q_head_stride, size),
-                     kv_rows_aligned(d_out, out_token_stride, out_head_stride, size), cut, plan.target, plan.least,
-                     plan.max_units, plan.rows, (unsigned*)d_work, (float*)((char*)d_work + kFewCountBytes)};
+  const AttnPlan few = few_plan(cache, batch, q_heads), many = many_plan(cache, batch, q_heads);
+  // rows and workgroups are counted in 32 bits
+  if (few.grid > 0x7FFFFFFFL || many.grid > 0x7FFFFFFFL || (long)batch->tokens * q_heads > 0x7FFFFFFFL) return (int)hipErrorInvalidValue;
+  KvAttnArgs a{(const int8_t*)cache->k, (const int8_t*)cache->v, cache->k_scale, cache->v_scale, batch->offsets,
+               batch->kv_lens, batch->table, d_q, d_out, d_lse, q_token_stride, q_head_stride, out_token_stride,
+               out_head_stride, batch->nseq, batch->tokens, batch->table_width, kv_block_shift(cache->block_size),
+               cache->num_blocks, cache->kv_heads, q_heads, softmax_scale, causal, window, type, q_heads / cache->kv_heads,
+               few_tokens(cache, batch, q_heads), kv_rows_aligned(d_q, q_token_stride, q_head_stride, size),
+               kv_rows_aligned(d_out, out_token_stride, out_head_stride, size)};
+  a.counters = (unsigned*)d_work;
+  a.partial = (float*)((char*)d_work + kCountBytes);
   hipStream_t s = (hipStream_t)stream;
-  if (plan.tokens > 0) {
-    const unsigned grid = (unsigned)(cut ? plan.grid : (long)batch->nseq * cache->kv_heads);
-    if (type == QHIP_TT_F32) launch_few<2>(a, cache->head_dim, grid, s);
-    else launch_few<1>(a, cache->head_dim, grid, s);
-  }
-  if (batch->max_new > plan.tokens) {
-    if (type == QHIP_TT_F32) launch_attention<float>(a, cache->head_dim, s);
-    else if (type == QHIP_TT_F16) launch_attention<f16_t>(a, cache->head_dim, s);
-    else launch_attention<bf16_t>(a, cache->head_dim, s);
-  }
+  // the two kernels share the workspace: they follow each other on the stream
+  // and each leaves the counters at zero
+  auto launch = [&](const AttnPlan& p, void (*f32_rows)(const KvAttnArgs&, int, unsigned, hipStream_t),
+                    void (*f16_rows)(const KvAttnArgs&, int, unsigned, hipStream_t)) {
+    if (p.grid == 0) return;
+    a.cut = p.work > 0 && d_work && work_bytes >= p.work;
+    a.target = p.target;
+    a.least = p.least;
+    a.max_units = p.max_units;
+    a.rows = p.rows;
+    a.slots = a.cut ? (p.work - kCountBytes) / ((long)p.rows * (cache->head_dim + 2) * 4) : 0;
+    (type == QHIP_TT_F32 ? f32_rows : f16_rows)(a, cache->head_dim, (unsigned)(a.cut ? p.cut_grid : p.grid), s);
+  };
+  launch(few, launch_few<2>, launch_few<1>);
+  launch(many, launch_many<2>, launch_many<1>);
   return (int)hipGetLastError();
 }
