@@ -24,7 +24,7 @@ struct KvAttnArgs {
   // the cut of long sequences: off, or items aimed for, fewest key units of one,
   // bound of a sequence's units, rows of a chunk's partial results
   bool cut;
-  int target, least, max_units, rows;
+  int target, least, max_units, max_chunks, rows;
   long slots;  // chunks that the workspace holds
   unsigned* counters;
   float* partial;
@@ -133,7 +133,7 @@ __device__ __forceinline__ FewSeq few_seq(const KvAttnArgs& a, int i) {
 
 // The item of a workgroup: key head, sequence and chunk.
 struct FewItem {
-  int seq, head, chunk, chunks, slot, unit;  // slot: of the first chunk's partial results; unit: 32-key units of a chunk
+  int seq, head, chunk, chunks, slot;  // slot: of the first chunk's partial results
   FewSeq s;
 };
 __device__ __forceinline__ bool few_item(const KvAttnArgs& a, int lane, FewItem& it) {
@@ -151,7 +151,7 @@ __device__ __forceinline__ bool few_item(const KvAttnArgs& a, int lane, FewItem&
   int items = 0, slots = 0;
   for (int i0 = 0; i0 < a.nseq; i0 += 64) {
     if (i0) s = few_seq(a, i0 + lane);
-    const int c = s.n ? max(1, (int)(((long)s.units + unit - 1) / unit)) : 0, cut = c > 1 ? c : 0;
+    const int c = s.n ? min(a.max_chunks, max(1, (int)(((long)s.units + unit - 1) / unit))) : 0, cut = c > 1 ? c : 0;
     const int ci = wave_scan(c, lane), cs = wave_scan(cut, lane);
     const int all = __shfl(ci, 63, 64);
     if (at < items + all) {
@@ -160,7 +160,6 @@ __device__ __forceinline__ bool few_item(const KvAttnArgs& a, int lane, FewItem&
       it.chunks = __shfl(c, owner, 64);
       it.chunk = at - (items + __shfl(ci, owner, 64) - it.chunks);
       it.slot = (slots + __shfl(cs, owner, 64) - it.chunks) * a.kv_heads + it.head * it.chunks;
-      it.unit = unit;
       it.s = FewSeq{__shfl(s.n, owner, 64), __shfl(s.len, owner, 64), __shfl(s.lo, owner, 64), __shfl(s.units, owner, 64)};
       return true;
     }
@@ -222,52 +221,123 @@ __device__ __forceinline__ void store_n(void* out, long at, int type, bool vec, 
 constexpr int kNoScale = -1000;
 __device__ __forceinline__ int scale_exp(float v) { return fabsf(v) > 0.0f ? __builtin_amdgcn_frexp_expf(v) : kNoScale; }
 
+// log(sum e^s) of a row whose maximum and sum are in powers of two
+__device__ __forceinline__ float row_lse(float m, float l) {
+  return l == 0.0f ? kMinusInf : (m + __builtin_log2f(l)) * 0.693147180559945309f;
+}
+
 // what e^-(m - M) leaves of a part whose maximum is m (both may be -infinity)
 __device__ __forceinline__ float weight_of(float m, float top) { return m == top ? 1.0f : __builtin_amdgcn_exp2f(m - top); }
 
-// One row of a sequence from its chunks' partial results, D / 64 values a lane:
-// `rows` x D outputs of the chunk's own keys, then each row's m and l, `stride`
-// floats a chunk.  row: of the partial results; seq_row: of the sequence's key head.
-template <int D>
-__device__ __forceinline__ void join_row(const KvAttnArgs& a, const float* parts, long stride, int rows, int row, int chunks,
-                                         int lane, int first_token, int seq_row, int head) {
-  constexpr int W = D / 64;
-  const float* stat = parts + (long)rows * D + 2 * row;
-  float top = kMinusInf;
-  for (int c0 = 0; c0 < chunks; c0 += 64) {
-    float x = c0 + lane < chunks ? sk_load(stat + (c0 + lane) * stride) : kMinusInf;
+// ---- joining the chunks of a sequence's rows ----------------------------------------
+//
+// A chunk's partial results are `rows` x D outputs of its own keys, then each
+// row's maximum m and sum l, `stride` floats in all, stored and loaded through
+// to the agent's point of coherence (sc1: sk_store's and sk_load's policy, 16
+// bytes at a time).  Every chunk adds one to the tile's counter; the last one
+// joins all in chunk order, so the result does not depend on which was last.
+constexpr int kSc1 = 16;  // cache policy of a buffer access: sc1
+
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t part_rsrc(float* p, long floats) {
+  return __builtin_amdgcn_make_buffer_rsrc(p, 0, (int)(4 * floats), 0x00027000);  // raw, 32-bit, bounds-checked
+}
+// N (2, 4, 8 or 16) consecutive values from float `at` on
+template <int N>
+__device__ __forceinline__ void part_store(__amdgpu_buffer_rsrc_t r, int at, const float* v) {
 #pragma unroll
-    for (int d = 1; d < 64; d <<= 1) x = fmaxf(x, __shfl_xor(x, d, 64));
-    top = fmaxf(top, x);
+  for (int i = 0; i < N; i += 4) {
+    if constexpr (N == 2)
+      __builtin_amdgcn_raw_buffer_store_b64(kv_u32x2{__float_as_uint(v[0]), __float_as_uint(v[1])}, r, 4 * at, 0, kSc1);
+    else
+      __builtin_amdgcn_raw_buffer_store_b128(kv_u32x4{__float_as_uint(v[i]), __float_as_uint(v[i + 1]), __float_as_uint(v[i + 2]),
+                                                      __float_as_uint(v[i + 3])}, r, 4 * (at + i), 0, kSc1);
   }
-  float acc[W], sum = 0.0f;
-#pragma unroll
-  for (int w = 0; w < W; ++w) acc[w] = 0.0f;
-  for (int c0 = 0; c0 < chunks; c0 += 64) {
-    const int cnt = min(64, chunks - c0);
-    float f = 0.0f;
-    if (lane < cnt) f = weight_of(sk_load(stat + (c0 + lane) * stride), top) * sk_load(stat + (c0 + lane) * stride + 1);
-    for (int i = 0; i < cnt; ++i) {
-      const float fi = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(f), i));
-      const float* x = parts + (c0 + i) * stride + (long)row * D + lane * W;
-      sum += fi;
-#pragma unroll
-      for (int w = 0; w < W; ++w) acc[w] += fi * sk_load(x + w);
+}
+
+// LDS of a join: m (then weights) and l of `rows` x `chunks`, 1 / sum of each
+// row, and 4 KB of sums
+constexpr int kJoinLds = 16384;
+constexpr int kJoinPairs = (kJoinLds - 4096 - 4 * 128) / 8;  // most rows x chunks
+
+// All 256 threads: the rows seq_row .. seq_row + count of key head `head`.
+template <int D>
+__device__ __forceinline__ void join_rows(const KvAttnArgs& a, float* lds, __amdgpu_buffer_rsrc_t parts, int stride, int rows,
+                                          int count, int chunks, int first_token, int seq_row, int head) {
+  const int tid = threadIdx.x;
+  float* s_acc = lds;               // [256][4]
+  float* s_inv = lds + 1024;        // [128]
+  float* s_m = lds + 1024 + 128;    // [chunks][count]
+  float* s_l = s_m + chunks * count;
+  for (int i = tid; i < chunks * count; i += 256) {
+    const int c = i / count, r = i - c * count;
+    const kv_u32x2 x = __builtin_amdgcn_raw_buffer_load_b64(parts, 4 * (c * stride + rows * D + 2 * r), 0, kSc1);
+    s_m[i] = __uint_as_float(x[0]);
+    s_l[i] = __uint_as_float(x[1]);
+  }
+  __syncthreads();
+  {
+    int team = 64;  // lanes of a row
+    while (team * count > 256) team >>= 1;
+    const int r = tid / team, tl = tid & (team - 1);
+    float top = kMinusInf, sum = 0.0f;
+    if (r < count)
+      for (int c = tl; c < chunks; c += team) top = fmaxf(top, s_m[c * count + r]);
+    for (int d = 1; d < team; d <<= 1) top = fmaxf(top, __shfl_xor(top, d, 64));
+    if (r < count)
+      for (int c = tl; c < chunks; c += team) {
+        const float f = weight_of(s_m[c * count + r], top) * s_l[c * count + r];
+        s_m[c * count + r] = f;
+        sum += f;
+      }
+    for (int d = 1; d < team; d <<= 1) sum += __shfl_xor(sum, d, 64);
+    if (r < count && tl == 0) {
+      s_inv[r] = sum == 0.0f ? 0.0f : 1.0f / sum;
+      const int tok = (seq_row + r) / a.group, t = first_token + tok, qh = head * a.group + (seq_row + r - tok * a.group);
+      if (a.lse && t >= 0 && t < a.tokens) a.lse[(long)t * a.q_heads + qh] = row_lse(top, sum);
     }
   }
-  const int tok = seq_row / a.group, t = first_token + tok, qh = head * a.group + (seq_row - tok * a.group);
-  if (t < 0 || t >= a.tokens) return;
-  const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+  __syncthreads();
+  // four values a thread; with fewer than 256 of them, slices of the chunks
+  const int pieces = count * (D / 4), slices = pieces < 256 ? 256 / pieces : 1;
+  for (int e0 = 0; e0 < pieces; e0 += 256) {
+    const int sl = slices > 1 ? tid / pieces : 0, e = slices > 1 ? tid - sl * pieces : e0 + tid;
+    const int r = e / (D / 4);
+    f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (e < pieces && sl < slices)
+      for (int c0 = sl; c0 < chunks; c0 += 8 * slices) {
+        kv_u32x4 x[8];
 #pragma unroll
-  for (int w = 0; w < W; ++w) store1(a.out, (long)t * a.out_token + (long)qh * a.out_head + lane * W + w, a.type, acc[w] * inv);
-  if (a.lse && lane == 0) a.lse[(long)t * a.q_heads + qh] = sum == 0.0f ? kMinusInf : (top + __builtin_log2f(sum)) * 0.693147180559945309f;
+        for (int j = 0; j < 8; ++j)  // past the last chunk: out of the buffer's bounds, 0
+          x[j] = __builtin_amdgcn_raw_buffer_load_b128(parts, 4 * ((c0 + j * slices) * stride + 4 * e), 0, kSc1);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const int c = c0 + j * slices;
+          const float f = c < chunks ? s_m[c * count + r] : 0.0f;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) acc[i] += f * __uint_as_float(x[j][i]);
+        }
+      }
+    if (slices > 1) {
+      ((f32x4*)s_acc)[tid] = acc;
+      __syncthreads();
+      if (sl == 0)
+        for (int k = 1; k < slices; ++k) acc += ((f32x4*)s_acc)[k * pieces + e];
+    }
+    const int tok = (seq_row + r) / a.group, t = first_token + tok, qh = head * a.group + (seq_row + r - tok * a.group);
+    if (e < pieces && sl == 0 && t >= 0 && t < a.tokens) {
+      const float inv = s_inv[r], v[4] = {acc[0] * inv, acc[1] * inv, acc[2] * inv, acc[3] * inv};
+      store_n<4>(a.out, (long)t * a.out_token + (long)qh * a.out_head + 4 * (e % (D / 4)), a.type, a.out_vec, v);
+    }
+  }
 }
 
 // SPLIT 2: f32 rows, queries and weights in two f16 parts each
 template <int D, int SPLIT>
 __global__ __launch_bounds__(256, D == 256 ? 2 : D == 128 ? 3 : 4) void k_kv_attention_few(KvAttnArgs a) {
   constexpr int J = D / 64, C = D / 16, W = D / 64;  // 64-dimension pieces, output tiles, dwords of a value load
-  __shared__ float s_o[2][C * 4 * 64], s_m[2][64], s_l[2][64];
+  constexpr int R = C * 4 * 64;  // floats of a wave's output
+  __shared__ __attribute__((aligned(16))) float s_o[2 * R > kJoinLds / 4 ? 2 * R : kJoinLds / 4];
+  __shared__ float s_m[2][64], s_l[2][64];
   __shared__ int s_e[2][64];
   const int tid = threadIdx.x, lane = tid & 63, r16 = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -276,10 +346,11 @@ __global__ __launch_bounds__(256, D == 256 ? 2 : D == 128 ? 3 : 4) void k_kv_att
   const int seq = __builtin_amdgcn_readfirstlane(it.seq), n = __builtin_amdgcn_readfirstlane(it.s.n);
   const int len = __builtin_amdgcn_readfirstlane(it.s.len), lo = __builtin_amdgcn_readfirstlane(it.s.lo);
   const int chunks = __builtin_amdgcn_readfirstlane(it.chunks), chunk = __builtin_amdgcn_readfirstlane(it.chunk);
-  const int head = __builtin_amdgcn_readfirstlane(it.head), unit = __builtin_amdgcn_readfirstlane(it.unit);
+  const int head = __builtin_amdgcn_readfirstlane(it.head);
   const int rows = n * a.group, tiles = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
-  const int key0 = lo + (chunks > 1 ? chunk * unit * 32 : 0);
-  const int key1 = chunk == chunks - 1 ? len : key0 + unit * 32;
+  const int units = max(0, len - lo + 31) >> 5;
+  const int key0 = lo + 32 * (int)((long)units * chunk / chunks);
+  const int key1 = min(len, lo + 32 * (int)((long)units * (chunk + 1) / chunks));
   const int part = wave / tiles, parts = 4 / tiles;
   const int row = (wave % tiles) * 16 + r16;  // this lane's row
   const bool own_row = row < rows;
@@ -497,7 +568,7 @@ __global__ __launch_bounds__(256, D == 256 ? 2 : D == 128 ? 3 : 4) void k_kv_att
 #pragma unroll
       for (int c = 0; c < C; ++c)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) s_o[slot][(4 * c + r) * 64 + lane] = o[c][r];
+        for (int r = 0; r < 4; ++r) s_o[slot * R + (4 * c + r) * 64 + lane] = o[c][r];
       s_m[slot][lane] = m;
       s_l[slot][lane] = l;
       s_e[slot][lane] = ve;
@@ -511,7 +582,7 @@ __global__ __launch_bounds__(256, D == 256 ? 2 : D == 128 ? 3 : 4) void k_kv_att
 #pragma unroll
       for (int c = 0; c < C; ++c)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) o[c][r] = o[c][r] * g1 + s_o[wave][(4 * c + r) * 64 + lane] * g2;
+        for (int r = 0; r < 4; ++r) o[c][r] = o[c][r] * g1 + s_o[wave * R + (4 * c + r) * 64 + lane] * g2;
       l = l * f1 + s_l[wave][lane] * f2;
       m = top;
       ve = e;
@@ -531,32 +602,29 @@ __global__ __launch_bounds__(256, D == 256 ? 2 : D == 128 ? 3 : 4) void k_kv_att
         for (int c = 0; c < C; ++c) v[c] = __builtin_ldexpf(o[c][r] * norm, ve - 14 + 9);
         store_n<C>(a.out, at + r * C, a.type, a.out_vec, v);
       }
-      if (a.lse && g == 0) a.lse[(long)t * a.q_heads + qh] = l == 0.0f ? kMinusInf : (m + __builtin_log2f(l)) * 0.693147180559945309f;
+      if (a.lse && g == 0) a.lse[(long)t * a.q_heads + qh] = row_lse(m, l);
     }
     return;
   }
   // partial results of the chunk: out [rows][D] (of its own keys), then m and l
   if (it.slot + chunks > a.slots) return;  // offsets or lengths that are none
-  const long stride = (long)a.rows * (D + 2);
-  float* parts_at = a.partial + (long)it.slot * stride;
+  const int stride = a.rows * (D + 2);
+  const __amdgpu_buffer_rsrc_t parts_at = part_rsrc(a.partial + (long)it.slot * stride, (long)chunks * stride);
   if (wave < tiles && own_row) {
-    float* mine = parts_at + chunk * stride;
 #pragma unroll
-    for (int r = 0; r < 4; ++r)
+    for (int r = 0; r < 4; ++r) {
+      float v[C];
 #pragma unroll
-      for (int c = 0; c < C; ++c)
-        sk_store(mine + row * D + (4 * g + r) * C + c, __builtin_ldexpf(o[c][r] * norm, ve - 14 + 9));
-    if (g == 0) {
-      sk_store(mine + a.rows * D + 2 * row, m);
-      sk_store(mine + a.rows * D + 2 * row + 1, l);
+      for (int c = 0; c < C; ++c) v[c] = __builtin_ldexpf(o[c][r] * norm, ve - 14 + 9);
+      part_store<C>(parts_at, chunk * stride + row * D + (4 * g + r) * C, v);
     }
+    const float stat[2] = {m, l};
+    if (g == 0) part_store<2>(parts_at, chunk * stride + a.rows * D + 2 * row, stat);
   }
   unsigned* count = a.counters + (long)seq * a.kv_heads + head;
   if (!sk_arrive(count, (unsigned)chunks)) return;
   sk_reset(count);
-  // the last workgroup: a wave a row
-  for (int rw = wave; rw < rows; rw += 4)
-    join_row<D>(a, parts_at, stride, a.rows, rw, chunks, lane, a.offsets[seq], rw, head);
+  join_rows<D>(a, s_o, parts_at, stride, a.rows, rows, chunks, a.offsets[seq], 0, head);
 }
 
 // ---- sequences of many rows: key tiles staged in LDS ---------------------------------
@@ -577,7 +645,7 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 constexpr int kManyRows = 128;
 constexpr int kManyKeys = 64;
-constexpr int kManyChunks = 16;  // most chunks of a sequence (their weights fit the smallest key tile's LDS)
+
 
 struct ManySeq {
   int n, len, tiles, units;  // new tokens (0: not one of these sequences), tokens, row tiles, key tiles to plan for
@@ -617,7 +685,7 @@ __device__ __forceinline__ bool many_item(const KvAttnArgs& a, int lane, ManyIte
   int items = 0, slots = 0, tiles = 0;
   for (int i0 = 0; i0 < a.nseq; i0 += 64) {
     if (i0) s = many_seq(a, i0 + lane);
-    const int c = min(kManyChunks, max(1, (int)(((long)s.units + unit - 1) / unit))), n = s.tiles * c, cut = c > 1 ? n : 0;
+    const int c = min(a.max_chunks, max(1, (int)(((long)s.units + unit - 1) / unit))), n = s.tiles * c, cut = c > 1 ? n : 0;
     const int ci = wave_scan(n, lane), cs = wave_scan(cut, lane), ct = wave_scan(s.tiles, lane);
     const int all = __shfl(ci, 63, 64);
     if (at < items + all) {
@@ -653,7 +721,9 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_kv_attention_many(KvA
   constexpr int KP = D / 64;                 // 16-byte pieces of a key tile a thread stages
   constexpr int VW = D == 256 ? 2 : 1;       // dwords of a value row a thread stages (8 keys of 4 VW dimensions)
   constexpr int VT = 8 * (D / (4 * VW));     // threads that stage values
-  __shared__ __attribute__((aligned(16))) uint8_t s_k[kManyKeys * D * 2], s_v[kManyKeys * D * 2];
+  __shared__ __attribute__((aligned(16))) uint8_t s_kv[2 * kManyKeys * D * 2];
+  uint8_t *const s_k = s_kv, *const s_v = s_kv + kManyKeys * D * 2;
+  static_assert(sizeof(s_kv) >= kJoinLds, "the join's LDS");
   const int tid = threadIdx.x, lane = tid & 63, r32 = lane & 31, h = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   ManyItem it;
@@ -903,81 +973,28 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_kv_attention_many(KvA
         for (int c = 0; c < C; ++c) v[c] = __builtin_ldexpf(o[c][r] * norm, ve - 14 + 9);
         store_n<C>(a.out, at + (8 * (r >> 2) + 4 * h + (r & 3)) * C, a.type, a.out_vec, v);
       }
-      if (a.lse && h == 0) a.lse[(long)t * a.q_heads + qh] = l == 0.0f ? kMinusInf : (m + __builtin_log2f(l)) * 0.693147180559945309f;
+      if (a.lse && h == 0) a.lse[(long)t * a.q_heads + qh] = row_lse(m, l);
     }
     return;
   }
   if (it.slot + chunks > a.slots || it.counter >= kMaxCut) return;  // offsets or lengths that are none
-  constexpr long kStride = (long)kManyRows * (D + 2);
-  float* parts_at = a.partial + (long)it.slot * kStride;
+  constexpr int kStride = kManyRows * (D + 2);
+  const __amdgpu_buffer_rsrc_t parts_at = part_rsrc(a.partial + (long)it.slot * kStride, (long)chunks * kStride);
   if (own_row) {
-    float* mine = parts_at + chunk * kStride;
 #pragma unroll
-    for (int r = 0; r < 16; ++r)
+    for (int r = 0; r < 16; ++r) {
+      float v[C];
 #pragma unroll
-      for (int c = 0; c < C; ++c)
-        sk_store(mine + row * D + (8 * (r >> 2) + 4 * h + (r & 3)) * C + c, __builtin_ldexpf(o[c][r] * norm, ve - 14 + 9));
-    if (h == 0) {
-      sk_store(mine + kManyRows * D + 2 * row, m);
-      sk_store(mine + kManyRows * D + 2 * row + 1, l);
+      for (int c = 0; c < C; ++c) v[c] = __builtin_ldexpf(o[c][r] * norm, ve - 14 + 9);
+      part_store<C>(parts_at, chunk * kStride + row * D + (8 * (r >> 2) + 4 * h + (r & 3)) * C, v);
     }
+    const float stat[2] = {m, l};
+    if (h == 0) part_store<2>(parts_at, chunk * kStride + kManyRows * D + 2 * row, stat);
   }
   unsigned* counter = a.counters + it.counter;
   if (!sk_arrive(counter, (unsigned)chunks)) return;
   sk_reset(counter);
-  // the last workgroup: each row's chunk weights into LDS, then two values a thread
-  float* s_f = (float*)s_k;
-  float* s_inv = (float*)s_v;
-  if (tid < rows) {
-    const float* stat = parts_at + kManyRows * D + 2 * tid;
-    float top = kMinusInf, sum = 0.0f;
-    for (int c = 0; c < chunks; ++c) {
-      const float x = sk_load(stat + c * kStride);
-      s_f[c * kManyRows + tid] = x;
-      top = fmaxf(top, x);
-    }
-    for (int c = 0; c < chunks; ++c) {
-      const float f = weight_of(s_f[c * kManyRows + tid], top) * sk_load(stat + c * kStride + 1);
-      s_f[c * kManyRows + tid] = f;
-      sum += f;
-    }
-    s_inv[tid] = sum == 0.0f ? 0.0f : 1.0f / sum;
-    const int tk = (row_first + tid) / a.group, tt = a.offsets[seq] + tk, qq = head * a.group + (row_first + tid - tk * a.group);
-    if (a.lse && tt >= 0 && tt < a.tokens)
-      a.lse[(long)tt * a.q_heads + qq] = sum == 0.0f ? kMinusInf : (top + __builtin_log2f(sum)) * 0.693147180559945309f;
-  }
-  __syncthreads();
-  constexpr int kFlight = 16;
-  for (int e0 = 0; e0 < rows * (D / 2); e0 += 256 * kFlight) {
-    float acc[kFlight][2] = {};
-    for (int c = 0; c < chunks; ++c) {
-      uint64_t x[kFlight];
-#pragma unroll
-      for (int j = 0; j < kFlight; ++j) {
-        const int e = e0 + 256 * j + tid;
-        x[j] = e < rows * (D / 2) ? __hip_atomic_load((const uint64_t*)(parts_at + c * kStride) + e, __ATOMIC_RELAXED,
-                                                      __HIP_MEMORY_SCOPE_AGENT)
-                                  : 0;
-      }
-#pragma unroll
-      for (int j = 0; j < kFlight; ++j) {
-        const float f = s_f[c * kManyRows + min(e0 + 256 * j + tid, rows * (D / 2) - 1) / (D / 2)];
-        acc[j][0] += f * __uint_as_float((uint32_t)x[j]);
-        acc[j][1] += f * __uint_as_float((uint32_t)(x[j] >> 32));
-      }
-    }
-#pragma unroll
-    for (int j = 0; j < kFlight; ++j) {
-      const int e = e0 + 256 * j + tid;
-      if (e >= rows * (D / 2)) break;
-      const int rw = e / (D / 2), d = 2 * (e % (D / 2));
-      const int tk = (row_first + rw) / a.group, tt = a.offsets[seq] + tk, qq = head * a.group + (row_first + rw - tk * a.group);
-      if (tt < 0 || tt >= a.tokens) continue;
-      const long at = (long)tt * a.out_token + (long)qq * a.out_head + d;
-      store1(a.out, at, a.type, acc[j][0] * s_inv[rw]);
-      store1(a.out, at + 1, a.type, acc[j][1] * s_inv[rw]);
-    }
-  }
+  join_rows<D>(a, (float*)s_kv, parts_at, kStride, kManyRows, rows, chunks, a.offsets[seq], row_first, head);
 }
 
 template <int SPLIT>
@@ -1088,6 +1105,7 @@ extern "C" int qhip_launch_kv_attention(const qhip_kv_cache* cache, const qhip_k
     a.target = p.target;
     a.least = p.least;
     a.max_units = p.max_units;
+    a.max_chunks = kJoinPairs / p.rows;
     a.rows = p.rows;
     a.slots = a.cut ? (p.work - kCountBytes) / ((long)p.rows * (cache->head_dim + 2) * 4) : 0;
     (type == QHIP_TT_F32 ? f32_rows : f16_rows)(a, cache->head_dim, (unsigned)(a.cut ? p.cut_grid : p.grid), s);
