@@ -1,12 +1,24 @@
 // kv_attention.hip -- attention over the 8-bit key/value cache.
 //
-// Two kernels, each for its own sequences of a batch: those of a few rows, whose
-// cost is reading the codes, and those of many, whose cost is the products.
+//   s_j = scale * q . k_j over the keys j that the row sees, out = sum
+//   softmax(s)_j v_j, lse = log(sum exp(s_j)); k_j = code * key scale of j's
+//   block, v_j likewise
+//
+// in one pass over the keys with a running maximum m and sum l in f32.  Two
+// kernels, each for its own sequences of a batch: one for those of a few rows,
+// whose cost is reading the codes, and one for those of many, whose cost is the
+// products.  A row is a query head of a new token; the rows of one key head (row
+// = token * G + head of the group) share every key.
 #include "kv_internal.hpp"
 #include "qhip_device.hpp"
 #include "qhip_internal.hpp"
 
 namespace qhip {
+
+typedef _Float16 h16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 h16x2 __attribute__((ext_vector_type(2)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 struct KvAttnArgs {
   const int8_t *k, *v;
@@ -18,60 +30,31 @@ struct KvAttnArgs {
   long q_token, q_head, out_token, out_head;
   int nseq, tokens, width, shift, num_blocks, kv_heads, q_heads;
   float scale;
-  int causal, window;
-  int type, group, few_tokens;  // group: query heads of a key head; sequences of up to few_tokens new tokens are few rows
-  bool q_vec, out_vec;          // rows that 16-byte accesses may touch
-  // the cut of long sequences: off, or items aimed for, fewest key units of one,
-  // bound of a sequence's units, rows of a chunk's partial results
+  int causal, window, type, group;
+  int group_inv;  // 65536 / group, rounded up
+  // the kernel's sequences (those of min_tokens < new tokens <= max_tokens), the
+  // rows of a workgroup and log2 of the keys of a unit
+  int min_tokens, max_tokens, tile_rows, key_shift;
+  // the cut of long sequences: off, or a unit count's share of the items aimed
+  // for, fewest key units of an item, bound of a sequence's units, most chunks,
+  // and the chunks that the workspace holds
   bool cut;
-  int target, least, max_units, max_chunks, rows;
-  long slots;  // chunks that the workspace holds
+  float share;
+  int least, max_units, max_chunks;
+  long slots;
   unsigned* counters;
   float* partial;
 };
 
-// ---- sequences of a few rows: the cache streamed once ------------------------------
-//
-// The rows of a sequence are its new tokens' query heads of one key head (row =
-// token * G + head of the group), up to 64 in tiles of 16.  The work is one
-// pass over the codes, 2 D bytes a key, so the kernel is built to keep loads in
-// flight and never puts a code anywhere but in a register:
-//
-//   S^T = K Q^T   16 keys x 16 rows a v_mfma_f32_16x16x32_f16; lane 16 g + i
-//                 loads 16-byte pieces of key i, whose dimensions (64 j + 16 g
-//                 ..+15) the query fragment has in the same order
-//   O^T = V^T P^T the accumulator of S^T (lane 16 g + r: row r, keys 4 g ..+3
-//                 of each of two tiles) is P's operand as it stands; lane 16 g +
-//                 i loads dimensions i D/16 ..+(D/16-1) of just those eight
-//                 keys, whole 16-lane rows contiguous, and picks a dimension's
-//                 eight codes with byte permutes
-//
-// so that a row's maximum, sum and output all stay in the four lanes 16 g + r.
-// Codes become f16 exactly: (code + 128) as a subnormal is (code + 128) 2^-24,
-// and one packed fma makes it code * 2^-9.  Queries are scaled by a power of two
-// per row to below 2^14 and f32 ones split into two f16 parts (22 bits); softmax
-// weights are scaled to 2^14 and, for f32 rows, split alike.  f16 and bf16 rows
-// take weights of 11 bits: their outputs are rounded to 11 and 8.  A block's key
-// scale multiplies the scores; its value scale, relative to the largest's power
-// of two, the weights.
-//
-// A workgroup's four waves take steps of 32 keys in turn (one, two or four row
-// tiles share a step's waves) and are merged in LDS.  Long sequences are cut
-// into chunks over workgroups; the chunk length follows from all sequences'
-// lengths, so that ragged batches spread evenly, and the last workgroup of a
-// sequence's key head joins the partial results in order.
-
-typedef _Float16 h16x8 __attribute__((ext_vector_type(8)));
-typedef _Float16 h16x2 __attribute__((ext_vector_type(2)));
-typedef float f32x4 __attribute__((ext_vector_type(4)));
-
-constexpr int kFewRows = 64;         // most rows of a sequence's key head
-constexpr long kCountBytes = 32768;
-constexpr int kMaxCut = kCountBytes / 4;  // most row tiles that are cut
-constexpr float kCodeScale = 0x1p9f;  // codes are held as code * 2^-9
 constexpr float kMinusInf = -INFINITY;
+constexpr float kLog2e = 1.44269504088896341f, kLn2 = 0.693147180559945309f;
 
-// pairs of codes (bytes 0 and 2 of p, biased by 128) as f16, times 2^-9
+// ---- codes as f16 ---------------------------------------------------------------------
+// A code + 128 read as a subnormal f16 is (code + 128) 2^-24; one packed fma
+// makes it code * 2^-9, exactly.
+constexpr float kCodeScale = 0x1p9f;
+
+// bytes 0 and 2 of p (biased by 128, bytes 1 and 3 zero)
 __device__ __forceinline__ h16x2 codes2(uint32_t p) {
   return __builtin_elementwise_fma(__builtin_bit_cast(h16x2, p), h16x2{(_Float16)32768.0f, (_Float16)32768.0f},
                                    h16x2{(_Float16)-0.25f, (_Float16)-0.25f});
@@ -82,161 +65,257 @@ __device__ __forceinline__ h16x8 codes8(uint32_t a, uint32_t b) {
   const h16x2 p2 = codes2(__builtin_amdgcn_perm(0u, b, 0x0C010C00u)), p3 = codes2(__builtin_amdgcn_perm(0u, b, 0x0C030C02u));
   return h16x8{p0[0], p0[1], p1[0], p1[1], p2[0], p2[1], p3[0], p3[1]};
 }
-// byte B of two dwords (biased)
+// byte B of eight dwords (biased): one dimension of eight keys
 template <int B>
-__device__ __forceinline__ h16x2 codes_of(uint32_t a, uint32_t b) {
-  return codes2(__builtin_amdgcn_perm(b, a, 0x0C000C00u | (unsigned)B | ((4u + B) << 16)));
+__device__ __forceinline__ h16x8 codes_across(const uint32_t* x) {
+  constexpr uint32_t sel = 0x0C000C00u | (unsigned)B | ((4u + B) << 16);
+  const h16x2 p0 = codes2(__builtin_amdgcn_perm(x[1], x[0], sel)), p1 = codes2(__builtin_amdgcn_perm(x[3], x[2], sel));
+  const h16x2 p2 = codes2(__builtin_amdgcn_perm(x[5], x[4], sel)), p3 = codes2(__builtin_amdgcn_perm(x[7], x[6], sel));
+  return h16x8{p0[0], p0[1], p1[0], p1[1], p2[0], p2[1], p3[0], p3[1]};
 }
 
-// maximum and sum over the four lanes of a row (lanes r, r + 16, r + 32, r + 48)
-__device__ __forceinline__ float row_max(float v) {
+// ---- lanes ------------------------------------------------------------------------------
+
+// maximum of a value over lanes l and l ^ 32 / over the four lanes l mod 16
+__device__ __forceinline__ float max32(float v) {
   const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  v = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  return fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+}
+__device__ __forceinline__ float sum32(float v) {
+  const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(a[0]) + __uint_as_float(a[1]);
+}
+__device__ __forceinline__ float max16(float v) {
+  v = max32(v);
   const auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
   return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
 }
-__device__ __forceinline__ float row_sum(float v) {
-  const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  v = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+__device__ __forceinline__ float sum16(float v) {
+  v = sum32(v);
   const auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
   return __uint_as_float(b[0]) + __uint_as_float(b[1]);
 }
-
-__device__ __forceinline__ int wave_sum(int v) {
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) v += __shfl_xor(v, d, 64);
-  return v;
+__device__ __forceinline__ float lane_f(float v, int i) {
+  return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(v), i));
 }
-__device__ __forceinline__ int wave_scan(int v, int lane) {  // inclusive
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const int o = __shfl_up(v, d, 64);
-    if (lane >= d) v += o;
-  }
-  return v;
-}
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
 
-struct FewSeq {
-  int n, len, lo, units;  // rows of queries (0: not one of these sequences), tokens, first key, 32-key units to plan for
+// ---- a workgroup's item -------------------------------------------------------------------
+//
+// Sequences in order, their row tiles from the last (which sees the most keys),
+// a tile's chunks of keys, and fastest the key heads.  A sequence's chunk count
+// follows from its share of all sequences' row tiles times key units, so that a
+// ragged batch spreads evenly over the workgroups; every wave works the plan out
+// for itself, 64 sequences at a time.  c = round(units / unit) chunks, at least
+// one: sequences that are cut have fewer than 4/3 of their units / unit, so all
+// chunks of cut sequences are fewer than 4/3 of the items aimed for.
+struct Item {
+  int seq, head, n, len, tile, chunk, chunks;
+  int slot, counter;  // of the tile's first chunk among the partial results, of the tile
 };
-__device__ __forceinline__ FewSeq few_seq(const KvAttnArgs& a, int i) {
-  FewSeq s{0, 0, 0, 0};
+struct SeqPlan {
+  int n, len, tiles, units;
+};
+__device__ __forceinline__ SeqPlan plan_seq(const KvAttnArgs& a, int i) {
+  SeqPlan s{0, 0, 0, 0};
   if (i >= a.nseq) return s;
-  const int n = a.offsets[i + 1] - a.offsets[i];
-  if (n <= 0 || n > a.few_tokens) return s;
+  const int first = a.offsets[i], end = a.offsets[i + 1], len = a.kv_lens[i];
+  const int n = end - first, here = min(end, a.tokens) - first;  // new tokens, and those among the packed rows
+  if (n <= a.min_tokens || n > a.max_tokens || here <= 0) return s;
   s.n = n;
-  s.len = max(a.kv_lens[i], 0);
-  if (a.causal && a.window > 0) s.lo = max(0, s.len - n - a.window + 1) & ~31;
-  s.units = min(max(s.len - s.lo + 31, 0) >> 5, a.max_units);
+  s.len = max(len, 0);
+  s.tiles = (here * a.group + a.tile_rows - 1) / a.tile_rows;
+  int keys = s.len;
+  if (a.window > 0) keys = (int)min((long)keys, (long)a.window + a.tile_rows + (2 << a.key_shift));
+  s.units = min((keys + (1 << a.key_shift) - 1) >> a.key_shift, a.max_units);
   return s;
 }
-
-// The item of a workgroup: key head, sequence and chunk.
-struct FewItem {
-  int seq, head, chunk, chunks, slot;  // slot: of the first chunk's partial results
-  FewSeq s;
-};
-__device__ __forceinline__ bool few_item(const KvAttnArgs& a, int lane, FewItem& it) {
+__device__ __forceinline__ bool find_item(const KvAttnArgs& a, int lane, Item& it) {
   const int at = blockIdx.x / a.kv_heads;
-  it.head = blockIdx.x - at * a.kv_heads;
-  int unit = 0x7FFFFFFF;
-  FewSeq s = few_seq(a, lane);
+  SeqPlan s = plan_seq(a, lane);
+  float per_unit = 0.0f;  // chunks of a key unit
   if (a.cut) {
-    int total = s.units;
-    for (int i = 64 + lane; i - lane < a.nseq; i += 64) total += few_seq(a, i).units;
-    total = wave_sum(total);
-    // about `target` items in all, none of fewer than `least` units
-    unit = max(a.least, (int)(((long)total * a.kv_heads + a.target - 1) / a.target));
+    int total = s.tiles * s.units;
+    for (int i = 64 + lane; i - lane < a.nseq; i += 64) {
+      const SeqPlan x = plan_seq(a, i);
+      total += x.tiles * x.units;
+    }
+    total = __builtin_amdgcn_readlane(scan64(total), 63);
+    per_unit = 1.0f / fmaxf((float)a.least, (float)total * a.share);
   }
-  int items = 0, slots = 0;
+  int items = 0, slots = 0, tiles = 0;
   for (int i0 = 0; i0 < a.nseq; i0 += 64) {
-    if (i0) s = few_seq(a, i0 + lane);
-    const int c = s.n ? min(a.max_chunks, max(1, (int)(((long)s.units + unit - 1) / unit))) : 0, cut = c > 1 ? c : 0;
-    const int ci = wave_scan(c, lane), cs = wave_scan(cut, lane);
-    const int all = __shfl(ci, 63, 64);
-    if (at < items + all) {
-      const int owner = __builtin_ctzll(__ballot(items + ci > at));
-      it.seq = i0 + owner;
-      it.chunks = __shfl(c, owner, 64);
-      it.chunk = at - (items + __shfl(ci, owner, 64) - it.chunks);
-      it.slot = (slots + __shfl(cs, owner, 64) - it.chunks) * a.kv_heads + it.head * it.chunks;
-      it.s = FewSeq{__shfl(s.n, owner, 64), __shfl(s.len, owner, 64), __shfl(s.lo, owner, 64), __shfl(s.units, owner, 64)};
+    if (i0) s = plan_seq(a, i0 + lane);
+    const int c = min(a.max_chunks, max(1, (int)((float)s.units * per_unit + 0.5f)));
+    const int n = s.tiles * c, cut = c > 1 ? n : 0;
+    const int ni = scan64(n);
+    const int all = __builtin_amdgcn_readlane(ni, 63);
+    const bool here = at < items + all;
+    if (a.cut) {
+      const int ci = scan64(cut), ti = scan64(s.tiles);
+      if (here) {
+        const int owner = __builtin_ctzll(__ballot(items + ni > at));
+        slots += __builtin_amdgcn_readlane(ci - cut, owner);
+        tiles += __builtin_amdgcn_readlane(ti - s.tiles, owner);
+      } else {
+        slots += __builtin_amdgcn_readlane(ci, 63);
+        tiles += __builtin_amdgcn_readlane(ti, 63);
+      }
+    }
+    if (here) {
+      const int owner = __builtin_ctzll(__ballot(items + ni > at));
+      const int count = __builtin_amdgcn_readlane(s.tiles, owner);
+      it.seq = uniform(i0 + owner);
+      it.head = uniform(blockIdx.x - at * a.kv_heads);
+      it.n = __builtin_amdgcn_readlane(s.n, owner);
+      it.len = __builtin_amdgcn_readlane(s.len, owner);
+      it.chunks = __builtin_amdgcn_readlane(c, owner);
+      const int local = at - (items + __builtin_amdgcn_readlane(ni - n, owner)), tile = uniform(local / it.chunks);
+      it.chunk = uniform(local - tile * it.chunks);
+      it.tile = count - 1 - tile;
+      it.slot = uniform((slots + tile * it.chunks) * a.kv_heads + it.head * it.chunks);
+      it.counter = uniform((tiles + tile) * a.kv_heads + it.head);
       return true;
     }
     items += all;
-    slots += __shfl(cs, 63, 64);
   }
   return false;
 }
 
-// eight query values from d on as f32
-__device__ __forceinline__ void load_q8(const void* q, long at, int type, bool vec, float* v) {
-  if (type == QHIP_TT_F32) {
-    const Raw8<float> r = vec ? load8<float, true>((const float*)q + at) : load8<float, false>((const float*)q + at);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = r.e[i];
-  } else if (type == QHIP_TT_F16) {
-    const Raw8<f16_t> r = vec ? load8<f16_t, true>((const f16_t*)q + at) : load8<f16_t, false>((const f16_t*)q + at);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = (float)r.e[i];
-  } else {
-    const Raw8<bf16_t> r = vec ? load8<bf16_t, true>((const bf16_t*)q + at) : load8<bf16_t, false>((const bf16_t*)q + at);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = (float)r.e[i];
+// The item's rows and keys.
+struct Span {
+  int row0, rows;    // first row and rows of the tile
+  int first;         // place of the sequence's first new token
+  int key0, key1;    // this chunk's keys, from a unit's start
+  int off;           // the sequence's first packed token
+};
+__device__ __forceinline__ Span find_span(const KvAttnArgs& a, const Item& it) {
+  Span s;
+  s.row0 = it.tile * a.tile_rows;
+  s.rows = (int)min((long)a.tile_rows, (long)it.n * a.group - s.row0);
+  s.first = it.len - it.n;
+  s.off = a.offsets[it.seq];
+  const int tok_a = uniform(s.row0 / a.group), tok_b = uniform((s.row0 + s.rows - 1) / a.group);
+  const int lo = a.window > 0 ? max(0, s.first + tok_a - a.window + 1) >> a.key_shift << a.key_shift : 0;
+  const int hi = a.causal ? s.first + tok_b + 1 : it.len;
+  const int units = max(0, hi - lo + (1 << a.key_shift) - 1) >> a.key_shift;
+  const int q = uniform(units / it.chunks), r = units - q * it.chunks;  // the first r chunks have one more
+  const int u0 = q * it.chunk + min(it.chunk, r), u1 = u0 + q + (it.chunk < r ? 1 : 0);
+  s.key0 = lo + (u0 << a.key_shift);
+  s.key1 = min(hi, lo + (u1 << a.key_shift));
+  return s;
+}
+// row r of the tile: its token among the sequence's new ones and its query head
+struct RowAt {
+  int tok, head;
+};
+__device__ __forceinline__ RowAt row_at(const KvAttnArgs& a, const Span& s, int r, int head) {
+  const int base = s.row0 / a.group, x = s.row0 - base * a.group + r;  // x < tile rows + group
+  const int t = (x * a.group_inv) >> 16;
+  return RowAt{base + t, head * a.group + (x - t * a.group)};
+}
+
+// ---- a 16-key tile's block ------------------------------------------------------------------
+// (a block holds whole 16-key tiles)  NaN scales where the table names no block
+// of the pool: the rows that see the tile become NaN; the address is block 0's.
+struct TileInfo {
+  int id;
+  float ks, vs;
+};
+__device__ __forceinline__ int tile_id(const KvAttnArgs& a, int seq, int key, int end) {
+  const int b = key >> a.shift;
+  return key < end && b < a.width ? a.table[(long)seq * a.width + b] : key < end ? -1 : -2;
+}
+__device__ __forceinline__ TileInfo tile_info(const KvAttnArgs& a, int id, int head) {
+  const bool in = (unsigned)id < (unsigned)a.num_blocks;
+  TileInfo x{in ? id : 0, 0.0f, 0.0f};
+  if (id != -2) {  // -2: past the last key, never seen
+    x.ks = a.k_scale[(long)x.id * a.kv_heads + head];
+    x.vs = a.v_scale[(long)x.id * a.kv_heads + head];
+    x.ks = in && finite_bits(__float_as_uint(x.ks)) ? x.ks : __builtin_nanf("");
+    x.vs = in && finite_bits(__float_as_uint(x.vs)) ? x.vs : __builtin_nanf("");
   }
+  return x;
 }
-__device__ __forceinline__ void store1(void* out, long at, int type, float v) {
-  if (type == QHIP_TT_F32) ((float*)out)[at] = v;
-  else if (type == QHIP_TT_F16) ((f16_t*)out)[at] = (f16_t)v;
-  else ((bf16_t*)out)[at] = (bf16_t)v;
+
+// ---- queries ----------------------------------------------------------------------------------
+// A lane's pieces of eight query values as they lie in memory (f32 rows where
+// SPLIT is 2, else 16-bit ones).
+template <int SPLIT>
+using QElem = typename std::conditional<SPLIT == 2, float, uint16_t>::type;
+template <int SPLIT>
+using QRaw = Raw8<QElem<SPLIT>>;
+
+template <int SPLIT>
+__device__ __forceinline__ float q_value(const QRaw<SPLIT>& raw, int i, int type) {
+  if constexpr (SPLIT == 2) return raw.e[i];
+  else if (type == QHIP_TT_F16) return (float)__builtin_bit_cast(f16_t, raw.e[i]);
+  else return __uint_as_float((uint32_t)raw.e[i] << 16);
 }
-// N (a power of two) consecutive values, in pieces of up to 16 bytes where vec
-template <typename T, int N>
-__device__ __forceinline__ void store_pieces(T* out, const float* v) {
+// The row's values times a power of two that brings the largest to below 2^14,
+// as f16 or, SPLIT 2, as the sum of two (22 bits); returns the power.
+template <int SPLIT, int N, typename RowMax>
+__device__ __forceinline__ int split_q(const QRaw<SPLIT>* raw, int type, RowMax row_max, h16x8* hi, h16x8* lo) {
+  float top = 0.0f;
+#pragma unroll
+  for (int n = 0; n < N; ++n)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(q_value<SPLIT>(raw[n], i, type)));
+  const int e = 14 - __builtin_amdgcn_frexp_expf(row_max(top));
+#pragma unroll
+  for (int n = 0; n < N; ++n)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float x = __builtin_ldexpf(q_value<SPLIT>(raw[n], i, type), e);
+      hi[n][i] = (_Float16)x;
+      if constexpr (SPLIT == 2) lo[n][i] = (_Float16)(x - (float)hi[n][i]);
+    }
+  return e;
+}
+
+// ---- results ------------------------------------------------------------------------------------
+// N (a power of two) consecutive values of a row, in pieces of up to 16 bytes
+template <int SPLIT, int N>
+__device__ __forceinline__ void store_row(void* out, long at, int type, const float* v) {
+  typedef QElem<SPLIT> T;
   constexpr int P = N * sizeof(T) < 16 ? N : 16 / sizeof(T);
-  typedef T piece __attribute__((ext_vector_type(P)));
+  typedef T value __attribute__((ext_vector_type(P)));
+  struct __attribute__((packed, aligned(2))) piece { value x; };
 #pragma unroll
   for (int i = 0; i < N; i += P) {
-    piece x;
+    value x;
 #pragma unroll
-    for (int j = 0; j < P; ++j) x[j] = (T)v[i + j];
-    *(piece*)(out + i) = x;
+    for (int j = 0; j < P; ++j) {
+      if constexpr (SPLIT == 2) x[j] = v[i + j];
+      else x[j] = type == QHIP_TT_F16 ? __builtin_bit_cast(uint16_t, (f16_t)v[i + j]) : __builtin_bit_cast(uint16_t, (bf16_t)v[i + j]);
+    }
+    ((piece*)((T*)out + at + i))->x = x;
   }
 }
-template <int N>
-__device__ __forceinline__ void store_n(void* out, long at, int type, bool vec, const float* v) {
-  if (!vec) {
-#pragma unroll
-    for (int i = 0; i < N; ++i) store1(out, at + i, type, v[i]);
-  } else if (type == QHIP_TT_F32) {
-    store_pieces<float, N>((float*)out + at, v);
-  } else if (type == QHIP_TT_F16) {
-    store_pieces<f16_t, N>((f16_t*)out + at, v);
-  } else {
-    store_pieces<bf16_t, N>((bf16_t*)out + at, v);
-  }
-}
-
-// power of two of a value scale (a zero or a NaN has none)
-constexpr int kNoScale = -1000;
-__device__ __forceinline__ int scale_exp(float v) { return fabsf(v) > 0.0f ? __builtin_amdgcn_frexp_expf(v) : kNoScale; }
-
-// log(sum e^s) of a row whose maximum and sum are in powers of two
+// log(sum e^s) of a row whose maximum is in powers of two
 __device__ __forceinline__ float row_lse(float m, float l) {
-  return l == 0.0f ? kMinusInf : (m + __builtin_log2f(l)) * 0.693147180559945309f;
+  return l == 0.0f ? kMinusInf : (m + __builtin_log2f(l)) * kLn2;
 }
-
-// what e^-(m - M) leaves of a part whose maximum is m (both may be -infinity)
+// what 2^(m - top) leaves of a part whose maximum is m (both may be -infinity)
 __device__ __forceinline__ float weight_of(float m, float top) { return m == top ? 1.0f : __builtin_amdgcn_exp2f(m - top); }
 
-// ---- joining the chunks of a sequence's rows ----------------------------------------
+// A row's weights are scaled by 2^(14 - e), e the power of two of the largest
+// value scale that the row has seen (so that hidden blocks change no bit of it):
+// its output is in units of 2^(e - 14) times kCodeScale.
+constexpr int kNoScale = -1000;  // of a zero or a NaN
+__device__ __forceinline__ int scale_exp(float v) { return fabsf(v) > 0.0f ? __builtin_amdgcn_frexp_expf(v) : kNoScale; }
+__device__ __forceinline__ float in_units(float o, int e) { return __builtin_ldexpf(o, e - 14 + 9); }
+
+// ---- joining a tile's chunks ----------------------------------------------------------------------
 //
-// A chunk's partial results are `rows` x D outputs of its own keys, then each
-// row's maximum m and sum l, `stride` floats in all, stored and loaded through
-// to the agent's point of coherence (sc1: sk_store's and sk_load's policy, 16
-// bytes at a time).  Every chunk adds one to the tile's counter; the last one
-// joins all in chunk order, so the result does not depend on which was last.
-constexpr int kSc1 = 16;  // cache policy of a buffer access: sc1
+// A chunk's partial results are tile_rows x D outputs of its own keys, then each
+// row's maximum m and sum l, stored and loaded through to the agent's point of
+// coherence (sc1: sk_store's and sk_load's policy, 16 bytes at a time).  Every
+// chunk adds one to the tile's counter; the last one joins all in chunk order,
+// so the result does not depend on which was last.
+constexpr int kSc1 = 16;  // cache policy of a buffer access
+constexpr long kCountBytes = 32768;
+constexpr int kMaxCut = kCountBytes / 4;  // most row tiles that are cut
 
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t part_rsrc(float* p, long floats) {
   return __builtin_amdgcn_make_buffer_rsrc(p, 0, (int)(4 * floats), 0x00027000);  // raw, 32-bit, bounds-checked
@@ -254,25 +333,38 @@ __device__ __forceinline__ void part_store(__amdgpu_buffer_rsrc_t r, int at, con
   }
 }
 
-// LDS of a join: m (then weights) and l of `rows` x `chunks`, 1 / sum of each
-// row, and 4 KB of sums
+// LDS of a join: 4 KB of sums, 1 / sum of each row, m (then weights) and l of
+// rows x chunks
 constexpr int kJoinLds = 16384;
 constexpr int kJoinPairs = (kJoinLds - 4096 - 4 * 128) / 8;  // most rows x chunks
 
-// All 256 threads: the rows seq_row .. seq_row + count of key head `head`.
-template <int D>
-__device__ __forceinline__ void join_rows(const KvAttnArgs& a, float* lds, __amdgpu_buffer_rsrc_t parts, int stride, int rows,
-                                          int count, int chunks, int first_token, int seq_row, int head) {
-  const int tid = threadIdx.x;
-  float* s_acc = lds;               // [256][4]
-  float* s_inv = lds + 1024;        // [128]
-  float* s_m = lds + 1024 + 128;    // [chunks][count]
+// All 256 threads.  EB pieces of four values a thread and CB chunks are loaded
+// at a time; with fewer than 256 pieces the threads share out the chunks.
+template <int D, int SPLIT, int EB, int CB>
+__device__ __forceinline__ void join_rows(const KvAttnArgs& a, float* lds, __amdgpu_buffer_rsrc_t parts, const Item& it,
+                                          const Span& sp) {
+  const int tid = threadIdx.x, count = sp.rows, chunks = it.chunks, stride = a.tile_rows * (D + 2);
+  float* s_acc = lds;             // [256][4]
+  float* s_inv = lds + 1024;      // [128]
+  float* s_m = lds + 1024 + 128;  // [chunks][count]
   float* s_l = s_m + chunks * count;
+  const int pieces = count * (D / 4), slices = EB == 1 ? 256 / pieces : 1;
+  const int sl = EB == 1 ? tid / pieces : 0, e0 = EB == 1 ? tid - sl * pieces : tid;
+  kv_u32x4 x[EB][CB];
+  auto load = [&](int e, int c) {  // past the last piece or chunk: out of the buffer's bounds, 0
+#pragma unroll
+    for (int j = 0; j < EB; ++j)
+#pragma unroll
+      for (int k = 0; k < CB; ++k)
+        x[j][k] = __builtin_amdgcn_raw_buffer_load_b128(
+            parts, e + 256 * j < pieces && sl < slices ? 4 * ((c + k * slices) * stride + 4 * (e + 256 * j)) : -1, 0, kSc1);
+  };
+  load(e0, sl);
   for (int i = tid; i < chunks * count; i += 256) {
     const int c = i / count, r = i - c * count;
-    const kv_u32x2 x = __builtin_amdgcn_raw_buffer_load_b64(parts, 4 * (c * stride + rows * D + 2 * r), 0, kSc1);
-    s_m[i] = __uint_as_float(x[0]);
-    s_l[i] = __uint_as_float(x[1]);
+    const kv_u32x2 y = __builtin_amdgcn_raw_buffer_load_b64(parts, 4 * (c * stride + a.tile_rows * D + 2 * r), 0, kSc1);
+    s_m[i] = __uint_as_float(y[0]);
+    s_l[i] = __uint_as_float(y[1]);
   }
   __syncthreads();
   {
@@ -292,178 +384,179 @@ __device__ __forceinline__ void join_rows(const KvAttnArgs& a, float* lds, __amd
     for (int d = 1; d < team; d <<= 1) sum += __shfl_xor(sum, d, 64);
     if (r < count && tl == 0) {
       s_inv[r] = sum == 0.0f ? 0.0f : 1.0f / sum;
-      const int tok = (seq_row + r) / a.group, t = first_token + tok, qh = head * a.group + (seq_row + r - tok * a.group);
-      if (a.lse && t >= 0 && t < a.tokens) a.lse[(long)t * a.q_heads + qh] = row_lse(top, sum);
+      const RowAt w = row_at(a, sp, r, it.head);
+      const int t = sp.off + w.tok;
+      if (a.lse && t >= 0 && t < a.tokens) a.lse[(long)t * a.q_heads + w.head] = row_lse(top, sum);
     }
   }
   __syncthreads();
-  // four values a thread; with fewer than 256 of them, slices of the chunks
-  const int pieces = count * (D / 4), slices = pieces < 256 ? 256 / pieces : 1;
-  for (int e0 = 0; e0 < pieces; e0 += 256) {
-    const int sl = slices > 1 ? tid / pieces : 0, e = slices > 1 ? tid - sl * pieces : e0 + tid;
-    const int r = e / (D / 4);
-    f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
-    if (e < pieces && sl < slices)
-      for (int c0 = sl; c0 < chunks; c0 += 8 * slices) {
-        kv_u32x4 x[8];
+  for (int e = e0; e - tid < pieces; e += 256 * EB) {
+    f32x4 acc[EB] = {};
+    for (int c = sl; c < chunks; c += CB * slices) {
+      if (e != e0 || c != sl) load(e, c);
 #pragma unroll
-        for (int j = 0; j < 8; ++j)  // past the last chunk: out of the buffer's bounds, 0
-          x[j] = __builtin_amdgcn_raw_buffer_load_b128(parts, 4 * ((c0 + j * slices) * stride + 4 * e), 0, kSc1);
+      for (int j = 0; j < EB; ++j)
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const int c = c0 + j * slices;
-          const float f = c < chunks ? s_m[c * count + r] : 0.0f;
+        for (int k = 0; k < CB; ++k) {
+          const int cc = c + k * slices, r = (e + 256 * j) / (D / 4);
+          const float f = cc < chunks && r < count ? s_m[cc * count + r] : 0.0f;
 #pragma unroll
-          for (int i = 0; i < 4; ++i) acc[i] += f * __uint_as_float(x[j][i]);
+          for (int i = 0; i < 4; ++i) acc[j][i] += f * __uint_as_float(x[j][k][i]);
         }
-      }
-    if (slices > 1) {
-      ((f32x4*)s_acc)[tid] = acc;
+    }
+    if constexpr (EB == 1) {
+      ((f32x4*)s_acc)[tid] = acc[0];
       __syncthreads();
       if (sl == 0)
-        for (int k = 1; k < slices; ++k) acc += ((f32x4*)s_acc)[k * pieces + e];
+        for (int k = 1; k < slices; ++k) acc[0] += ((f32x4*)s_acc)[k * pieces + e];
     }
-    const int tok = (seq_row + r) / a.group, t = first_token + tok, qh = head * a.group + (seq_row + r - tok * a.group);
-    if (e < pieces && sl == 0 && t >= 0 && t < a.tokens) {
-      const float inv = s_inv[r], v[4] = {acc[0] * inv, acc[1] * inv, acc[2] * inv, acc[3] * inv};
-      store_n<4>(a.out, (long)t * a.out_token + (long)qh * a.out_head + 4 * (e % (D / 4)), a.type, a.out_vec, v);
+#pragma unroll
+    for (int j = 0; j < EB; ++j) {
+      const int ee = e + 256 * j, r = ee / (D / 4);
+      if (ee >= pieces || sl != 0) continue;
+      const RowAt w = row_at(a, sp, r, it.head);
+      const int t = sp.off + w.tok;
+      if (t < 0 || t >= a.tokens) continue;
+      const float inv = s_inv[r], v[4] = {acc[j][0] * inv, acc[j][1] * inv, acc[j][2] * inv, acc[j][3] * inv};
+      store_row<SPLIT, 4>(a.out, (long)t * a.out_token + (long)w.head * a.out_head + 4 * (ee % (D / 4)), a.type, v);
     }
+    if constexpr (EB == 1) break;
   }
 }
+// After every thread's part_stores: whether this workgroup was the tile's last,
+// which then joins.
+template <int D, int SPLIT>
+__device__ __forceinline__ void arrive_and_join(const KvAttnArgs& a, float* lds, __amdgpu_buffer_rsrc_t parts, const Item& it,
+                                                const Span& sp) {
+  unsigned* counter = a.counters + it.counter;
+  if (!sk_arrive(counter, (unsigned)it.chunks)) return;
+  sk_reset(counter);
+  constexpr int F = D == 64 ? 2 : 4;  // 16 pieces in flight a thread, where the registers allow it
+  if (sp.rows * (D / 4) <= 256) join_rows<D, SPLIT, 1, 4 * F>(a, lds, parts, it, sp);
+  else join_rows<D, SPLIT, F, 4>(a, lds, parts, it, sp);
+}
 
-// SPLIT 2: f32 rows, queries and weights in two f16 parts each
+// ---- sequences of a few rows: the cache streamed once ------------------------------
+//
+// Row tiles of 16, up to four in a workgroup.  The work is one pass over the
+// codes, 2 D bytes a key, so the kernel is built to keep loads in flight and
+// never puts a code anywhere but in a register:
+//
+//   S^T = K Q^T   16 keys x 16 rows a v_mfma_f32_16x16x32_f16; lane 16 g + i
+//                 loads 16-byte pieces of key i, whose dimensions (64 j + 16 g
+//                 ..+15) the query fragment has in the same order
+//   O^T = V^T P^T the accumulator of S^T (lane 16 g + r: row r, keys 4 g ..+3
+//                 of each of two tiles) is P's operand as it stands; lane 16 g +
+//                 i loads dimensions i D/16 ..+(D/16-1) of just those eight
+//                 keys, whole 16-lane rows contiguous, and picks a dimension's
+//                 eight codes with byte permutes
+//
+// so that a row's maximum, sum and output all stay in the four lanes 16 g + r.
+// f32 rows (SPLIT 2) take queries and softmax weights in two f16 parts each, 22
+// bits; f16 and bf16 rows, whose outputs are rounded to 11 and 8 bits, weights of
+// 11.  A block's key scale multiplies the scores, its value scale the weights.
+//
+// A workgroup's four waves take steps of 32 keys in turn (one, two or four row
+// tiles share a step's waves) and are merged in LDS.  Long sequences are cut
+// into chunks over workgroups (find_item).
+constexpr int kFewRows = 64;
+
 template <int D, int SPLIT>
 __global__ __launch_bounds__(256, D == 256 ? 2 : D == 128 ? 3 : 4) void k_kv_attention_few(KvAttnArgs a) {
   constexpr int J = D / 64, C = D / 16, W = D / 64;  // 64-dimension pieces, output tiles, dwords of a value load
-  constexpr int R = C * 4 * 64;  // floats of a wave's output
+  constexpr int R = C * 4 * 64;                      // floats of a wave's output
   __shared__ __attribute__((aligned(16))) float s_o[2 * R > kJoinLds / 4 ? 2 * R : kJoinLds / 4];
   __shared__ float s_m[2][64], s_l[2][64];
   __shared__ int s_e[2][64];
   const int tid = threadIdx.x, lane = tid & 63, r16 = lane & 15, g = lane >> 4;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  FewItem it;
-  if (!few_item(a, lane, it)) return;  // all four waves alike
-  const int seq = __builtin_amdgcn_readfirstlane(it.seq), n = __builtin_amdgcn_readfirstlane(it.s.n);
-  const int len = __builtin_amdgcn_readfirstlane(it.s.len), lo = __builtin_amdgcn_readfirstlane(it.s.lo);
-  const int chunks = __builtin_amdgcn_readfirstlane(it.chunks), chunk = __builtin_amdgcn_readfirstlane(it.chunk);
-  const int head = __builtin_amdgcn_readfirstlane(it.head);
-  const int rows = n * a.group, tiles = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
-  const int units = max(0, len - lo + 31) >> 5;
-  const int key0 = lo + 32 * (int)((long)units * chunk / chunks);
-  const int key1 = min(len, lo + 32 * (int)((long)units * (chunk + 1) / chunks));
+  const int wave = uniform(tid >> 6);
+  Item it;
+  if (!find_item(a, lane, it)) return;  // all four waves alike
+  const Span sp = find_span(a, it);
+  const int tiles = sp.rows <= 16 ? 1 : sp.rows <= 32 ? 2 : 4;
   const int part = wave / tiles, parts = 4 / tiles;
-  const int row = (wave % tiles) * 16 + r16;  // this lane's row
-  const bool own_row = row < rows;
-  const int tok = own_row ? row / a.group : 0, p = len - n + tok;
-  const int t = a.offsets[seq] + tok, qh = head * a.group + (row - tok * a.group);
-  const bool live = own_row && t >= 0 && t < a.tokens;
-  const int vis_hi = a.causal ? p + 1 : len, vis_lo = a.causal && a.window > 0 ? p - a.window + 1 : 0;
-  // keys that every row of the sequence sees
-  const int all_hi = a.causal ? len - n + 1 : len, all_lo = a.causal && a.window > 0 ? len - a.window : 0;
 
-  // the row's queries, scaled by a power of two
-  h16x8 qh_[J][2], ql_[SPLIT == 2 ? J : 1][2];
-  float c_row;
-  {
-    float v[J][2][8], top = 0.0f;
+  // lane i: tile i & 1 of this wave's step i / 2 of a round of 32 steps
+  int s0 = part;
+  auto round_id = [&]() { return tile_id(a, it.seq, sp.key0 + 32 * (s0 + parts * (lane >> 1)) + 16 * (lane & 1), sp.key1); };
+  const int id0 = round_id();
+
+  const int row = (wave % tiles) * 16 + r16;  // this lane's row
+  const RowAt w = row_at(a, sp, row < sp.rows ? row : 0, it.head);
+  const int p = sp.first + w.tok, t = sp.off + w.tok;
+  const bool live = row < sp.rows && t >= 0 && t < a.tokens;
+  const int vis_hi = a.causal ? p + 1 : it.len, vis_lo = a.window > 0 ? p - a.window + 1 : 0;
+  // keys that every row of the tile sees
+  const RowAt last = row_at(a, sp, sp.rows - 1, it.head);
+  const int all_hi = a.causal ? sp.first + uniform(sp.row0 / a.group) + 1 : it.len;
+  const int all_lo = a.window > 0 ? sp.first + uniform(last.tok) - a.window + 1 : 0;
+  QRaw<SPLIT> raw[2 * J] = {};
+  if (live) {
+    const long at = (long)t * a.q_token + (long)w.head * a.q_head + 16 * g;
 #pragma unroll
-    for (int j = 0; j < J; ++j)
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        if (live)
-          load_q8(a.q, (long)t * a.q_token + (long)qh * a.q_head + 64 * j + 16 * g + 8 * h, a.type, a.q_vec, v[j][h]);
-        else
-#pragma unroll
-          for (int i = 0; i < 8; ++i) v[j][h][i] = 0.0f;
-      }
-#pragma unroll
-    for (int j = 0; j < J; ++j)
-#pragma unroll
-      for (int h = 0; h < 2; ++h)
-#pragma unroll
-        for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(v[j][h][i]));
-    const int e = 14 - __builtin_amdgcn_frexp_expf(row_max(top));
-#pragma unroll
-    for (int j = 0; j < J; ++j)
-#pragma unroll
-      for (int h = 0; h < 2; ++h)
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const float x = __builtin_ldexpf(v[j][h][i], e);
-          const _Float16 hi = (_Float16)x;
-          qh_[j][h][i] = hi;
-          if constexpr (SPLIT == 2) ql_[j][h][i] = (_Float16)(x - (float)hi);
-        }
-    c_row = __builtin_ldexpf(a.scale * 1.44269504088896341f * kCodeScale, -e);
+    for (int i = 0; i < 2 * J; ++i) raw[i] = load8((const QElem<SPLIT>*)a.q + at + 64 * (i >> 1) + 8 * (i & 1));
   }
 
-  f32x4 o[C];
-#pragma unroll
-  for (int c = 0; c < C; ++c) o[c] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-  float m = kMinusInf, l = 0.0f;
-  int ve = kNoScale;  // power of two of the largest value scale that the row has seen: o is in units of 2^(ve - 14 + 9)
-
+  TileInfo info = tile_info(a, id0, it.head);
   const uint8_t* kc = (const uint8_t*)a.k;
   const uint8_t* vc = (const uint8_t*)a.v;
   const int mask = (1 << a.shift) - 1;
   const uint32_t koff = (uint32_t)(r16 * D + 16 * g), voff = (uint32_t)(4 * g * D + r16 * C);
-  for (int s0 = part; key0 + 32 * s0 < key1; s0 += 32 * parts) {
-    // lane i: tile i & 1 of this wave's step i / 2
-    const int mine = key0 + 32 * (s0 + parts * (lane >> 1)) + 16 * (lane & 1);
-    int id = 0;
-    float ks = 0.0f, vs = 0.0f;
-    if (mine < key1) {
-      const int b = mine >> a.shift;
-      id = b < a.width ? a.table[(long)seq * a.width + b] : -1;
-      const bool in = (unsigned)id < (unsigned)a.num_blocks;
-      id = in ? id : 0;
-      ks = a.k_scale[(long)id * a.kv_heads + head];
-      vs = a.v_scale[(long)id * a.kv_heads + head];
-      ks = in && finite_bits(__float_as_uint(ks)) ? ks : __builtin_nanf("");
-      vs = in && finite_bits(__float_as_uint(vs)) ? vs : __builtin_nanf("");
+  kv_u32x4 kr[2][J];
+  uint32_t vr[8][W];
+  auto tile_at = [&](int i) {  // byte offset of tile i's first code
+    const long b = __builtin_amdgcn_readlane(info.id, i);
+    const int first = (sp.key0 + 32 * (s0 + parts * (i >> 1)) + 16 * (i & 1)) & mask;
+    return ((b * a.kv_heads + it.head) << a.shift | first) * D;
+  };
+  auto load_k = [&](int st) {
+#pragma unroll
+    for (int tt = 0; tt < 2; ++tt) {
+      const uint8_t* b = kc + tile_at(2 * st + tt);
+#pragma unroll
+      for (int j = 0; j < J; ++j) kr[tt][j] = *(const kv_u32x4*)(b + koff + 64 * j);
     }
-    const int steps = min(32, (key1 - key0 - 32 * s0 + 32 * parts - 1) / (32 * parts));
-
-    kv_u32x4 kr[2][J];
-    uint32_t vr[8][W];
-    auto tile_at = [&](int i) {  // byte offset of tile i's first code
-      const long b = __builtin_amdgcn_readlane(id, i);
-      const int first = (key0 + 32 * (s0 + parts * (i >> 1)) + 16 * (i & 1)) & mask;
-      return ((b * a.kv_heads + head) << a.shift | first) * D;
-    };
-    auto load_k = [&](int st) {
+  };
+  auto load_v = [&](int st) {
 #pragma unroll
-      for (int tt = 0; tt < 2; ++tt) {
-        const uint8_t* b = kc + tile_at(2 * st + tt);
+    for (int tt = 0; tt < 2; ++tt) {
+      const uint8_t* b = vc + tile_at(2 * st + tt);
 #pragma unroll
-        for (int j = 0; j < J; ++j) kr[tt][j] = *(const kv_u32x4*)(b + koff + 64 * j);
-      }
-    };
-    auto load_v = [&](int st) {
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t* x = (const uint32_t*)(b + voff + i * D);
+        if constexpr (W == 4) {
+          const kv_u32x4 y = *(const kv_u32x4*)x;
 #pragma unroll
-      for (int tt = 0; tt < 2; ++tt) {
-        const uint8_t* b = vc + tile_at(2 * st + tt);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const uint32_t* x = (const uint32_t*)(b + voff + i * D);
-          if constexpr (W == 4) {
-            const kv_u32x4 y = *(const kv_u32x4*)x;
-#pragma unroll
-            for (int w = 0; w < 4; ++w) vr[4 * tt + i][w] = y[w];
-          } else if constexpr (W == 2) {
-            const kv_u32x2 y = *(const kv_u32x2*)x;
-            vr[4 * tt + i][0] = y[0];
-            vr[4 * tt + i][1] = y[1];
-          } else {
-            vr[4 * tt + i][0] = x[0];
-          }
+          for (int w = 0; w < 4; ++w) vr[4 * tt + i][w] = y[w];
+        } else if constexpr (W == 2) {
+          const kv_u32x2 y = *(const kv_u32x2*)x;
+          vr[4 * tt + i][0] = y[0];
+          vr[4 * tt + i][1] = y[1];
+        } else {
+          vr[4 * tt + i][0] = x[0];
         }
       }
-    };
+    }
+  };
+  const bool any = sp.key0 + 32 * s0 < sp.key1;
+  if (any) {
     load_k(0);
     load_v(0);
+  }
+
+  h16x8 q_hi[2 * J], q_lo[SPLIT == 2 ? 2 * J : 1];
+  const int qe = split_q<SPLIT, 2 * J>(raw, a.type, max16, q_hi, q_lo);
+  const float c_row = __builtin_ldexpf(a.scale * kLog2e * kCodeScale, -qe);
+  f32x4 o[C];
+#pragma unroll
+  for (int c = 0; c < C; ++c) o[c] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  float m = kMinusInf, l = 0.0f;
+  int ve = kNoScale;
+
+  while (any) {
+    const int steps = min(32, (sp.key1 - sp.key0 - 32 * s0 + 32 * parts - 1) / (32 * parts));
     for (int st = 0; st < steps; ++st) {
-      const int key = key0 + 32 * (s0 + parts * st);
+      const int key = sp.key0 + 32 * (s0 + parts * st);
       float s[2][4];
 #pragma unroll
       for (int tt = 0; tt < 2; ++tt) {
@@ -472,31 +565,28 @@ __global__ __launch_bounds__(256, D == 256 ? 2 : D == 128 ? 3 : 4) void k_kv_att
         for (int j = 0; j < J; ++j) {
           const kv_u32x4 x = kr[tt][j] ^ 0x80808080u;
           const h16x8 k0 = codes8(x[0], x[1]), k1 = codes8(x[2], x[3]);
-          hi = __builtin_amdgcn_mfma_f32_16x16x32_f16(k0, qh_[j][0], hi, 0, 0, 0);
-          hi = __builtin_amdgcn_mfma_f32_16x16x32_f16(k1, qh_[j][1], hi, 0, 0, 0);
+          hi = __builtin_amdgcn_mfma_f32_16x16x32_f16(k0, q_hi[2 * j], hi, 0, 0, 0);
+          hi = __builtin_amdgcn_mfma_f32_16x16x32_f16(k1, q_hi[2 * j + 1], hi, 0, 0, 0);
           if constexpr (SPLIT == 2) {
-            low = __builtin_amdgcn_mfma_f32_16x16x32_f16(k0, ql_[j][0], low, 0, 0, 0);
-            low = __builtin_amdgcn_mfma_f32_16x16x32_f16(k1, ql_[j][1], low, 0, 0, 0);
+            low = __builtin_amdgcn_mfma_f32_16x16x32_f16(k0, q_lo[2 * j], low, 0, 0, 0);
+            low = __builtin_amdgcn_mfma_f32_16x16x32_f16(k1, q_lo[2 * j + 1], low, 0, 0, 0);
           }
         }
 #pragma unroll
         for (int r = 0; r < 4; ++r) s[tt][r] = SPLIT == 2 ? hi[r] + low[r] : hi[r];
       }
       if (st + 1 < steps) load_k(st + 1);
-      const float c0 = c_row * __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(ks), 2 * st));
-      const float c1 = c_row * __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(ks), 2 * st + 1));
-      const float v0 = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(vs), 2 * st));
-      const float v1 = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(vs), 2 * st + 1));
-      float top = kMinusInf;
-      const bool edge = key < all_lo || key + 32 > min(all_hi, key1);  // some row does not see some key
+      const float c0 = c_row * lane_f(info.ks, 2 * st), c1 = c_row * lane_f(info.ks, 2 * st + 1);
+      const float v0 = lane_f(info.vs, 2 * st), v1 = lane_f(info.vs, 2 * st + 1);
+      const bool edge = key < all_lo || key + 32 > min(all_hi, sp.key1);  // some row does not see some key
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         s[0][r] *= c0;
         s[1][r] *= c1;
       }
       int e0 = scale_exp(v0), e1 = scale_exp(v1);
+      const int end = min(vis_hi, sp.key1);
       if (edge) {
-        const int end = min(vis_hi, key1);
 #pragma unroll
         for (int tt = 0; tt < 2; ++tt)
 #pragma unroll
@@ -508,9 +598,10 @@ __global__ __launch_bounds__(256, D == 256 ? 2 : D == 128 ? 3 : 4) void k_kv_att
         if (key + 16 >= end || key + 32 <= vis_lo) e1 = kNoScale;
       }
       e0 = max(ve, max(e0, e1));
+      float top = fmaxf(s[0][0], s[1][0]);
 #pragma unroll
-      for (int r = 0; r < 4; ++r) top = fmaxf(top, fmaxf(s[0][r], s[1][r]));
-      top = fmaxf(m, row_max(top));
+      for (int r = 1; r < 4; ++r) top = fmaxf(top, fmaxf(s[0][r], s[1][r]));
+      top = fmaxf(m, max16(top));
       if (__any(top != m || e0 != ve)) {
         const float f = weight_of(m, top), fo = __builtin_ldexpf(f, ve - e0);
         l *= f;
@@ -526,12 +617,12 @@ __global__ __launch_bounds__(256, D == 256 ? 2 : D == 128 ? 3 : 4) void k_kv_att
       for (int tt = 0; tt < 2; ++tt)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          // m is -infinity where the row has seen nothing yet; what it does not
-          // see has weight 0 whatever its block's scales are
           float e = __builtin_amdgcn_exp2f(s[tt][r] - m), x = e * (tt ? w1 : w0);
           if (edge) {
+            // m is -infinity where the row has seen nothing yet; what it does not
+            // see has weight 0 whatever its block's scales are
             const int j = key + 16 * tt + 4 * g + r;
-            if (j < vis_lo || j >= vis_hi || j >= key1) e = x = 0.0f;
+            if (j < vis_lo || j >= end) e = x = 0.0f;
           }
           sum += e;
           const _Float16 hi = (_Float16)x;
@@ -546,20 +637,20 @@ __global__ __launch_bounds__(256, D == 256 ? 2 : D == 128 ? 3 : 4) void k_kv_att
         for (int i = 0; i < 8; ++i) x[i] = vr[i][w] ^ 0x80808080u;
 #pragma unroll
         for (int b = 0; b < 4; ++b) {
-          h16x2 y[4];
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            y[i] = b == 0 ? codes_of<0>(x[2 * i], x[2 * i + 1]) : b == 1 ? codes_of<1>(x[2 * i], x[2 * i + 1])
-                 : b == 2 ? codes_of<2>(x[2 * i], x[2 * i + 1]) : codes_of<3>(x[2 * i], x[2 * i + 1]);
-          const h16x8 v8 = {y[0][0], y[0][1], y[1][0], y[1][1], y[2][0], y[2][1], y[3][0], y[3][1]};
+          const h16x8 v8 = b == 0 ? codes_across<0>(x) : b == 1 ? codes_across<1>(x) : b == 2 ? codes_across<2>(x) : codes_across<3>(x);
           o[4 * w + b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v8, ph, o[4 * w + b], 0, 0, 0);
           if constexpr (SPLIT == 2) o[4 * w + b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v8, pl, o[4 * w + b], 0, 0, 0);
         }
       }
       if (st + 1 < steps) load_v(st + 1);
     }
+    s0 += 32 * parts;
+    if (sp.key0 + 32 * s0 >= sp.key1) break;
+    info = tile_info(a, round_id(), it.head);
+    load_k(0);
+    load_v(0);
   }
-  l = row_sum(l);
+  l = sum16(l);
 
   // merge the waves that share a row tile: the upper half of the parts into the lower
   for (int half = parts / 2; half >= 1; half >>= 1) {
@@ -592,39 +683,39 @@ __global__ __launch_bounds__(256, D == 256 ? 2 : D == 128 ? 3 : 4) void k_kv_att
 
   // a row that sees nothing: 0 and -infinity (l is 0); NaN stays
   const float norm = l == 0.0f ? 0.0f : 1.0f / l;
-  if (chunks == 1) {
+#pragma unroll
+  for (int c = 0; c < C; ++c)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) o[c][r] = in_units(o[c][r] * norm, ve);
+  if (it.chunks == 1) {
     if (wave < tiles && live) {
-      const long at = (long)t * a.out_token + (long)qh * a.out_head + (4 * g) * C;
+      const long at = (long)t * a.out_token + (long)w.head * a.out_head + 4 * g * C;
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         float v[C];
 #pragma unroll
-        for (int c = 0; c < C; ++c) v[c] = __builtin_ldexpf(o[c][r] * norm, ve - 14 + 9);
-        store_n<C>(a.out, at + r * C, a.type, a.out_vec, v);
+        for (int c = 0; c < C; ++c) v[c] = o[c][r];
+        store_row<SPLIT, C>(a.out, at + r * C, a.type, v);
       }
-      if (a.lse && g == 0) a.lse[(long)t * a.q_heads + qh] = row_lse(m, l);
+      if (a.lse && g == 0) a.lse[(long)t * a.q_heads + w.head] = row_lse(m, l);
     }
     return;
   }
-  // partial results of the chunk: out [rows][D] (of its own keys), then m and l
-  if (it.slot + chunks > a.slots) return;  // offsets or lengths that are none
-  const int stride = a.rows * (D + 2);
-  const __amdgpu_buffer_rsrc_t parts_at = part_rsrc(a.partial + (long)it.slot * stride, (long)chunks * stride);
-  if (wave < tiles && own_row) {
+  if (it.slot + it.chunks > a.slots || it.counter >= kMaxCut) return;  // offsets or lengths that are none
+  const int stride = a.tile_rows * (D + 2);
+  const __amdgpu_buffer_rsrc_t parts_at = part_rsrc(a.partial + (long)it.slot * stride, (long)it.chunks * stride);
+  if (wave < tiles && row < sp.rows) {
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       float v[C];
 #pragma unroll
-      for (int c = 0; c < C; ++c) v[c] = __builtin_ldexpf(o[c][r] * norm, ve - 14 + 9);
-      part_store<C>(parts_at, chunk * stride + row * D + (4 * g + r) * C, v);
+      for (int c = 0; c < C; ++c) v[c] = o[c][r];
+      part_store<C>(parts_at, it.chunk * stride + row * D + (4 * g + r) * C, v);
     }
     const float stat[2] = {m, l};
-    if (g == 0) part_store<2>(parts_at, chunk * stride + a.rows * D + 2 * row, stat);
+    if (g == 0) part_store<2>(parts_at, it.chunk * stride + a.tile_rows * D + 2 * row, stat);
   }
-  unsigned* count = a.counters + (long)seq * a.kv_heads + head;
-  if (!sk_arrive(count, (unsigned)chunks)) return;
-  sk_reset(count);
-  join_rows<D>(a, s_o, parts_at, stride, a.rows, rows, chunks, a.offsets[seq], 0, head);
+  arrive_and_join<D, SPLIT>(a, s_o, parts_at, it, sp);
 }
 
 // ---- sequences of many rows: key tiles staged in LDS ---------------------------------
@@ -641,72 +732,8 @@ __global__ __launch_bounds__(256, D == 256 ? 2 : D == 128 ? 3 : 4) void k_kv_att
 // tile c holds dimensions i D/32 + c.  The next tile's codes are in flight in
 // registers while this one is multiplied.
 
-typedef float f32x16 __attribute__((ext_vector_type(16)));
-
 constexpr int kManyRows = 128;
 constexpr int kManyKeys = 64;
-
-
-struct ManySeq {
-  int n, len, tiles, units;  // new tokens (0: not one of these sequences), tokens, row tiles, key tiles to plan for
-};
-__device__ __forceinline__ ManySeq many_seq(const KvAttnArgs& a, int i) {
-  ManySeq s{0, 0, 0, 0};
-  if (i >= a.nseq) return s;
-  const int n = a.offsets[i + 1] - a.offsets[i];
-  if (n <= a.few_tokens || n > a.tokens) return s;
-  s.n = n;
-  s.len = max(a.kv_lens[i], 0);
-  s.tiles = (int)(((long)(min(a.offsets[i + 1], a.tokens) - a.offsets[i]) * a.group + kManyRows - 1) / kManyRows);
-  if (s.tiles <= 0) return ManySeq{0, 0, 0, 0};
-  int keys = s.len;
-  if (a.causal && a.window > 0) keys = (int)min((long)keys, (long)a.window + kManyRows / a.group + 2 * kManyKeys);
-  s.units = min((keys + kManyKeys - 1) / kManyKeys, a.max_units);
-  return s;
-}
-struct ManyItem {
-  int seq, head, tile, chunk, chunks, slot, counter;
-  ManySeq s;
-};
-__device__ __forceinline__ bool many_item(const KvAttnArgs& a, int lane, ManyItem& it) {
-  const int at = blockIdx.x / a.kv_heads;
-  it.head = blockIdx.x - at * a.kv_heads;
-  int unit = 0x7FFFFFFF;
-  ManySeq s = many_seq(a, lane);
-  if (a.cut) {
-    int total = s.tiles * s.units;
-    for (int i = 64 + lane; i - lane < a.nseq; i += 64) {
-      const ManySeq x = many_seq(a, i);
-      total += x.tiles * x.units;
-    }
-    total = wave_sum(total);
-    unit = max(a.least, (int)(((long)total * a.kv_heads + a.target - 1) / a.target));
-  }
-  int items = 0, slots = 0, tiles = 0;
-  for (int i0 = 0; i0 < a.nseq; i0 += 64) {
-    if (i0) s = many_seq(a, i0 + lane);
-    const int c = min(a.max_chunks, max(1, (int)(((long)s.units + unit - 1) / unit))), n = s.tiles * c, cut = c > 1 ? n : 0;
-    const int ci = wave_scan(n, lane), cs = wave_scan(cut, lane), ct = wave_scan(s.tiles, lane);
-    const int all = __shfl(ci, 63, 64);
-    if (at < items + all) {
-      const int owner = __builtin_ctzll(__ballot(items + ci > at));
-      it.seq = i0 + owner;
-      it.s = ManySeq{__shfl(s.n, owner, 64), __shfl(s.len, owner, 64), __shfl(s.tiles, owner, 64), 0};
-      it.chunks = __shfl(c, owner, 64);
-      const int local = at - (items + __shfl(ci, owner, 64) - it.s.tiles * it.chunks);
-      const int tile = local / it.chunks;
-      it.chunk = local - tile * it.chunks;
-      it.tile = it.s.tiles - 1 - tile;  // the last rows see the most keys: they begin first
-      it.slot = (slots + __shfl(cs, owner, 64) - (it.s.tiles - tile) * it.chunks) * a.kv_heads + it.head * it.chunks;
-      it.counter = (tiles + __shfl(ct, owner, 64) - it.s.tiles + it.tile) * a.kv_heads + it.head;
-      return true;
-    }
-    items += all;
-    slots += __shfl(cs, 63, 64);
-    tiles += __shfl(ct, 63, 64);
-  }
-  return false;
-}
 
 // the 16-byte piece of a value row that holds piece x of dimension `dim`
 template <int D>
@@ -725,104 +752,47 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_kv_attention_many(KvA
   uint8_t *const s_k = s_kv, *const s_v = s_kv + kManyKeys * D * 2;
   static_assert(sizeof(s_kv) >= kJoinLds, "the join's LDS");
   const int tid = threadIdx.x, lane = tid & 63, r32 = lane & 31, h = lane >> 5;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  ManyItem it;
-  if (!many_item(a, lane, it)) return;
-  const int seq = __builtin_amdgcn_readfirstlane(it.seq), n = __builtin_amdgcn_readfirstlane(it.s.n);
-  const int len = __builtin_amdgcn_readfirstlane(it.s.len), head = __builtin_amdgcn_readfirstlane(it.head);
-  const int chunks = __builtin_amdgcn_readfirstlane(it.chunks), chunk = __builtin_amdgcn_readfirstlane(it.chunk);
-  const int row_first = __builtin_amdgcn_readfirstlane(it.tile) * kManyRows;
-  const int rows = (int)min((long)kManyRows, (long)n * a.group - row_first);
-  const int first = len - n;  // place of the sequence's first new token
-  const bool windowed = a.causal && a.window > 0;
-  // the tile's keys, and this chunk's
-  const int tok_a = row_first / a.group, tok_b = (row_first + rows - 1) / a.group;
-  const int lo = windowed ? max(0, first + tok_a - a.window + 1) & ~(kManyKeys - 1) : 0;
-  const int hi = a.causal ? first + tok_b + 1 : len;
-  const int all_tiles = max(0, hi - lo + kManyKeys - 1) / kManyKeys;
-  const int tile0 = (int)((long)all_tiles * chunk / chunks), tile1 = (int)((long)all_tiles * (chunk + 1) / chunks);
-  const int key0 = lo + tile0 * kManyKeys, count = tile1 - tile0;
+  const int wave = uniform(tid >> 6);
+  Item it;
+  if (!find_item(a, lane, it)) return;
+  const Span sp = find_span(a, it);
+  const int count = max(0, sp.key1 - sp.key0 + kManyKeys - 1) / kManyKeys;  // key tiles
+
+  // lane i: 16-key tile i of a round of 16 key tiles
+  auto round_id = [&](int round) { return tile_id(a, it.seq, sp.key0 + round * 16 * kManyKeys + 16 * lane, sp.key1); };
+  const int id0 = round_id(0), id1 = round_id(1);
 
   // this lane's row, and what the wave's rows see
   const int wrow = wave * 32, row = wrow + r32;
-  const bool own_row = row < rows;
-  const int tok = own_row ? (row_first + row) / a.group : tok_a, p = first + tok;
-  const int t = a.offsets[seq] + tok, qh = head * a.group + (row_first + row - tok * a.group);
-  const bool live = own_row && t >= 0 && t < a.tokens;
-  const int vis_hi = a.causal ? p + 1 : len, vis_lo = windowed ? p - a.window + 1 : 0;
-  const int wtok_a = (row_first + wrow) / a.group, wtok_b = (row_first + min(wrow + 31, rows - 1)) / a.group;
-  const bool busy = wrow < rows;
-  const int all_hi = a.causal ? first + wtok_a + 1 : len, all_lo = windowed ? first + wtok_b - a.window + 1 : 0;
-  const int any_hi = a.causal ? first + wtok_b + 1 : len, any_lo = windowed ? first + wtok_a - a.window + 1 : 0;
-
-  h16x8 q_hi[S], q_lo[SPLIT == 2 ? S : 1];
-  float c_row;
-  {
-    float top = 0.0f;
-    const long at = (long)t * a.q_token + (long)qh * a.q_head + 8 * h;
+  const bool busy = wrow < sp.rows;
+  const RowAt w = row_at(a, sp, row < sp.rows ? row : 0, it.head);
+  const int p = sp.first + w.tok, t = sp.off + w.tok;
+  const bool live = row < sp.rows && t >= 0 && t < a.tokens;
+  const int vis_hi = a.causal ? p + 1 : it.len, vis_lo = a.window > 0 ? p - a.window + 1 : 0;
+  const int tok_a = uniform(row_at(a, sp, wrow, it.head).tok);
+  const int tok_b = uniform(row_at(a, sp, min(wrow + 31, sp.rows - 1), it.head).tok);
+  const int all_hi = a.causal ? sp.first + tok_a + 1 : it.len, all_lo = a.window > 0 ? sp.first + tok_b - a.window + 1 : 0;
+  const int any_hi = a.causal ? sp.first + tok_b + 1 : it.len, any_lo = a.window > 0 ? sp.first + tok_a - a.window + 1 : 0;
+  QRaw<SPLIT> raw[S] = {};
+  if (live) {
+    const long at = (long)t * a.q_token + (long)w.head * a.q_head + 8 * h;
 #pragma unroll
-    for (int s = 0; s < S; ++s) {
-      float v[8] = {};
-      if (live) load_q8(a.q, at + 16 * s, a.type, a.q_vec, v);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(v[i]));
-    }
-    const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
-    const int e = 14 - __builtin_amdgcn_frexp_expf(fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1])));
-#pragma unroll
-    for (int s = 0; s < S; ++s) {
-      float v[8] = {};
-      if (live) load_q8(a.q, at + 16 * s, a.type, a.q_vec, v);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float x = __builtin_ldexpf(v[i], e);
-        q_hi[s][i] = (_Float16)x;
-        if constexpr (SPLIT == 2) q_lo[s][i] = (_Float16)(x - (float)q_hi[s][i]);
-      }
-    }
-    c_row = __builtin_ldexpf(a.scale * 1.44269504088896341f * kCodeScale, -e);
+    for (int i = 0; i < S; ++i) raw[i] = load8((const QElem<SPLIT>*)a.q + at + 16 * i);
   }
 
-  f32x16 o[C];
-#pragma unroll
-  for (int c = 0; c < C; ++c)
-#pragma unroll
-    for (int i = 0; i < 16; ++i) o[c][i] = 0.0f;
-  float m = kMinusInf, l = 0.0f;
-  int ve = kNoScale;
-
-  // lane i: the 16-key tile i of a round of 16 key tiles
-  struct Info {
-    int id;
-    float ks, vs;
-  };
-  auto load_info = [&](int round) {
-    Info x{0, 0.0f, 0.0f};
-    const int mine = key0 + round * 16 * kManyKeys + 16 * lane;
-    if (mine < hi) {
-      const int b = mine >> a.shift;
-      const int id = b < a.width ? a.table[(long)seq * a.width + b] : -1;
-      const bool in = (unsigned)id < (unsigned)a.num_blocks;
-      x.id = in ? id : 0;
-      x.ks = a.k_scale[(long)x.id * a.kv_heads + head];
-      x.vs = a.v_scale[(long)x.id * a.kv_heads + head];
-      x.ks = in && finite_bits(__float_as_uint(x.ks)) ? x.ks : __builtin_nanf("");
-      x.vs = in && finite_bits(__float_as_uint(x.vs)) ? x.vs : __builtin_nanf("");
-    }
-    return x;
-  };
+  TileInfo info = tile_info(a, id0, it.head), next = tile_info(a, id1, it.head);
   const int mask = (1 << a.shift) - 1;
   // staging: pieces of keys (D / 16 a key), then 8 keys of 4 VW dimensions of the values
-  const int kkey = tid / (D / 16), kpc = tid % (D / 16);   // first key (a step of 4096 / D further each piece)
+  const int kkey = tid / (D / 16), kpc = tid % (D / 16);  // first key (4096 / D further each piece)
   const int vgrp = tid / (D / (4 * VW)), vdim = (tid % (D / (4 * VW))) * 4 * VW;
   // group x of the values' eight: keys 32 (x >> 2) + 16 (x >> 1 & 1) + 4 (x & 1) + {0..3, 8..11}
   const int vkey = 32 * (vgrp >> 2) + 16 * ((vgrp >> 1) & 1) + 4 * (vgrp & 1);
   kv_u32x4 kr[KP];
   uint32_t vr[8][VW];
-  auto load_tile = [&](const Info& x, int i) {  // key tile i of the round
+  auto load_tile = [&](const TileInfo& x, int i) {  // key tile i of the round
     auto at = [&](int key) {  // byte offset of a key's codes
       const long id = __shfl(x.id, 4 * i + (key >> 4), 64);
-      return ((id * a.kv_heads + head) << a.shift | ((16 * (4 * i + (key >> 4)) + key0 + (key & 15)) & mask)) * D;
+      return ((id * a.kv_heads + it.head) << a.shift | ((sp.key0 + 16 * (4 * i + (key >> 4)) + (key & 15)) & mask)) * D;
     };
 #pragma unroll
     for (int j = 0; j < KP; ++j) kr[j] = *(const kv_u32x4*)((const uint8_t*)a.k + at(kkey + j * (4096 / D)) + 16 * kpc);
@@ -858,26 +828,31 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_kv_attention_many(KvA
         for (int j = 0; j < 8; ++j) x[j] = vr[j][w] ^ 0x80808080u;
 #pragma unroll
         for (int b = 0; b < 4; ++b) {
-          h16x2 y[4];
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-            y[j] = b == 0 ? codes_of<0>(x[2 * j], x[2 * j + 1]) : b == 1 ? codes_of<1>(x[2 * j], x[2 * j + 1])
-                 : b == 2 ? codes_of<2>(x[2 * j], x[2 * j + 1]) : codes_of<3>(x[2 * j], x[2 * j + 1]);
           const int dim = vdim + 4 * w + b;
           *(h16x8*)(s_v + dim * 128 + value_piece<D>(dim, vgrp) * 16) =
-              h16x8{y[0][0], y[0][1], y[1][0], y[1][1], y[2][0], y[2][1], y[3][0], y[3][1]};
+              b == 0 ? codes_across<0>(x) : b == 1 ? codes_across<1>(x) : b == 2 ? codes_across<2>(x) : codes_across<3>(x);
         }
       }
     }
   };
-
-  Info info = load_info(0), next = load_info(1);
   if (count > 0) load_tile(info, 0);
+
+  h16x8 q_hi[S], q_lo[SPLIT == 2 ? S : 1];
+  const int qe = split_q<SPLIT, S>(raw, a.type, max32, q_hi, q_lo);
+  const float c_row = __builtin_ldexpf(a.scale * kLog2e * kCodeScale, -qe);
+  f32x16 o[C];
+#pragma unroll
+  for (int c = 0; c < C; ++c)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) o[c][i] = 0.0f;
+  float m = kMinusInf, l = 0.0f;
+  int ve = kNoScale;
+
   for (int i = 0; i < count; ++i) {
     const int ri = i & 15;
     if (ri == 0 && i) {
       info = next;
-      next = load_info((i >> 4) + 1);
+      next = tile_info(a, round_id((i >> 4) + 1), it.head);
     }
     __syncthreads();  // the previous tile has been read
     store_tile();
@@ -886,7 +861,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_kv_attention_many(KvA
       if (ri == 15) load_tile(next, 0);
       else load_tile(info, ri + 1);
     }
-    const int key = key0 + i * kManyKeys;
+    const int key = sp.key0 + i * kManyKeys;
 #pragma unroll 1
     for (int mt = 0; mt < 2; ++mt) {
       const int kt = key + 32 * mt;
@@ -900,10 +875,10 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_kv_attention_many(KvA
         if constexpr (SPLIT == 2) sl = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, q_lo[st], sl, 0, 0, 0);
       }
       const int sc = 4 * ri + 2 * mt;
-      const float c0 = c_row * __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(info.ks), sc));
-      const float c1 = c_row * __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(info.ks), sc + 1));
-      const float v0 = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(info.vs), sc));
-      const float v1 = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(info.vs), sc + 1));
+      const float c0 = c_row * lane_f(info.ks, sc);
+      const float c1 = c_row * lane_f(info.ks, sc + 1);
+      const float v0 = lane_f(info.vs, sc);
+      const float v1 = lane_f(info.vs, sc + 1);
       const bool edge = kt < all_lo || kt + 32 > all_hi;
 #pragma unroll
       for (int r = 0; r < 16; ++r) s[r] = (SPLIT == 2 ? s[r] + sl[r] : s[r]) * (r < 8 ? c0 : c1);
@@ -921,8 +896,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_kv_attention_many(KvA
       float top = s[0];
 #pragma unroll
       for (int r = 1; r < 16; ++r) top = fmaxf(top, s[r]);
-      const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
-      top = fmaxf(m, fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1])));
+      top = fmaxf(m, max32(top));
       if (__any(top != m || e0 != ve)) {
         const float f = weight_of(m, top), fo = __builtin_ldexpf(f, ve - e0);
         l *= f;
@@ -958,43 +932,41 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_kv_attention_many(KvA
         }
     }
   }
-  {
-    const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(l), __float_as_uint(l), false, false);
-    l = __uint_as_float(sw[0]) + __uint_as_float(sw[1]);
-  }
+  l = sum32(l);
   const float norm = l == 0.0f ? 0.0f : 1.0f / l;
-  if (chunks == 1) {
+#pragma unroll
+  for (int c = 0; c < C; ++c)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) o[c][r] = in_units(o[c][r] * norm, ve);
+  if (it.chunks == 1) {
     if (live) {
-      const long at = (long)t * a.out_token + (long)qh * a.out_head;
+      const long at = (long)t * a.out_token + (long)w.head * a.out_head;
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
         float v[C];
 #pragma unroll
-        for (int c = 0; c < C; ++c) v[c] = __builtin_ldexpf(o[c][r] * norm, ve - 14 + 9);
-        store_n<C>(a.out, at + (8 * (r >> 2) + 4 * h + (r & 3)) * C, a.type, a.out_vec, v);
+        for (int c = 0; c < C; ++c) v[c] = o[c][r];
+        store_row<SPLIT, C>(a.out, at + (8 * (r >> 2) + 4 * h + (r & 3)) * C, a.type, v);
       }
-      if (a.lse && h == 0) a.lse[(long)t * a.q_heads + qh] = row_lse(m, l);
+      if (a.lse && h == 0) a.lse[(long)t * a.q_heads + w.head] = row_lse(m, l);
     }
     return;
   }
-  if (it.slot + chunks > a.slots || it.counter >= kMaxCut) return;  // offsets or lengths that are none
+  if (it.slot + it.chunks > a.slots || it.counter >= kMaxCut) return;  // offsets or lengths that are none
   constexpr int kStride = kManyRows * (D + 2);
-  const __amdgpu_buffer_rsrc_t parts_at = part_rsrc(a.partial + (long)it.slot * kStride, (long)chunks * kStride);
-  if (own_row) {
+  const __amdgpu_buffer_rsrc_t parts_at = part_rsrc(a.partial + (long)it.slot * kStride, (long)it.chunks * kStride);
+  if (row < sp.rows) {
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
       float v[C];
 #pragma unroll
-      for (int c = 0; c < C; ++c) v[c] = __builtin_ldexpf(o[c][r] * norm, ve - 14 + 9);
-      part_store<C>(parts_at, chunk * kStride + row * D + (8 * (r >> 2) + 4 * h + (r & 3)) * C, v);
+      for (int c = 0; c < C; ++c) v[c] = o[c][r];
+      part_store<C>(parts_at, it.chunk * kStride + row * D + (8 * (r >> 2) + 4 * h + (r & 3)) * C, v);
     }
     const float stat[2] = {m, l};
-    if (h == 0) part_store<2>(parts_at, chunk * kStride + kManyRows * D + 2 * row, stat);
+    if (h == 0) part_store<2>(parts_at, it.chunk * kStride + kManyRows * D + 2 * row, stat);
   }
-  unsigned* counter = a.counters + it.counter;
-  if (!sk_arrive(counter, (unsigned)chunks)) return;
-  sk_reset(counter);
-  join_rows<D>(a, (float*)s_kv, parts_at, kStride, kManyRows, rows, chunks, a.offsets[seq], row_first, head);
+  arrive_and_join<D, SPLIT>(a, (float*)s_kv, parts_at, it, sp);
 }
 
 template <int SPLIT>
@@ -1020,43 +992,51 @@ static int check_batch(const qhip_kv_cache* cache, const qhip_kv_batch* b, int q
   return rc;
 }
 
-// How one of the two kernels' sequences are cut: grid without and with a cut,
-// key units of the longest sequence, items aimed for, fewest units of one, and
-// the workspace (0: no cut).
+// One kernel's share of a batch: its sequences, tile and unit sizes, grid without
+// and with a cut, items aimed for, and the workspace (0: no cut).
 struct AttnPlan {
-  int rows, max_units, target, least;
+  int min_tokens, max_tokens, rows, key_shift, units, target, least;
   long grid, cut_grid, work;
 };
-// `tiles`: bound of the row tiles over all sequences and key heads; a sequence
-// that is cut has less than twice units / unit chunks, where a chunk's unit is
-// at least a target-th of all units, so the chunks are less than twice target.
-static AttnPlan attn_plan(long tiles, int rows, int units, int target, int least, int dim) {
-  AttnPlan p{rows, units, target, least, tiles, tiles, 0};
-  const long most = (units + least - 1) / least;
-  if (tiles > 0 && most > 1 && tiles <= kMaxCut && tiles * units < 0x7FFFFFFFL) {
-    p.cut_grid = tiles * most < target + tiles ? tiles * most : target + tiles;
-    const long slots = tiles * most < 2L * target ? tiles * most : 2L * target;
-    p.work = kCountBytes + slots * rows * (dim + 2) * 4;
+// `tiles`: bound of the row tiles over all sequences and key heads.  Chunks of
+// cut sequences are fewer than 4/3 of target (find_item), items than target +
+// tiles.
+static void plan_cut(AttnPlan& p, long tiles, int dim) {
+  p.grid = p.cut_grid = tiles;
+  const long most = (p.units + p.least - 1) / p.least;  // chunks of a tile
+  if (tiles > 0 && most > 1 && tiles <= kMaxCut && tiles * p.units < 0x7FFFFFFFL) {
+    p.cut_grid = tiles * most < p.target + tiles ? tiles * most : p.target + tiles;
+    const long slots = tiles * most < 4L * p.target / 3 + 1 ? tiles * most : 4L * p.target / 3 + 1;
+    p.work = kCountBytes + slots * p.rows * (dim + 2) * 4;
   }
-  return p;
 }
-// most new tokens of a few-row sequence
-static int few_tokens(const qhip_kv_cache* c, const qhip_kv_batch* b, int q_heads) {
-  const int most = kFewRows / (q_heads / c->kv_heads);
-  return most < b->max_new ? most : b->max_new;
-}
-static AttnPlan few_plan(const qhip_kv_cache* c, const qhip_kv_batch* b, int q_heads) {
-  const int rows = few_tokens(c, b, q_heads) * (q_heads / c->kv_heads);
-  const long tiles = rows ? (long)b->nseq * c->kv_heads : 0;
-  return attn_plan(tiles, rows, (int)(((long)b->max_kv + 31) / 32), rows <= 16 ? 1024 : 512, 16, c->head_dim);
-}
-static AttnPlan many_plan(const qhip_kv_cache* c, const qhip_kv_batch* b, int q_heads) {
-  if (b->max_new <= few_tokens(c, b, q_heads)) return AttnPlan{};
-  const long tiles = ((long)b->tokens * (q_heads / c->kv_heads) / kManyRows + b->nseq) * c->kv_heads;
-  const int target = 512;
-  AttnPlan p = attn_plan(tiles, kManyRows, (int)(((long)b->max_kv + kManyKeys - 1) / kManyKeys), target, 8, c->head_dim);
-  if (tiles >= 2 * target) p.work = 0;  // enough workgroups as it is
-  return p;
+static int units_of(int keys, int shift) { return (int)(((long)keys + (1 << shift) - 1) >> shift); }
+
+// the few-row kernel's plan, then the many-row kernel's
+static void attn_plans(const qhip_kv_cache* c, const qhip_kv_batch* b, int q_heads, AttnPlan* p) {
+  const int group = q_heads / c->kv_heads;
+  AttnPlan &few = p[0], &many = p[1];
+  few = many = AttnPlan{};
+  few.max_tokens = many.min_tokens = kFewRows / group < b->max_new ? kFewRows / group : b->max_new;
+  many.max_tokens = 0x7FFFFFFF;
+  if (few.max_tokens > 0) {
+    few.rows = few.max_tokens * group;
+    few.key_shift = 5;
+    few.units = units_of(b->max_kv, 5);
+    few.target = few.rows <= 16 ? 1024 : 512;
+    few.least = 16;
+    plan_cut(few, (long)b->nseq * c->kv_heads, c->head_dim);
+  }
+  if (b->max_new > many.min_tokens) {
+    many.rows = kManyRows;
+    many.key_shift = 6;
+    many.units = units_of(b->max_kv, 6);
+    many.target = 512;
+    many.least = 8;
+    const long tiles = ((long)b->tokens * group / kManyRows + b->nseq) * c->kv_heads;
+    plan_cut(many, tiles, c->head_dim);
+    if (tiles >= 2 * many.target) many.work = 0;  // enough workgroups as it is
+  }
 }
 
 }  // namespace qhip
@@ -1065,8 +1045,9 @@ using namespace qhip;
 
 extern "C" long qhip_kv_attention_work_bytes(const qhip_kv_cache* cache, const qhip_kv_batch* batch, int q_heads) {
   if (check_batch(cache, batch, q_heads)) return -1;
-  const long few = few_plan(cache, batch, q_heads).work, many = many_plan(cache, batch, q_heads).work;
-  return few > many ? few : many;
+  AttnPlan p[2];
+  attn_plans(cache, batch, q_heads, p);
+  return p[0].work > p[1].work ? p[0].work : p[1].work;
 }
 
 extern "C" int qhip_launch_kv_attention(const qhip_kv_cache* cache, const qhip_kv_batch* batch, int type,
@@ -1084,33 +1065,62 @@ extern "C" int qhip_launch_kv_attention(const qhip_kv_cache* cache, const qhip_k
     return (int)hipErrorInvalidValue;
   if (rc) return rc;
   if (batch->tokens == 0 || batch->nseq == 0) return 0;
-  const AttnPlan few = few_plan(cache, batch, q_heads), many = many_plan(cache, batch, q_heads);
+  AttnPlan plans[2];
+  attn_plans(cache, batch, q_heads, plans);
   // rows and workgroups are counted in 32 bits
-  if (few.grid > 0x7FFFFFFFL || many.grid > 0x7FFFFFFFL || (long)batch->tokens * q_heads > 0x7FFFFFFFL) return (int)hipErrorInvalidValue;
-  KvAttnArgs a{(const int8_t*)cache->k, (const int8_t*)cache->v, cache->k_scale, cache->v_scale, batch->offsets,
-               batch->kv_lens, batch->table, d_q, d_out, d_lse, q_token_stride, q_head_stride, out_token_stride,
-               out_head_stride, batch->nseq, batch->tokens, batch->table_width, kv_block_shift(cache->block_size),
-               cache->num_blocks, cache->kv_heads, q_heads, softmax_scale, causal, window, type, q_heads / cache->kv_heads,
-               few_tokens(cache, batch, q_heads), kv_rows_aligned(d_q, q_token_stride, q_head_stride, size),
-               kv_rows_aligned(d_out, out_token_stride, out_head_stride, size)};
+  if (plans[0].cut_grid > 0x7FFFFFFFL || plans[1].cut_grid > 0x7FFFFFFFL || (long)batch->tokens * q_heads > 0x7FFFFFFFL)
+    return (int)hipErrorInvalidValue;
+  KvAttnArgs a{};
+  a.k = (const int8_t*)cache->k;
+  a.v = (const int8_t*)cache->v;
+  a.k_scale = cache->k_scale;
+  a.v_scale = cache->v_scale;
+  a.offsets = batch->offsets;
+  a.kv_lens = batch->kv_lens;
+  a.table = batch->table;
+  a.q = d_q;
+  a.out = d_out;
+  a.lse = d_lse;
+  a.q_token = q_token_stride;
+  a.q_head = q_head_stride;
+  a.out_token = out_token_stride;
+  a.out_head = out_head_stride;
+  a.nseq = batch->nseq;
+  a.tokens = batch->tokens;
+  a.width = batch->table_width;
+  a.shift = kv_block_shift(cache->block_size);
+  a.num_blocks = cache->num_blocks;
+  a.kv_heads = cache->kv_heads;
+  a.q_heads = q_heads;
+  a.scale = softmax_scale;
+  a.causal = causal;
+  a.window = window;
+  a.type = type;
+  a.group = q_heads / cache->kv_heads;
+  a.group_inv = (65536 + a.group - 1) / a.group;
   a.counters = (unsigned*)d_work;
   a.partial = (float*)((char*)d_work + kCountBytes);
-  hipStream_t s = (hipStream_t)stream;
   // the two kernels share the workspace: they follow each other on the stream
   // and each leaves the counters at zero
-  auto launch = [&](const AttnPlan& p, void (*f32_rows)(const KvAttnArgs&, int, unsigned, hipStream_t),
-                    void (*f16_rows)(const KvAttnArgs&, int, unsigned, hipStream_t)) {
-    if (p.grid == 0) return;
+  for (int i = 0; i < 2; ++i) {
+    const AttnPlan& p = plans[i];
+    if (p.grid == 0) continue;
+    a.min_tokens = p.min_tokens;
+    a.max_tokens = p.max_tokens;
+    a.tile_rows = p.rows;
+    a.key_shift = p.key_shift;
     a.cut = p.work > 0 && d_work && work_bytes >= p.work;
-    a.target = p.target;
+    // a little above kv_heads / target, so that rounding makes no item too many
+    a.share = (float)cache->kv_heads / (float)p.target * 1.00001f;
     a.least = p.least;
-    a.max_units = p.max_units;
+    a.max_units = p.units;
     a.max_chunks = kJoinPairs / p.rows;
-    a.rows = p.rows;
     a.slots = a.cut ? (p.work - kCountBytes) / ((long)p.rows * (cache->head_dim + 2) * 4) : 0;
-    (type == QHIP_TT_F32 ? f32_rows : f16_rows)(a, cache->head_dim, (unsigned)(a.cut ? p.cut_grid : p.grid), s);
-  };
-  launch(few, launch_few<2>, launch_few<1>);
-  launch(many, launch_many<2>, launch_many<1>);
+    const unsigned grid = (unsigned)(a.cut ? p.cut_grid : p.grid);
+    if (i == 0) type == QHIP_TT_F32 ? launch_few<2>(a, cache->head_dim, grid, (hipStream_t)stream)
+                                    : launch_few<1>(a, cache->head_dim, grid, (hipStream_t)stream);
+    else type == QHIP_TT_F32 ? launch_many<2>(a, cache->head_dim, grid, (hipStream_t)stream)
+                             : launch_many<1>(a, cache->head_dim, grid, (hipStream_t)stream);
+  }
   return (int)hipGetLastError();
 }

@@ -24,15 +24,6 @@ struct KvTablesArgs {
   int *table, *offsets, *kv_lens, *slots, *positions, *taken_out;
 };
 
-__device__ __forceinline__ int scan64(int v, int lane) {
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const int o = __shfl_up(v, d, 64);
-    if (lane >= d) v += o;
-  }
-  return v;
-}
-
 // largest i in [0, cnt) with a[i] <= x (a ascending, a[0] <= x)
 __device__ __forceinline__ int find_le(const int* a, int cnt, int x) {
   int lo = 0, hi = cnt;
@@ -66,7 +57,7 @@ __global__ __launch_bounds__(256) void k_kv_tables(KvTablesArgs a) {
       nsum += n[k];
       fsum += f[k];
     }
-    const int ni = scan64(nsum, lane), fi = scan64(fsum, lane);
+    const int ni = scan64(nsum), fi = scan64(fsum);
     if (lane == 63) {
       s_wave[0][wave] = ni;
       s_wave[1][wave] = fi;
@@ -157,7 +148,7 @@ __device__ __forceinline__ int code8(float x, float m) {
   return r == r ? (int)fminf(fmaxf(r, -127.0f), 127.0f) : 0;
 }
 
-template <typename T, bool VEC>
+template <typename T>
 __global__ __launch_bounds__(256) void k_kv_append(KvAppendArgs a) {
   __shared__ uint32_t s_max[4];
   const int t = blockIdx.x, h = blockIdx.y, z = blockIdx.z, tid = threadIdx.x, lane = tid & 63;
@@ -182,7 +173,7 @@ __global__ __launch_bounds__(256) void k_kv_append(KvAppendArgs a) {
 #pragma unroll
   for (int k = 0; k < kAppKeep; ++k) {
     const int r = row0 + k * rows;
-    if (r < n) keep[k] = load8<T, VEC>(x + r * stride);
+    if (r < n) keep[k] = load8(x + r * stride);
   }
 #pragma unroll
   for (int k = 0; k < kAppKeep; ++k)
@@ -190,7 +181,7 @@ __global__ __launch_bounds__(256) void k_kv_append(KvAppendArgs a) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint((float)keep[k].e[i]) & 0x7FFFFFFFu);
   for (int r = row0 + kAppKeep * rows; r < n; r += rows) {
-    const Raw8<T> v = load8<T, VEC>(x + r * stride);
+    const Raw8<T> v = load8(x + r * stride);
 #pragma unroll
     for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint((float)v.e[i]) & 0x7FFFFFFFu);
   }
@@ -226,7 +217,7 @@ __global__ __launch_bounds__(256) void k_kv_append(KvAppendArgs a) {
 #pragma unroll
   for (int k = 0; k < kAppKeep; ++k)
     if (row0 + k * rows < n) put(row0 + k * rows, keep[k]);
-  for (int r = row0 + kAppKeep * rows; r < n; r += rows) put(r, load8<T, VEC>(x + r * stride));
+  for (int r = row0 + kAppKeep * rows; r < n; r += rows) put(r, load8(x + r * stride));
   if (tid == 0) a.scales[z][bh] = scale;
 }
 
@@ -286,15 +277,6 @@ extern "C" int qhip_launch_kv_tables(const int* d_cached, const int* d_new, int 
   return (int)hipGetLastError();
 }
 
-template <typename T>
-static void launch_append(const KvAppendArgs& a, bool vec, hipStream_t s) {
-  const dim3 grid((unsigned)a.tokens, (unsigned)a.heads, 2);
-  if (vec)
-    hipLaunchKernelGGL((k_kv_append<T, true>), grid, dim3(256), 0, s, a);
-  else
-    hipLaunchKernelGGL((k_kv_append<T, false>), grid, dim3(256), 0, s, a);
-}
-
 extern "C" int qhip_launch_kv_append(const qhip_kv_cache* cache, int type, const void* d_k, long k_token_stride,
                                      long k_head_stride, const void* d_v, long v_token_stride, long v_head_stride,
                                      const int* d_slots, int tokens, void* stream) {
@@ -308,12 +290,11 @@ extern "C" int qhip_launch_kv_append(const qhip_kv_cache* cache, int type, const
   const KvAppendArgs a{{(int8_t*)cache->k, (int8_t*)cache->v}, {cache->k_scale, cache->v_scale}, {d_k, d_v},
                        {k_token_stride, v_token_stride}, {k_head_stride, v_head_stride}, d_slots, tokens, num_slots,
                        kv_block_shift(cache->block_size), cache->kv_heads, cache->head_dim};
-  const bool vec = kv_rows_aligned(d_k, k_token_stride, k_head_stride, size) &&
-                   kv_rows_aligned(d_v, v_token_stride, v_head_stride, size);
+  const dim3 grid((unsigned)tokens, (unsigned)cache->kv_heads, 2);
   hipStream_t s = (hipStream_t)stream;
-  if (type == QHIP_TT_F32) launch_append<float>(a, vec, s);
-  else if (type == QHIP_TT_F16) launch_append<f16_t>(a, vec, s);
-  else launch_append<bf16_t>(a, vec, s);
+  if (type == QHIP_TT_F32) hipLaunchKernelGGL(k_kv_append<float>, grid, dim3(256), 0, s, a);
+  else if (type == QHIP_TT_F16) hipLaunchKernelGGL(k_kv_append<f16_t>, grid, dim3(256), 0, s, a);
+  else hipLaunchKernelGGL(k_kv_append<bf16_t>, grid, dim3(256), 0, s, a);
   return (int)hipGetLastError();
 }
 

@@ -16,25 +16,34 @@ typedef uint32_t kv_u32x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16_t;
 typedef __bf16 bf16_t;
 
-// Eight consecutive elements as they lie in memory; VEC: p is 16-byte aligned.
+// Eight consecutive elements as they lie in memory, in 16-byte loads from any
+// element's address (rows inside a wider tensor may begin anywhere).
 template <typename T>
 struct Raw8 {
   T e[8];
 };
-template <typename T, bool VEC>
+template <typename T>
 __device__ __forceinline__ Raw8<T> load8(const T* p) {
-  Raw8<T> r;
-  if constexpr (VEC) {
+  typedef uint32_t piece __attribute__((ext_vector_type(4), aligned(2)));
+  kv_u32x4 r[sizeof(Raw8<T>) / 16];
 #pragma unroll
-    for (unsigned i = 0; i < sizeof(r) / 16; ++i) ((kv_u32x4*)&r)[i] = ((const kv_u32x4*)p)[i];
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) r.e[i] = p[i];
-  }
-  return r;
+  for (unsigned i = 0; i < sizeof(r) / 16; ++i) r[i] = ((const piece*)p)[i];
+  return __builtin_bit_cast(Raw8<T>, r);
 }
 
 __device__ __forceinline__ bool finite_bits(uint32_t u) { return (u & 0x7F800000u) != 0x7F800000u; }
+
+// inclusive sum over the wave's lanes up to this one (rows of 16, then their ends
+// handed on)
+__device__ __forceinline__ int scan64(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false);  // row_shr:1
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);  // row_bcast:15 into rows 1 and 3
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);  // row_bcast:31 into rows 2 and 3
+  return v;
+}
 
 inline int kv_type_size(int type) {
   return type == QHIP_TT_F32 ? 4 : type == QHIP_TT_F16 || type == QHIP_TT_BF16 ? 2 : 0;
@@ -59,11 +68,6 @@ inline int kv_check_cache(const qhip_kv_cache* c) {
     return (int)hipErrorInvalidValue;
   if (c->head_dim != 64 && c->head_dim != 128 && c->head_dim != 256) return QHIP_DECLINE;
   return 0;
-}
-
-// element strides of rows that 16-byte loads may read
-inline bool kv_rows_aligned(const void* p, long token_stride, long head_stride, int size) {
-  return aligned16(p) && (token_stride * size) % 16 == 0 && (head_stride * size) % 16 == 0;
 }
 
 }  // namespace qhip
