@@ -3,6 +3,8 @@
 // reading blocks back.
 #include "kv_internal.hpp"
 
+#include <type_traits>
+
 namespace qhip {
 
 // ---- block tables and slot maps --------------------------------------------------
@@ -126,13 +128,17 @@ __global__ __launch_bounds__(256) void k_kv_tables(KvTablesArgs a) {
 // ---- append -----------------------------------------------------------------------
 //
 // A run is the new tokens of one block: a token begins one unless its slot
-// follows the previous token's in the same block.  The workgroup of a run's
-// first token handles the run for one head of the keys or of the values, the
-// others end.  The values are read once into registers (up to kAppKeep pieces
-// of eight a thread; what a longer run has beyond them is read again), their
-// largest |x| taken as the maximum of the bit patterns (a NaN's is above an
-// infinity's, so neither is lost), and the codes written.
+// follows the previous token's in the same block.  A workgroup finds the runs
+// that begin among its kAppTokens (or, in a batch of few tokens, at its one)
+// token, for one head of the keys or of the values.  A run whose values fit one
+// wave's registers is a wave's, so that a batch of single tokens keeps all four
+// busy; a longer one is the workgroup's.  The values are read once, into
+// registers (kAppKeep pieces of eight a thread; what a run has beyond them is
+// read again), their largest |x| taken as the maximum of the bit patterns (a
+// NaN's is above an infinity's, so neither is lost), and the codes written.
 constexpr int kAppKeep = 8;
+constexpr int kAppTokens = 16;
+constexpr int kAppFew = 256;  // tokens up to which a workgroup looks at one
 
 struct KvAppendArgs {
   int8_t* codes[2];
@@ -140,117 +146,147 @@ struct KvAppendArgs {
   const void* x[2];
   long token_stride[2], head_stride[2];
   const int* slots;
-  int tokens, num_slots, shift, heads, dim;
+  int tokens, num_slots, shift, heads, dim, tile;
 };
 
 __device__ __forceinline__ int code8(float x, float m) {
   const float r = __builtin_rintf(x * m);
   return r == r ? (int)fminf(fmaxf(r, -127.0f), 127.0f) : 0;
 }
+// four codes in a dword
+__device__ __forceinline__ uint32_t codes4(float a, float b, float c, float d, float m) {
+  return (code8(a, m) & 0xFF) | (code8(b, m) & 0xFF) << 8 | (code8(c, m) & 0xFF) << 16 | (uint32_t)code8(d, m) << 24;
+}
+__device__ __forceinline__ float sbyte(uint32_t w, int i) { return (float)(int8_t)(w >> (8 * i)); }
 
-template <typename T>
-__global__ __launch_bounds__(256) void k_kv_append(KvAppendArgs a) {
-  __shared__ uint32_t s_max[4];
-  const int t = blockIdx.x, h = blockIdx.y, z = blockIdx.z, tid = threadIdx.x, lane = tid & 63;
-  const int slot = a.slots[t], size = 1 << a.shift, place = slot & (size - 1);
-  if ((unsigned)slot >= (unsigned)a.num_slots) return;
-  if (place > 0 && t > 0 && a.slots[t - 1] == slot - 1) return;
-  // the run's length: the tokens whose slots follow, up to the block's end
-  int n = 0;
-  for (int c = 0; c < size; c += 64) {
-    const int i = c + lane;
-    const bool in = i < size - place && t + i < a.tokens && a.slots[t + i] == slot + i;
-    const uint64_t m = __ballot(in);
-    n += m == ~0ull ? 64 : __builtin_ctzll(~m);
-    if (m != ~0ull) break;
-  }
-  const int lanes = a.dim >> 3, rows = 256 / lanes;  // lanes of a row, rows of a pass
-  const int row0 = tid / lanes, d0 = (tid & (lanes - 1)) * 8;
-  const T* x = (const T*)a.x[z] + (long)t * a.token_stride[z] + (long)h * a.head_stride[z] + d0;
+// The run of `n` tokens from token t on, at `slot`; this thread is `id` of NT
+// (a wave, or the workgroup's four with s_max between them), keeping KEEP pieces.
+template <typename T, int NT, int KEEP>
+__device__ __forceinline__ void append_run(const KvAppendArgs& a, int t, int slot, int n, int h, int z, int id, uint32_t* s_max) {
+  const int size = 1 << a.shift, place = slot & (size - 1);
+  const int lanes = a.dim >> 3, rows = NT / lanes;  // lanes of a row, rows of a pass
+  const int row0 = id / lanes, d0 = (id & (lanes - 1)) * 8;
   const long stride = a.token_stride[z];
-  Raw8<T> keep[kAppKeep];
-  uint32_t top = 0;
-#pragma unroll
-  for (int k = 0; k < kAppKeep; ++k) {
-    const int r = row0 + k * rows;
-    if (r < n) keep[k] = load8(x + r * stride);
-  }
-#pragma unroll
-  for (int k = 0; k < kAppKeep; ++k)
-    if (row0 + k * rows < n)
-#pragma unroll
-      for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint((float)keep[k].e[i]) & 0x7FFFFFFFu);
-  for (int r = row0 + kAppKeep * rows; r < n; r += rows) {
-    const Raw8<T> v = load8(x + r * stride);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint((float)v.e[i]) & 0x7FFFFFFFu);
-  }
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) top = max(top, (uint32_t)__shfl_xor((int)top, d, 64));
-  if (lane == 0) s_max[tid >> 6] = top;
+  const T* x = (const T*)a.x[z] + (long)t * stride + (long)h * a.head_stride[z] + d0;
   const long bh = (long)(slot >> a.shift) * a.heads + h;
   const float old = place > 0 ? a.scales[z][bh] : 0.0f;
-  __syncthreads();
-  top = max(max(s_max[0], s_max[1]), max(s_max[2], s_max[3]));
+  Raw8<T> keep[KEEP];
+  uint32_t top = 0;
+#pragma unroll
+  for (int k = 0; k < KEEP; ++k)
+    if (row0 + k * rows < n) keep[k] = load8(x + (row0 + k * rows) * stride);
+  auto see = [&](const Raw8<T>& v) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint((float)v.e[i]) & 0x7FFFFFFFu);
+  };
+#pragma unroll
+  for (int k = 0; k < KEEP; ++k)
+    if (row0 + k * rows < n) see(keep[k]);
+  for (int r = row0 + KEEP * rows; r < n; r += rows) see(load8(x + r * stride));
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) top = max(top, (uint32_t)__shfl_xor((int)top, d, 64));
+  if constexpr (NT > 64) {
+    if ((id & 63) == 0) s_max[id >> 6] = top;
+    __syncthreads();
+    top = max(max(s_max[0], s_max[1]), max(s_max[2], s_max[3]));
+    __syncthreads();  // read before the next run's
+  }
   // maximum of non-negative floats as integers: NaN above infinity above all others
   const uint32_t sbits = max(__float_as_uint(__uint_as_float(top) / 127.0f) & 0x7FFFFFFFu, __float_as_uint(old));
   const float scale = __uint_as_float(sbits);
   const float inv = scale > 0.0f ? 1.0f / scale : 0.0f;
   int8_t* codes = a.codes[z] + bh * ((long)size * a.dim);
-  if (place > 0 && sbits != __float_as_uint(old)) {
+  if (place > 0 && sbits != __float_as_uint(old)) {  // the tokens before the run, to the new scale
     const float ratio = scale > 0.0f ? old / scale : 0.0f;
-    for (int i = tid; i < place * a.dim / 8; i += 256) {
-      kv_u32x2 v = ((kv_u32x2*)codes)[i];
-      int8_t* b = (int8_t*)&v;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) b[j] = (int8_t)code8((float)b[j], ratio);
-      ((kv_u32x2*)codes)[i] = v;
+    for (int i = id; i < place * a.dim / 8; i += NT) {
+      const kv_u32x2 v = ((const kv_u32x2*)codes)[i];
+      ((kv_u32x2*)codes)[i] = kv_u32x2{codes4(sbyte(v[0], 0), sbyte(v[0], 1), sbyte(v[0], 2), sbyte(v[0], 3), ratio),
+                                       codes4(sbyte(v[1], 0), sbyte(v[1], 1), sbyte(v[1], 2), sbyte(v[1], 3), ratio)};
     }
   }
   auto put = [&](int r, const Raw8<T>& v) {
-    kv_u32x2 w;
-    int8_t* b = (int8_t*)&w;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) b[j] = (int8_t)code8((float)v.e[j], inv);
-    *(kv_u32x2*)(codes + (long)(place + r) * a.dim + d0) = w;
+    *(kv_u32x2*)(codes + (long)(place + r) * a.dim + d0) =
+        kv_u32x2{codes4((float)v.e[0], (float)v.e[1], (float)v.e[2], (float)v.e[3], inv),
+                 codes4((float)v.e[4], (float)v.e[5], (float)v.e[6], (float)v.e[7], inv)};
   };
 #pragma unroll
-  for (int k = 0; k < kAppKeep; ++k)
+  for (int k = 0; k < KEEP; ++k)
     if (row0 + k * rows < n) put(row0 + k * rows, keep[k]);
-  for (int r = row0 + kAppKeep * rows; r < n; r += rows) put(r, load8(x + r * stride));
-  if (tid == 0) a.scales[z][bh] = scale;
+  for (int r = row0 + KEEP * rows; r < n; r += rows) put(r, load8(x + r * stride));
+  if (id == 0) a.scales[z][bh] = scale;
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void k_kv_append(KvAppendArgs a) {
+  __shared__ uint32_t s_max[4];
+  const int h = blockIdx.y, z = blockIdx.z, tid = threadIdx.x, lane = tid & 63, size = 1 << a.shift;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int t0 = (int)blockIdx.x * a.tile;
+  // the tokens of the tile that begin a run (a lane each)
+  int slot = -1;
+  bool begins = false;
+  if (lane < a.tile && t0 + lane < a.tokens) {
+    slot = a.slots[t0 + lane];
+    const int before = t0 + lane > 0 ? a.slots[t0 + lane - 1] : -1;
+    begins = (unsigned)slot < (unsigned)a.num_slots && ((slot & (size - 1)) == 0 || before != slot - 1 || t0 + lane == 0);
+  }
+  uint64_t runs = __ballot(begins);
+  for (int i = 0; runs; ++i, runs &= runs - 1) {
+    const int at = __builtin_ctzll(runs), t = t0 + at, first = __builtin_amdgcn_readlane(slot, at);
+    // its length: the tokens whose slots follow, up to the block's end
+    int n = 0;
+    for (int c = 0; c < size; c += 64) {
+      const int j = c + lane;
+      const bool in = j < size - (first & (size - 1)) && t + j < a.tokens && a.slots[t + j] == first + j;
+      const uint64_t m = __ballot(in);
+      n += m == ~0ull ? 64 : __builtin_ctzll(~m);
+      if (m != ~0ull) break;
+    }
+    if (n * a.dim <= 64 * 8) {
+      if ((i & 3) == wave) append_run<T, 64, 1>(a, t, first, n, h, z, lane, s_max);
+    } else {
+      append_run<T, 256, kAppKeep>(a, t, first, n, h, z, tid, s_max);
+    }
+  }
 }
 
 // ---- read back ----------------------------------------------------------------------
+//
+// A workgroup's share of one block's head: kReadCodes codes, a 16-byte piece of
+// the output a thread and pass, so that a wave's stores are contiguous.
+constexpr int kReadCodes = 4096;
 
 struct KvReadArgs {
   const int8_t* codes[2];
   const float* scales[2];
   void* out[2];
   const int* blocks;
-  long pieces;  // 16-code pieces of one block's head
-  int num_blocks, heads;
+  int size, num_blocks, heads;  // size: codes of a block's head
 };
 
 template <typename T>
 __global__ __launch_bounds__(256) void k_kv_read(KvReadArgs a) {
-  const int h = blockIdx.y, z = blockIdx.z;
+  constexpr int P = 16 / sizeof(T);  // values of a piece
+  typedef typename std::conditional<P == 4, uint32_t, kv_u32x2>::type Codes;
+  const int z = blockIdx.z;
   if (!a.out[z]) return;
-  const int id = a.blocks[blockIdx.x];
+  const int i = (int)blockIdx.x / a.heads, h = (int)blockIdx.x - i * a.heads, id = a.blocks[i];
   const bool in = (unsigned)id < (unsigned)a.num_blocks;
   const long bh = in ? (long)id * a.heads + h : 0;
   const float scale = in ? a.scales[z][bh] : __builtin_nanf("");
-  const long to = ((long)blockIdx.x * a.heads + h) * a.pieces;
-  for (long i = threadIdx.x; i < a.pieces; i += 256) {
-    kv_u32x4 c = {0, 0, 0, 0};
-    if (in) c = ((const kv_u32x4*)a.codes[z])[bh * a.pieces + i];
-    const int8_t* b = (const int8_t*)&c;
-    T v[16];
+  const int8_t* codes = a.codes[z] + bh * a.size;
+  T* out = (T*)a.out[z] + (long)blockIdx.x * a.size;
+  const int c0 = (int)blockIdx.y * kReadCodes, c1 = min(a.size, c0 + kReadCodes);
 #pragma unroll
-    for (int j = 0; j < 16; ++j) v[j] = (T)((float)b[j] * scale);
-    kv_u32x4* o = (kv_u32x4*)((T*)a.out[z] + 16 * (to + i));
+  for (int k = 0; k < kReadCodes / (256 * P); ++k) {
+    const int c = c0 + (k * 256 + (int)threadIdx.x) * P;
+    if (c >= c1) break;
+    const Codes x = *(const Codes*)(codes + c);
+    const uint32_t* w = (const uint32_t*)&x;
+    T v[P];
 #pragma unroll
-    for (unsigned j = 0; j < sizeof(v) / 16; ++j) o[j] = ((const kv_u32x4*)v)[j];
+    for (int j = 0; j < P; ++j) v[j] = (T)(sbyte(w[j >> 2], j & 3) * scale);
+    *(kv_u32x4*)(out + c) = *(const kv_u32x4*)v;
   }
 }
 
@@ -289,8 +325,9 @@ extern "C" int qhip_launch_kv_append(const qhip_kv_cache* cache, int type, const
   const int num_slots = cache->num_blocks * cache->block_size;
   const KvAppendArgs a{{(int8_t*)cache->k, (int8_t*)cache->v}, {cache->k_scale, cache->v_scale}, {d_k, d_v},
                        {k_token_stride, v_token_stride}, {k_head_stride, v_head_stride}, d_slots, tokens, num_slots,
-                       kv_block_shift(cache->block_size), cache->kv_heads, cache->head_dim};
-  const dim3 grid((unsigned)tokens, (unsigned)cache->kv_heads, 2);
+                       kv_block_shift(cache->block_size), cache->kv_heads, cache->head_dim,
+                       tokens > kAppFew ? kAppTokens : 1};
+  const dim3 grid((unsigned)((tokens + a.tile - 1) / a.tile), (unsigned)cache->kv_heads, 2);
   hipStream_t s = (hipStream_t)stream;
   if (type == QHIP_TT_F32) hipLaunchKernelGGL(k_kv_append<float>, grid, dim3(256), 0, s, a);
   else if (type == QHIP_TT_F16) hipLaunchKernelGGL(k_kv_append<f16_t>, grid, dim3(256), 0, s, a);
@@ -307,9 +344,9 @@ extern "C" int qhip_launch_kv_read(const qhip_kv_cache* cache, const int* d_bloc
   if (rc) return rc;
   if (nblocks == 0 || (!d_k_out && !d_v_out)) return 0;
   const KvReadArgs a{{(const int8_t*)cache->k, (const int8_t*)cache->v}, {cache->k_scale, cache->v_scale},
-                     {d_k_out, d_v_out}, d_blocks, (long)cache->block_size * cache->head_dim / 16, cache->num_blocks,
-                     cache->kv_heads};
-  const dim3 grid((unsigned)nblocks, (unsigned)cache->kv_heads, 2);
+                     {d_k_out, d_v_out}, d_blocks, cache->block_size * cache->head_dim, cache->num_blocks, cache->kv_heads};
+  if ((long)nblocks * a.heads > 0x7FFFFFFFL) return (int)hipErrorInvalidValue;
+  const dim3 grid((unsigned)(nblocks * a.heads), (unsigned)((a.size + kReadCodes - 1) / kReadCodes), 2);
   hipStream_t s = (hipStream_t)stream;
   if (type == QHIP_TT_F32) hipLaunchKernelGGL(k_kv_read<float>, grid, dim3(256), 0, s, a);
   else if (type == QHIP_TT_F16) hipLaunchKernelGGL(k_kv_read<f16_t>, grid, dim3(256), 0, s, a);
