@@ -102,26 +102,28 @@ __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirs
 
 // ---- a workgroup's item -------------------------------------------------------------------
 //
-// Sequences in order, their row tiles from the last (which sees the most keys),
-// a tile's chunks of keys, and fastest the key heads.  A sequence's chunk count
-// follows from its share of all sequences' row tiles times key units, so that a
-// ragged batch spreads evenly over the workgroups; every wave works the plan out
-// for itself, 64 sequences at a time.  c = round(units / unit) chunks, at least
-// one: sequences that are cut have fewer than 4/3 of their units / unit, so all
+// Sequences that are cut into chunks of keys come first, so that the short ones
+// fill the end; a sequence's row tiles from the last (which sees the most keys),
+// a tile's chunks, and fastest the key heads.  The chunk count follows from a
+// sequence's share of all sequences' row tiles times key units, so that a ragged
+// batch spreads evenly over the workgroups; every wave works the plan out for
+// itself, 64 sequences at a time.  c = round(units / unit) chunks, at least one:
+// sequences that are cut have fewer than 4/3 of their units / unit, so all
 // chunks of cut sequences are fewer than 4/3 of the items aimed for.
 struct Item {
-  int seq, head, n, len, tile, chunk, chunks;
+  int seq, head, off, n, len, tile, chunk, chunks;  // off: the sequence's first packed token
   int slot, counter;  // of the tile's first chunk among the partial results, of the tile
 };
 struct SeqPlan {
-  int n, len, tiles, units;
+  int first, n, len, tiles, units;
 };
 __device__ __forceinline__ SeqPlan plan_seq(const KvAttnArgs& a, int i) {
-  SeqPlan s{0, 0, 0, 0};
+  SeqPlan s{0, 0, 0, 0, 0};
   if (i >= a.nseq) return s;
   const int first = a.offsets[i], end = a.offsets[i + 1], len = a.kv_lens[i];
   const int n = end - first, here = min(end, a.tokens) - first;  // new tokens, and those among the packed rows
   if (n <= a.min_tokens || n > a.max_tokens || here <= 0) return s;
+  s.first = first;
   s.n = n;
   s.len = max(len, 0);
   s.tiles = (here * a.group + a.tile_rows - 1) / a.tile_rows;
@@ -143,42 +145,34 @@ __device__ __forceinline__ bool find_item(const KvAttnArgs& a, int lane, Item& i
     total = __builtin_amdgcn_readlane(scan64(total), 63);
     per_unit = 1.0f / fmaxf((float)a.least, (float)total * a.share);
   }
-  int items = 0, slots = 0, tiles = 0;
-  for (int i0 = 0; i0 < a.nseq; i0 += 64) {
-    if (i0) s = plan_seq(a, i0 + lane);
-    const int c = min(a.max_chunks, max(1, (int)((float)s.units * per_unit + 0.5f)));
-    const int n = s.tiles * c, cut = c > 1 ? n : 0;
-    const int ni = scan64(n);
-    const int all = __builtin_amdgcn_readlane(ni, 63);
-    const bool here = at < items + all;
-    if (a.cut) {
-      const int ci = scan64(cut), ti = scan64(s.tiles);
-      if (here) {
+  int items = 0, tiles = 0;  // before the 64 sequences, of the cut ones
+  for (int pass = a.cut ? 0 : 1; pass < 2; ++pass)
+    for (int i0 = 0; i0 < a.nseq; i0 += 64) {
+      if (a.nseq > 64) s = plan_seq(a, i0 + lane);
+      const int c = min(a.max_chunks, max(1, (int)((float)s.units * per_unit + 0.5f)));
+      const int here = (c > 1) == (pass == 0) ? s.tiles : 0;
+      const int ni = scan64(here * c), ti = scan64(here);
+      const int all = __builtin_amdgcn_readlane(ni, 63);
+      if (at < items + all) {
         const int owner = __builtin_ctzll(__ballot(items + ni > at));
-        slots += __builtin_amdgcn_readlane(ci - cut, owner);
-        tiles += __builtin_amdgcn_readlane(ti - s.tiles, owner);
-      } else {
-        slots += __builtin_amdgcn_readlane(ci, 63);
-        tiles += __builtin_amdgcn_readlane(ti, 63);
+        const int count = __builtin_amdgcn_readlane(s.tiles, owner);
+        it.seq = uniform(i0 + owner);
+        it.head = uniform(blockIdx.x - at * a.kv_heads);
+        it.off = __builtin_amdgcn_readlane(s.first, owner);
+        it.n = __builtin_amdgcn_readlane(s.n, owner);
+        it.len = __builtin_amdgcn_readlane(s.len, owner);
+        it.chunks = __builtin_amdgcn_readlane(c, owner);
+        const int first = items + __builtin_amdgcn_readlane(ni, owner) - count * it.chunks;
+        const int tile = uniform((at - first) / it.chunks);
+        it.chunk = uniform(at - first - tile * it.chunks);
+        it.tile = count - 1 - tile;
+        it.slot = uniform((first + tile * it.chunks) * a.kv_heads + it.head * it.chunks);
+        it.counter = uniform((tiles + __builtin_amdgcn_readlane(ti, owner) - 1 - tile) * a.kv_heads + it.head);
+        return true;
       }
+      items += all;
+      tiles += __builtin_amdgcn_readlane(ti, 63);
     }
-    if (here) {
-      const int owner = __builtin_ctzll(__ballot(items + ni > at));
-      const int count = __builtin_amdgcn_readlane(s.tiles, owner);
-      it.seq = uniform(i0 + owner);
-      it.head = uniform(blockIdx.x - at * a.kv_heads);
-      it.n = __builtin_amdgcn_readlane(s.n, owner);
-      it.len = __builtin_amdgcn_readlane(s.len, owner);
-      it.chunks = __builtin_amdgcn_readlane(c, owner);
-      const int local = at - (items + __builtin_amdgcn_readlane(ni - n, owner)), tile = uniform(local / it.chunks);
-      it.chunk = uniform(local - tile * it.chunks);
-      it.tile = count - 1 - tile;
-      it.slot = uniform((slots + tile * it.chunks) * a.kv_heads + it.head * it.chunks);
-      it.counter = uniform((tiles + tile) * a.kv_heads + it.head);
-      return true;
-    }
-    items += all;
-  }
   return false;
 }
 
@@ -187,14 +181,12 @@ struct Span {
   int row0, rows;    // first row and rows of the tile
   int first;         // place of the sequence's first new token
   int key0, key1;    // this chunk's keys, from a unit's start
-  int off;           // the sequence's first packed token
 };
 __device__ __forceinline__ Span find_span(const KvAttnArgs& a, const Item& it) {
   Span s;
   s.row0 = it.tile * a.tile_rows;
   s.rows = (int)min((long)a.tile_rows, (long)it.n * a.group - s.row0);
   s.first = it.len - it.n;
-  s.off = a.offsets[it.seq];
   const int tok_a = uniform(s.row0 / a.group), tok_b = uniform((s.row0 + s.rows - 1) / a.group);
   const int lo = a.window > 0 ? max(0, s.first + tok_a - a.window + 1) >> a.key_shift << a.key_shift : 0;
   const int hi = a.causal ? s.first + tok_b + 1 : it.len;
@@ -385,7 +377,7 @@ __device__ __forceinline__ void join_rows(const KvAttnArgs& a, float* lds, __amd
     if (r < count && tl == 0) {
       s_inv[r] = sum == 0.0f ? 0.0f : 1.0f / sum;
       const RowAt w = row_at(a, sp, r, it.head);
-      const int t = sp.off + w.tok;
+      const int t = it.off + w.tok;
       if (a.lse && t >= 0 && t < a.tokens) a.lse[(long)t * a.q_heads + w.head] = row_lse(top, sum);
     }
   }
@@ -415,7 +407,7 @@ __device__ __forceinline__ void join_rows(const KvAttnArgs& a, float* lds, __amd
       const int ee = e + 256 * j, r = ee / (D / 4);
       if (ee >= pieces || sl != 0) continue;
       const RowAt w = row_at(a, sp, r, it.head);
-      const int t = sp.off + w.tok;
+      const int t = it.off + w.tok;
       if (t < 0 || t >= a.tokens) continue;
       const float inv = s_inv[r], v[4] = {acc[j][0] * inv, acc[j][1] * inv, acc[j][2] * inv, acc[j][3] * inv};
       store_row<SPLIT, 4>(a.out, (long)t * a.out_token + (long)w.head * a.out_head + 4 * (ee % (D / 4)), a.type, v);
@@ -461,19 +453,19 @@ __device__ __forceinline__ void arrive_and_join(const KvAttnArgs& a, float* lds,
 // into chunks over workgroups (find_item).
 constexpr int kFewRows = 64;
 
-template <int D, int SPLIT>
-__global__ __launch_bounds__(256, D == 256 ? 2 : D == 128 ? 3 : 4) void k_kv_attention_few(KvAttnArgs a) {
+template <int D, int SPLIT, int NT>
+__global__ __launch_bounds__(256, NT == 1 ? (D == 256 ? 2 : D == 128 ? 3 : 4) : (D == 256 ? 1 : 2)) void k_kv_attention_few(KvAttnArgs a) {
   constexpr int J = D / 64, C = D / 16, W = D / 64;  // 64-dimension pieces, output tiles, dwords of a value load
-  constexpr int R = C * 4 * 64;                      // floats of a wave's output
+  constexpr int R = NT * C * 4 * 64;                 // floats of a wave's output
   __shared__ __attribute__((aligned(16))) float s_o[2 * R > kJoinLds / 4 ? 2 * R : kJoinLds / 4];
-  __shared__ float s_m[2][64], s_l[2][64];
-  __shared__ int s_e[2][64];
+  __shared__ float s_m[2][NT][64], s_l[2][NT][64];
+  __shared__ int s_e[2][NT][64];
   const int tid = threadIdx.x, lane = tid & 63, r16 = lane & 15, g = lane >> 4;
   const int wave = uniform(tid >> 6);
   Item it;
   if (!find_item(a, lane, it)) return;  // all four waves alike
   const Span sp = find_span(a, it);
-  const int tiles = sp.rows <= 16 ? 1 : sp.rows <= 32 ? 2 : 4;
+  const int tiles = sp.rows <= 16 * NT ? 1 : sp.rows <= 32 * NT ? 2 : 4;
   const int part = wave / tiles, parts = 4 / tiles;
 
   // lane i: tile i & 1 of this wave's step i / 2 of a round of 32 steps
@@ -481,21 +473,29 @@ __global__ __launch_bounds__(256, D == 256 ? 2 : D == 128 ? 3 : 4) void k_kv_att
   auto round_id = [&]() { return tile_id(a, it.seq, sp.key0 + 32 * (s0 + parts * (lane >> 1)) + 16 * (lane & 1), sp.key1); };
   const int id0 = round_id();
 
-  const int row = (wave % tiles) * 16 + r16;  // this lane's row
-  const RowAt w = row_at(a, sp, row < sp.rows ? row : 0, it.head);
-  const int p = sp.first + w.tok, t = sp.off + w.tok;
-  const bool live = row < sp.rows && t >= 0 && t < a.tokens;
-  const int vis_hi = a.causal ? p + 1 : it.len, vis_lo = a.window > 0 ? p - a.window + 1 : 0;
-  // keys that every row of the tile sees
-  const RowAt last = row_at(a, sp, sp.rows - 1, it.head);
-  const int all_hi = a.causal ? sp.first + uniform(sp.row0 / a.group) + 1 : it.len;
-  const int all_lo = a.window > 0 ? sp.first + uniform(last.tok) - a.window + 1 : 0;
-  QRaw<SPLIT> raw[2 * J] = {};
-  if (live) {
-    const long at = (long)t * a.q_token + (long)w.head * a.q_head + 16 * g;
+  // this lane's rows
+  int row[NT], t[NT], qh[NT], vis_hi[NT], vis_lo[NT];
+  bool live[NT];
+  QRaw<SPLIT> raw[NT][2 * J] = {};
 #pragma unroll
-    for (int i = 0; i < 2 * J; ++i) raw[i] = load8((const QElem<SPLIT>*)a.q + at + 64 * (i >> 1) + 8 * (i & 1));
+  for (int nt = 0; nt < NT; ++nt) {
+    row[nt] = ((wave % tiles) * NT + nt) * 16 + r16;
+    const RowAt w = row_at(a, sp, row[nt] < sp.rows ? row[nt] : 0, it.head);
+    const int p = sp.first + w.tok;
+    t[nt] = it.off + w.tok;
+    qh[nt] = w.head;
+    live[nt] = row[nt] < sp.rows && t[nt] >= 0 && t[nt] < a.tokens;
+    vis_hi[nt] = a.causal ? p + 1 : it.len;
+    vis_lo[nt] = a.window > 0 ? p - a.window + 1 : 0;
+    if (live[nt]) {
+      const long at = (long)t[nt] * a.q_token + (long)w.head * a.q_head + 16 * g;
+#pragma unroll
+      for (int i = 0; i < 2 * J; ++i) raw[nt][i] = load8((const QElem<SPLIT>*)a.q + at + 64 * (i >> 1) + 8 * (i & 1));
+    }
   }
+  // keys that every row of the tile sees
+  const int all_hi = a.causal ? sp.first + uniform(sp.row0 / a.group) + 1 : it.len;
+  const int all_lo = a.window > 0 ? sp.first + uniform(row_at(a, sp, sp.rows - 1, it.head).tok) - a.window + 1 : 0;
 
   TileInfo info = tile_info(a, id0, it.head);
   const uint8_t* kc = (const uint8_t*)a.k;
@@ -544,92 +544,105 @@ __global__ __launch_bounds__(256, D == 256 ? 2 : D == 128 ? 3 : 4) void k_kv_att
     load_v(0);
   }
 
-  h16x8 q_hi[2 * J], q_lo[SPLIT == 2 ? 2 * J : 1];
-  const int qe = split_q<SPLIT, 2 * J>(raw, a.type, max16, q_hi, q_lo);
-  const float c_row = __builtin_ldexpf(a.scale * kLog2e * kCodeScale, -qe);
-  f32x4 o[C];
+  h16x8 q_hi[NT][2 * J], q_lo[NT][SPLIT == 2 ? 2 * J : 1];
+  float c_row[NT], m[NT], l[NT];
+  int ve[NT];
+  f32x4 o[NT][C];
 #pragma unroll
-  for (int c = 0; c < C; ++c) o[c] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-  float m = kMinusInf, l = 0.0f;
-  int ve = kNoScale;
+  for (int nt = 0; nt < NT; ++nt) {
+    const int qe = split_q<SPLIT, 2 * J>(raw[nt], a.type, max16, q_hi[nt], q_lo[nt]);
+    c_row[nt] = __builtin_ldexpf(a.scale * kLog2e * kCodeScale, -qe);
+    m[nt] = kMinusInf;
+    l[nt] = 0.0f;
+    ve[nt] = kNoScale;
+#pragma unroll
+    for (int c = 0; c < C; ++c) o[nt][c] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  }
 
   while (any) {
     const int steps = min(32, (sp.key1 - sp.key0 - 32 * s0 + 32 * parts - 1) / (32 * parts));
     for (int st = 0; st < steps; ++st) {
       const int key = sp.key0 + 32 * (s0 + parts * st);
-      float s[2][4];
+      float s[NT][2][4];
 #pragma unroll
       for (int tt = 0; tt < 2; ++tt) {
-        f32x4 hi = {0.0f, 0.0f, 0.0f, 0.0f}, low = {0.0f, 0.0f, 0.0f, 0.0f};
+        f32x4 hi[NT], low[NT];
 #pragma unroll
-        for (int j = 0; j < J; ++j) {
-          const kv_u32x4 x = kr[tt][j] ^ 0x80808080u;
-          const h16x8 k0 = codes8(x[0], x[1]), k1 = codes8(x[2], x[3]);
-          hi = __builtin_amdgcn_mfma_f32_16x16x32_f16(k0, q_hi[2 * j], hi, 0, 0, 0);
-          hi = __builtin_amdgcn_mfma_f32_16x16x32_f16(k1, q_hi[2 * j + 1], hi, 0, 0, 0);
-          if constexpr (SPLIT == 2) {
-            low = __builtin_amdgcn_mfma_f32_16x16x32_f16(k0, q_lo[2 * j], low, 0, 0, 0);
-            low = __builtin_amdgcn_mfma_f32_16x16x32_f16(k1, q_lo[2 * j + 1], low, 0, 0, 0);
+        for (int nt = 0; nt < NT; ++nt) hi[nt] = low[nt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int j = 0; j < 2 * J; ++j) {
+          const kv_u32x4 x = kr[tt][j >> 1] ^ 0x80808080u;
+          const h16x8 k = j & 1 ? codes8(x[2], x[3]) : codes8(x[0], x[1]);
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            hi[nt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, q_hi[nt][j], hi[nt], 0, 0, 0);
+            if constexpr (SPLIT == 2) low[nt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, q_lo[nt][j], low[nt], 0, 0, 0);
           }
         }
 #pragma unroll
-        for (int r = 0; r < 4; ++r) s[tt][r] = SPLIT == 2 ? hi[r] + low[r] : hi[r];
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) s[nt][tt][r] = SPLIT == 2 ? hi[nt][r] + low[nt][r] : hi[nt][r];
       }
       if (st + 1 < steps) load_k(st + 1);
-      const float c0 = c_row * lane_f(info.ks, 2 * st), c1 = c_row * lane_f(info.ks, 2 * st + 1);
+      const float k0 = lane_f(info.ks, 2 * st), k1 = lane_f(info.ks, 2 * st + 1);
       const float v0 = lane_f(info.vs, 2 * st), v1 = lane_f(info.vs, 2 * st + 1);
       const bool edge = key < all_lo || key + 32 > min(all_hi, sp.key1);  // some row does not see some key
+      h16x8 ph[NT], pl[NT];
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        s[0][r] *= c0;
-        s[1][r] *= c1;
-      }
-      int e0 = scale_exp(v0), e1 = scale_exp(v1);
-      const int end = min(vis_hi, sp.key1);
-      if (edge) {
+      for (int nt = 0; nt < NT; ++nt) {
+        const float c0 = c_row[nt] * k0, c1 = c_row[nt] * k1;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          s[nt][0][r] *= c0;
+          s[nt][1][r] *= c1;
+        }
+        int e0 = scale_exp(v0), e1 = scale_exp(v1);
+        const int end = min(vis_hi[nt], sp.key1);
+        if (edge) {
+#pragma unroll
+          for (int tt = 0; tt < 2; ++tt)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              const int j = key + 16 * tt + 4 * g + r;
+              if (j < vis_lo[nt] || j >= end) s[nt][tt][r] = kMinusInf;
+            }
+          if (key >= end || key + 16 <= vis_lo[nt]) e0 = kNoScale;
+          if (key + 16 >= end || key + 32 <= vis_lo[nt]) e1 = kNoScale;
+        }
+        e0 = max(ve[nt], max(e0, e1));
+        float top = fmaxf(s[nt][0][0], s[nt][1][0]);
+#pragma unroll
+        for (int r = 1; r < 4; ++r) top = fmaxf(top, fmaxf(s[nt][0][r], s[nt][1][r]));
+        top = fmaxf(m[nt], max16(top));
+        if (__any(top != m[nt] || e0 != ve[nt])) {
+          const float f = weight_of(m[nt], top), fo = __builtin_ldexpf(f, ve[nt] - e0);
+          l[nt] *= f;
+#pragma unroll
+          for (int c = 0; c < C; ++c) o[nt][c] *= fo;
+          m[nt] = top;
+          ve[nt] = e0;
+        }
+        const float w0 = __builtin_ldexpf(v0, 14 - ve[nt]), w1 = __builtin_ldexpf(v1, 14 - ve[nt]);
+        float sum = 0.0f;
 #pragma unroll
         for (int tt = 0; tt < 2; ++tt)
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
-            const int j = key + 16 * tt + 4 * g + r;
-            if (j < vis_lo || j >= end) s[tt][r] = kMinusInf;
+            float e = __builtin_amdgcn_exp2f(s[nt][tt][r] - m[nt]), x = e * (tt ? w1 : w0);
+            if (edge) {
+              // m is -infinity where the row has seen nothing yet; what it does not
+              // see has weight 0 whatever its block's scales are
+              const int j = key + 16 * tt + 4 * g + r;
+              if (j < vis_lo[nt] || j >= end) e = x = 0.0f;
+            }
+            sum += e;
+            const _Float16 hi = (_Float16)x;
+            ph[nt][4 * tt + r] = hi;
+            if constexpr (SPLIT == 2) pl[nt][4 * tt + r] = (_Float16)(x - (float)hi);
           }
-        if (key >= end || key + 16 <= vis_lo) e0 = kNoScale;
-        if (key + 16 >= end || key + 32 <= vis_lo) e1 = kNoScale;
+        l[nt] += sum;
       }
-      e0 = max(ve, max(e0, e1));
-      float top = fmaxf(s[0][0], s[1][0]);
-#pragma unroll
-      for (int r = 1; r < 4; ++r) top = fmaxf(top, fmaxf(s[0][r], s[1][r]));
-      top = fmaxf(m, max16(top));
-      if (__any(top != m || e0 != ve)) {
-        const float f = weight_of(m, top), fo = __builtin_ldexpf(f, ve - e0);
-        l *= f;
-#pragma unroll
-        for (int c = 0; c < C; ++c) o[c] *= fo;
-        m = top;
-        ve = e0;
-      }
-      const float w0 = __builtin_ldexpf(v0, 14 - ve), w1 = __builtin_ldexpf(v1, 14 - ve);
-      h16x8 ph, pl;
-      float sum = 0.0f;
-#pragma unroll
-      for (int tt = 0; tt < 2; ++tt)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          float e = __builtin_amdgcn_exp2f(s[tt][r] - m), x = e * (tt ? w1 : w0);
-          if (edge) {
-            // m is -infinity where the row has seen nothing yet; what it does not
-            // see has weight 0 whatever its block's scales are
-            const int j = key + 16 * tt + 4 * g + r;
-            if (j < vis_lo || j >= end) e = x = 0.0f;
-          }
-          sum += e;
-          const _Float16 hi = (_Float16)x;
-          ph[4 * tt + r] = hi;
-          if constexpr (SPLIT == 2) pl[4 * tt + r] = (_Float16)(x - (float)hi);
-        }
-      l += sum;
 #pragma unroll
       for (int w = 0; w < W; ++w) {
         uint32_t x[8];
@@ -638,8 +651,12 @@ __global__ __launch_bounds__(256, D == 256 ? 2 : D == 128 ? 3 : 4) void k_kv_att
 #pragma unroll
         for (int b = 0; b < 4; ++b) {
           const h16x8 v8 = b == 0 ? codes_across<0>(x) : b == 1 ? codes_across<1>(x) : b == 2 ? codes_across<2>(x) : codes_across<3>(x);
-          o[4 * w + b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v8, ph, o[4 * w + b], 0, 0, 0);
-          if constexpr (SPLIT == 2) o[4 * w + b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v8, pl, o[4 * w + b], 0, 0, 0);
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            f32x4& y = o[nt][4 * w + b];
+            y = __builtin_amdgcn_mfma_f32_16x16x32_f16(v8, ph[nt], y, 0, 0, 0);
+            if constexpr (SPLIT == 2) y = __builtin_amdgcn_mfma_f32_16x16x32_f16(v8, pl[nt], y, 0, 0, 0);
+          }
         }
       }
       if (st + 1 < steps) load_v(st + 1);
@@ -650,71 +667,85 @@ __global__ __launch_bounds__(256, D == 256 ? 2 : D == 128 ? 3 : 4) void k_kv_att
     load_k(0);
     load_v(0);
   }
-  l = sum16(l);
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) l[nt] = sum16(l[nt]);
 
   // merge the waves that share a row tile: the upper half of the parts into the lower
   for (int half = parts / 2; half >= 1; half >>= 1) {
     const int slot = wave - half * tiles;  // waves [half * tiles, 2 half * tiles) give
     if (slot >= 0 && slot < half * tiles) {
 #pragma unroll
-      for (int c = 0; c < C; ++c)
+      for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
-        for (int r = 0; r < 4; ++r) s_o[slot * R + (4 * c + r) * 64 + lane] = o[c][r];
-      s_m[slot][lane] = m;
-      s_l[slot][lane] = l;
-      s_e[slot][lane] = ve;
+        for (int c = 0; c < C; ++c)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) s_o[slot * R + ((nt * C + c) * 4 + r) * 64 + lane] = o[nt][c][r];
+        s_m[slot][nt][lane] = m[nt];
+        s_l[slot][nt][lane] = l[nt];
+        s_e[slot][nt][lane] = ve[nt];
+      }
     }
     __syncthreads();
     if (wave < half * tiles) {
-      const float m2 = s_m[wave][lane], top = fmaxf(m, m2);
-      const int ve2 = s_e[wave][lane], e = max(ve, ve2);
-      const float f1 = weight_of(m, top), f2 = weight_of(m2, top);
-      const float g1 = __builtin_ldexpf(f1, ve - e), g2 = __builtin_ldexpf(f2, ve2 - e);
 #pragma unroll
-      for (int c = 0; c < C; ++c)
+      for (int nt = 0; nt < NT; ++nt) {
+        const float m2 = s_m[wave][nt][lane], top = fmaxf(m[nt], m2);
+        const int ve2 = s_e[wave][nt][lane], e = max(ve[nt], ve2);
+        const float f1 = weight_of(m[nt], top), f2 = weight_of(m2, top);
+        const float g1 = __builtin_ldexpf(f1, ve[nt] - e), g2 = __builtin_ldexpf(f2, ve2 - e);
 #pragma unroll
-        for (int r = 0; r < 4; ++r) o[c][r] = o[c][r] * g1 + s_o[wave * R + (4 * c + r) * 64 + lane] * g2;
-      l = l * f1 + s_l[wave][lane] * f2;
-      m = top;
-      ve = e;
+        for (int c = 0; c < C; ++c)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) o[nt][c][r] = o[nt][c][r] * g1 + s_o[wave * R + ((nt * C + c) * 4 + r) * 64 + lane] * g2;
+        l[nt] = l[nt] * f1 + s_l[wave][nt][lane] * f2;
+        m[nt] = top;
+        ve[nt] = e;
+      }
     }
     __syncthreads();
   }
 
-  // a row that sees nothing: 0 and -infinity (l is 0); NaN stays
-  const float norm = l == 0.0f ? 0.0f : 1.0f / l;
 #pragma unroll
-  for (int c = 0; c < C; ++c)
+  for (int nt = 0; nt < NT; ++nt) {
+    // a row that sees nothing: 0 and -infinity (l is 0); NaN stays
+    const float norm = l[nt] == 0.0f ? 0.0f : 1.0f / l[nt];
 #pragma unroll
-    for (int r = 0; r < 4; ++r) o[c][r] = in_units(o[c][r] * norm, ve);
+    for (int c = 0; c < C; ++c)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) o[nt][c][r] = in_units(o[nt][c][r] * norm, ve[nt]);
+  }
   if (it.chunks == 1) {
-    if (wave < tiles && live) {
-      const long at = (long)t * a.out_token + (long)w.head * a.out_head + 4 * g * C;
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        float v[C];
+    for (int nt = 0; nt < NT; ++nt)
+      if (wave < tiles && live[nt]) {
+        const long at = (long)t[nt] * a.out_token + (long)qh[nt] * a.out_head + 4 * g * C;
 #pragma unroll
-        for (int c = 0; c < C; ++c) v[c] = o[c][r];
-        store_row<SPLIT, C>(a.out, at + r * C, a.type, v);
+        for (int r = 0; r < 4; ++r) {
+          float v[C];
+#pragma unroll
+          for (int c = 0; c < C; ++c) v[c] = o[nt][c][r];
+          store_row<SPLIT, C>(a.out, at + r * C, a.type, v);
+        }
+        if (a.lse && g == 0) a.lse[(long)t[nt] * a.q_heads + qh[nt]] = row_lse(m[nt], l[nt]);
       }
-      if (a.lse && g == 0) a.lse[(long)t * a.q_heads + w.head] = row_lse(m, l);
-    }
     return;
   }
   if (it.slot + it.chunks > a.slots || it.counter >= kMaxCut) return;  // offsets or lengths that are none
   const int stride = a.tile_rows * (D + 2);
   const __amdgpu_buffer_rsrc_t parts_at = part_rsrc(a.partial + (long)it.slot * stride, (long)it.chunks * stride);
-  if (wave < tiles && row < sp.rows) {
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      float v[C];
+  for (int nt = 0; nt < NT; ++nt)
+    if (wave < tiles && row[nt] < sp.rows) {
 #pragma unroll
-      for (int c = 0; c < C; ++c) v[c] = o[c][r];
-      part_store<C>(parts_at, it.chunk * stride + row * D + (4 * g + r) * C, v);
+      for (int r = 0; r < 4; ++r) {
+        float v[C];
+#pragma unroll
+        for (int c = 0; c < C; ++c) v[c] = o[nt][c][r];
+        part_store<C>(parts_at, it.chunk * stride + row[nt] * D + (4 * g + r) * C, v);
+      }
+      const float stat[2] = {m[nt], l[nt]};
+      if (g == 0) part_store<2>(parts_at, it.chunk * stride + a.tile_rows * D + 2 * row[nt], stat);
     }
-    const float stat[2] = {m, l};
-    if (g == 0) part_store<2>(parts_at, it.chunk * stride + a.tile_rows * D + 2 * row, stat);
-  }
   arrive_and_join<D, SPLIT>(a, s_o, parts_at, it, sp);
 }
 
@@ -766,7 +797,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_kv_attention_many(KvA
   const int wrow = wave * 32, row = wrow + r32;
   const bool busy = wrow < sp.rows;
   const RowAt w = row_at(a, sp, row < sp.rows ? row : 0, it.head);
-  const int p = sp.first + w.tok, t = sp.off + w.tok;
+  const int p = sp.first + w.tok, t = it.off + w.tok;
   const bool live = row < sp.rows && t >= 0 && t < a.tokens;
   const int vis_hi = a.causal ? p + 1 : it.len, vis_lo = a.window > 0 ? p - a.window + 1 : 0;
   const int tok_a = uniform(row_at(a, sp, wrow, it.head).tok);
@@ -969,11 +1000,11 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_kv_attention_many(KvA
   arrive_and_join<D, SPLIT>(a, (float*)s_kv, parts_at, it, sp);
 }
 
-template <int SPLIT>
+template <int SPLIT, int NT>
 static void launch_few(const KvAttnArgs& a, int dim, unsigned grid, hipStream_t s) {
-  if (dim == 64) hipLaunchKernelGGL((k_kv_attention_few<64, SPLIT>), dim3(grid), dim3(256), 0, s, a);
-  else if (dim == 128) hipLaunchKernelGGL((k_kv_attention_few<128, SPLIT>), dim3(grid), dim3(256), 0, s, a);
-  else hipLaunchKernelGGL((k_kv_attention_few<256, SPLIT>), dim3(grid), dim3(256), 0, s, a);
+  if (dim == 64) hipLaunchKernelGGL((k_kv_attention_few<64, SPLIT, NT>), dim3(grid), dim3(256), 0, s, a);
+  else if (dim == 128) hipLaunchKernelGGL((k_kv_attention_few<128, SPLIT, NT>), dim3(grid), dim3(256), 0, s, a);
+  else hipLaunchKernelGGL((k_kv_attention_few<256, SPLIT, NT>), dim3(grid), dim3(256), 0, s, a);
 }
 
 template <int SPLIT>
@@ -1017,15 +1048,16 @@ static void attn_plans(const qhip_kv_cache* c, const qhip_kv_batch* b, int q_hea
   const int group = q_heads / c->kv_heads;
   AttnPlan &few = p[0], &many = p[1];
   few = many = AttnPlan{};
-  few.max_tokens = many.min_tokens = kFewRows / group < b->max_new ? kFewRows / group : b->max_new;
+  const int all_rows = 0;
+  few.max_tokens = many.min_tokens = all_rows ? 0x7FFFFFFF : kFewRows / group < b->max_new ? kFewRows / group : b->max_new;
   many.max_tokens = 0x7FFFFFFF;
   if (few.max_tokens > 0) {
-    few.rows = few.max_tokens * group;
+    few.rows = all_rows ? all_rows : few.max_tokens * group;
     few.key_shift = 5;
     few.units = units_of(b->max_kv, 5);
-    few.target = few.rows <= 16 ? 1024 : 512;
-    few.least = 16;
-    plan_cut(few, (long)b->nseq * c->kv_heads, c->head_dim);
+    few.target = c->head_dim == 256 ? 256 : 384;
+    few.least = few.rows <= 16 ? 8 : 16;
+    plan_cut(few, ((all_rows ? (long)b->tokens * group / all_rows : 0) + b->nseq) * c->kv_heads, c->head_dim);
   }
   if (b->max_new > many.min_tokens) {
     many.rows = kManyRows;
@@ -1117,8 +1149,10 @@ extern "C" int qhip_launch_kv_attention(const qhip_kv_cache* cache, const qhip_k
     a.max_chunks = kJoinPairs / p.rows;
     a.slots = a.cut ? (p.work - kCountBytes) / ((long)p.rows * (cache->head_dim + 2) * 4) : 0;
     const unsigned grid = (unsigned)(a.cut ? p.cut_grid : p.grid);
-    if (i == 0) type == QHIP_TT_F32 ? launch_few<2>(a, cache->head_dim, grid, (hipStream_t)stream)
-                                    : launch_few<1>(a, cache->head_dim, grid, (hipStream_t)stream);
+    if (i == 0 && p.rows > 16) type == QHIP_TT_F32 ? launch_few<2, 2>(a, cache->head_dim, grid, (hipStream_t)stream)
+                                                   : launch_few<1, 2>(a, cache->head_dim, grid, (hipStream_t)stream);
+    else if (i == 0) type == QHIP_TT_F32 ? launch_few<2, 1>(a, cache->head_dim, grid, (hipStream_t)stream)
+                                         : launch_few<1, 1>(a, cache->head_dim, grid, (hipStream_t)stream);
     else type == QHIP_TT_F32 ? launch_many<2>(a, cache->head_dim, grid, (hipStream_t)stream)
                              : launch_many<1>(a, cache->head_dim, grid, (hipStream_t)stream);
   }

@@ -21,7 +21,8 @@ _NINTS_SB = {12: 2, 13: 2, 10: 2, 23: 8, 18: 8, 21: 8}
 
 
 def _stream() -> ctypes.c_void_p:
-    return ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
+    """The current torch stream's handle (torch.cuda.current_stream builds a stream object first: 2.8 us a call)."""
+    return ctypes.c_void_p(torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice()))
 
 
 def _p(t: torch.Tensor) -> ctypes.c_void_p:
@@ -338,15 +339,21 @@ class KvCache:
 
 
 class KvStep:
-    """What kv_tables writes for a step of `nseq` sequences and `tokens` packed tokens."""
+    """What kv_tables writes for a step of `nseq` sequences and `tokens` packed tokens: offsets [nseq + 1], kv_lens
+    [nseq], slots and positions [tokens], taken [1].  Tensors put in their place are checked once, when they are set."""
 
     def __init__(self, nseq: int, tokens: int, device="cuda"):
-        def ints(n):
-            return torch.empty(n, dtype=torch.int32, device=device)
-
         self.nseq, self.tokens = nseq, tokens
-        self.offsets, self.kv_lens, self.taken = ints(nseq + 1), ints(nseq), ints(1)
-        self.slots, self.positions = ints(tokens), ints(tokens)
+        for name, n in (("offsets", nseq + 1), ("kv_lens", nseq), ("slots", tokens), ("positions", tokens), ("taken", 1)):
+            setattr(self, name, torch.empty(n, dtype=torch.int32, device=device))
+
+    def __setattr__(self, name, value):
+        if isinstance(value, torch.Tensor):
+            n = {"offsets": self.nseq + 1, "kv_lens": self.nseq, "taken": 1}.get(name, self.tokens)
+            _ints(name, value)
+            if value.shape != (n,):
+                raise ValueError(f"{name}: {n} entries")
+        super().__setattr__(name, value)
 
 
 def kv_tables(cached: torch.Tensor, new: torch.Tensor, free: torch.Tensor, table: torch.Tensor, block_size: int,
@@ -354,11 +361,12 @@ def kv_tables(cached: torch.Tensor, new: torch.Tensor, free: torch.Tensor, table
     """Blocks and slots for `new` [nseq] tokens behind `cached` [nseq]: the new entries of `table` [nseq, width] come
     from `free`, from entry `taken` [1] on; `step` receives the rest."""
     nseq = step.nseq
-    if table.dim() != 2 or len(cached) != nseq or len(new) != nseq or len(table) != nseq:
+    c, n, f, t = _ints("cached", cached), _ints("new", new), _ints("free", free), _ints("table", table, 2)
+    rows, width = table.shape
+    if cached.shape[0] != nseq or new.shape[0] != nseq or rows != nseq:
         raise ValueError(f"cached, new, table: {nseq} sequences")
     check("kv_tables", load().qhip_launch_kv_tables(
-        _ints("cached", cached), _ints("new", new), nseq, _ints("free", free), len(free),
-        None if taken is None else _ints("taken", taken), block_size, _ints("table", table, 2), table.shape[1], step.tokens,
+        c, n, nseq, f, free.shape[0], None if taken is None else _ints("taken", taken), block_size, t, width, step.tokens,
         step.offsets.data_ptr(), step.kv_lens.data_ptr(), step.slots.data_ptr(), step.positions.data_ptr(),
         step.taken.data_ptr(), _stream()))
     return step
@@ -379,8 +387,7 @@ def kv_read(cache: KvCache, blocks: torch.Tensor, dtype: torch.dtype = torch.flo
     if dtype not in _KV_TYPES:
         raise ValueError("dtype: f32, f16 or bf16")
     shape = (len(blocks), cache.kv_heads, cache.block_size, cache.head_dim)
-    k = torch.empty(shape, dtype=dtype, device=blocks.device)
-    v = torch.empty(shape, dtype=dtype, device=blocks.device)
+    k, v = torch.empty((2, *shape), dtype=dtype, device=blocks.device)
     check("kv_read", load().qhip_launch_kv_read(cache._ref, _ints("blocks", blocks), len(blocks), _KV_TYPES[dtype],
                                                 k.data_ptr(), v.data_ptr(), _stream()))
     return k, v
