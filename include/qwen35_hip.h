@@ -364,7 +364,7 @@ int qhip_launch_mul_mat_ragged(const void *d_w, const void *d_xq_packed, float *
  * calls allocates, waits or keeps anything.
  *
  *   k, v              int8 [num_blocks][kv_heads][block_size][head_dim], 16-byte aligned
- *   k_scale, v_scale  f32  [num_blocks][kv_heads]
+ *   k_scale, v_scale  f32  [num_blocks][kv_heads], not negative
  *   block_size        16, 32, 64, 128 or 256; 0 < num_blocks * block_size < 2^31
  *   head_dim          64, 128 or 256 (others: QHIP_DECLINE)
  *

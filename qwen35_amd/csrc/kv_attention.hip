@@ -29,7 +29,7 @@ struct KvAttnArgs {
   float* lse;
   long q_token, q_head, out_token, out_head;
   int nseq, tokens, width, shift, num_blocks, kv_heads, q_heads;
-  float scale;
+  float scale, sign;  // the softmax scale's absolute value and sign
   int causal, window, type, group;
   int group_inv;  // 65536 / group, rounded up
   // the kernel's sequences (those of min_tokens < new tokens <= max_tokens), the
@@ -244,10 +244,11 @@ __device__ __forceinline__ float q_value(const QRaw<SPLIT>& raw, int i, int type
   else if (type == QHIP_TT_F16) return (float)__builtin_bit_cast(f16_t, raw.e[i]);
   else return __uint_as_float((uint32_t)raw.e[i] << 16);
 }
-// The row's values times a power of two that brings the largest to below 2^14,
-// as f16 or, SPLIT 2, as the sum of two (22 bits); returns the power.
+// The row's values times a power of two that brings the largest to below 2^14
+// (and the softmax scale's sign), as f16 or, SPLIT 2, as the sum of two (22
+// bits); returns the power.
 template <int SPLIT, int N, typename RowMax>
-__device__ __forceinline__ int split_q(const QRaw<SPLIT>* raw, int type, RowMax row_max, h16x8* hi, h16x8* lo) {
+__device__ __forceinline__ int split_q(const QRaw<SPLIT>* raw, int type, float sign, RowMax row_max, h16x8* hi, h16x8* lo) {
   float top = 0.0f;
 #pragma unroll
   for (int n = 0; n < N; ++n)
@@ -258,7 +259,7 @@ __device__ __forceinline__ int split_q(const QRaw<SPLIT>* raw, int type, RowMax 
   for (int n = 0; n < N; ++n)
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const float x = __builtin_ldexpf(q_value<SPLIT>(raw[n], i, type), e);
+      const float x = __builtin_ldexpf(q_value<SPLIT>(raw[n], i, type) * sign, e);
       hi[n][i] = (_Float16)x;
       if constexpr (SPLIT == 2) lo[n][i] = (_Float16)(x - (float)hi[n][i]);
     }
@@ -550,7 +551,7 @@ __global__ __launch_bounds__(256, NT == 1 ? (D == 256 ? 2 : D == 128 ? 3 : 4) : 
   f32x4 o[NT][C];
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
-    const int qe = split_q<SPLIT, 2 * J>(raw[nt], a.type, max16, q_hi[nt], q_lo[nt]);
+    const int qe = split_q<SPLIT, 2 * J>(raw[nt], a.type, a.sign, max16, q_hi[nt], q_lo[nt]);
     c_row[nt] = __builtin_ldexpf(a.scale * kLog2e * kCodeScale, -qe);
     m[nt] = kMinusInf;
     l[nt] = 0.0f;
@@ -592,11 +593,6 @@ __global__ __launch_bounds__(256, NT == 1 ? (D == 256 ? 2 : D == 128 ? 3 : 4) : 
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
         const float c0 = c_row[nt] * k0, c1 = c_row[nt] * k1;
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          s[nt][0][r] *= c0;
-          s[nt][1][r] *= c1;
-        }
         int e0 = scale_exp(v0), e1 = scale_exp(v1);
         const int end = min(vis_hi[nt], sp.key1);
         if (edge) {
@@ -611,10 +607,10 @@ __global__ __launch_bounds__(256, NT == 1 ? (D == 256 ? 2 : D == 128 ? 3 : 4) : 
           if (key + 16 >= end || key + 32 <= vis_lo[nt]) e1 = kNoScale;
         }
         e0 = max(ve[nt], max(e0, e1));
-        float top = fmaxf(s[nt][0][0], s[nt][1][0]);
-#pragma unroll
-        for (int r = 1; r < 4; ++r) top = fmaxf(top, fmaxf(s[nt][0][r], s[nt][1][r]));
-        top = fmaxf(m[nt], max16(top));
+        // the scores' factors c0, c1 are not negative, so each tile's largest is that of the products
+        const float top0 = fmaxf(fmaxf(s[nt][0][0], s[nt][0][1]), fmaxf(s[nt][0][2], s[nt][0][3]));
+        const float top1 = fmaxf(fmaxf(s[nt][1][0], s[nt][1][1]), fmaxf(s[nt][1][2], s[nt][1][3]));
+        const float top = fmaxf(m[nt], max16(fmaxf(top0 * c0, top1 * c1)));
         if (__any(top != m[nt] || e0 != ve[nt])) {
           const float f = weight_of(m[nt], top), fo = __builtin_ldexpf(f, ve[nt] - e0);
           l[nt] *= f;
@@ -624,22 +620,35 @@ __global__ __launch_bounds__(256, NT == 1 ? (D == 256 ? 2 : D == 128 ? 3 : 4) : 
           ve[nt] = e0;
         }
         const float w0 = __builtin_ldexpf(v0, 14 - ve[nt]), w1 = __builtin_ldexpf(v1, 14 - ve[nt]);
+        auto hide = [&]() {  // what the row does not see has weight 0 whatever its block's scales are
+#pragma unroll
+          for (int tt = 0; tt < 2; ++tt)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              const int j = key + 16 * tt + 4 * g + r;
+              s[nt][tt][r] = j < vis_lo[nt] || j >= end ? 0.0f : s[nt][tt][r];
+            }
+        };
+#pragma unroll
+        for (int tt = 0; tt < 2; ++tt)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) s[nt][tt][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[nt][tt][r], tt ? c1 : c0, -m[nt]));
+        if (edge) hide();
         float sum = 0.0f;
 #pragma unroll
         for (int tt = 0; tt < 2; ++tt)
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
-            float e = __builtin_amdgcn_exp2f(s[nt][tt][r] - m[nt]), x = e * (tt ? w1 : w0);
-            if (edge) {
-              // m is -infinity where the row has seen nothing yet; what it does not
-              // see has weight 0 whatever its block's scales are
-              const int j = key + 16 * tt + 4 * g + r;
-              if (j < vis_lo[nt] || j >= end) e = x = 0.0f;
-            }
-            sum += e;
-            const _Float16 hi = (_Float16)x;
-            ph[nt][4 * tt + r] = hi;
-            if constexpr (SPLIT == 2) pl[nt][4 * tt + r] = (_Float16)(x - (float)hi);
+            sum += s[nt][tt][r];
+            s[nt][tt][r] *= tt ? w1 : w0;
+          }
+        if (edge && __any(!(w0 * 0.0f + w1 * 0.0f == 0.0f))) hide();  // 0 * NaN, 0 * infinity
+#pragma unroll
+        for (int tt = 0; tt < 2; ++tt)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            ph[nt][4 * tt + r] = (_Float16)s[nt][tt][r];
+            if constexpr (SPLIT == 2) pl[nt][4 * tt + r] = (_Float16)(s[nt][tt][r] - (float)ph[nt][4 * tt + r]);
           }
         l[nt] += sum;
       }
@@ -756,8 +765,9 @@ __global__ __launch_bounds__(256, NT == 1 ? (D == 256 ? 2 : D == 128 ? 3 : 4) : 
 // Per tile of 64 keys the codes are read once from memory, turned into f16 and
 // laid down in LDS as v_mfma_f32_32x32x16_f16 wants them: keys row by row
 // (16-byte pieces of 8 dimensions), values dimension by dimension (16-byte
-// pieces of the 8 keys that a lane's weights belong to), both with the piece
-// index xor-ed so that eight lanes hit eight pieces of a 128-byte row of banks.
+// pieces of the 8 keys that a lane's weights belong to; dimensions in the order
+// of the output tiles' rows), the rows padded by 16 bytes so that eight lanes hit
+// eight different 16-byte banks.
 // S^T and O^T as for few rows: lane 32 h + r holds row r; keys 8 i + 4 h ..+3 of
 // a 32-key half are its scores and its half of the weights' operand, and output
 // tile c holds dimensions i D/32 + c.  The next tile's codes are in flight in
@@ -766,21 +776,15 @@ __global__ __launch_bounds__(256, NT == 1 ? (D == 256 ? 2 : D == 128 ? 3 : 4) : 
 constexpr int kManyRows = 128;
 constexpr int kManyKeys = 64;
 
-// the 16-byte piece of a value row that holds piece x of dimension `dim`
-template <int D>
-__device__ __forceinline__ int value_piece(int dim, int x) {
-  if constexpr (D == 64) return x ^ (((dim >> 1) ^ (dim >> 4)) & 7);
-  else return x ^ ((dim / (D / 32)) & 7);
-}
-
 template <int D, int SPLIT>
 __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_kv_attention_many(KvAttnArgs a) {
   constexpr int S = D / 16, C = D / 32;      // 16-dimension steps, output tiles
   constexpr int KP = D / 64;                 // 16-byte pieces of a key tile a thread stages
   constexpr int VW = D == 256 ? 2 : 1;       // dwords of a value row a thread stages (8 keys of 4 VW dimensions)
   constexpr int VT = 8 * (D / (4 * VW));     // threads that stage values
-  __shared__ __attribute__((aligned(16))) uint8_t s_kv[2 * kManyKeys * D * 2];
-  uint8_t *const s_k = s_kv, *const s_v = s_kv + kManyKeys * D * 2;
+  constexpr int KB = 2 * D + 16, VB = 2 * kManyKeys + 16;  // bytes of a key row, of a dimension's row
+  __shared__ __attribute__((aligned(16))) uint8_t s_kv[kManyKeys * KB + D * VB];
+  uint8_t *const s_k = s_kv, *const s_v = s_kv + kManyKeys * KB;
   static_assert(sizeof(s_kv) >= kJoinLds, "the join's LDS");
   const int tid = threadIdx.x, lane = tid & 63, r32 = lane & 31, h = lane >> 5;
   const int wave = uniform(tid >> 6);
@@ -847,9 +851,8 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_kv_attention_many(KvA
     for (int j = 0; j < KP; ++j) {
       const int key = kkey + j * (4096 / D);
       const kv_u32x4 x = kr[j] ^ 0x80808080u;
-      uint8_t* row_at = s_k + key * (D * 2);
-      *(h16x8*)(row_at + ((2 * kpc) ^ (key & 7)) * 16) = codes8(x[0], x[1]);
-      *(h16x8*)(row_at + ((2 * kpc + 1) ^ (key & 7)) * 16) = codes8(x[2], x[3]);
+      *(h16x8*)(s_k + key * KB + 32 * kpc) = codes8(x[0], x[1]);
+      *(h16x8*)(s_k + key * KB + 32 * kpc + 16) = codes8(x[2], x[3]);
     }
     if (VT == 256 || tid < VT) {
 #pragma unroll
@@ -860,7 +863,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_kv_attention_many(KvA
 #pragma unroll
         for (int b = 0; b < 4; ++b) {
           const int dim = vdim + 4 * w + b;
-          *(h16x8*)(s_v + dim * 128 + value_piece<D>(dim, vgrp) * 16) =
+          *(h16x8*)(s_v + ((dim % C) * 32 + dim / C) * VB + 16 * vgrp) =
               b == 0 ? codes_across<0>(x) : b == 1 ? codes_across<1>(x) : b == 2 ? codes_across<2>(x) : codes_across<3>(x);
         }
       }
@@ -869,7 +872,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_kv_attention_many(KvA
   if (count > 0) load_tile(info, 0);
 
   h16x8 q_hi[S], q_lo[SPLIT == 2 ? S : 1];
-  const int qe = split_q<SPLIT, S>(raw, a.type, max32, q_hi, q_lo);
+  const int qe = split_q<SPLIT, S>(raw, a.type, a.sign, max32, q_hi, q_lo);
   const float c_row = __builtin_ldexpf(a.scale * kLog2e * kCodeScale, -qe);
   f32x16 o[C];
 #pragma unroll
@@ -879,6 +882,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_kv_attention_many(KvA
   float m = kMinusInf, l = 0.0f;
   int ve = kNoScale;
 
+  const uint8_t *const k_at = s_k + r32 * KB + 16 * h, *const v_at = s_v + r32 * VB + 16 * h;  // this lane's operands
   for (int i = 0; i < count; ++i) {
     const int ri = i & 15;
     if (ri == 0 && i) {
@@ -893,71 +897,92 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_kv_attention_many(KvA
       else load_tile(info, ri + 1);
     }
     const int key = sp.key0 + i * kManyKeys;
-#pragma unroll 1
+    if (!busy || key >= any_hi || key + kManyKeys <= any_lo) continue;  // no row of the wave sees it
+    // both 32-key halves' scores, then both halves' weights: the second half's
+    // products run beside the first's exponentials
+    f32x16 s[2];
+#pragma unroll
     for (int mt = 0; mt < 2; ++mt) {
-      const int kt = key + 32 * mt;
-      if (!busy || kt >= any_hi || kt + 32 <= any_lo) continue;  // no row of the wave sees it
-      f32x16 s = {}, sl = {};
+      f32x16 hi = {}, low = {};
 #pragma unroll
       for (int st = 0; st < S; ++st) {
-        const int kk = 32 * mt + r32;
-        const h16x8 x = *(const h16x8*)(s_k + kk * (D * 2) + ((2 * st + h) ^ (kk & 7)) * 16);
-        s = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, q_hi[st], s, 0, 0, 0);
-        if constexpr (SPLIT == 2) sl = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, q_lo[st], sl, 0, 0, 0);
+        const h16x8 x = *(const h16x8*)(k_at + 32 * mt * KB + 32 * st);
+        hi = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, q_hi[st], hi, 0, 0, 0);
+        if constexpr (SPLIT == 2) low = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, q_lo[st], low, 0, 0, 0);
       }
-      const int sc = 4 * ri + 2 * mt;
-      const float c0 = c_row * lane_f(info.ks, sc);
-      const float c1 = c_row * lane_f(info.ks, sc + 1);
-      const float v0 = lane_f(info.vs, sc);
-      const float v1 = lane_f(info.vs, sc + 1);
-      const bool edge = kt < all_lo || kt + 32 > all_hi;
+      s[mt] = SPLIT == 2 ? hi + low : hi;
+    }
+    const bool edge = key < all_lo || key + kManyKeys > all_hi;
+    float cs[4], vs[4];  // of the four 16-key tiles
+    int e0 = ve;
 #pragma unroll
-      for (int r = 0; r < 16; ++r) s[r] = (SPLIT == 2 ? s[r] + sl[r] : s[r]) * (r < 8 ? c0 : c1);
-      int e0 = scale_exp(v0), e1 = scale_exp(v1);
-      if (edge) {
+    for (int q = 0; q < 4; ++q) {
+      cs[q] = c_row * lane_f(info.ks, 4 * ri + q);
+      vs[q] = lane_f(info.vs, 4 * ri + q);
+      const int e = scale_exp(vs[q]);
+      e0 = max(e0, edge && (key + 16 * q >= vis_hi || key + 16 * q + 16 <= vis_lo) ? kNoScale : e);
+    }
+    if (edge) {
+#pragma unroll
+      for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
-          const int j = kt + 8 * (r >> 2) + 4 * h + (r & 3);
-          if (j < vis_lo || j >= vis_hi) s[r] = kMinusInf;
+          const int j = key + 32 * mt + 8 * (r >> 2) + 4 * h + (r & 3);
+          if (j < vis_lo || j >= vis_hi) s[mt][r] = kMinusInf;
         }
-        if (kt >= vis_hi || kt + 16 <= vis_lo) e0 = kNoScale;
-        if (kt + 16 >= vis_hi || kt + 32 <= vis_lo) e1 = kNoScale;
-      }
-      e0 = max(ve, max(e0, e1));
-      float top = s[0];
+    }
+    // the scores' factors are not negative, so each tile's largest is that of the products
+    float top = kMinusInf;
 #pragma unroll
-      for (int r = 1; r < 16; ++r) top = fmaxf(top, s[r]);
-      top = fmaxf(m, max32(top));
-      if (__any(top != m || e0 != ve)) {
-        const float f = weight_of(m, top), fo = __builtin_ldexpf(f, ve - e0);
-        l *= f;
+    for (int q = 0; q < 4; ++q) {
+      float x = s[q >> 1][8 * (q & 1)];
 #pragma unroll
-        for (int c = 0; c < C; ++c) o[c] *= fo;
-        m = top;
-        ve = e0;
-      }
-      const float w0 = __builtin_ldexpf(v0, 14 - ve), w1 = __builtin_ldexpf(v1, 14 - ve);
-      h16x8 p_hi[2], p_lo[2];
-      float sum = 0.0f;
+      for (int r = 1; r < 8; ++r) x = fmaxf(x, s[q >> 1][8 * (q & 1) + r]);
+      top = fmaxf(top, x * cs[q]);
+    }
+    top = fmaxf(m, max32(top));
+    if (__any(top != m || e0 != ve)) {
+      const float f = weight_of(m, top), fo = __builtin_ldexpf(f, ve - e0);
+      l *= f;
+#pragma unroll
+      for (int c = 0; c < C; ++c) o[c] *= fo;
+      m = top;
+      ve = e0;
+    }
+    auto hide = [&](int mt, f32x16& x) {  // what the row does not see has weight 0 whatever its block's scales are
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
-        float e = __builtin_amdgcn_exp2f(s[r] - m), x = e * (r < 8 ? w0 : w1);
-        if (edge) {
-          const int j = kt + 8 * (r >> 2) + 4 * h + (r & 3);
-          if (j < vis_lo || j >= vis_hi) e = x = 0.0f;
-        }
-        sum += e;
-        const _Float16 y = (_Float16)x;
-        p_hi[r >> 3][r & 7] = y;
-        if constexpr (SPLIT == 2) p_lo[r >> 3][r & 7] = (_Float16)(x - (float)y);
+        const int j = key + 32 * mt + 8 * (r >> 2) + 4 * h + (r & 3);
+        x[r] = j < vis_lo || j >= vis_hi ? 0.0f : x[r];
       }
+    };
+    float ws[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) ws[q] = __builtin_ldexpf(vs[q], 14 - ve);
+#pragma unroll
+    for (int mt = 0; mt < 2; ++mt) {
+      f32x16& x = s[mt];
+#pragma unroll
+      for (int r = 0; r < 16; ++r) x[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[r], cs[2 * mt + (r >> 3)], -m));
+      if (edge) hide(mt, x);
+      float sum = 0.0f;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) sum += x[r];
       l += sum;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) x[r] *= ws[2 * mt + (r >> 3)];
+      if (edge && __any(!(ws[2 * mt] * 0.0f + ws[2 * mt + 1] * 0.0f == 0.0f))) hide(mt, x);  // 0 * NaN, 0 * infinity
+      h16x8 p_hi[2], p_lo[2];
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        p_hi[r >> 3][r & 7] = (_Float16)x[r];
+        if constexpr (SPLIT == 2) p_lo[r >> 3][r & 7] = (_Float16)(x[r] - (float)p_hi[r >> 3][r & 7]);
+      }
 #pragma unroll
       for (int st = 0; st < 2; ++st)
 #pragma unroll
         for (int c = 0; c < C; ++c) {
-          const int dim = r32 * C + c;
-          const h16x8 x = *(const h16x8*)(s_v + dim * 128 + value_piece<D>(dim, 4 * mt + 2 * st + h) * 16);
+          const h16x8 x = *(const h16x8*)(v_at + 64 * mt + 32 * st + 32 * c * VB);
           o[c] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, p_hi[st], o[c], 0, 0, 0);
           if constexpr (SPLIT == 2) o[c] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, p_lo[st], o[c], 0, 0, 0);
         }
@@ -1124,7 +1149,8 @@ extern "C" int qhip_launch_kv_attention(const qhip_kv_cache* cache, const qhip_k
   a.num_blocks = cache->num_blocks;
   a.kv_heads = cache->kv_heads;
   a.q_heads = q_heads;
-  a.scale = softmax_scale;
+  a.scale = fabsf(softmax_scale);
+  a.sign = softmax_scale < 0.0f ? -1.0f : 1.0f;
   a.causal = causal;
   a.window = window;
   a.type = type;
