@@ -100,6 +100,13 @@ __device__ __forceinline__ float lane_f(float v, int i) {
 }
 __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
 
+// A uniform value that the compiler takes as new here, so that what is computed
+// from it stays in its branch (it would otherwise be done on every path).
+__device__ __forceinline__ int here(int v) {
+  asm volatile("" : "+s"(v));
+  return v;
+}
+
 // ---- a workgroup's item -------------------------------------------------------------------
 //
 // Sequences that are cut into chunks of keys come first, so that the short ones
@@ -292,12 +299,24 @@ __device__ __forceinline__ float row_lse(float m, float l) {
 // what 2^(m - top) leaves of a part whose maximum is m (both may be -infinity)
 __device__ __forceinline__ float weight_of(float m, float top) { return m == top ? 1.0f : __builtin_amdgcn_exp2f(m - top); }
 
-// A row's weights are scaled by 2^(14 - e), e the power of two of the largest
-// value scale that the row has seen (so that hidden blocks change no bit of it):
-// its output is in units of 2^(e - 14) times kCodeScale.
+// A row's weights are taken relative to a maximum m and to the power of two e of
+// a value scale, times 2^kShift: its output is in units of 2^(e - kShift) times
+// kCodeScale.  m and e are those of what the row itself has seen (so that hidden
+// blocks change no bit of it), and move only when a score passes m by more than
+// kLag or a scale 2^(e + kLagExp): the output is then rescaled, which at every
+// new maximum would cost a tile of many rows a tenth of its time.  Weights stay
+// below 2^15, inside f16.  Two-part weights keep the larger shift: what is below
+// 2^-24 of it is lost, and they are to be good to 22 bits.
+template <int SPLIT>
+constexpr int kShift = SPLIT == 2 ? 14 : 7;
+template <int SPLIT>
+constexpr float kLag = SPLIT == 2 ? 1.0f : 7.0f;
+template <int SPLIT>
+constexpr int kLagExp = SPLIT == 2 ? 0 : 1;
 constexpr int kNoScale = -1000;  // of a zero or a NaN
 __device__ __forceinline__ int scale_exp(float v) { return fabsf(v) > 0.0f ? __builtin_amdgcn_frexp_expf(v) : kNoScale; }
-__device__ __forceinline__ float in_units(float o, int e) { return __builtin_ldexpf(o, e - 14 + 9); }
+template <int SPLIT>
+__device__ __forceinline__ float in_units(float o, int e) { return __builtin_ldexpf(o, e - kShift<SPLIT> + 9); }
 
 // ---- joining a tile's chunks ----------------------------------------------------------------------
 //
@@ -486,7 +505,7 @@ __global__ __launch_bounds__(256, NT == 1 ? (D == 256 ? 2 : D == 128 ? 3 : 4) : 
     t[nt] = it.off + w.tok;
     qh[nt] = w.head;
     live[nt] = row[nt] < sp.rows && t[nt] >= 0 && t[nt] < a.tokens;
-    vis_hi[nt] = a.causal ? p + 1 : it.len;
+    vis_hi[nt] = min(a.causal ? p + 1 : it.len, sp.key1);  // of this chunk
     vis_lo[nt] = a.window > 0 ? p - a.window + 1 : 0;
     if (live[nt]) {
       const long at = (long)t[nt] * a.q_token + (long)w.head * a.q_head + 16 * g;
@@ -594,39 +613,42 @@ __global__ __launch_bounds__(256, NT == 1 ? (D == 256 ? 2 : D == 128 ? 3 : 4) : 
       for (int nt = 0; nt < NT; ++nt) {
         const float c0 = c_row[nt] * k0, c1 = c_row[nt] * k1;
         int e0 = scale_exp(v0), e1 = scale_exp(v1);
-        const int end = min(vis_hi[nt], sp.key1);
         if (edge) {
+          const int from = vis_lo[nt], to = vis_hi[nt];
 #pragma unroll
           for (int tt = 0; tt < 2; ++tt)
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
               const int j = key + 16 * tt + 4 * g + r;
-              if (j < vis_lo[nt] || j >= end) s[nt][tt][r] = kMinusInf;
+              s[nt][tt][r] = j < from || j >= to ? kMinusInf : s[nt][tt][r];
             }
-          if (key >= end || key + 16 <= vis_lo[nt]) e0 = kNoScale;
-          if (key + 16 >= end || key + 32 <= vis_lo[nt]) e1 = kNoScale;
+          e0 = key >= to || key + 16 <= from ? kNoScale : e0;
+          e1 = key + 16 >= to || key + 32 <= from ? kNoScale : e1;
         }
-        e0 = max(ve[nt], max(e0, e1));
+        e0 = max(e0, e1);
         // the scores' factors c0, c1 are not negative, so each tile's largest is that of the products
         const float top0 = fmaxf(fmaxf(s[nt][0][0], s[nt][0][1]), fmaxf(s[nt][0][2], s[nt][0][3]));
         const float top1 = fmaxf(fmaxf(s[nt][1][0], s[nt][1][1]), fmaxf(s[nt][1][2], s[nt][1][3]));
-        const float top = fmaxf(m[nt], max16(fmaxf(top0 * c0, top1 * c1)));
-        if (__any(top != m[nt] || e0 != ve[nt])) {
-          const float f = weight_of(m[nt], top), fo = __builtin_ldexpf(f, ve[nt] - e0);
+        const float top = max16(fmaxf(top0 * c0, top1 * c1));
+        if (__any(top > m[nt] + kLag<SPLIT> || e0 > ve[nt] + kLagExp<SPLIT>)) {
+          const float m1 = top > m[nt] + kLag<SPLIT> ? top : m[nt];
+          e0 = e0 > ve[nt] + kLagExp<SPLIT> ? e0 : ve[nt];
+          const float f = weight_of(m[nt], m1), fo = __builtin_ldexpf(f, ve[nt] - e0);
           l[nt] *= f;
 #pragma unroll
           for (int c = 0; c < C; ++c) o[nt][c] *= fo;
-          m[nt] = top;
+          m[nt] = m1;
           ve[nt] = e0;
         }
-        const float w0 = __builtin_ldexpf(v0, 14 - ve[nt]), w1 = __builtin_ldexpf(v1, 14 - ve[nt]);
+        const float w0 = __builtin_ldexpf(v0, kShift<SPLIT> - ve[nt]), w1 = __builtin_ldexpf(v1, kShift<SPLIT> - ve[nt]);
         auto hide = [&]() {  // what the row does not see has weight 0 whatever its block's scales are
+          const int from = vis_lo[nt], to = vis_hi[nt], first = here(key);
 #pragma unroll
           for (int tt = 0; tt < 2; ++tt)
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-              const int j = key + 16 * tt + 4 * g + r;
-              s[nt][tt][r] = j < vis_lo[nt] || j >= end ? 0.0f : s[nt][tt][r];
+              const int j = first + 16 * tt + 4 * g + r;
+              s[nt][tt][r] = j < from || j >= to ? 0.0f : s[nt][tt][r];
             }
         };
 #pragma unroll
@@ -721,7 +743,7 @@ __global__ __launch_bounds__(256, NT == 1 ? (D == 256 ? 2 : D == 128 ? 3 : 4) : 
 #pragma unroll
     for (int c = 0; c < C; ++c)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) o[nt][c][r] = in_units(o[nt][c][r] * norm, ve[nt]);
+      for (int r = 0; r < 4; ++r) o[nt][c][r] = in_units<SPLIT>(o[nt][c][r] * norm, ve[nt]);
   }
   if (it.chunks == 1) {
 #pragma unroll
@@ -914,22 +936,25 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_kv_attention_many(KvA
     }
     const bool edge = key < all_lo || key + kManyKeys > all_hi;
     float cs[4], vs[4];  // of the four 16-key tiles
-    int e0 = ve;
+    int e0 = kNoScale;
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
       cs[q] = c_row * lane_f(info.ks, 4 * ri + q);
       vs[q] = lane_f(info.vs, 4 * ri + q);
-      const int e = scale_exp(vs[q]);
-      e0 = max(e0, edge && (key + 16 * q >= vis_hi || key + 16 * q + 16 <= vis_lo) ? kNoScale : e);
+      if (!edge) e0 = max(e0, scale_exp(vs[q]));
     }
     if (edge) {
+      const int from = vis_lo, to = vis_hi;
 #pragma unroll
       for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
           const int j = key + 32 * mt + 8 * (r >> 2) + 4 * h + (r & 3);
-          if (j < vis_lo || j >= vis_hi) s[mt][r] = kMinusInf;
+          s[mt][r] = j < from || j >= to ? kMinusInf : s[mt][r];
         }
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        e0 = max(e0, key + 16 * q >= to || key + 16 * q + 16 <= from ? kNoScale : scale_exp(vs[q]));
     }
     // the scores' factors are not negative, so each tile's largest is that of the products
     float top = kMinusInf;
@@ -940,25 +965,28 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_kv_attention_many(KvA
       for (int r = 1; r < 8; ++r) x = fmaxf(x, s[q >> 1][8 * (q & 1) + r]);
       top = fmaxf(top, x * cs[q]);
     }
-    top = fmaxf(m, max32(top));
-    if (__any(top != m || e0 != ve)) {
-      const float f = weight_of(m, top), fo = __builtin_ldexpf(f, ve - e0);
+    top = max32(top);
+    if (__any(top > m + kLag<SPLIT> || e0 > ve + kLagExp<SPLIT>)) {
+      const float m1 = top > m + kLag<SPLIT> ? top : m;
+      e0 = e0 > ve + kLagExp<SPLIT> ? e0 : ve;
+      const float f = weight_of(m, m1), fo = __builtin_ldexpf(f, ve - e0);
       l *= f;
 #pragma unroll
       for (int c = 0; c < C; ++c) o[c] *= fo;
-      m = top;
+      m = m1;
       ve = e0;
     }
     auto hide = [&](int mt, f32x16& x) {  // what the row does not see has weight 0 whatever its block's scales are
+      const int from = vis_lo, to = vis_hi, first = here(key);
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
-        const int j = key + 32 * mt + 8 * (r >> 2) + 4 * h + (r & 3);
-        x[r] = j < vis_lo || j >= vis_hi ? 0.0f : x[r];
+        const int j = first + 32 * mt + 8 * (r >> 2) + 4 * h + (r & 3);
+        x[r] = j < from || j >= to ? 0.0f : x[r];
       }
     };
     float ws[4];
 #pragma unroll
-    for (int q = 0; q < 4; ++q) ws[q] = __builtin_ldexpf(vs[q], 14 - ve);
+    for (int q = 0; q < 4; ++q) ws[q] = __builtin_ldexpf(vs[q], kShift<SPLIT> - ve);
 #pragma unroll
     for (int mt = 0; mt < 2; ++mt) {
       f32x16& x = s[mt];
@@ -993,7 +1021,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_kv_attention_many(KvA
 #pragma unroll
   for (int c = 0; c < C; ++c)
 #pragma unroll
-    for (int r = 0; r < 16; ++r) o[c][r] = in_units(o[c][r] * norm, ve);
+    for (int r = 0; r < 16; ++r) o[c][r] = in_units<SPLIT>(o[c][r] * norm, ve);
   if (it.chunks == 1) {
     if (live) {
       const long at = (long)t * a.out_token + (long)w.head * a.out_head;
