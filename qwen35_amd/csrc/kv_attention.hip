@@ -798,8 +798,9 @@ __global__ __launch_bounds__(256, NT == 1 ? (D == 256 ? 2 : D == 128 ? 3 : 4) : 
 constexpr int kManyRows = 128;
 constexpr int kManyKeys = 64;
 
-template <int D, int SPLIT>
+template <int D>
 __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_kv_attention_many(KvAttnArgs a) {
+  constexpr int SPLIT = 1;
   constexpr int S = D / 16, C = D / 32;      // 16-dimension steps, output tiles
   constexpr int KP = D / 64;                 // 16-byte pieces of a key tile a thread stages
   constexpr int VW = D == 256 ? 2 : 1;       // dwords of a value row a thread stages (8 keys of 4 VW dimensions)
@@ -893,8 +894,8 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_kv_attention_many(KvA
   };
   if (count > 0) load_tile(info, 0);
 
-  h16x8 q_hi[S], q_lo[SPLIT == 2 ? S : 1];
-  const int qe = split_q<SPLIT, S>(raw, a.type, a.sign, max32, q_hi, q_lo);
+  h16x8 qf[S];
+  const int qe = split_q<SPLIT, S>(raw, a.type, a.sign, max32, qf, nullptr);
   const float c_row = __builtin_ldexpf(a.scale * kLog2e * kCodeScale, -qe);
   f32x16 o[C];
 #pragma unroll
@@ -925,14 +926,13 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_kv_attention_many(KvA
     f32x16 s[2];
 #pragma unroll
     for (int mt = 0; mt < 2; ++mt) {
-      f32x16 hi = {}, low = {};
+      f32x16 x = {};
 #pragma unroll
       for (int st = 0; st < S; ++st) {
-        const h16x8 x = *(const h16x8*)(k_at + 32 * mt * KB + 32 * st);
-        hi = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, q_hi[st], hi, 0, 0, 0);
-        if constexpr (SPLIT == 2) low = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, q_lo[st], low, 0, 0, 0);
+        const h16x8 k = *(const h16x8*)(k_at + 32 * mt * KB + 32 * st);
+        x = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, qf[st], x, 0, 0, 0);
       }
-      s[mt] = SPLIT == 2 ? hi + low : hi;
+      s[mt] = x;
     }
     const bool edge = key < all_lo || key + kManyKeys > all_hi;
     float cs[4], vs[4];  // of the four 16-key tiles
@@ -1000,19 +1000,15 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_kv_attention_many(KvA
 #pragma unroll
       for (int r = 0; r < 16; ++r) x[r] *= ws[2 * mt + (r >> 3)];
       if (edge && __any(!(ws[2 * mt] * 0.0f + ws[2 * mt + 1] * 0.0f == 0.0f))) hide(mt, x);  // 0 * NaN, 0 * infinity
-      h16x8 p_hi[2], p_lo[2];
+      h16x8 pf[2];
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        p_hi[r >> 3][r & 7] = (_Float16)x[r];
-        if constexpr (SPLIT == 2) p_lo[r >> 3][r & 7] = (_Float16)(x[r] - (float)p_hi[r >> 3][r & 7]);
-      }
+      for (int r = 0; r < 16; ++r) pf[r >> 3][r & 7] = (_Float16)x[r];
 #pragma unroll
       for (int st = 0; st < 2; ++st)
 #pragma unroll
         for (int c = 0; c < C; ++c) {
-          const h16x8 x = *(const h16x8*)(v_at + 64 * mt + 32 * st + 32 * c * VB);
-          o[c] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, p_hi[st], o[c], 0, 0, 0);
-          if constexpr (SPLIT == 2) o[c] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, p_lo[st], o[c], 0, 0, 0);
+          const h16x8 v = *(const h16x8*)(v_at + 64 * mt + 32 * st + 32 * c * VB);
+          o[c] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, pf[st], o[c], 0, 0, 0);
         }
     }
   }
@@ -1053,18 +1049,26 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_kv_attention_many(KvA
   arrive_and_join<D, SPLIT>(a, (float*)s_kv, parts_at, it, sp);
 }
 
-template <int SPLIT, int NT>
-static void launch_few(const KvAttnArgs& a, int dim, unsigned grid, hipStream_t s) {
-  if (dim == 64) hipLaunchKernelGGL((k_kv_attention_few<64, SPLIT, NT>), dim3(grid), dim3(256), 0, s, a);
-  else if (dim == 128) hipLaunchKernelGGL((k_kv_attention_few<128, SPLIT, NT>), dim3(grid), dim3(256), 0, s, a);
-  else hipLaunchKernelGGL((k_kv_attention_few<256, SPLIT, NT>), dim3(grid), dim3(256), 0, s, a);
+template <int D>
+static void launch_few(const KvAttnArgs& a, bool f32, bool pairs, unsigned grid, hipStream_t s) {
+  if constexpr (D < 256)
+    if (pairs) {
+      if (f32) hipLaunchKernelGGL((k_kv_attention_few<D, 2, 2>), dim3(grid), dim3(256), 0, s, a);
+      else hipLaunchKernelGGL((k_kv_attention_few<D, 1, 2>), dim3(grid), dim3(256), 0, s, a);
+      return;
+    }
+  if (f32) hipLaunchKernelGGL((k_kv_attention_few<D, 2, 1>), dim3(grid), dim3(256), 0, s, a);
+  else hipLaunchKernelGGL((k_kv_attention_few<D, 1, 1>), dim3(grid), dim3(256), 0, s, a);
 }
-
-template <int SPLIT>
+static void launch_few(const KvAttnArgs& a, int dim, bool f32, bool pairs, unsigned grid, hipStream_t s) {
+  if (dim == 64) launch_few<64>(a, f32, pairs, grid, s);
+  else if (dim == 128) launch_few<128>(a, f32, pairs, grid, s);
+  else launch_few<256>(a, f32, pairs, grid, s);
+}
 static void launch_many(const KvAttnArgs& a, int dim, unsigned grid, hipStream_t s) {
-  if (dim == 64) hipLaunchKernelGGL((k_kv_attention_many<64, SPLIT>), dim3(grid), dim3(256), 0, s, a);
-  else if (dim == 128) hipLaunchKernelGGL((k_kv_attention_many<128, SPLIT>), dim3(grid), dim3(256), 0, s, a);
-  else hipLaunchKernelGGL((k_kv_attention_many<256, SPLIT>), dim3(grid), dim3(256), 0, s, a);
+  if (dim == 64) hipLaunchKernelGGL(k_kv_attention_many<64>, dim3(grid), dim3(256), 0, s, a);
+  else if (dim == 128) hipLaunchKernelGGL(k_kv_attention_many<128>, dim3(grid), dim3(256), 0, s, a);
+  else hipLaunchKernelGGL(k_kv_attention_many<256>, dim3(grid), dim3(256), 0, s, a);
 }
 
 // 0, hipErrorInvalidValue or QHIP_DECLINE
@@ -1084,11 +1088,11 @@ struct AttnPlan {
 };
 // `tiles`: bound of the row tiles over all sequences and key heads.  Chunks of
 // cut sequences are fewer than 4/3 of target (find_item), items than target +
-// tiles.
+// tiles.  Twice as many tiles as items aimed for are enough as they are.
 static void plan_cut(AttnPlan& p, long tiles, int dim) {
   p.grid = p.cut_grid = tiles;
   const long most = (p.units + p.least - 1) / p.least;  // chunks of a tile
-  if (tiles > 0 && most > 1 && tiles <= kMaxCut && tiles * p.units < 0x7FFFFFFFL) {
+  if (tiles > 0 && most > 1 && tiles < 2L * p.target && tiles <= kMaxCut && tiles * p.units < 0x7FFFFFFFL) {
     p.cut_grid = tiles * most < p.target + tiles ? tiles * most : p.target + tiles;
     const long slots = tiles * most < 4L * p.target / 3 + 1 ? tiles * most : 4L * p.target / 3 + 1;
     p.work = kCountBytes + slots * p.rows * (dim + 2) * 4;
@@ -1097,30 +1101,38 @@ static void plan_cut(AttnPlan& p, long tiles, int dim) {
 static int units_of(int keys, int shift) { return (int)(((long)keys + (1 << shift) - 1) >> shift); }
 
 // the few-row kernel's plan, then the many-row kernel's
-static void attn_plans(const qhip_kv_cache* c, const qhip_kv_batch* b, int q_heads, AttnPlan* p) {
+static void attn_plans(const qhip_kv_cache* c, const qhip_kv_batch* b, int q_heads, int window, bool f32, AttnPlan* p) {
   const int group = q_heads / c->kv_heads;
+  const long rows = (long)b->tokens * q_heads, most_rows = (long)b->max_new * group;  // in all, of a sequence's key head
   AttnPlan &few = p[0], &many = p[1];
   few = many = AttnPlan{};
-  const int all_rows = 0;
-  few.max_tokens = many.min_tokens = all_rows ? 0x7FFFFFFF : kFewRows / group < b->max_new ? kFewRows / group : b->max_new;
+  if (b->max_new == 0) return;
+  const long many_tiles = rows / kManyRows + (long)b->nseq * c->kv_heads;
+  // row tiles times key tiles (at most) from which the many-row kernel runs
+  const long work = many_tiles * units_of(window > 0 && window < b->max_kv ? window : b->max_kv, 6);
+  const bool use_many = !f32 && most_rows > kFewRows && work >= (c->head_dim == 256 ? 20000 : 8500);
+  few.max_tokens = many.min_tokens = use_many ? kFewRows / group : 0x7FFFFFFF;
   many.max_tokens = 0x7FFFFFFF;
-  if (few.max_tokens > 0) {
-    few.rows = all_rows ? all_rows : few.max_tokens * group;
+  // all sequences alike: the few-row kernel has none
+  const bool none = use_many && (long)b->nseq * b->max_new == b->tokens;
+  if (few.max_tokens > 0 && !none) {
+    few.rows = most_rows <= 16 ? (int)most_rows : use_many || rows <= 8192 ? 16 : c->head_dim == 256 || rows < 40000 ? 32 : 64;
     few.key_shift = 5;
     few.units = units_of(b->max_kv, 5);
     few.target = c->head_dim == 256 ? 256 : 384;
     few.least = few.rows <= 16 ? 8 : 16;
-    plan_cut(few, ((all_rows ? (long)b->tokens * group / all_rows : 0) + b->nseq) * c->kv_heads, c->head_dim);
+    // beyond one a sequence and key head
+    long more = most_rows <= few.rows ? 0 : rows / few.rows;
+    if (use_many && more > 3L * b->nseq * c->kv_heads) more = 3L * b->nseq * c->kv_heads;
+    plan_cut(few, more + (long)b->nseq * c->kv_heads, c->head_dim);
   }
-  if (b->max_new > many.min_tokens) {
+  if (use_many) {
     many.rows = kManyRows;
     many.key_shift = 6;
     many.units = units_of(b->max_kv, 6);
-    many.target = 512;
+    many.target = c->head_dim == 256 ? 256 : 512;
     many.least = 8;
-    const long tiles = ((long)b->tokens * group / kManyRows + b->nseq) * c->kv_heads;
-    plan_cut(many, tiles, c->head_dim);
-    if (tiles >= 2 * many.target) many.work = 0;  // enough workgroups as it is
+    plan_cut(many, many_tiles, c->head_dim);
   }
 }
 
@@ -1130,9 +1142,13 @@ using namespace qhip;
 
 extern "C" long qhip_kv_attention_work_bytes(const qhip_kv_cache* cache, const qhip_kv_batch* batch, int q_heads) {
   if (check_batch(cache, batch, q_heads)) return -1;
-  AttnPlan p[2];
-  attn_plans(cache, batch, q_heads, p);
-  return p[0].work > p[1].work ? p[0].work : p[1].work;
+  long work = 0;
+  for (int f32 = 0; f32 < 2; ++f32) {
+    AttnPlan p[2];
+    attn_plans(cache, batch, q_heads, 0, f32, p);  // a window may only move rows to the plan of f32 rows
+    for (const AttnPlan& x : p) work = x.work > work ? x.work : work;
+  }
+  return work;
 }
 
 extern "C" int qhip_launch_kv_attention(const qhip_kv_cache* cache, const qhip_kv_batch* batch, int type,
@@ -1151,7 +1167,7 @@ extern "C" int qhip_launch_kv_attention(const qhip_kv_cache* cache, const qhip_k
   if (rc) return rc;
   if (batch->tokens == 0 || batch->nseq == 0) return 0;
   AttnPlan plans[2];
-  attn_plans(cache, batch, q_heads, plans);
+  attn_plans(cache, batch, q_heads, window, type == QHIP_TT_F32, plans);
   // rows and workgroups are counted in 32 bits
   if (plans[0].cut_grid > 0x7FFFFFFFL || plans[1].cut_grid > 0x7FFFFFFFL || (long)batch->tokens * q_heads > 0x7FFFFFFFL)
     return (int)hipErrorInvalidValue;
@@ -1203,12 +1219,8 @@ extern "C" int qhip_launch_kv_attention(const qhip_kv_cache* cache, const qhip_k
     a.max_chunks = kJoinPairs / p.rows;
     a.slots = a.cut ? (p.work - kCountBytes) / ((long)p.rows * (cache->head_dim + 2) * 4) : 0;
     const unsigned grid = (unsigned)(a.cut ? p.cut_grid : p.grid);
-    if (i == 0 && p.rows > 16) type == QHIP_TT_F32 ? launch_few<2, 2>(a, cache->head_dim, grid, (hipStream_t)stream)
-                                                   : launch_few<1, 2>(a, cache->head_dim, grid, (hipStream_t)stream);
-    else if (i == 0) type == QHIP_TT_F32 ? launch_few<2, 1>(a, cache->head_dim, grid, (hipStream_t)stream)
-                                         : launch_few<1, 1>(a, cache->head_dim, grid, (hipStream_t)stream);
-    else type == QHIP_TT_F32 ? launch_many<2>(a, cache->head_dim, grid, (hipStream_t)stream)
-                             : launch_many<1>(a, cache->head_dim, grid, (hipStream_t)stream);
+    if (i == 0) launch_few(a, cache->head_dim, type == QHIP_TT_F32, p.rows > 16, grid, (hipStream_t)stream);
+    else launch_many(a, cache->head_dim, grid, (hipStream_t)stream);
   }
   return (int)hipGetLastError();
 }

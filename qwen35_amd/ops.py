@@ -394,7 +394,8 @@ def kv_read(cache: KvCache, blocks: torch.Tensor, dtype: torch.dtype = torch.flo
 
 
 def kv_attention_work(cache: KvCache, q_heads: int, nseq: int, tokens: int, max_new: int, max_kv: int) -> torch.Tensor | None:
-    """Zeroed workspace for kv_attention's batches of up to these sizes (None when nothing would be cut)."""
+    """Zeroed workspace for kv_attention of a batch of these sizes (None when nothing would be cut); with another
+    batch's, long sequences may go uncut."""
     b = QhipKvBatch(None, None, None, nseq, tokens, max_new, max_kv, 0)
     n = load().qhip_kv_attention_work_bytes(cache._ref, ctypes.byref(b), q_heads)
     if n < 0:
