@@ -387,7 +387,7 @@ def kv_read(cache: KvCache, blocks: torch.Tensor, dtype: torch.dtype = torch.flo
     if dtype not in _KV_TYPES:
         raise ValueError("dtype: f32, f16 or bf16")
     shape = (len(blocks), cache.kv_heads, cache.block_size, cache.head_dim)
-    k, v = torch.empty((2, *shape), dtype=dtype, device=blocks.device)
+    k, v = torch.empty((2, *shape), dtype=dtype, device=blocks.device).unbind(0)
     check("kv_read", load().qhip_launch_kv_read(cache._ref, _ints("blocks", blocks), len(blocks), _KV_TYPES[dtype],
                                                 k.data_ptr(), v.data_ptr(), _stream()))
     return k, v
