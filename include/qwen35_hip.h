@@ -385,7 +385,8 @@ typedef struct qhip_kv_cache {
 
 /* Block tables and slot maps from the lengths of a step's requests.  Sequence
  * i < nseq has d_cached[i] tokens in the cache and brings d_new[i] (either may
- * be 0; negative counts as 0); its blocks are d_table[i * table_width ...], of
+ * be 0; negative counts as 0, cached + new is cut at 2^30, the sum of d_new is
+ * below 2^31); its blocks are d_table[i * table_width ...], of
  * which the first ceil(cached / block_size) are there.  Sequences take the
  * further blocks that they need from d_free[0 .. nfree) in order, from entry
  * d_taken[0] (NULL = 0) on.  Written:
@@ -441,13 +442,15 @@ typedef struct qhip_kv_batch {
 } qhip_kv_batch;
 
 /* Attention of each packed token's q_heads query heads over its own sequence's
- * cached keys and values; query head h reads key head h / (q_heads / kv_heads).
+ * cached keys and values; query head h reads key head h / (q_heads / kv_heads)
+ * (at most 512 query heads a key head; more: QHIP_DECLINE).
  *   s_j = softmax_scale * q . k_j over the visible j, out = sum softmax(s)_j v_j,
  *   lse = log(sum exp(s_j))
  * The n-th of a sequence's new tokens is its token p = kv_len - new + n; causal
  * (0 or 1): it sees j <= p, and with window > 0 only j > p - window.  A row that
  * sees nothing gets out = 0 and lse = -infinity.  A visible token whose table
- * entry names no block of the pool makes its rows NaN.  d_q, d_out: head_dim
+ * entry names no block of the pool makes its rows NaN; lengths above 2^30 are
+ * taken as 2^30.  d_q, d_out: head_dim
  * contiguous elements of `type` at token * token_stride + head * head_stride
  * (elements); d_lse (nullable): f32 [tokens][q_heads].  Rows of tokens at or
  * past offsets[nseq] are not written.

@@ -31,7 +31,7 @@ struct KvAttnArgs {
   int nseq, tokens, width, shift, num_blocks, kv_heads, q_heads;
   float scale, sign;  // the softmax scale's absolute value and sign
   int causal, window, type, group;
-  int group_inv;  // 65536 / group, rounded up
+  int group_inv;  // 2^20 / group, rounded up
   // the kernel's sequences (those of min_tokens < new tokens <= max_tokens), the
   // rows of a workgroup and log2 of the keys of a unit
   int min_tokens, max_tokens, tile_rows, key_shift;
@@ -128,11 +128,12 @@ __device__ __forceinline__ SeqPlan plan_seq(const KvAttnArgs& a, int i) {
   SeqPlan s{0, 0, 0, 0, 0};
   if (i >= a.nseq) return s;
   const int first = a.offsets[i], end = a.offsets[i + 1], len = a.kv_lens[i];
+  if (first < 0 || end <= first) return s;
   const int n = end - first, here = min(end, a.tokens) - first;  // new tokens, and those among the packed rows
-  if (n <= a.min_tokens || n > a.max_tokens || here <= 0) return s;
+  if (n <= a.min_tokens || n > a.max_tokens || n > kMaxLen || here <= 0) return s;
   s.first = first;
   s.n = n;
-  s.len = max(len, 0);
+  s.len = min(max(len, 0), kMaxLen);
   s.tiles = (here * a.group + a.tile_rows - 1) / a.tile_rows;
   int keys = s.len;
   if (a.window > 0) keys = (int)min((long)keys, (long)a.window + a.tile_rows + (2 << a.key_shift));
@@ -183,6 +184,8 @@ __device__ __forceinline__ bool find_item(const KvAttnArgs& a, int lane, Item& i
   return false;
 }
 
+constexpr int kBehind = 1 << 20;
+
 // The item's rows and keys.
 struct Span {
   int row0, rows;    // first row and rows of the tile
@@ -196,7 +199,9 @@ __device__ __forceinline__ Span find_span(const KvAttnArgs& a, const Item& it) {
   s.first = it.len - it.n;
   const int tok_a = uniform(s.row0 / a.group), tok_b = uniform((s.row0 + s.rows - 1) / a.group);
   const int lo = a.window > 0 ? max(0, s.first + tok_a - a.window + 1) >> a.key_shift << a.key_shift : 0;
-  const int hi = a.causal ? s.first + tok_b + 1 : it.len;
+  // (lengths that the table cannot hold end a little behind it: enough for their rows to be NaN)
+  const long cap = max((long)a.width << a.shift, (long)lo) + kBehind;
+  const int hi = (int)min((long)(a.causal ? s.first + tok_b + 1 : it.len), cap);
   const int units = max(0, hi - lo + (1 << a.key_shift) - 1) >> a.key_shift;
   const int q = uniform(units / it.chunks), r = units - q * it.chunks;  // the first r chunks have one more
   const int u0 = q * it.chunk + min(it.chunk, r), u1 = u0 + q + (it.chunk < r ? 1 : 0);
@@ -209,8 +214,8 @@ struct RowAt {
   int tok, head;
 };
 __device__ __forceinline__ RowAt row_at(const KvAttnArgs& a, const Span& s, int r, int head) {
-  const int base = s.row0 / a.group, x = s.row0 - base * a.group + r;  // x < tile rows + group
-  const int t = (x * a.group_inv) >> 16;
+  const int base = s.row0 / a.group, x = s.row0 - base * a.group + r;
+  const int t = (x * a.group_inv) >> 20;  // x / group, exact: x < 128 + group, so x * group < 2^20
   return RowAt{base + t, head * a.group + (x - t * a.group)};
 }
 
@@ -223,7 +228,7 @@ struct TileInfo {
 };
 __device__ __forceinline__ int tile_id(const KvAttnArgs& a, int seq, int key, int end) {
   const int b = key >> a.shift;
-  return key < end && b < a.width ? a.table[(long)seq * a.width + b] : key < end ? -1 : -2;
+  return key >= end ? -2 : (unsigned)b < (unsigned)a.width ? a.table[(long)seq * a.width + b] : -1;
 }
 __device__ __forceinline__ TileInfo tile_info(const KvAttnArgs& a, int id, int head) {
   const bool in = (unsigned)id < (unsigned)a.num_blocks;
@@ -369,7 +374,7 @@ __device__ __forceinline__ void join_rows(const KvAttnArgs& a, float* lds, __amd
 #pragma unroll
       for (int k = 0; k < CB; ++k)
         x[j][k] = __builtin_amdgcn_raw_buffer_load_b128(
-            parts, e + 256 * j < pieces && sl < slices ? 4 * ((c + k * slices) * stride + 4 * (e + 256 * j)) : -1, 0, kSc1);
+            parts, 4 * (e + 256 * j < pieces && sl < slices ? (c + k * slices) * stride + 4 * (e + 256 * j) : chunks * stride), 0, kSc1);
   };
   load(e0, sl);
   for (int i = tid; i < chunks * count; i += 256) {
@@ -1071,13 +1076,14 @@ static void launch_many(const KvAttnArgs& a, int dim, unsigned grid, hipStream_t
   else hipLaunchKernelGGL(k_kv_attention_many<256>, dim3(grid), dim3(256), 0, s, a);
 }
 
+constexpr int kMaxGroup = 512;  // most query heads of a key head (row_at)
 // 0, hipErrorInvalidValue or QHIP_DECLINE
 static int check_batch(const qhip_kv_cache* cache, const qhip_kv_batch* b, int q_heads) {
   const int rc = kv_check_cache(cache);
   if (rc == (int)hipErrorInvalidValue || !b) return (int)hipErrorInvalidValue;
   if (b->nseq < 0 || b->tokens < 0 || b->max_new < 0 || b->max_kv < 0 || b->table_width < 0) return (int)hipErrorInvalidValue;
   if (q_heads <= 0 || q_heads > 65535 || q_heads % cache->kv_heads) return (int)hipErrorInvalidValue;
-  return rc;
+  return rc ? rc : q_heads / cache->kv_heads > kMaxGroup ? QHIP_DECLINE : 0;
 }
 
 // One kernel's share of a batch: its sequences, tile and unit sizes, grid without
@@ -1196,10 +1202,10 @@ extern "C" int qhip_launch_kv_attention(const qhip_kv_cache* cache, const qhip_k
   a.scale = fabsf(softmax_scale);
   a.sign = softmax_scale < 0.0f ? -1.0f : 1.0f;
   a.causal = causal;
-  a.window = window;
+  a.window = window < kMaxLen ? window : kMaxLen;
   a.type = type;
   a.group = q_heads / cache->kv_heads;
-  a.group_inv = (65536 + a.group - 1) / a.group;
+  a.group_inv = ((1 << 20) + a.group - 1) / a.group;
   a.counters = (unsigned*)d_work;
   a.partial = (float*)((char*)d_work + kCountBytes);
   // the two kernels share the workspace: they follow each other on the stream

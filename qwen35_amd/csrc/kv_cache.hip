@@ -17,7 +17,7 @@ namespace qhip {
 // two scans), and then fills its own share of the tokens and of the table's
 // new entries, each by a search in the sums: one launch, nothing handed from
 // one workgroup to another.
-constexpr int kTabSeqs = 1024;    // sequences of a chunk (256 threads x 4)
+constexpr int kTabSeqs = 1024;  // sequences of a chunk (256 threads x 4)
 
 struct KvTablesArgs {
   const int *cached, *fresh, *free_list, *taken;
@@ -40,7 +40,7 @@ __global__ __launch_bounds__(256) void k_kv_tables(KvTablesArgs a) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const bool last = blockIdx.x == gridDim.x - 1;
   const int t_lo = (int)blockIdx.x * 256 * a.each, t_hi = min(a.tokens, t_lo + 256 * a.each);
-  const int e_lo = (int)blockIdx.x * a.entries, e_hi = last ? 0x7FFFFFFF : e_lo + a.entries;
+  const int e_lo = (int)blockIdx.x * a.entries, e_hi = last ? 0x7FFFFF00 : e_lo + a.entries;
   const int mask = (1 << a.shift) - 1;
   const int taken = a.taken ? a.taken[0] : 0;
   int off0 = 0, fresh0 = 0;  // sums before the chunk
@@ -49,8 +49,8 @@ __global__ __launch_bounds__(256) void k_kv_tables(KvTablesArgs a) {
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
       const int i = s0 + 4 * tid + k;
-      c[k] = i < a.nseq ? max(a.cached[i], 0) : 0;
-      n[k] = i < a.nseq ? max(a.fresh[i], 0) : 0;
+      c[k] = i < a.nseq ? min(max(a.cached[i], 0), kMaxLen) : 0;
+      n[k] = i < a.nseq ? min(max(a.fresh[i], 0), kMaxLen - c[k]) : 0;
     }
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
@@ -97,7 +97,7 @@ __global__ __launch_bounds__(256) void k_kv_tables(KvTablesArgs a) {
       for (int k = 0; k < 4; ++k) {
         const int t = t0 + k;
         if (t < tb || t >= t1) continue;
-        while (s_off[i + 1] <= t) ++i;
+        while (i + 1 < cnt && s_off[i + 1] <= t) ++i;
         const int p = s_len[i] + (t - s_off[i]);
         const int j = p >> a.shift, before = (s_len[i] + mask) >> a.shift;
         int entry = -1;

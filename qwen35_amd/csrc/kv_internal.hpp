@@ -12,6 +12,10 @@ namespace qhip {
 typedef uint32_t kv_u32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t kv_u32x2 __attribute__((ext_vector_type(2)));
 
+// Longest sequence: places are ints, and some are counted a round of steps past
+// the last.
+constexpr int kMaxLen = 1 << 30;
+
 // NaN payloads aside, (float)T is exact and T(float) rounds to nearest even.
 typedef _Float16 f16_t;
 typedef __bf16 bf16_t;

@@ -92,3 +92,15 @@ def test_attention_workspace(lib):
     assert lib.qhip_kv_attention_work_bytes(cache(), batch(tokens=-1), 4) == -1
     assert lib.qhip_kv_attention_work_bytes(cache(), batch(), 3) == -1
     assert lib.qhip_kv_attention_work_bytes(cache(), batch(), 4) >= 0
+
+
+def test_attention_workspace_covers_the_types_and_stays_moderate(lib):
+    c = cache(kv_heads=4, head_dim=128, block_size=64, num_blocks=100)
+    for nseq, tokens, new, kv in [(1, 1, 1, 131072), (64, 64, 1, 8192), (13, 65, 5, 4000), (12, 1032, 1021, 6021)]:
+        n = lib.qhip_kv_attention_work_bytes(c, batch(nseq=nseq, tokens=tokens, max_new=new, max_kv=kv), 16)
+        assert 32768 < n <= 64 << 20, (nseq, tokens, n)
+    # enough row tiles as they are, nothing to cut, no rows
+    assert lib.qhip_kv_attention_work_bytes(c, batch(nseq=2000, tokens=2000, max_new=1, max_kv=9000), 16) == 0
+    assert lib.qhip_kv_attention_work_bytes(c, batch(nseq=1, tokens=1, max_new=1, max_kv=32), 16) == 0
+    assert lib.qhip_kv_attention_work_bytes(c, batch(nseq=1, tokens=1, max_new=0, max_kv=9000), 16) == 0
+    assert lib.qhip_kv_attention_work_bytes(cache(kv_heads=1), batch(), 513) == -1
