@@ -313,6 +313,8 @@ __global__ __launch_bounds__(256) void k_kv_read(KvReadArgs a) {
 
 using namespace qhip;
 
+static bool overlap(const int* a, int na, const int* b, int nb) { return a && b && a < b + nb && b < a + na; }
+
 extern "C" int qhip_launch_kv_tables(const int* d_cached, const int* d_new, int nseq, const int* d_free, int nfree,
                                      const int* d_taken, int block_size, int* d_table, int table_width, int tokens,
                                      int* d_offsets, int* d_kv_lens, int* d_slots, int* d_positions, int* d_taken_out,
@@ -322,6 +324,12 @@ extern "C" int qhip_launch_kv_tables(const int* d_cached, const int* d_new, int 
   if (!d_offsets || !d_taken_out || (nseq > 0 && (!d_cached || !d_new || !d_kv_lens)) || (nfree > 0 && !d_free) ||
       (nseq > 0 && table_width > 0 && !d_table) || (tokens > 0 && !d_slots))
     return (int)hipErrorInvalidValue;
+  // (an output in an input's place would be read by workgroups that start later)
+  const struct { const int* at; int n; } in[] = {{d_cached, nseq}, {d_new, nseq}, {d_taken, 1}, {d_free, nfree}},
+                                         out[] = {{d_offsets, nseq + 1}, {d_kv_lens, nseq}, {d_taken_out, 1}};
+  for (const auto& x : in)
+    for (const auto& y : out)
+      if (overlap(x.at, x.n, y.at, y.n)) return (int)hipErrorInvalidValue;
   // every workgroup walks all sequences, so the grid follows the tokens; the
   // fresh blocks number at most tokens / block_size + nseq
   // (four tokens a thread share a search and 16-byte stores: 100,000 tokens of

@@ -42,6 +42,15 @@ def test_tables(lib):
         assert lib.qhip_launch_kv_tables(*args) == INVALID, (at, bad)
 
 
+def test_tables_in_place_are_refused(lib):
+    at = [P + 0x100 * i for i in range(9)]  # cached, new, free, taken, table, offsets, kv_lens, slots, taken_out
+    for inp, out in [(0, 5), (0, 6), (1, 6), (2, 8), (3, 8), (3, 5)]:
+        x = list(at)
+        x[out] = x[inp]
+        assert lib.qhip_launch_kv_tables(x[0], x[1], 2, x[2], 3, x[3], 16, x[4], 4, 5, x[5], x[6], x[7], None, x[8],
+                                         None) == INVALID, (inp, out)
+
+
 def test_append(lib):
     def call(c, type=0, k=P, v=P, slots=P, tokens=3):
         return lib.qhip_launch_kv_append(c, type, k, 128, 64, v, 128, 64, slots, tokens, None)
