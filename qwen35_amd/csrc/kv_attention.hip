@@ -946,22 +946,30 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_kv_attention_many(KvA
     for (int q = 0; q < 4; ++q) {
       cs[q] = c_row * lane_f(info.ks, 4 * ri + q);
       vs[q] = lane_f(info.vs, 4 * ri + q);
-      if (!edge) e0 = max(e0, scale_exp(vs[q]));
+      // frexp_exp of a normal number, on the scalar unit (0 and what is below 2^-126 count as 2^-126)
+      const int e = ((int)__float_as_uint(vs[q]) >> 23) - 126;
+      e0 = max(e0, e < 129 ? e : kNoScale);
     }
+    const int from = vis_lo, to = vis_hi;
+    auto hide = [&](int mt, float with) {
+      const int lo = from - 4 * h - here(key), hi = to - 4 * h - here(key);
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const int j = 32 * mt + 8 * (r >> 2) + (r & 3);
+        s[mt][r] = j < lo || j >= hi ? with : s[mt][r];
+      }
+    };
     if (edge) {
-      const int from = vis_lo, to = vis_hi;
+      hide(0, kMinusInf);
+      hide(1, kMinusInf);
+      e0 = kNoScale;
 #pragma unroll
-      for (int mt = 0; mt < 2; ++mt)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const int j = key + 32 * mt + 8 * (r >> 2) + 4 * h + (r & 3);
-          s[mt][r] = j < from || j >= to ? kMinusInf : s[mt][r];
-        }
-#pragma unroll
-      for (int q = 0; q < 4; ++q)
-        e0 = max(e0, key + 16 * q >= to || key + 16 * q + 16 <= from ? kNoScale : scale_exp(vs[q]));
+      for (int q = 0; q < 4; ++q) {
+        const int e = scale_exp(vs[q]);
+        e0 = max(e0, key + 16 * q >= to || key + 16 * q + 16 <= from ? kNoScale : e);
+      }
     }
-    // the scores' factors are not negative, so each tile's largest is that of the products
+    // the scores' factors are not negative, so each 16-key tile's largest is that of the products
     float top = kMinusInf;
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
@@ -981,33 +989,32 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_kv_attention_many(KvA
       m = m1;
       ve = e0;
     }
-    auto hide = [&](int mt, f32x16& x) {  // what the row does not see has weight 0 whatever its block's scales are
-      const int from = vis_lo, to = vis_hi, first = here(key);
-#pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const int j = first + 32 * mt + 8 * (r >> 2) + 4 * h + (r & 3);
-        x[r] = j < from || j >= to ? 0.0f : x[r];
-      }
-    };
     float ws[4];
 #pragma unroll
     for (int q = 0; q < 4; ++q) ws[q] = __builtin_ldexpf(vs[q], kShift<SPLIT> - ve);
+    float sum[2] = {};
+    auto weights = [&](auto masked) {
+#pragma unroll
+      for (int mt = 0; mt < 2; ++mt) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[mt][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[mt][r], cs[2 * mt + (r >> 3)], -m));
+        if constexpr (masked) hide(mt, 0.0f);  // what the row does not see has weight 0 whatever its block's scales are
+#pragma unroll
+        for (int r = 0; r < 16; ++r) sum[mt] += s[mt][r];
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[mt][r] *= ws[2 * mt + (r >> 3)];
+        if constexpr (masked) hide(mt, 0.0f);  // 0 * NaN, 0 * infinity
+      }
+    };
+    if (edge) weights(std::true_type{});
+    else weights(std::false_type{});
+    l += sum[0];
+    l += sum[1];
 #pragma unroll
     for (int mt = 0; mt < 2; ++mt) {
-      f32x16& x = s[mt];
-#pragma unroll
-      for (int r = 0; r < 16; ++r) x[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[r], cs[2 * mt + (r >> 3)], -m));
-      if (edge) hide(mt, x);
-      float sum = 0.0f;
-#pragma unroll
-      for (int r = 0; r < 16; ++r) sum += x[r];
-      l += sum;
-#pragma unroll
-      for (int r = 0; r < 16; ++r) x[r] *= ws[2 * mt + (r >> 3)];
-      if (edge && __any(!(ws[2 * mt] * 0.0f + ws[2 * mt + 1] * 0.0f == 0.0f))) hide(mt, x);  // 0 * NaN, 0 * infinity
       h16x8 pf[2];
 #pragma unroll
-      for (int r = 0; r < 16; ++r) pf[r >> 3][r & 7] = (_Float16)x[r];
+      for (int r = 0; r < 16; ++r) pf[r >> 3][r & 7] = (_Float16)s[mt][r];
 #pragma unroll
       for (int st = 0; st < 2; ++st)
 #pragma unroll
