@@ -412,8 +412,8 @@ int qhip_launch_kv_tables(const int *d_cached, const int *d_new, int nseq, const
  * (-1) skips the token, whose values are not read.  Tokens of one block must be
  * adjacent and in slot order, as qhip_launch_kv_tables lays them out.  For each
  * block and head that gets tokens
- *   scale = max(old scale, max |x| / 127), without the old one where the first
- *   new token is the block's first;
+ *   scale = max(old scale, max |x| * (1/127)), without the old one where the
+ *   first new token is the block's first;
  *   codes of the tokens before it: round(code * (old / scale));
  *   new codes: round(x * (1 / scale)), each an f32 operation, ties to even.
  * A NaN among the new values makes the scale NaN, an infinity makes it

@@ -211,7 +211,7 @@ __device__ __forceinline__ void append_run(const KvAppendArgs& a, int t, int slo
     __syncthreads();  // read before the next run's
   }
   // maximum of non-negative floats as integers: NaN above infinity above all others
-  const uint32_t sbits = max(__float_as_uint(__uint_as_float(top) / 127.0f) & 0x7FFFFFFFu, __float_as_uint(old));
+  const uint32_t sbits = max(__float_as_uint(__uint_as_float(top) * (1.0f / 127.0f)) & 0x7FFFFFFFu, __float_as_uint(old));
   const float scale = __uint_as_float(sbits);
   const float inv = scale > 0.0f ? 1.0f / scale : 0.0f;
   int8_t* codes = a.codes[z] + bh * ((long)size * a.dim);

@@ -25,6 +25,10 @@ def tables(cached, new, free, taken, table, block, tokens):
     return table, offsets, kv_lens, (slots + [-1] * pad)[:tokens], (positions + [0] * pad)[:tokens], taken
 
 
+#: a code step's share of the largest value: the f32 nearest 1/127
+PART = float(torch.tensor(1.0) / torch.tensor(127.0))
+
+
 def _f32(x):
     return x.float().double()
 
@@ -43,7 +47,7 @@ def append(codes, scales, x, slots):
         for h in range(codes.shape[1]):
             old = scales[b, h].double() if first else torch.zeros((), dtype=torch.float64, device=x.device)
             top = x[rows, h].abs().max()
-            scale = torch.maximum(old, _f32(top / 127))
+            scale = torch.maximum(old, _f32(top * PART))
             c = codes[b, h].double()
             usable = bool(torch.isfinite(scale) and scale > 0)
             ratio = _f32(old / scale) if usable else torch.zeros_like(old)
