@@ -1124,11 +1124,13 @@ static void attn_plans(const qhip_kv_cache* c, const qhip_kv_batch* b, int q_hea
   // row tiles times key tiles (at most) from which the many-row kernel runs
   const long work = many_tiles * units_of(window > 0 && window < b->max_kv ? window : b->max_kv, 6);
   const bool use_many = !f32 && most_rows > kFewRows && work >= (c->head_dim == 256 ? 20000 : 8500);
-  few.max_tokens = many.min_tokens = use_many ? kFewRows / group : 0x7FFFFFFF;
+  // where the sequences are half as long as the longest on average, what single
+  // tokens there may be are few beside the tiles of the others, and a launch
+  // that mostly finds no sequence costs 3 to 4 us
+  const bool alike = use_many && (long)b->nseq * b->max_new <= 2L * b->tokens;
+  few.max_tokens = many.min_tokens = alike ? 0 : use_many ? kFewRows / group : 0x7FFFFFFF;
   many.max_tokens = 0x7FFFFFFF;
-  // all sequences alike: the few-row kernel has none
-  const bool none = use_many && (long)b->nseq * b->max_new == b->tokens;
-  if (few.max_tokens > 0 && !none) {
+  if (few.max_tokens > 0) {
     few.rows = most_rows <= 16 ? (int)most_rows : use_many || rows <= 8192 ? 16 : c->head_dim == 256 || rows < 40000 ? 32 : 64;
     few.key_shift = 5;
     few.units = units_of(b->max_kv, 5);

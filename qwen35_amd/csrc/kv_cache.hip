@@ -166,6 +166,7 @@ struct KvAppendArgs {
   long token_stride[2], head_stride[2];
   const int* slots;
   int tokens, num_slots, shift, heads, dim, tile;
+  bool near;
 };
 
 __device__ __forceinline__ int code8(float x, float m) {
@@ -238,9 +239,11 @@ __device__ __forceinline__ void append_run(const KvAppendArgs& a, int t, int slo
 template <typename T>
 __global__ __launch_bounds__(256) void k_kv_append(KvAppendArgs a) {
   __shared__ uint32_t s_max[4];
-  const int h = blockIdx.y, z = blockIdx.z, tid = threadIdx.x, lane = tid & 63, size = 1 << a.shift;
+  const int tid = threadIdx.x, lane = tid & 63, size = 1 << a.shift;
+  const int item = a.near ? blockIdx.y : blockIdx.x;
+  const int z = a.near ? (int)blockIdx.x >= a.heads : blockIdx.z, h = a.near ? (int)blockIdx.x - z * a.heads : blockIdx.y;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int t0 = (int)blockIdx.x * a.tile;
+  const int t0 = item * a.tile;
   // the tokens of the tile that begin a run (a lane each)
   int slot = -1;
   bool begins = false;
@@ -352,12 +355,13 @@ extern "C" int qhip_launch_kv_append(const qhip_kv_cache* cache, int type, const
     return (int)hipErrorInvalidValue;
   if (rc) return rc;
   if (tokens == 0) return 0;
-  const int num_slots = cache->num_blocks * cache->block_size;
+  const int num_slots = cache->num_blocks * cache->block_size, tile = tokens > kAppFew ? kAppTokens : 1;
+  const int tiles = (tokens - 1) / tile + 1;
   const KvAppendArgs a{{(int8_t*)cache->k, (int8_t*)cache->v}, {cache->k_scale, cache->v_scale}, {d_k, d_v},
                        {k_token_stride, v_token_stride}, {k_head_stride, v_head_stride}, d_slots, tokens, num_slots,
                        kv_block_shift(cache->block_size), cache->kv_heads, cache->head_dim,
-                       tokens > kAppFew ? kAppTokens : 1};
-  const dim3 grid((unsigned)((tokens + a.tile - 1) / a.tile), (unsigned)cache->kv_heads, 2);
+                       tile, tile > 1 && tiles <= 65535};
+  const dim3 grid = a.near ? dim3(2 * cache->kv_heads, tiles) : dim3(tiles, cache->kv_heads, 2);
   hipStream_t s = (hipStream_t)stream;
   if (type == QHIP_TT_F32) hipLaunchKernelGGL(k_kv_append<float>, grid, dim3(256), 0, s, a);
   else if (type == QHIP_TT_F16) hipLaunchKernelGGL(k_kv_append<f16_t>, grid, dim3(256), 0, s, a);

@@ -25,6 +25,14 @@ def test_batches(gpu, lens, dim, heads, group, dtype):
     t.check(lens, heads, group, 64, dim, dtype, seed=dim)
 
 
+@pytest.mark.parametrize("dtype", t.DTYPES)
+@pytest.mark.parametrize("dim,heads,group", [(64, 2, 8), (128, 2, 8), (256, 3, 8), (64, 12, 1)])
+def test_a_short_sequence_among_long_ones(gpu, dim, heads, group, dtype):
+    lens = [(3001, 3001), (2500, 1), (2900, 2500), (0, 0)]
+    t.check(lens, heads, group, 64, dim, dtype, seed=dim)
+    t.check(lens, heads, group, 64, dim, dtype, seed=dim, window=700)
+
+
 @pytest.mark.parametrize("block", [16, 32, 128, 256])
 @pytest.mark.parametrize("dim", [64, 128, 256])
 def test_block_sizes(gpu, dim, block):
