@@ -329,7 +329,11 @@ __device__ __forceinline__ float in_units(float o, int e) { return __builtin_lde
 // row's maximum m and sum l, stored and loaded through to the agent's point of
 // coherence (sc1: sk_store's and sk_load's policy, 16 bytes at a time).  Every
 // chunk adds one to the tile's counter; the last one joins all in chunk order,
-// so the result does not depend on which was last.
+// so the result does not depend on which was last.  A join is bound by the
+// latency of its loads, so 16 pieces a thread are in flight: 4 chunks of 128 rows
+// of 128 dimensions take 10 us, a decode's chunks of 4 rows 3.7.  (32 in
+// flight spill the products' registers: 96 us against 86 for 512 rows behind 8000
+// keys.)
 constexpr int kSc1 = 16;  // cache policy of a buffer access
 constexpr long kCountBytes = 32768;
 constexpr int kMaxCut = kCountBytes / 4;  // most row tiles that are cut
@@ -455,7 +459,8 @@ __device__ __forceinline__ void arrive_and_join(const KvAttnArgs& a, float* lds,
 
 // ---- sequences of a few rows: the cache streamed once ------------------------------
 //
-// Row tiles of 16, up to four in a workgroup.  The work is one pass over the
+// Row tiles of 16 (NT = 2: pairs of them in a wave, 32 rows on each step's codes),
+// up to four a workgroup.  The work is one pass over the
 // codes, 2 D bytes a key, so the kernel is built to keep loads in flight and
 // never puts a code anywhere but in a register:
 //
@@ -476,7 +481,17 @@ __device__ __forceinline__ void arrive_and_join(const KvAttnArgs& a, float* lds,
 // A workgroup's four waves take steps of 32 keys in turn (one, two or four row
 // tiles share a step's waves) and are merged in LDS.  Long sequences are cut
 // into chunks over workgroups (find_item).
-constexpr int kFewRows = 64;
+//
+// Bound by memory where sequences are long: one f32 token on 131071 keys (4 key
+// heads of 256, 268 MB) 60 us, 4.5 TB/s; 64 tokens on 2000 keys each, 53 us at 4.9
+// TB/s (256) and 30 us at 4.2 TB/s (8 heads of 128).  Short ones are bound by
+// chains of latencies: lengths - plan - table - scales 5 us and codes 3 us before
+// the first product, 2 us to merge the waves, partial results - counter - join 5
+// us where a sequence is cut: one token on 333 keys takes 13 us.  f32 rows in number are bound by the matrix pipe
+// at twice the products for either operand: 4096 tokens, 16 heads of 128, 170 us
+// (400 TFLOP/s).  The registers allow two waves a SIMD for D = 256 and three for
+// 128; a fourth would spill (60 us against 44 for 64 ragged decodes).
+constexpr int kFewRows = 64;  // rows up to which a sequence beside long ones is this kernel's
 
 template <int D, int SPLIT, int NT>
 __global__ __launch_bounds__(256, NT == 1 ? (D == 256 ? 2 : D == 128 ? 3 : 4) : (D == 256 ? 1 : 2)) void k_kv_attention_few(KvAttnArgs a) {
@@ -799,6 +814,17 @@ __global__ __launch_bounds__(256, NT == 1 ? (D == 256 ? 2 : D == 128 ? 3 : 4) : 
 // a 32-key half are its scores and its half of the weights' operand, and output
 // tile c holds dimensions i D/32 + c.  The next tile's codes are in flight in
 // registers while this one is multiplied.
+//
+// Bound by the SIMDs' issue: of a tile's time the matrix pipe is busy for 38% and
+// the vector pipe issues for 61% (32 exponentials and some 300 other operations a
+// lane and tile of 64 keys, a quarter of them the staging), and the two hardly
+// overlap with two waves a SIMD.  A prompt of 8192 tokens, 32 heads of 128 on 8,
+// takes 650 us (850 TFLOP/s); 4096 tokens of 16 heads 127 us (531), of 256
+// dimensions 242 us (563), of 64 95 us (350: half the products to the same
+// exponentials).  Tried and not kept: LDS for two tiles with one barrier (the
+// same for 128, 285 us against 242 for 256), loops of their own for tiles without
+// masks (64: 88 against 94, but 256: 402 against 242 for its spills), three waves a
+// SIMD for 64 (116 against 99), priority for the products (702 us against 696).
 
 constexpr int kManyRows = 128;
 constexpr int kManyKeys = 64;
@@ -1123,6 +1149,10 @@ static void attn_plans(const qhip_kv_cache* c, const qhip_kv_batch* b, int q_hea
   const long many_tiles = rows / kManyRows + (long)b->nseq * c->kv_heads;
   // row tiles times key tiles (at most) from which the many-row kernel runs
   const long work = many_tiles * units_of(window > 0 && window < b->max_kv ? window : b->max_kv, 6);
+  // (us, few-row / many-row kernel, bf16, 16 heads on 4: 2048 tokens of 128 48 / 57,
+  // 4096 129 / 127, of 256 100 / 116 and 321 / 242; 512 tokens behind 8000 keys of 128
+  // 97 / 87, 256 behind 4000 37 / 51; of 64 512 behind 8000 66 / 51, 8192 tokens 288 /
+  // 262, but 4096 87 / 95, whose 512 uneven tiles are one round of workgroups.)
   const bool use_many = !f32 && most_rows > kFewRows && work >= (c->head_dim == 256 ? 20000 : 8500);
   // where the sequences are half as long as the longest on average, what single
   // tokens there may be are few beside the tiles of the others, and a launch
@@ -1131,9 +1161,20 @@ static void attn_plans(const qhip_kv_cache* c, const qhip_kv_batch* b, int q_hea
   few.max_tokens = many.min_tokens = alike ? 0 : use_many ? kFewRows / group : 0x7FFFFFFF;
   many.max_tokens = 0x7FFFFFFF;
   if (few.max_tokens > 0) {
+    // Rows of a workgroup: more of them share the codes, fewer make more
+    // workgroups.  (us at 16 / 32 / 64 rows, f32, 16 heads: 512 tokens of 128
+    // dimensions 18.5 / 17.5 / 22.4, 1024 32 / 29 / 36, 4096 224 / 181 / 170, of 64
+    // dimensions 131 / 128 / 127; of 256 512 tokens 23 / 26, 1024 52 / 46.  13
+    // sequences of 5 tokens with 24 heads of 256: 24 / 30.  64 rows of 256
+    // dimensions do not fit the registers.)
     few.rows = most_rows <= 16 ? (int)most_rows : use_many || rows <= 8192 ? 16 : c->head_dim == 256 || rows < 40000 ? 32 : 64;
     few.key_shift = 5;
     few.units = units_of(b->max_kv, 5);
+    // Items aimed for: a cut costs partial results and a join, too few leave CUs
+    // idle.  (us at 384 / 512 / 768: 64 sequences of 2000 keys of 128 dimensions 30 /
+    // 34 / 35, of 256 at 256 / 512 / 768 52 / 59 / 69.)  Fewest 32-key units of an
+    // item: one token on 8000 keys 15.5 us with 4, 14.8 with 8; 256 f32 tokens behind
+    // 4000 45.3 with 8, 44.0 with 16.
     few.target = c->head_dim == 256 ? 256 : 384;
     few.least = few.rows <= 16 ? 8 : 16;
     // beyond one a sequence and key head
@@ -1145,8 +1186,11 @@ static void attn_plans(const qhip_kv_cache* c, const qhip_kv_batch* b, int q_hea
     many.rows = kManyRows;
     many.key_shift = 6;
     many.units = units_of(b->max_kv, 6);
+    // two workgroups a CU, one where they have 256 dimensions (1021 tokens behind 5000
+    // keys of 128: 103 us with 512, 115 with 256, 140 with 768; 512 behind 8000 of 256:
+    // 156 with 256, 229 with 512)
     many.target = c->head_dim == 256 ? 256 : 512;
-    many.least = 8;
+    many.least = 8;  // 64-key units (4: 91 us, 8: 88, 16: 87 for 512 tokens behind 8000)
     plan_cut(many, many_tiles, c->head_dim);
   }
 }
