@@ -494,7 +494,8 @@ __device__ __forceinline__ void arrive_and_join(const KvAttnArgs& a, float* lds,
 constexpr int kFewRows = 64;  // rows up to which a sequence beside long ones is this kernel's
 
 template <int D, int SPLIT, int NT>
-__global__ __launch_bounds__(256, NT == 1 ? (D == 256 ? 2 : D == 128 ? 3 : 4) : (D == 256 ? 1 : 2)) void k_kv_attention_few(KvAttnArgs a) {
+__global__ __launch_bounds__(256, NT == 1 ? (D == 256 ? 2 : D == 128 ? 3 : 4) : 2)
+void k_kv_attention_few(KvAttnArgs a) {
   constexpr int J = D / 64, C = D / 16, W = D / 64;  // 64-dimension pieces, output tiles, dwords of a value load
   constexpr int R = NT * C * 4 * 64;                 // floats of a wave's output
   __shared__ __attribute__((aligned(16))) float s_o[2 * R > kJoinLds / 4 ? 2 * R : kJoinLds / 4];
