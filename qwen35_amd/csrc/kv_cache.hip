@@ -163,15 +163,16 @@ __global__ __launch_bounds__(256) void k_kv_tables(KvTablesArgs a) {
 // place of the quotient, and one multiply.
 //
 // Prompts are bound by reading the new values: 4600 f32 tokens of 4 heads of 256
-// (47 MB) 15.4 us, 3.1 TB/s.  Single tokens are bound by the chain slots - values
+// (47 MB) 12.2 us, 3.9 TB/s.  Single tokens are bound by the chain slots - values
 // - maximum - codes: 64 tokens of 8 heads of 128 in 4.5 us.
 constexpr int kAppKeep = 8;
 // One token a workgroup up to kAppFew tokens: single tokens are a run each, which
 // a wave would otherwise take in turn, a prompt's workgroups mostly find no run.
-// (us, one / 16 a workgroup, bf16 8 heads of 128: 32 single tokens 3.6 / 10.2, 256
-// 8.8 / 10.0, 512 14.9 / 11.4; a prompt of 256 6.1 / 4.8, of 1024 12.5 / 6.8)
+// (us, one / 16 a workgroup, bf16 8 heads of 128: 32 single tokens 3.7 / 9.8, 128
+// 5.9 / 11.2, 256 8.9 / 11.2, 512 15.2 / 11.3; a prompt of 32 4.3 / 4.1, of 128 7.8 /
+// 4.7, of 256 12.3 / 4.8, of 1024 45 / 5.6)
 constexpr int kAppTokens = 16;
-constexpr int kAppFew = 256;
+constexpr int kAppFew = 128;
 
 struct KvAppendArgs {
   int8_t* codes[2];
@@ -179,8 +180,7 @@ struct KvAppendArgs {
   const void* x[2];
   long token_stride[2], head_stride[2];
   const int* slots;
-  int tokens, num_slots, shift, heads, dim, tile;
-  bool near;
+  int tokens, num_slots, shift, heads, dim, tile, tiles, span;  // span: log2 of the tiles of a block
 };
 
 __device__ __forceinline__ int code8(float x, float m) {
@@ -254,8 +254,15 @@ template <typename T>
 __global__ __launch_bounds__(256) void k_kv_append(KvAppendArgs a) {
   __shared__ uint32_t s_max[4];
   const int tid = threadIdx.x, lane = tid & 63, size = 1 << a.shift;
-  const int item = a.near ? blockIdx.y : blockIdx.x;
-  const int z = a.near ? (int)blockIdx.x >= a.heads : blockIdx.z, h = a.near ? (int)blockIdx.x - z * a.heads : blockIdx.y;
+  int item = blockIdx.x, h = blockIdx.y, z = blockIdx.z;
+  if (a.tile > 1) {  // eight blocks' tiles side by side (an XCD each), of a tile all heads, keys and values
+    const unsigned parts = 2u * a.heads, at = blockIdx.x >> 3;
+    const unsigned tile = __builtin_amdgcn_readfirstlane(at / parts), part = at - tile * parts;  // (a division is a vector's)
+    item = (int)(((((tile >> a.span) << 3) + (blockIdx.x & 7)) << a.span) + (tile & ((1u << a.span) - 1)));
+    if (item >= a.tiles) return;
+    z = (int)part >= a.heads;
+    h = (int)part - z * a.heads;
+  }
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int t0 = item * a.tile;
   // the tokens of the tile that begin a run (a lane each)
@@ -372,16 +379,20 @@ extern "C" int qhip_launch_kv_append(const qhip_kv_cache* cache, int type, const
   if (rc) return rc;
   if (tokens == 0) return 0;
   const int num_slots = cache->num_blocks * cache->block_size, tile = tokens > kAppFew ? kAppTokens : 1;
-  const int tiles = (tokens - 1) / tile + 1;
+  const int tiles = (tokens - 1) / tile + 1, span = kv_block_shift(cache->block_size) - 4;
+  static_assert(kAppTokens == 16, "span");
   const KvAppendArgs a{{(int8_t*)cache->k, (int8_t*)cache->v}, {cache->k_scale, cache->v_scale}, {d_k, d_v},
                        {k_token_stride, v_token_stride}, {k_head_stride, v_head_stride}, d_slots, tokens, num_slots,
                        kv_block_shift(cache->block_size), cache->kv_heads, cache->head_dim,
-                       tile, tile > 1 && tiles <= 65535};
-  // Heads, keys and values of the same tokens side by side: their rows share
-  // pages and their power-of-two strides spread over the channels (4600 bf16
-  // tokens of 8 heads of 128: 15.4 us, 24.1 with the tokens side by side).  Single
-  // tokens the other way round (64 of 8 heads: 4.5 us against 5.8).
-  const dim3 grid = a.near ? dim3(2 * cache->kv_heads, tiles) : dim3(tiles, cache->kv_heads, 2);
+                       tile, tiles, span};
+  // An XCD takes all heads of a block's tokens: whole rows through one L2, and a
+  // run (mostly a whole block) on each of the eight.  4600 tokens, us, so / the
+  // tokens in the grid's order, whose runs fall on two XCDs / one XCD a head: bf16 8
+  // heads of 128 13.7 / 24.1 / 15.4, 4 of 256 12.8 / 21.9 / 18.8, f32 12.2 / 19.5 / 15.4.
+  // Single tokens in the grid's order (64 of 8 heads: 4.5 against 5.8 by head).
+  const long round = 8L << span, parts = 2L * cache->kv_heads, items = (tiles + round - 1) / round * round * parts;
+  if (tile > 1 && items > 0x7FFFFFFFL) return (int)hipErrorInvalidValue;
+  const dim3 grid = tile > 1 ? dim3((unsigned)items) : dim3(tiles, cache->kv_heads, 2);
   hipStream_t s = (hipStream_t)stream;
   if (type == QHIP_TT_F32) hipLaunchKernelGGL(k_kv_append<float>, grid, dim3(256), 0, s, a);
   else if (type == QHIP_TT_F16) hipLaunchKernelGGL(k_kv_append<f16_t>, grid, dim3(256), 0, s, a);
