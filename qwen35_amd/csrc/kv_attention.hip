@@ -356,8 +356,8 @@ __device__ __forceinline__ void part_store(__amdgpu_buffer_rsrc_t r, int at, con
 
 // LDS of a join: 4 KB of sums, 1 / sum of each row, m (then weights) and l of
 // rows x chunks
-constexpr int kJoinLds = 16384;
-constexpr int kJoinPairs = (kJoinLds - 4096 - 4 * 128) / 8;  // most rows x chunks
+constexpr int kJoinLds = 16384;  // least that a kernel has
+constexpr int join_pairs(int lds) { return (lds - 4096 - 4 * 128) / 8; }  // most rows x chunks
 
 // All 256 threads.  EB pieces of four values a thread and CB chunks are loaded
 // at a time; with fewer than 256 pieces the threads share out the chunks.
@@ -829,6 +829,12 @@ void k_kv_attention_few(KvAttnArgs a) {
 
 constexpr int kManyRows = 128;
 constexpr int kManyKeys = 64;
+// LDS: a tile's keys and values, and for 31 chunks of a tile or more in a join
+// (64 tokens of 16 heads of 128 behind 100,000 keys, 8 tiles: 182 us, 287 with 11)
+constexpr int many_lds(int dim) {
+  const int tile = kManyKeys * (2 * dim + 16) + dim * (2 * kManyKeys + 16);
+  return tile > 36864 ? tile : 36864;
+}
 
 template <int D>
 __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_kv_attention_many(KvAttnArgs a) {
@@ -838,9 +844,9 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_kv_attention_many(KvA
   constexpr int VW = D == 256 ? 2 : 1;       // dwords of a value row a thread stages (8 keys of 4 VW dimensions)
   constexpr int VT = 8 * (D / (4 * VW));     // threads that stage values
   constexpr int KB = 2 * D + 16, VB = 2 * kManyKeys + 16;  // bytes of a key row, of a dimension's row
-  __shared__ __attribute__((aligned(16))) uint8_t s_kv[kManyKeys * KB + D * VB];
+  __shared__ __attribute__((aligned(16))) uint8_t s_kv[many_lds(D)];
   uint8_t *const s_k = s_kv, *const s_v = s_kv + kManyKeys * KB;
-  static_assert(sizeof(s_kv) >= kJoinLds, "the join's LDS");
+  static_assert(sizeof(s_kv) >= kManyKeys * KB + D * VB && sizeof(s_kv) >= kJoinLds, "a tile's and the join's LDS");
   const int tid = threadIdx.x, lane = tid & 63, r32 = lane & 31, h = lane >> 5;
   const int wave = uniform(tid >> 6);
   Item it;
@@ -934,7 +940,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_kv_attention_many(KvA
   for (int c = 0; c < C; ++c)
 #pragma unroll
     for (int i = 0; i < 16; ++i) o[c][i] = 0.0f;
-  float m = kMinusInf, l = 0.0f;
+  float m = kMinusInf, l = 0.0f, l_before = 0.0f;  // l: of this round of tiles
   int ve = kNoScale;
 
   const uint8_t *const k_at = s_k + r32 * KB + 16 * h, *const v_at = s_v + r32 * VB + 16 * h;  // this lane's operands
@@ -943,6 +949,8 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_kv_attention_many(KvA
     if (ri == 0 && i) {
       info = next;
       next = tile_info(a, round_id((i >> 4) + 1), it.head);
+      l_before += l;  // one long sum of like terms would round the same way each time (4e-5 in 90,000 keys)
+      l = 0.0f;
     }
     __syncthreads();  // the previous tile has been read
     store_tile();
@@ -1011,6 +1019,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_kv_attention_many(KvA
       e0 = e0 > ve + kLagExp<SPLIT> ? e0 : ve;
       const float f = weight_of(m, m1), fo = __builtin_ldexpf(f, ve - e0);
       l *= f;
+      l_before *= f;
 #pragma unroll
       for (int c = 0; c < C; ++c) o[c] *= fo;
       m = m1;
@@ -1051,7 +1060,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_kv_attention_many(KvA
         }
     }
   }
-  l = sum32(l);
+  l = sum32(l_before + l);
   const float norm = l == 0.0f ? 0.0f : 1.0f / l;
 #pragma unroll
   for (int c = 0; c < C; ++c)
@@ -1152,9 +1161,10 @@ static void attn_plans(const qhip_kv_cache* c, const qhip_kv_batch* b, int q_hea
   const long work = many_tiles * units_of(window > 0 && window < b->max_kv ? window : b->max_kv, 6);
   // (us, few-row / many-row kernel, bf16, 16 heads on 4: 2048 tokens of 128 48 / 57,
   // 4096 129 / 127, of 256 100 / 116 and 321 / 242; 512 tokens behind 8000 keys of 128
-  // 97 / 87, 256 behind 4000 37 / 51; of 64 512 behind 8000 66 / 51, 8192 tokens 288 /
+  // 97 / 87, 256 behind 4000 37 / 51; 256 behind 30,000 of 256 337 / 254, 64 behind
+  // 100,000 332 / 349; of 64 512 behind 8000 66 / 51, 8192 tokens 288 /
   // 262, but 4096 87 / 95, whose 512 uneven tiles are one round of workgroups.)
-  const bool use_many = !f32 && most_rows > kFewRows && work >= (c->head_dim == 256 ? 20000 : 8500);
+  const bool use_many = !f32 && most_rows > kFewRows && work >= (c->head_dim == 256 ? 12000 : 8500);
   // where the sequences are half as long as the longest on average, what single
   // tokens there may be are few beside the tiles of the others, and a launch
   // that mostly finds no sequence costs 3 to 4 us
@@ -1276,7 +1286,7 @@ extern "C" int qhip_launch_kv_attention(const qhip_kv_cache* cache, const qhip_k
     a.share = (float)cache->kv_heads / (float)p.target * 1.00001f;
     a.least = p.least;
     a.max_units = p.units;
-    a.max_chunks = kJoinPairs / p.rows;
+    a.max_chunks = join_pairs(i == 0 ? kJoinLds : many_lds(cache->head_dim)) / p.rows;
     a.slots = a.cut ? (p.work - kCountBytes) / ((long)p.rows * (cache->head_dim + 2) * 4) : 0;
     const unsigned grid = (unsigned)(a.cut ? p.cut_grid : p.grid);
     if (i == 0) launch_few(a, cache->head_dim, type == QHIP_TT_F32, p.rows > 16, grid, (hipStream_t)stream);

@@ -70,6 +70,13 @@ def test_scales_of_queries_values_and_softmax(gpu, dtype):
     assert torch.equal(torch.isfinite(lse), torch.isfinite(want[1]))
 
 
+@pytest.mark.parametrize("dtype", t.DTYPES)
+@pytest.mark.parametrize("dim,lens", [(64, [(90000, 40)]), (128, [(90000, 40), (70, 9)]), (256, [(150000, 60)])])
+def test_few_tiles_on_many_keys(gpu, dim, lens, dtype):
+    """As many chunks of a row tile as a join takes."""
+    t.check(lens, 2, 8, 64, dim, dtype, seed=dim)
+
+
 @pytest.mark.parametrize("odd", [math.nan, math.inf])
 def test_poisoned_blocks_reach_their_rows_only(gpu, odd):
     lens = [(4000, 1500), (3000, 700)]
