@@ -498,9 +498,10 @@ __global__ __launch_bounds__(256, NT == 1 ? (D == 256 ? 2 : D == 128 ? 3 : 4) : 
 void k_kv_attention_few(KvAttnArgs a) {
   constexpr int J = D / 64, C = D / 16, W = D / 64;  // 64-dimension pieces, output tiles, dwords of a value load
   constexpr int R = NT * C * 4 * 64;                 // floats of a wave's output
-  __shared__ __attribute__((aligned(16))) float s_o[2 * R > kJoinLds / 4 ? 2 * R : kJoinLds / 4];
-  __shared__ float s_m[2][NT][64], s_l[2][NT][64];
-  __shared__ int s_e[2][NT][64];
+  __shared__ __attribute__((aligned(16))) float s_o[4 * R];
+  static_assert(sizeof(s_o) >= kJoinLds, "the join's LDS");
+  __shared__ float s_m[4][NT][64], s_l[4][NT][64];
+  __shared__ int s_e[4][NT][64];
   const int tid = threadIdx.x, lane = tid & 63, r16 = lane & 15, g = lane >> 4;
   const int wave = uniform(tid >> 6);
   Item it;
@@ -515,21 +516,17 @@ void k_kv_attention_few(KvAttnArgs a) {
   const int id0 = round_id();
 
   // this lane's rows
-  int row[NT], t[NT], qh[NT], vis_hi[NT], vis_lo[NT];
-  bool live[NT];
+  int vis_hi[NT], vis_lo[NT];
   QRaw<SPLIT> raw[NT][2 * J] = {};
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
-    row[nt] = ((wave % tiles) * NT + nt) * 16 + r16;
-    const RowAt w = row_at(a, sp, row[nt] < sp.rows ? row[nt] : 0, it.head);
-    const int p = sp.first + w.tok;
-    t[nt] = it.off + w.tok;
-    qh[nt] = w.head;
-    live[nt] = row[nt] < sp.rows && t[nt] >= 0 && t[nt] < a.tokens;
+    const int row = ((wave % tiles) * NT + nt) * 16 + r16;
+    const RowAt w = row_at(a, sp, row < sp.rows ? row : 0, it.head);
+    const int p = sp.first + w.tok, t = it.off + w.tok;
     vis_hi[nt] = min(a.causal ? p + 1 : it.len, sp.key1);  // of this chunk
     vis_lo[nt] = a.window > 0 ? p - a.window + 1 : 0;
-    if (live[nt]) {
-      const long at = (long)t[nt] * a.q_token + (long)w.head * a.q_head + 16 * g;
+    if (row < sp.rows && t >= 0 && t < a.tokens) {
+      const long at = (long)t * a.q_token + (long)w.head * a.q_head + 16 * g;
 #pragma unroll
       for (int i = 0; i < 2 * J; ++i) raw[nt][i] = load8((const QElem<SPLIT>*)a.q + at + 64 * (i >> 1) + 8 * (i & 1));
     }
@@ -546,9 +543,9 @@ void k_kv_attention_few(KvAttnArgs a) {
   kv_u32x4 kr[2][J];
   uint32_t vr[8][W];
   auto tile_at = [&](int i) {  // byte offset of tile i's first code
-    const long b = __builtin_amdgcn_readlane(info.id, i);
-    const int first = (sp.key0 + 32 * (s0 + parts * (i >> 1)) + 16 * (i & 1)) & mask;
-    return ((b * a.kv_heads + it.head) << a.shift | first) * D;
+    const uint64_t b = (uint32_t)__builtin_amdgcn_readlane(info.id, i);
+    const unsigned first = (sp.key0 + 32 * (s0 + parts * (i >> 1)) + 16 * (i & 1)) & mask;
+    return ((b * (uint32_t)a.kv_heads + (uint32_t)it.head) << a.shift | first) * D;
   };
   auto load_k = [&](int st) {
 #pragma unroll
@@ -600,6 +597,40 @@ void k_kv_attention_few(KvAttnArgs a) {
     for (int c = 0; c < C; ++c) o[nt][c] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
   }
 
+  // a wave's results into its part of the LDS, and those of a wave's part added to this one's
+  // (the lane counted anew, here and for the results: what is kept over the loop spills)
+  auto lane_here = [&]() { return (int)__builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, (unsigned)here(0))); };
+  auto give = [&]() {
+    const int lane = lane_here();
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+      for (int c = 0; c < C; ++c)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) s_o[wave * R + ((nt * C + c) * 4 + r) * 64 + lane] = o[nt][c][r];
+      s_m[wave][nt][lane] = m[nt];
+      s_l[wave][nt][lane] = l[nt];
+      s_e[wave][nt][lane] = ve[nt];
+    }
+  };
+  auto take = [&](int from) {
+    const int lane = lane_here();
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const float m2 = s_m[from][nt][lane], top = fmaxf(m[nt], m2);
+      const int ve2 = s_e[from][nt][lane], e = max(ve[nt], ve2);
+      const float f1 = weight_of(m[nt], top), f2 = weight_of(m2, top);
+      const float g1 = __builtin_ldexpf(f1, ve[nt] - e), g2 = __builtin_ldexpf(f2, ve2 - e);
+#pragma unroll
+      for (int c = 0; c < C; ++c)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) o[nt][c][r] = o[nt][c][r] * g1 + s_o[from * R + ((nt * C + c) * 4 + r) * 64 + lane] * g2;
+      l[nt] = l[nt] * f1 + s_l[from][nt][lane] * f2;
+      m[nt] = top;
+      ve[nt] = e;
+    }
+  };
+  bool aside = false;  // results of earlier rounds wait in the LDS
   while (any) {
     const int steps = min(32, (sp.key1 - sp.key0 - 32 * s0 + 32 * parts - 1) / (32 * parts));
     for (int st = 0; st < steps; ++st) {
@@ -714,7 +745,22 @@ void k_kv_attention_few(KvAttnArgs a) {
       if (st + 1 < steps) load_v(st + 1);
     }
     s0 += 32 * parts;
-    if (sp.key0 + 32 * s0 >= sp.key1) break;
+    const bool more = sp.key0 + 32 * s0 < sp.key1;
+    // One long sum of like terms would round the same way each time (1.2e-4 of an
+    // output in 131,072 keys, now 2e-6): two rounds are summed by themselves and then
+    // added to what waits in the LDS.
+    if (!more || !((s0 >> 5) & parts)) {
+      if (aside) take(wave);
+      if (!more) break;
+      give();
+      aside = true;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        l[nt] = 0.0f;
+#pragma unroll
+        for (int c = 0; c < C; ++c) o[nt][c] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+      }
+    }
     info = tile_info(a, round_id(), it.head);
     load_k(0);
     load_v(0);
@@ -724,37 +770,10 @@ void k_kv_attention_few(KvAttnArgs a) {
 
   // merge the waves that share a row tile: the upper half of the parts into the lower
   for (int half = parts / 2; half >= 1; half >>= 1) {
-    const int slot = wave - half * tiles;  // waves [half * tiles, 2 half * tiles) give
-    if (slot >= 0 && slot < half * tiles) {
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-#pragma unroll
-        for (int c = 0; c < C; ++c)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) s_o[slot * R + ((nt * C + c) * 4 + r) * 64 + lane] = o[nt][c][r];
-        s_m[slot][nt][lane] = m[nt];
-        s_l[slot][nt][lane] = l[nt];
-        s_e[slot][nt][lane] = ve[nt];
-      }
-    }
+    const int at = wave - half * tiles;  // waves [half * tiles, 2 half * tiles) give
+    if (at >= 0 && at < half * tiles) give();
     __syncthreads();
-    if (wave < half * tiles) {
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        const float m2 = s_m[wave][nt][lane], top = fmaxf(m[nt], m2);
-        const int ve2 = s_e[wave][nt][lane], e = max(ve[nt], ve2);
-        const float f1 = weight_of(m[nt], top), f2 = weight_of(m2, top);
-        const float g1 = __builtin_ldexpf(f1, ve[nt] - e), g2 = __builtin_ldexpf(f2, ve2 - e);
-#pragma unroll
-        for (int c = 0; c < C; ++c)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) o[nt][c][r] = o[nt][c][r] * g1 + s_o[wave * R + ((nt * C + c) * 4 + r) * 64 + lane] * g2;
-        l[nt] = l[nt] * f1 + s_l[wave][nt][lane] * f2;
-        m[nt] = top;
-        ve[nt] = e;
-      }
-    }
-    __syncthreads();
+    if (at < 0) take(wave + half * tiles);
   }
 
 #pragma unroll
@@ -766,11 +785,15 @@ void k_kv_attention_few(KvAttnArgs a) {
 #pragma unroll
       for (int r = 0; r < 4; ++r) o[nt][c][r] = in_units<SPLIT>(o[nt][c][r] * norm, ve[nt]);
   }
+  const int lane_end = lane_here(), g_end = lane_end >> 4, row_end = (wave % tiles) * NT * 16 + (lane_end & 15);
   if (it.chunks == 1) {
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
-      if (wave < tiles && live[nt]) {
-        const long at = (long)t[nt] * a.out_token + (long)qh[nt] * a.out_head + 4 * g * C;
+    for (int nt = 0; nt < NT; ++nt) {
+      const int row = row_end + 16 * nt;
+      const RowAt w = row_at(a, sp, row < sp.rows ? row : 0, it.head);
+      const int t = it.off + w.tok;
+      if (wave < tiles && row < sp.rows && t >= 0 && t < a.tokens) {
+        const long at = (long)t * a.out_token + (long)w.head * a.out_head + 4 * g_end * C;
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           float v[C];
@@ -778,8 +801,9 @@ void k_kv_attention_few(KvAttnArgs a) {
           for (int c = 0; c < C; ++c) v[c] = o[nt][c][r];
           store_row<SPLIT, C>(a.out, at + r * C, a.type, v);
         }
-        if (a.lse && g == 0) a.lse[(long)t[nt] * a.q_heads + qh[nt]] = row_lse(m[nt], l[nt]);
+        if (a.lse && g_end == 0) a.lse[(long)t * a.q_heads + w.head] = row_lse(m[nt], l[nt]);
       }
+    }
     return;
   }
   if (it.slot + it.chunks > a.slots || it.counter >= kMaxCut) return;  // offsets or lengths that are none
@@ -787,16 +811,17 @@ void k_kv_attention_few(KvAttnArgs a) {
   const __amdgpu_buffer_rsrc_t parts_at = part_rsrc(a.partial + (long)it.slot * stride, (long)it.chunks * stride);
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt)
-    if (wave < tiles && row[nt] < sp.rows) {
+    if (wave < tiles && row_end + 16 * nt < sp.rows) {
+      const int row = row_end + 16 * nt;
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         float v[C];
 #pragma unroll
         for (int c = 0; c < C; ++c) v[c] = o[nt][c][r];
-        part_store<C>(parts_at, it.chunk * stride + row[nt] * D + (4 * g + r) * C, v);
+        part_store<C>(parts_at, it.chunk * stride + row * D + (4 * g_end + r) * C, v);
       }
       const float stat[2] = {m[nt], l[nt]};
-      if (g == 0) part_store<2>(parts_at, it.chunk * stride + a.tile_rows * D + 2 * row[nt], stat);
+      if (g_end == 0) part_store<2>(parts_at, it.chunk * stride + a.tile_rows * D + 2 * row, stat);
     }
   arrive_and_join<D, SPLIT>(a, s_o, parts_at, it, sp);
 }
