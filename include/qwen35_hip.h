@@ -394,8 +394,9 @@ typedef struct qhip_kv_cache {
  *   d_offsets   [nseq + 1] prefix sums of d_new: the packed tokens' order
  *   d_kv_lens   [nseq] cached + new
  *   d_slots     [tokens] block * block_size + place in the block of each packed
- *               token; -1 where no block was left or the row of the table is too
- *               short, and for tokens at or past the sum of d_new (a batch that
+ *               token; -1 where no block was left, the row of the table is too
+ *               short or its entry is no block (negative, or too large for a slot
+ *               below 2^31), and for tokens at or past the sum of d_new (a batch that
  *               is padded to `tokens`)
  *   d_positions [tokens] (nullable) each token's place in its sequence, 0 for padding
  *   d_taken_out the free-list entries taken, these included: more than nfree

@@ -112,7 +112,8 @@ __global__ __launch_bounds__(256) void k_kv_tables(KvTablesArgs a) {
           else if ((unsigned)at < (unsigned)a.nfree)
             entry = a.free_list[at];
         }
-        slot[k] = entry >= 0 ? (entry << a.shift) | (p & mask) : -1;
+        // (a larger id is outside every pool, and its slot would not fit 31 bits)
+        slot[k] = (unsigned)entry <= 0x7FFFFFFFu >> a.shift ? (entry << a.shift) | (p & mask) : -1;
         place[k] = p;
       }
       typedef int int4_a4 __attribute__((ext_vector_type(4), aligned(4)));
