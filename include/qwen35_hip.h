@@ -401,7 +401,7 @@ typedef struct qhip_kv_cache {
  *   d_positions [tokens] (nullable) each token's place in its sequence, 0 for padding
  *   d_taken_out the free-list entries taken, these included: more than nfree
  *               says that blocks were short
- * Outputs must not overlap inputs, d_table apart. */
+ * The arrays must not overlap (hipErrorInvalidValue). */
 int qhip_launch_kv_tables(const int *d_cached, const int *d_new, int nseq, const int *d_free, int nfree,
                           const int *d_taken, int block_size, int *d_table, int table_width, int tokens,
                           int *d_offsets, int *d_kv_lens, int *d_slots, int *d_positions, int *d_taken_out,

@@ -339,7 +339,13 @@ __global__ __launch_bounds__(256) void k_kv_read(KvReadArgs a) {
 
 using namespace qhip;
 
-static bool overlap(const int* a, int na, const int* b, int nb) { return a && b && a < b + nb && b < a + na; }
+struct Ints {
+  const int* at;
+  long n;
+};
+static bool overlap(const Ints& a, const Ints& b) {
+  return a.at && b.at && a.n > 0 && b.n > 0 && a.at < b.at + b.n && b.at < a.at + a.n;
+}
 
 extern "C" int qhip_launch_kv_tables(const int* d_cached, const int* d_new, int nseq, const int* d_free, int nfree,
                                      const int* d_taken, int block_size, int* d_table, int table_width, int tokens,
@@ -351,11 +357,17 @@ extern "C" int qhip_launch_kv_tables(const int* d_cached, const int* d_new, int 
       (nseq > 0 && table_width > 0 && !d_table) || (tokens > 0 && !d_slots))
     return (int)hipErrorInvalidValue;
   // (an output in an input's place would be read by workgroups that start later)
-  const struct { const int* at; int n; } in[] = {{d_cached, nseq}, {d_new, nseq}, {d_taken, 1}, {d_free, nfree}},
-                                         out[] = {{d_offsets, nseq + 1}, {d_kv_lens, nseq}, {d_taken_out, 1}};
-  for (const auto& x : in)
-    for (const auto& y : out)
-      if (overlap(x.at, x.n, y.at, y.n)) return (int)hipErrorInvalidValue;
+  const Ints table{d_table, (long)nseq * table_width}, in[] = {{d_cached, nseq}, {d_new, nseq}, {d_taken, 1}, {d_free, nfree}},
+             out[] = {{d_offsets, nseq + 1L}, {d_kv_lens, nseq}, {d_slots, tokens}, {d_positions, tokens}, {d_taken_out, 1}};
+  for (const Ints& x : in)
+    if (overlap(x, table)) return (int)hipErrorInvalidValue;
+  for (const Ints& y : out) {
+    for (const Ints& x : in)
+      if (overlap(x, y)) return (int)hipErrorInvalidValue;
+    for (const Ints& z : out)
+      if (&z != &y && overlap(z, y)) return (int)hipErrorInvalidValue;
+    if (overlap(table, y)) return (int)hipErrorInvalidValue;
+  }
   // every workgroup walks all sequences, so the grid follows the tokens; the
   // fresh blocks number at most tokens / block_size + nseq
   // (four tokens a thread share a search and 16-byte stores: 100,000 tokens of
