@@ -459,9 +459,8 @@ __device__ __forceinline__ void arrive_and_join(const KvAttnArgs& a, float* lds,
 
 // ---- sequences of a few rows: the cache streamed once ------------------------------
 //
-// Row tiles of 16 (NT = 2: pairs of them in a wave, 32 rows on each step's codes),
-// up to four a workgroup.  The work is one pass over the
-// codes, 2 D bytes a key, so the kernel is built to keep loads in flight and
+// A wave has 16 rows (NT = 2: two times 16, on each step's codes), a workgroup that
+// many or twice as many (attn_plans).  The work is one pass over the codes, 2 D bytes a key, so the kernel is built to keep loads in flight and
 // never puts a code anywhere but in a register:
 //
 //   S^T = K Q^T   16 keys x 16 rows a v_mfma_f32_16x16x32_f16; lane 16 g + i
@@ -478,9 +477,9 @@ __device__ __forceinline__ void arrive_and_join(const KvAttnArgs& a, float* lds,
 // bits; f16 and bf16 rows, whose outputs are rounded to 11 and 8 bits, weights of
 // 11.  A block's key scale multiplies the scores, its value scale the weights.
 //
-// A workgroup's four waves take steps of 32 keys in turn (one, two or four row
-// tiles share a step's waves) and are merged in LDS.  Long sequences are cut
-// into chunks over workgroups (find_item).
+// A workgroup's four waves take steps of 32 keys in turn (with twice a wave's rows,
+// two and two of them) and are merged in LDS.  Long sequences are cut into chunks
+// over workgroups (find_item).
 //
 // Bound by memory where sequences are long: one f32 token on 131071 keys (4 key
 // heads of 256, 268 MB) 60 us, 4.5 TB/s; 64 tokens on 2000 keys each, 53 us at 4.9
@@ -507,8 +506,7 @@ void k_kv_attention_few(KvAttnArgs a) {
   Item it;
   if (!find_item(a, lane, it)) return;  // all four waves alike
   const Span sp = find_span(a, it);
-  const int tiles = sp.rows <= 16 * NT ? 1 : sp.rows <= 32 * NT ? 2 : 4;
-  const int part = wave / tiles, parts = 4 / tiles;
+  const int tiles = sp.rows <= 16 * NT ? 1 : 2, part = wave / tiles, parts = 4 / tiles;
 
   // lane i: tile i & 1 of this wave's step i / 2 of a round of 32 steps
   int s0 = part;
@@ -1202,7 +1200,8 @@ static void attn_plans(const qhip_kv_cache* c, const qhip_kv_batch* b, int q_hea
     // dimensions 18.5 / 17.5 / 22.4, 1024 32 / 29 / 36, 4096 224 / 181 / 170, of 64
     // dimensions 131 / 128 / 127; of 256 512 tokens 23 / 26, 1024 52 / 46.  13
     // sequences of 5 tokens with 24 heads of 256: 24 / 30.  64 rows of 256
-    // dimensions do not fit the registers.)
+    // dimensions do not fit the registers.)  Twice a wave's rows at most: 32 of 256
+    // dimensions, and beyond 16 (pairs) 64 of fewer.
     few.rows = most_rows <= 16 ? (int)most_rows : use_many || rows <= 8192 ? 16 : c->head_dim == 256 || rows < 40000 ? 32 : 64;
     few.key_shift = 5;
     few.units = units_of(b->max_kv, 5);
