@@ -423,6 +423,8 @@ def kv_attention(q: torch.Tensor, cache: KvCache, table: torch.Tensor, offsets: 
         lse = torch.empty((tokens, heads), dtype=torch.float32, device=q.device)
     elif lse.dtype != torch.float32 or lse.shape != (tokens, heads) or not lse.is_contiguous() or not lse.is_cuda:
         raise ValueError("lse: f32 [tokens, q_heads]")
+    if work is not None and (work.dtype != torch.uint8 or work.dim() != 1 or not work.is_cuda or not work.is_contiguous()):
+        raise ValueError("work: a contiguous uint8 GPU tensor (kv_attention_work)")
     b = QhipKvBatch(_ints("offsets", offsets), _ints("kv_lens", kv_lens), _ints("table", table, 2), nseq, tokens, max_new,
                     max_kv, table.shape[1])
     check("kv_attention", load().qhip_launch_kv_attention(
