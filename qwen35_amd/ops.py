@@ -365,8 +365,11 @@ def kv_tables(cached: torch.Tensor, new: torch.Tensor, free: torch.Tensor, table
     rows, width = table.shape
     if cached.shape[0] != nseq or new.shape[0] != nseq or rows != nseq:
         raise ValueError(f"cached, new, table: {nseq} sequences")
+    at = None if taken is None else _ints("taken", taken)
+    if taken is not None and taken.shape != (1,):
+        raise ValueError("taken: one entry")
     check("kv_tables", load().qhip_launch_kv_tables(
-        c, n, nseq, f, free.shape[0], None if taken is None else _ints("taken", taken), block_size, t, width, step.tokens,
+        c, n, nseq, f, free.shape[0], at, block_size, t, width, step.tokens,
         step.offsets.data_ptr(), step.kv_lens.data_ptr(), step.slots.data_ptr(), step.positions.data_ptr(),
         step.taken.data_ptr(), _stream()))
     return step

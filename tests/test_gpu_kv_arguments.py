@@ -3,6 +3,7 @@ import pytest
 import torch
 
 import test_gpu_kv_attention as t
+import test_gpu_kv_cache as c
 from qwen35_amd import ops
 
 pytestmark = pytest.mark.gpu
@@ -17,3 +18,11 @@ def test_work_is_a_byte_tensor_on_the_gpu(gpu):
             ops.kv_attention(*args, work=bad)
     ops.kv_attention(*args, work=work)
     assert not bool(work[:32768].any())
+
+
+def test_taken_has_one_entry(gpu):
+    """No entry would count as none taken, and read nothing."""
+    step = ops.KvStep(2, 4)
+    for bad in (c.ints([]), c.ints([1, 2]), c.ints([[1]]), torch.tensor([1], device="cuda"), torch.tensor([1], dtype=torch.int32)):
+        with pytest.raises(ValueError):
+            ops.kv_tables(c.ints([0, 0]), c.ints([2, 2]), c.ints([4, 5, 6]), c.ints([[0], [0]]), 16, step, taken=bad)
