@@ -316,20 +316,29 @@ def _kv_rows(name: str, t: torch.Tensor, dim: int) -> int:
 
 
 class KvCache:
-    """One layer's keys and values: int8 [blocks, kv_heads, block_size, head_dim] with f32 scales [blocks, kv_heads]."""
+    """One layer's keys and values: int8 [blocks, kv_heads, block_size, head_dim] with f32 scales [blocks, kv_heads].
+    Tensors of the same sizes may be put in their place (they are checked when they are set); the sizes are fixed."""
 
     def __init__(self, k: torch.Tensor, v: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor):
-        for t in (k, v):
-            if t.dtype != torch.int8 or t.dim() != 4 or t.shape != k.shape or not t.is_cuda or not t.is_contiguous():
-                raise ValueError("k, v: contiguous int8 GPU tensors [blocks, kv_heads, block_size, head_dim]")
-        for t in (k_scale, v_scale):
-            if t.dtype != torch.float32 or t.shape != k.shape[:2] or not t.is_cuda or not t.is_contiguous():
-                raise ValueError("k_scale, v_scale: contiguous f32 GPU tensors [blocks, kv_heads]")
-        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
-        self.num_blocks, self.kv_heads, self.block_size, self.head_dim = k.shape
-        self._c = QhipKvCache(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), self.num_blocks,
-                              self.block_size, self.kv_heads, self.head_dim)
+        sizes = k.shape if k.dim() == 4 else (0, 0, 0, 0)
+        self._c = QhipKvCache(None, None, None, None, sizes[0], sizes[2], sizes[1], sizes[3])
         self._ref = ctypes.byref(self._c)
+        self.__dict__.update(zip(("num_blocks", "kv_heads", "block_size", "head_dim"), sizes))
+        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+
+    def __setattr__(self, name, value):
+        if name in ("num_blocks", "kv_heads", "block_size", "head_dim"):
+            raise AttributeError(f"{name}: fixed (another KvCache has other sizes)")
+        if name in ("k", "v", "k_scale", "v_scale"):
+            dtype, shape = torch.int8, (self.num_blocks, self.kv_heads, self.block_size, self.head_dim)
+            if name in ("k_scale", "v_scale"):
+                dtype, shape = torch.float32, shape[:2]
+            if (not isinstance(value, torch.Tensor) or value.dtype != dtype or value.shape != shape or not value.is_cuda
+                    or not value.is_contiguous()):
+                raise ValueError("k, v: contiguous int8 GPU tensors [blocks, kv_heads, block_size, head_dim]; "
+                                 "k_scale, v_scale: contiguous f32 GPU tensors [blocks, kv_heads]")
+            setattr(self._c, name, value.data_ptr())
+        super().__setattr__(name, value)
 
     @classmethod
     def empty(cls, num_blocks: int, kv_heads: int, block_size: int, head_dim: int, device="cuda") -> "KvCache":

@@ -7,6 +7,7 @@ import test_gpu_kv_cache as c
 from qwen35_amd import ops
 
 pytestmark = pytest.mark.gpu
+FIELDS = ("k", "v", "k_scale", "v_scale")
 
 
 def test_work_is_a_byte_tensor_on_the_gpu(gpu):
@@ -26,3 +27,34 @@ def test_taken_has_one_entry(gpu):
     for bad in (c.ints([]), c.ints([1, 2]), c.ints([[1]]), torch.tensor([1], device="cuda"), torch.tensor([1], dtype=torch.int32)):
         with pytest.raises(ValueError):
             ops.kv_tables(c.ints([0, 0]), c.ints([2, 2]), c.ints([4, 5, 6]), c.ints([[0], [0]]), 16, step, taken=bad)
+
+
+def test_tensors_put_in_a_caches_place_are_the_ones_used(gpu):
+    cache, other = c.pool(3, 2, 16, 64), c.pool(3, 2, 16, 64, seed=1)
+    old = [getattr(cache, n).clone() for n in FIELDS]
+    kept = [getattr(cache, n) for n in FIELDS]
+    want = c.pool(3, 2, 16, 64, seed=1)
+    for name in FIELDS:
+        setattr(cache, name, getattr(other, name))
+    kv = torch.randn((2, 3, 2, 64), device="cuda")
+    slots = c.ints([16, 17, 18])
+    ops.kv_append(want, kv[0], kv[1], slots)
+    ops.kv_append(cache, kv[0], kv[1], slots)
+    assert all(torch.equal(getattr(other, n), getattr(want, n)) for n in FIELDS)
+    assert all(torch.equal(a, b) for a, b in zip(old, kept))
+
+
+def test_what_does_not_fit_a_cache_is_refused(gpu):
+    cache = c.pool(3, 2, 16, 64)
+    before = [getattr(cache, n).data_ptr() for n in FIELDS]
+    for name, bad in [("k", cache.k.float()), ("k", cache.k[:2]), ("v", cache.v.cpu()), ("v", cache.v.transpose(0, 1)), ("k", None),
+                      ("k_scale", cache.k_scale[:2]), ("v_scale", cache.v_scale.double()), ("v_scale", cache.v_scale.t())]:
+        with pytest.raises(ValueError):
+            setattr(cache, name, bad)
+    for name in ("num_blocks", "kv_heads", "block_size", "head_dim"):
+        with pytest.raises(AttributeError):
+            setattr(cache, name, 1)
+    assert before == [getattr(cache, n).data_ptr() for n in FIELDS]
+    for bad in ((cache.k[0], cache.v[0]), (cache.k.cpu(), cache.v)):
+        with pytest.raises(ValueError):
+            ops.KvCache(*bad, cache.k_scale, cache.v_scale)
