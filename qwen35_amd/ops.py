@@ -349,19 +349,25 @@ class KvCache:
 
 class KvStep:
     """What kv_tables writes for a step of `nseq` sequences and `tokens` packed tokens: offsets [nseq + 1], kv_lens
-    [nseq], slots and positions [tokens], taken [1].  Tensors put in their place are checked once, when they are set."""
+    [nseq], slots and positions [tokens], taken [1].  Tensors put in their place are checked once, when they are set; the
+    sizes are fixed."""
 
     def __init__(self, nseq: int, tokens: int, device="cuda"):
-        self.nseq, self.tokens = nseq, tokens
-        for name, n in (("offsets", nseq + 1), ("kv_lens", nseq), ("slots", tokens), ("positions", tokens), ("taken", 1)):
+        self.__dict__.update(nseq=nseq, tokens=tokens)
+        for name, n in self._entries().items():
             setattr(self, name, torch.empty(n, dtype=torch.int32, device=device))
 
+    def _entries(self) -> dict[str, int]:
+        return {"offsets": self.nseq + 1, "kv_lens": self.nseq, "slots": self.tokens, "positions": self.tokens, "taken": 1}
+
     def __setattr__(self, name, value):
-        if isinstance(value, torch.Tensor):
-            n = {"offsets": self.nseq + 1, "kv_lens": self.nseq, "taken": 1}.get(name, self.tokens)
-            _ints(name, value)
-            if value.shape != (n,):
+        if name in ("nseq", "tokens"):
+            raise AttributeError(f"{name}: fixed (another KvStep has other sizes)")
+        n = self._entries().get(name)
+        if n is not None:
+            if not isinstance(value, torch.Tensor) or value.shape != (n,):
                 raise ValueError(f"{name}: {n} entries")
+            _ints(name, value)
         super().__setattr__(name, value)
 
 

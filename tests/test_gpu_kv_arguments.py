@@ -58,3 +58,16 @@ def test_what_does_not_fit_a_cache_is_refused(gpu):
     for bad in ((cache.k[0], cache.v[0]), (cache.k.cpu(), cache.v)):
         with pytest.raises(ValueError):
             ops.KvCache(*bad, cache.k_scale, cache.v_scale)
+
+
+def test_a_steps_sizes_are_fixed(gpu):
+    """The kernel writes as many entries as the step says."""
+    step = ops.KvStep(2, 4)
+    for name in ("nseq", "tokens"):
+        with pytest.raises(AttributeError):
+            setattr(step, name, 100)
+    step.slots = c.ints([0] * 4)
+    for name, bad in (("slots", c.ints([0] * 3)), ("offsets", c.ints([0] * 2)), ("taken", c.ints([])), ("kv_lens", None)):
+        with pytest.raises(ValueError):
+            setattr(step, name, bad)
+    assert (step.nseq, step.tokens) == (2, 4)
