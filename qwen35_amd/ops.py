@@ -20,9 +20,9 @@ _NINTS_32 = {3: 2}
 _NINTS_SB = {12: 2, 13: 2, 10: 2, 23: 8, 18: 8, 21: 8}
 
 
-def _stream() -> ctypes.c_void_p:
-    """The current torch stream's handle (torch.cuda.current_stream builds a stream object first: 2.8 us a call)."""
-    return ctypes.c_void_p(torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice()))
+def _stream(device: int | None = None) -> ctypes.c_void_p:
+    """The current stream's handle on the current device (torch.cuda.current_stream builds a stream object first: 2.8 us)."""
+    return ctypes.c_void_p(torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if device is None else device))
 
 
 def _p(t: torch.Tensor) -> ctypes.c_void_p:
@@ -302,17 +302,28 @@ def mul_mat_ragged(ttype: int, w: torch.Tensor, xq: torch.Tensor, off_d: torch.T
 _KV_TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 30}
 
 
-def _ints(name: str, t: torch.Tensor, dims: int = 1) -> int:
-    if t.dtype != torch.int32 or t.dim() != dims or not t.is_cuda or not t.is_contiguous():
-        raise ValueError(f"{name}: a contiguous int32 GPU tensor of {dims} dimension(s)")
+# Launches go to the current device's stream, so a call's tensors have to lie on that device.
+
+def _ints(name: str, t: torch.Tensor, device: int, dims: int = 1) -> int:
+    if t.dtype != torch.int32 or t.dim() != dims or t.get_device() != device or not t.is_contiguous():
+        raise ValueError(f"{name}: a contiguous int32 tensor of {dims} dimension(s) on the current GPU")
     return t.data_ptr()
 
 
-def _kv_rows(name: str, t: torch.Tensor, dim: int) -> int:
+def _kv_rows(name: str, t: torch.Tensor, dim: int, device: int) -> int:
     """The GGUF type id of token rows [tokens, heads, dim] whose last dimension is contiguous."""
-    if t.dim() != 3 or t.shape[2] != dim or t.stride(2) != 1 or not t.is_cuda or t.dtype not in _KV_TYPES:
-        raise ValueError(f"{name}: a GPU tensor [tokens, heads, {dim}] of f32, f16 or bf16 with contiguous heads")
+    if t.dim() != 3 or t.shape[2] != dim or t.stride(2) != 1 or t.get_device() != device or t.dtype not in _KV_TYPES:
+        raise ValueError(f"{name}: a tensor [tokens, heads, {dim}] of f32, f16 or bf16 with contiguous heads on the current GPU")
     return _KV_TYPES[t.dtype]
+
+
+def _kv_device(*owners) -> int:
+    """The current device, on which the tensors of a cache or a step lie."""
+    device = torch.cuda.current_device()
+    for x in owners:
+        if x._device != device:
+            raise ValueError(f"{type(x).__name__}: on device {x._device}, the current one is {device}")
+    return device
 
 
 class KvCache:
@@ -323,7 +334,7 @@ class KvCache:
         sizes = k.shape if k.dim() == 4 else (0, 0, 0, 0)
         self._c = QhipKvCache(None, None, None, None, sizes[0], sizes[2], sizes[1], sizes[3])
         self._ref = ctypes.byref(self._c)
-        self.__dict__.update(zip(("num_blocks", "kv_heads", "block_size", "head_dim"), sizes))
+        self.__dict__.update(zip(("num_blocks", "kv_heads", "block_size", "head_dim"), sizes), _device=k.get_device())
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
 
     def __setattr__(self, name, value):
@@ -334,9 +345,9 @@ class KvCache:
             if name in ("k_scale", "v_scale"):
                 dtype, shape = torch.float32, shape[:2]
             if (not isinstance(value, torch.Tensor) or value.dtype != dtype or value.shape != shape or not value.is_cuda
-                    or not value.is_contiguous()):
-                raise ValueError("k, v: contiguous int8 GPU tensors [blocks, kv_heads, block_size, head_dim]; "
-                                 "k_scale, v_scale: contiguous f32 GPU tensors [blocks, kv_heads]")
+                    or value.get_device() != self._device or not value.is_contiguous()):
+                raise ValueError("k, v: contiguous int8 tensors [blocks, kv_heads, block_size, head_dim], k_scale, v_scale: "
+                                 "f32 ones [blocks, kv_heads], all on one GPU")
             setattr(self._c, name, value.data_ptr())
         super().__setattr__(name, value)
 
@@ -355,7 +366,9 @@ class KvStep:
     def __init__(self, nseq: int, tokens: int, device="cuda"):
         self.__dict__.update(nseq=nseq, tokens=tokens)
         for name, n in self._entries().items():
-            setattr(self, name, torch.empty(n, dtype=torch.int32, device=device))
+            t = torch.empty(n, dtype=torch.int32, device=device)
+            self.__dict__.setdefault("_device", t.get_device())
+            setattr(self, name, t)
 
     def _entries(self) -> dict[str, int]:
         return {"offsets": self.nseq + 1, "kv_lens": self.nseq, "slots": self.tokens, "positions": self.tokens, "taken": 1}
@@ -367,7 +380,9 @@ class KvStep:
         if n is not None:
             if not isinstance(value, torch.Tensor) or value.shape != (n,):
                 raise ValueError(f"{name}: {n} entries")
-            _ints(name, value)
+            if not value.is_cuda:
+                raise ValueError(f"{name}: on a GPU")
+            _ints(name, value, self._device)
         super().__setattr__(name, value)
 
 
@@ -375,39 +390,42 @@ def kv_tables(cached: torch.Tensor, new: torch.Tensor, free: torch.Tensor, table
               step: KvStep, taken: torch.Tensor | None = None) -> KvStep:
     """Blocks and slots for `new` [nseq] tokens behind `cached` [nseq]: the new entries of `table` [nseq, width] come
     from `free`, from entry `taken` [1] on; `step` receives the rest."""
-    nseq = step.nseq
-    c, n, f, t = _ints("cached", cached), _ints("new", new), _ints("free", free), _ints("table", table, 2)
+    nseq, dev = step.nseq, _kv_device(step)
+    c, n, f, t = _ints("cached", cached, dev), _ints("new", new, dev), _ints("free", free, dev), _ints("table", table, dev, 2)
     rows, width = table.shape
     if cached.shape[0] != nseq or new.shape[0] != nseq or rows != nseq:
         raise ValueError(f"cached, new, table: {nseq} sequences")
-    at = None if taken is None else _ints("taken", taken)
+    at = None if taken is None else _ints("taken", taken, dev)
     if taken is not None and taken.shape != (1,):
         raise ValueError("taken: one entry")
     check("kv_tables", load().qhip_launch_kv_tables(
         c, n, nseq, f, free.shape[0], at, block_size, t, width, step.tokens,
         step.offsets.data_ptr(), step.kv_lens.data_ptr(), step.slots.data_ptr(), step.positions.data_ptr(),
-        step.taken.data_ptr(), _stream()))
+        step.taken.data_ptr(), _stream(dev)))
     return step
 
 
 def kv_append(cache: KvCache, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor) -> None:
     """Write k, v [tokens, kv_heads, head_dim] into `slots` [tokens] (-1: skip); the blocks' scales grow as needed."""
-    tt = _kv_rows("k", k, cache.head_dim)
-    if _kv_rows("v", v, cache.head_dim) != tt or k.shape != v.shape or k.shape[1] != cache.kv_heads or len(slots) != len(k):
+    dev = _kv_device(cache)
+    tt = _kv_rows("k", k, cache.head_dim, dev)
+    if _kv_rows("v", v, cache.head_dim, dev) != tt or k.shape != v.shape or k.shape[1] != cache.kv_heads or len(slots) != len(k):
         raise ValueError("k, v: one type, [tokens, kv_heads, head_dim]; slots: [tokens]")
     check("kv_append", load().qhip_launch_kv_append(
         cache._ref, tt, k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1),
-        _ints("slots", slots), len(k), _stream()))
+        _ints("slots", slots, dev), len(k), _stream(dev)))
 
 
 def kv_read(cache: KvCache, blocks: torch.Tensor, dtype: torch.dtype = torch.float32) -> tuple[torch.Tensor, torch.Tensor]:
     """The keys and values of whole blocks, [len(blocks), kv_heads, block_size, head_dim] each."""
     if dtype not in _KV_TYPES:
         raise ValueError("dtype: f32, f16 or bf16")
+    dev = _kv_device(cache)
+    ids = _ints("blocks", blocks, dev)
     shape = (len(blocks), cache.kv_heads, cache.block_size, cache.head_dim)
     k, v = torch.empty((2, *shape), dtype=dtype, device=blocks.device).unbind(0)
-    check("kv_read", load().qhip_launch_kv_read(cache._ref, _ints("blocks", blocks), len(blocks), _KV_TYPES[dtype],
-                                                k.data_ptr(), v.data_ptr(), _stream()))
+    check("kv_read", load().qhip_launch_kv_read(cache._ref, ids, len(blocks), _KV_TYPES[dtype], k.data_ptr(), v.data_ptr(),
+                                                _stream(dev)))
     return k, v
 
 
@@ -429,26 +447,27 @@ def kv_attention(q: torch.Tensor, cache: KvCache, table: torch.Tensor, offsets: 
 
     Sequence i has rows offsets[i] .. offsets[i + 1] and kv_lens[i] cached tokens (its new ones included); no sequence
     has more than max_new rows or max_kv tokens.  scale: 1 / sqrt(head_dim) by default."""
-    tt, nseq = _kv_rows("q", q, cache.head_dim), len(kv_lens)
+    dev = _kv_device(cache)
+    tt, nseq = _kv_rows("q", q, cache.head_dim, dev), len(kv_lens)
     tokens, heads = q.shape[0], q.shape[1]
     if len(table) != nseq or len(offsets) != nseq + 1:
         raise ValueError(f"table: {nseq} rows, offsets: {nseq + 1}")
     if out is None:
         out = torch.empty((tokens, heads, cache.head_dim), dtype=q.dtype, device=q.device)
-    elif _kv_rows("out", out, cache.head_dim) != tt or out.shape != q.shape:
+    elif _kv_rows("out", out, cache.head_dim, dev) != tt or out.shape != q.shape:
         raise ValueError("out: as q")
     if lse is None:
         lse = torch.empty((tokens, heads), dtype=torch.float32, device=q.device)
-    elif lse.dtype != torch.float32 or lse.shape != (tokens, heads) or not lse.is_contiguous() or not lse.is_cuda:
+    elif lse.dtype != torch.float32 or lse.shape != (tokens, heads) or not lse.is_contiguous() or lse.get_device() != dev:
         raise ValueError("lse: f32 [tokens, q_heads]")
-    if work is not None and (work.dtype != torch.uint8 or work.dim() != 1 or not work.is_cuda or not work.is_contiguous()):
-        raise ValueError("work: a contiguous uint8 GPU tensor (kv_attention_work)")
-    b = QhipKvBatch(_ints("offsets", offsets), _ints("kv_lens", kv_lens), _ints("table", table, 2), nseq, tokens, max_new,
-                    max_kv, table.shape[1])
+    if work is not None and (work.dtype != torch.uint8 or work.dim() != 1 or work.get_device() != dev or not work.is_contiguous()):
+        raise ValueError("work: a contiguous uint8 tensor on the current GPU (kv_attention_work)")
+    b = QhipKvBatch(_ints("offsets", offsets, dev), _ints("kv_lens", kv_lens, dev), _ints("table", table, dev, 2), nseq, tokens,
+                    max_new, max_kv, table.shape[1])
     check("kv_attention", load().qhip_launch_kv_attention(
         cache._ref, ctypes.byref(b), tt, q.data_ptr(), q.stride(0), q.stride(1), heads,
         cache.head_dim ** -0.5 if scale is None else scale, int(causal), window, out.data_ptr(), out.stride(0), out.stride(1),
-        lse.data_ptr(), None if work is None else work.data_ptr(), 0 if work is None else work.numel(), _stream()))
+        lse.data_ptr(), None if work is None else work.data_ptr(), 0 if work is None else work.numel(), _stream(dev)))
     return out, lse
 
 

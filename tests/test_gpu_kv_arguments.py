@@ -71,3 +71,22 @@ def test_a_steps_sizes_are_fixed(gpu):
         with pytest.raises(ValueError):
             setattr(step, name, bad)
     assert (step.nseq, step.tokens) == (2, 4)
+
+
+def test_tensors_of_another_device_are_refused(gpu, monkeypatch):
+    """Launches go to the current device's stream: as if that were another one."""
+    cache, table, offsets, kv_lens, q = t.make([(40, 2), (70, 1)], 2, 2, 32, 64, torch.float32)
+    step, slots = ops.KvStep(2, 4), c.ints([0, 1, 2])
+    table, offsets, kv_lens = t.ints(table), t.ints(offsets), t.ints(kv_lens)
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 1)
+    for call in (lambda: ops.kv_tables(slots[:2], slots[:2], slots, table, 16, step), lambda: ops.kv_append(cache, q[:, :2], q[:, 2:], slots),
+                 lambda: ops.kv_read(cache, slots), lambda: ops.kv_attention(q, cache, table, offsets, kv_lens, 2, 70)):
+        with pytest.raises(ValueError):
+            call()
+
+
+def test_launches_go_to_the_current_stream(gpu):
+    side = torch.cuda.Stream()
+    for stream in (torch.cuda.default_stream(), side):
+        with torch.cuda.stream(stream):
+            assert (ops._stream().value or 0) == torch.cuda.current_stream().cuda_stream == stream.cuda_stream
