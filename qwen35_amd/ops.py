@@ -317,6 +317,13 @@ def _kv_rows(name: str, t: torch.Tensor, dim: int, device: int) -> int:
     return _KV_TYPES[t.dtype]
 
 
+def _c_ints(names: str, *numbers: int) -> None:
+    """(ctypes would cut a number to its lowest 32 bits)"""
+    for n in numbers:
+        if not -0x80000000 <= n <= 0x7FFFFFFF:
+            raise ValueError(f"{names}: {n} does not fit 32 bits")
+
+
 def _kv_device(*owners) -> int:
     """The current device, on which the tensors of a cache or a step lie."""
     device = torch.cuda.current_device()
@@ -395,6 +402,7 @@ def kv_tables(cached: torch.Tensor, new: torch.Tensor, free: torch.Tensor, table
     rows, width = table.shape
     if cached.shape[0] != nseq or new.shape[0] != nseq or rows != nseq:
         raise ValueError(f"cached, new, table: {nseq} sequences")
+    _c_ints("block_size", block_size)
     at = None if taken is None else _ints("taken", taken, dev)
     if taken is not None and taken.shape != (1,):
         raise ValueError("taken: one entry")
@@ -432,6 +440,7 @@ def kv_read(cache: KvCache, blocks: torch.Tensor, dtype: torch.dtype = torch.flo
 def kv_attention_work(cache: KvCache, q_heads: int, nseq: int, tokens: int, max_new: int, max_kv: int) -> torch.Tensor | None:
     """Zeroed workspace for kv_attention of a batch of these sizes (None when nothing would be cut); with another
     batch's, long sequences may go uncut."""
+    _c_ints("nseq, tokens, max_new, max_kv", nseq, tokens, max_new, max_kv)
     b = QhipKvBatch(None, None, None, nseq, tokens, max_new, max_kv, 0)
     n = load().qhip_kv_attention_work_bytes(cache._ref, ctypes.byref(b), q_heads)
     if n < 0:
@@ -462,6 +471,7 @@ def kv_attention(q: torch.Tensor, cache: KvCache, table: torch.Tensor, offsets: 
         raise ValueError("lse: f32 [tokens, q_heads]")
     if work is not None and (work.dtype != torch.uint8 or work.dim() != 1 or work.get_device() != dev or not work.is_contiguous()):
         raise ValueError("work: a contiguous uint8 tensor on the current GPU (kv_attention_work)")
+    _c_ints("max_new, max_kv, window", max_new, max_kv, window)
     b = QhipKvBatch(_ints("offsets", offsets, dev), _ints("kv_lens", kv_lens, dev), _ints("table", table, dev, 2), nseq, tokens,
                     max_new, max_kv, table.shape[1])
     check("kv_attention", load().qhip_launch_kv_attention(

@@ -90,3 +90,18 @@ def test_launches_go_to_the_current_stream(gpu):
     for stream in (torch.cuda.default_stream(), side):
         with torch.cuda.stream(stream):
             assert (ops._stream().value or 0) == torch.cuda.current_stream().cuda_stream == stream.cuda_stream
+
+
+def test_numbers_past_32_bits_are_refused(gpu):
+    """They would be cut to their lowest 32 bits: a bound of 2^32 to none."""
+    cache, table, offsets, kv_lens, q = t.make([(40, 2), (70, 1)], 2, 2, 32, 64, torch.float32)
+    args = (q, cache, t.ints(table), t.ints(offsets), t.ints(kv_lens))
+    for most, longest, window in ((2 ** 32, 70, 0), (2, 2 ** 32 + 70, 0), (2, 70, 2 ** 32 + 3), (2 ** 31, 70, 0),
+                                  (-2 ** 32, 70, 0)):
+        with pytest.raises(ValueError):
+            ops.kv_attention(*args, most, longest, window=window)
+    for bad in ((2 ** 32 + 2, 3, 2, 70), (2, 2 ** 32 + 3, 2, 70), (2, 3, 2 ** 32, 70), (2, 3, 2, 2 ** 32 + 70)):
+        with pytest.raises(ValueError):
+            ops.kv_attention_work(cache, 4, *bad)
+    with pytest.raises(ValueError):
+        ops.kv_tables(c.ints([0]), c.ints([0]), c.ints([1]), c.ints([[0]]), 2 ** 32 + 16, ops.KvStep(1, 0))
