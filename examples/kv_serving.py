@@ -56,7 +56,7 @@ class Server:
         self.table = torch.full((nseq, -(-max_kv // c.block_size)), -1, **ints)
         self.free = torch.randperm(c.num_blocks, device="cuda").to(torch.int32)  # any order
         self.cached, self.taken = torch.zeros(nseq, **ints), torch.zeros(1, **ints)
-        self.work = {}
+        self.work = None
 
     def step(self, x, new):
         """x [sum(new), hidden]: `new` tokens of each sequence."""
@@ -66,12 +66,10 @@ class Server:
         ops.kv_tables(self.cached, torch.tensor(new, dtype=torch.int32, device="cuda"), self.free, self.table,
                       self.layer.cache.block_size, step, taken=self.taken)
         self.cached, self.taken = step.kv_lens, step.taken
-        # a workspace is kept for each kind of step and grows with the longest sequence
+        # one workspace serves every kind of step; it grows with what they need
         max_kv = 1 << (max(self.lens) - 1).bit_length()
-        key = (tokens, most, max_kv)
-        if key not in self.work:
-            self.work[key] = ops.kv_attention_work(self.layer.cache, self.layer.q_heads, self.nseq, tokens, most, max_kv)
-        return self.layer.step(x, step, self.table, most, max_kv, self.work[key])
+        self.work = ops.kv_attention_work(self.layer.cache, self.layer.q_heads, self.nseq, tokens, most, max_kv, work=self.work)
+        return self.layer.step(x, step, self.table, most, max_kv, self.work)
 
 
 def exact(layer, history, new):

@@ -437,14 +437,24 @@ def kv_read(cache: KvCache, blocks: torch.Tensor, dtype: torch.dtype = torch.flo
     return k, v
 
 
-def kv_attention_work(cache: KvCache, q_heads: int, nseq: int, tokens: int, max_new: int, max_kv: int) -> torch.Tensor | None:
-    """Zeroed workspace for kv_attention of a batch of these sizes (None when nothing would be cut); with another
-    batch's, long sequences may go uncut."""
+def _kv_work(work: torch.Tensor, device: int) -> None:
+    if work.dtype != torch.uint8 or work.dim() != 1 or work.get_device() != device or not work.is_contiguous():
+        raise ValueError("work: a contiguous uint8 tensor on the current GPU (kv_attention_work)")
+
+
+def kv_attention_work(cache: KvCache, q_heads: int, nseq: int, tokens: int, max_new: int, max_kv: int,
+                      work: torch.Tensor | None = None) -> torch.Tensor | None:
+    """Zeroed workspace for kv_attention of a batch of these sizes (None when nothing would be cut), or `work` itself, an
+    earlier one, if it is large enough; with a smaller one, long sequences may go uncut."""
     _c_ints("nseq, tokens, max_new, max_kv", nseq, tokens, max_new, max_kv)
     b = QhipKvBatch(None, None, None, nseq, tokens, max_new, max_kv, 0)
     n = load().qhip_kv_attention_work_bytes(cache._ref, ctypes.byref(b), q_heads)
     if n < 0:
         raise ValueError(f"bad ({q_heads} query heads, {nseq} sequences, {tokens} tokens)")
+    if work is not None:
+        _kv_work(work, cache._device)
+        if work.numel() >= n:
+            return work
     return torch.zeros(n, dtype=torch.uint8, device=cache.k.device) if n > 0 else None
 
 
@@ -469,8 +479,8 @@ def kv_attention(q: torch.Tensor, cache: KvCache, table: torch.Tensor, offsets: 
         lse = torch.empty((tokens, heads), dtype=torch.float32, device=q.device)
     elif lse.dtype != torch.float32 or lse.shape != (tokens, heads) or not lse.is_contiguous() or lse.get_device() != dev:
         raise ValueError("lse: f32 [tokens, q_heads]")
-    if work is not None and (work.dtype != torch.uint8 or work.dim() != 1 or work.get_device() != dev or not work.is_contiguous()):
-        raise ValueError("work: a contiguous uint8 tensor on the current GPU (kv_attention_work)")
+    if work is not None:
+        _kv_work(work, dev)
     _c_ints("max_new, max_kv, window", max_new, max_kv, window)
     b = QhipKvBatch(_ints("offsets", offsets, dev), _ints("kv_lens", kv_lens, dev), _ints("table", table, dev, 2), nseq, tokens,
                     max_new, max_kv, table.shape[1])
