@@ -401,7 +401,12 @@ typedef struct qhip_kv_cache {
  *   d_positions [tokens] (nullable) each token's place in its sequence, 0 for padding
  *   d_taken_out the free-list entries taken, these included: more than nfree
  *               says that blocks were short
- * The arrays must not overlap (hipErrorInvalidValue). */
+ * The arrays must not overlap (hipErrorInvalidValue).
+ * A sequence may fall back (draft tokens that were rejected): its next d_cached
+ * is smaller.  Blocks from ceil(cached / block_size) on are then no longer its
+ * own, and the next call that needs their entries overwrites them: the caller
+ * puts their ids back into the free list first (the entries before d_taken[0]
+ * are spent), or they are lost. */
 int qhip_launch_kv_tables(const int *d_cached, const int *d_new, int nseq, const int *d_free, int nfree,
                           const int *d_taken, int block_size, int *d_table, int table_width, int tokens,
                           int *d_offsets, int *d_kv_lens, int *d_slots, int *d_positions, int *d_taken_out,
@@ -417,6 +422,8 @@ int qhip_launch_kv_tables(const int *d_cached, const int *d_new, int nseq, const
  *   first new token is the block's first;
  *   codes of the tokens before it: round(code * (old / scale));
  *   new codes: round(x * (1 / scale)), each an f32 operation, ties to even.
+ * Tokens that a sequence gave up leave their share in the scale of a block that
+ * it keeps, until the block is begun anew.
  * A NaN among the new values makes the scale NaN, an infinity makes it
  * infinite: the block's head then reads as NaN until the block is begun anew. */
 int qhip_launch_kv_append(const qhip_kv_cache *cache, int type, const void *d_k, long k_token_stride,

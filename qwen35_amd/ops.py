@@ -396,7 +396,10 @@ class KvStep:
 def kv_tables(cached: torch.Tensor, new: torch.Tensor, free: torch.Tensor, table: torch.Tensor, block_size: int,
               step: KvStep, taken: torch.Tensor | None = None) -> KvStep:
     """Blocks and slots for `new` [nseq] tokens behind `cached` [nseq]: the new entries of `table` [nseq, width] come
-    from `free`, from entry `taken` [1] on; `step` receives the rest."""
+    from `free`, from entry `taken` [1] on; `step` receives the rest.
+
+    A sequence that falls back (rejected drafts) comes with a smaller `cached`; put its blocks behind that back into `free`
+    (the entries before `taken` are spent) first, since their entries of `table` are overwritten."""
     nseq, dev = step.nseq, _kv_device(step)
     c, n, f, t = _ints("cached", cached, dev), _ints("new", new, dev), _ints("free", free, dev), _ints("table", table, dev, 2)
     rows, width = table.shape
