@@ -458,9 +458,14 @@ typedef struct qhip_kv_batch {
  * (0 or 1): it sees j <= p, and with window > 0 only j > p - window.  A row that
  * sees nothing gets out = 0 and lse = -infinity.  A visible token whose table
  * entry names no block of the pool makes its rows NaN; lengths above 2^30 are
- * taken as 2^30.  d_q, d_out: head_dim
- * contiguous elements of `type` at token * token_stride + head * head_stride
- * (elements); d_lse (nullable): f32 [tokens][q_heads].  Rows of tokens at or
+ * taken as 2^30.
+ * Maxima, sums, scores and lse are f32 for every type.  f32 rows take queries and
+ * softmax weights in 22 bits: outputs are good to 1e-6 relative L2.  f16 and bf16
+ * rows round the softmax weights to 11 bits before the product with the values:
+ * 2e-4 relative L2 beside the outputs' own rounding (f16 2e-4, together 3e-4; bf16
+ * 1.7e-3, together the same).  A caller who wants less passes f32 rows.
+ * d_q, d_out: head_dim contiguous elements of `type` at token * token_stride +
+ * head * head_stride (elements); d_lse (nullable): f32 [tokens][q_heads].  Rows of tokens at or
  * past offsets[nseq] are not written.
  * d_work (nullable): qhip_kv_attention_work_bytes of the same batch, 16-byte
  * aligned, its first 32 KiB zero before the first launch and zero again after

@@ -303,7 +303,6 @@ _KV_TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 30}
 
 
 # Launches go to the current device's stream, so a call's tensors have to lie on that device.
-
 def _ints(name: str, t: torch.Tensor, device: int, dims: int = 1) -> int:
     if t.dtype != torch.int32 or t.dim() != dims or t.get_device() != device or not t.is_contiguous():
         raise ValueError(f"{name}: a contiguous int32 tensor of {dims} dimension(s) on the current GPU")
@@ -324,12 +323,11 @@ def _c_ints(names: str, *numbers: int) -> None:
             raise ValueError(f"{names}: {n} does not fit 32 bits")
 
 
-def _kv_device(*owners) -> int:
-    """The current device, on which the tensors of a cache or a step lie."""
+def _kv_device(owner) -> int:
+    """The current device, on which the tensors of the cache or step lie."""
     device = torch.cuda.current_device()
-    for x in owners:
-        if x._device != device:
-            raise ValueError(f"{type(x).__name__}: on device {x._device}, the current one is {device}")
+    if owner._device != device:
+        raise ValueError(f"{type(owner).__name__}: on device {owner._device}, the current one is {device}")
     return device
 
 
@@ -468,7 +466,10 @@ def kv_attention(q: torch.Tensor, cache: KvCache, table: torch.Tensor, offsets: 
     """Attention of q [tokens, q_heads, head_dim] over the cached tokens of each row's sequence: (out, lse [tokens, q_heads]).
 
     Sequence i has rows offsets[i] .. offsets[i + 1] and kv_lens[i] cached tokens (its new ones included); no sequence
-    has more than max_new rows or max_kv tokens.  scale: 1 / sqrt(head_dim) by default."""
+    has more than max_new rows or max_kv tokens.  scale: 1 / sqrt(head_dim) by default.  Rows at or past offsets[-1] are not
+    written (where out or lse is not given: whatever the memory held).  work: kv_attention_work's tensor, whose first 32 KiB
+    are zero before and after every call; calls that share one must not overlap (two streams need two).  f32 rows are good
+    to f32; f16 and bf16 rows take softmax weights of 11 bits, which adds 2e-4 of an output to its own rounding."""
     dev = _kv_device(cache)
     tt, nseq = _kv_rows("q", q, cache.head_dim, dev), len(kv_lens)
     tokens, heads = q.shape[0], q.shape[1]
