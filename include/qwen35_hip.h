@@ -437,7 +437,8 @@ int qhip_launch_kv_read(const qhip_kv_cache *cache, const int *d_blocks, int nbl
                         void *d_v_out, void *stream);
 
 /* A step's sequences as qhip_launch_kv_tables leaves them.  max_new, max_kv:
- * no sequence has more new tokens, or more tokens in all. */
+ * no sequence has more new tokens, or more tokens in all (rows of one that has
+ * more new ones may stay unwritten). */
 typedef struct qhip_kv_batch {
   const int *offsets; /* [nseq + 1] packed tokens of sequence i: [offsets[i], offsets[i + 1]) */
   const int *kv_lens; /* [nseq] its tokens in the cache, the new ones included */

@@ -444,6 +444,13 @@ __device__ __forceinline__ void join_rows(const KvAttnArgs& a, float* lds, __amd
     if constexpr (EB == 1) break;
   }
 }
+// Whether each chunk of the item's tile has its place in the workspace and its
+// workgroup in the grid.  Always, but for offsets that are none and sequences of
+// more than the stated tokens, whose counters would stay behind.
+__device__ __forceinline__ bool all_arrive(const KvAttnArgs& a, const Item& it) {
+  const int last = it.slot + (it.chunks - 1) * a.kv_heads - it.head * (it.chunks - 1);  // workgroup of the last chunk
+  return it.slot + it.chunks <= a.slots && it.counter < kMaxCut && last < (int)gridDim.x;
+}
 // After every thread's part_stores: whether this workgroup was the tile's last,
 // which then joins.
 template <int D, int SPLIT>
@@ -804,7 +811,7 @@ void k_kv_attention_few(KvAttnArgs a) {
     }
     return;
   }
-  if (it.slot + it.chunks > a.slots || it.counter >= kMaxCut) return;  // offsets or lengths that are none
+  if (!all_arrive(a, it)) return;
   const int stride = a.tile_rows * (D + 2);
   const __amdgpu_buffer_rsrc_t parts_at = part_rsrc(a.partial + (long)it.slot * stride, (long)it.chunks * stride);
 #pragma unroll
@@ -1103,7 +1110,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_kv_attention_many(KvA
     }
     return;
   }
-  if (it.slot + it.chunks > a.slots || it.counter >= kMaxCut) return;  // offsets or lengths that are none
+  if (!all_arrive(a, it)) return;
   constexpr int kStride = kManyRows * (D + 2);
   const __amdgpu_buffer_rsrc_t parts_at = part_rsrc(a.partial + (long)it.slot * kStride, (long)it.chunks * kStride);
   if (row < sp.rows) {

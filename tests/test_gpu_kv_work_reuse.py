@@ -56,3 +56,17 @@ def test_a_workspace_that_is_large_enough_is_kept(gpu):
     for bad in (work.cpu(), work.view(torch.float32)):
         with pytest.raises(ValueError):
             ops.kv_attention_work(cache, 8, 2, 2, 1, 4000, work=bad)
+
+
+def test_a_batch_past_its_bounds_leaves_the_workspace_usable(gpu):
+    """More new tokens than max_new says: rows may stay unwritten, but no counter is left for the next call."""
+    lens = [(9000, 508)] + [(0, 0)] * 12
+    cache, table, offsets, kv_lens, q = t.make(lens, 2, 4, 64, 128, torch.float32)
+    args = (q, cache, t.ints(table), t.ints(offsets), t.ints(kv_lens))
+    work = ops.kv_attention_work(cache, 8, 13, 508, 508, 9000)
+    work = ops.kv_attention_work(cache, 8, 13, 508, 4, 9000, work=work)
+    ops.kv_attention(*args, 4, 9000, work=work)
+    assert not bool(work[:32768].any())
+    want = t.attend(cache, table, offsets, kv_lens, q)
+    got = ops.kv_attention(*args, 508, 9000, work=work)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
