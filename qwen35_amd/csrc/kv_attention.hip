@@ -489,13 +489,16 @@ __device__ __forceinline__ void arrive_and_join(const KvAttnArgs& a, float* lds,
 // over workgroups (find_item).
 //
 // Bound by memory where sequences are long: one f32 token on 131071 keys (4 key
-// heads of 256, 268 MB) 60 us, 4.5 TB/s; 64 tokens on 2000 keys each, 53 us at 4.9
-// TB/s (256) and 30 us at 4.2 TB/s (8 heads of 128).  Short ones are bound by
+// heads of 256, 268 MB) 60 us, 4.5 TB/s; 64 tokens on 2000 keys each (262 MB), 54 us at
+// 4.9 TB/s (4 heads of 256) and 51 us at 5.1 (8 of 128).  Short ones are bound by
 // chains of latencies: lengths - plan - table - scales 5 us and codes 3 us before
 // the first product, 2 us to merge the waves, partial results - counter - join 5
-// us where a sequence is cut: one token on 333 keys takes 13 us.  f32 rows in number are bound by the matrix pipe
-// at twice the products for either operand: 4096 tokens, 16 heads of 128, 170 us
-// (400 TFLOP/s).  The registers allow two waves a SIMD for D = 256 and three for
+// us where a sequence is cut: one token on 333 keys takes 13 us.  Every wave walks
+// all sequences for the plan, so many short ones cost more: 512 decodes of up to
+// 2000 keys 104 us (306 MB, 62 at the copy's rate), 1000 of them 199 (547 MB, 111).
+// f32 rows in number are bound by the matrix pipe at twice the products for either
+// operand: 4096 tokens, 16 heads of 128, 170 to 195 us by the card (350 to 400
+// TFLOP/s), of 256 365 to 375.  The registers allow two waves a SIMD for D = 256 and three for
 // 128; a fourth would spill (60 us against 44 for 64 ragged decodes).
 constexpr int kFewRows = 64;  // rows up to which a sequence beside long ones is this kernel's
 
@@ -851,8 +854,8 @@ void k_kv_attention_few(KvAttnArgs a) {
 // lane and tile of 64 keys, a quarter of them the staging), and the two hardly
 // overlap with two waves a SIMD.  A prompt of 8192 tokens, 32 heads of 128 on 8,
 // takes 650 us (850 TFLOP/s); 4096 tokens of 16 heads 127 us (531), of 256
-// dimensions 242 us (563), of 64 95 us (350: half the products to the same
-// exponentials).  Tried and not kept: LDS for two tiles with one barrier (the
+// dimensions 245 us (560), of 64 92 us (370: half the products to the same
+// exponentials); 8192 tokens of 16 heads of 256 900 us (610).  Tried and not kept: LDS for two tiles with one barrier (the
 // same for 128, 285 us against 242 for 256), loops of their own for tiles without
 // masks (64: 88 against 94, but 256: 402 against 242 for its spills), three waves a
 // SIMD for 64 (116 against 99), priority for the products (702 us against 696).
@@ -979,7 +982,11 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_kv_attention_many(KvA
     if (ri == 0 && i) {
       info = next;
       next = tile_info(a, round_id((i >> 4) + 1), it.head);
-      l_before += l;  // one long sum of like terms would round the same way each time (4e-5 in 90,000 keys)
+      // One long sum of like terms would round the same way each time (4e-5 in 90,000
+      // keys).  The outputs' accumulators stay: uncut rows of 131,072 keys alike are off
+      // by up to 6e-4, where f16 rows allow 1e-3 and 128 rows' outputs of 128 dimensions
+      // would take another 64 KB of LDS, half the workgroups.
+      l_before += l;
       l = 0.0f;
     }
     __syncthreads();  // the previous tile has been read

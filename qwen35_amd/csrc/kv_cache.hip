@@ -164,7 +164,9 @@ __global__ __launch_bounds__(256) void k_kv_tables(KvTablesArgs a) {
 // place of the quotient, and one multiply.
 //
 // Prompts are bound by reading the new values: 4600 f32 tokens of 4 heads of 256
-// (47 MB) 12.2 us, 3.9 TB/s.  Single tokens are bound by the chain slots - values
+// (47 MB) 12.4 us, 3.8 TB/s.  16-bit ones take as long for 28 MB (13.0 us, of 8 heads of
+// 128 13.6): as many pieces in flight, each of half the bytes, and of blocks of 64
+// tokens three tiles in four find no run.  Single tokens are bound by the chain slots - values
 // - maximum - codes: 64 tokens of 8 heads of 128 in 4.5 us.
 constexpr int kAppKeep = 8;
 // One token a workgroup up to kAppFew tokens: single tokens are a run each, which
