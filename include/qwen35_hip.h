@@ -368,6 +368,8 @@ int qhip_launch_mul_mat_ragged(const void *d_w, const void *d_xq_packed, float *
  *   block_size        16, 32, 64, 128 or 256; 0 < num_blocks * block_size < 2^31
  *   head_dim          64, 128 or 256 (others: QHIP_DECLINE)
  *
+ * A call takes at most 2^31 - 1025 tokens and as many sequences.
+ *
  * Element types of keys, values, queries and outputs are GGUF type ids. */
 #define QHIP_TT_F32 0
 #define QHIP_TT_F16 1

@@ -1161,7 +1161,7 @@ constexpr int kMaxGroup = 512;  // most query heads of a key head (row_at)
 static int check_batch(const qhip_kv_cache* cache, const qhip_kv_batch* b, int q_heads) {
   const int rc = kv_check_cache(cache);
   if (rc == (int)hipErrorInvalidValue || !b) return (int)hipErrorInvalidValue;
-  if (b->nseq < 0 || b->tokens < 0 || b->max_new < 0 || b->max_kv < 0 || b->table_width < 0) return (int)hipErrorInvalidValue;
+  if (b->nseq < 0 || b->nseq > kMaxCount || b->tokens < 0 || b->max_new < 0 || b->max_kv < 0 || b->table_width < 0) return (int)hipErrorInvalidValue;
   if (q_heads <= 0 || q_heads > 65535 || q_heads % cache->kv_heads) return (int)hipErrorInvalidValue;
   return rc ? rc : q_heads / cache->kv_heads > kMaxGroup ? QHIP_DECLINE : 0;
 }

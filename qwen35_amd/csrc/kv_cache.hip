@@ -354,7 +354,8 @@ extern "C" int qhip_launch_kv_tables(const int* d_cached, const int* d_new, int 
                                      int* d_offsets, int* d_kv_lens, int* d_slots, int* d_positions, int* d_taken_out,
                                      void* stream) {
   const int shift = kv_block_shift(block_size);
-  if (shift < 0 || nseq < 0 || nfree < 0 || table_width < 0 || tokens < 0) return (int)hipErrorInvalidValue;
+  if (shift < 0 || nseq < 0 || nseq > kMaxCount || nfree < 0 || table_width < 0 || tokens < 0 || tokens > kMaxCount)
+    return (int)hipErrorInvalidValue;
   if (!d_offsets || !d_taken_out || (nseq > 0 && (!d_cached || !d_new || !d_kv_lens)) || (nfree > 0 && !d_free) ||
       (nseq > 0 && table_width > 0 && !d_table) || (tokens > 0 && !d_slots))
     return (int)hipErrorInvalidValue;
@@ -388,7 +389,7 @@ extern "C" int qhip_launch_kv_append(const qhip_kv_cache* cache, int type, const
                                      long k_head_stride, const void* d_v, long v_token_stride, long v_head_stride,
                                      const int* d_slots, int tokens, void* stream) {
   const int rc = kv_check_cache(cache), size = kv_type_size(type);
-  if (rc == (int)hipErrorInvalidValue || !size || tokens < 0) return (int)hipErrorInvalidValue;
+  if (rc == (int)hipErrorInvalidValue || !size || tokens < 0 || tokens > kMaxCount) return (int)hipErrorInvalidValue;
   if (tokens > 0 && (!d_k || !d_v || !d_slots || ((uintptr_t)d_k % size) || ((uintptr_t)d_v % size)))
     return (int)hipErrorInvalidValue;
   if (rc) return rc;

@@ -15,6 +15,9 @@ typedef uint32_t kv_u32x2 __attribute__((ext_vector_type(2)));
 // Longest sequence: places are ints, and some are counted a round of steps past
 // the last.
 constexpr int kMaxLen = 1 << 30;
+// Most tokens and sequences of a call: indexes run up to a workgroup's or a block's
+// past the last.
+constexpr int kMaxCount = 0x7FFFFFFF - 1024;
 
 // NaN payloads aside, (float)T is exact and T(float) rounds to nearest even.
 typedef _Float16 f16_t;
