@@ -466,7 +466,8 @@ typedef struct qhip_kv_batch {
  * softmax weights in 22 bits: outputs are good to 1e-6 relative L2.  f16 and bf16
  * rows round the softmax weights to 11 bits before the product with the values:
  * 2e-4 relative L2 beside the outputs' own rounding (f16 2e-4, together 3e-4; bf16
- * 1.7e-3, together the same).  A caller who wants less passes f32 rows.
+ * 1.7e-3, together the same), and where their keys are not cut, long sums of like
+ * terms up to 6e-4 on 131,072 keys.  A caller who wants less passes f32 rows.
  * d_q, d_out: head_dim contiguous elements of `type` at token * token_stride +
  * head * head_stride (elements); d_lse (nullable): f32 [tokens][q_heads].  Rows of tokens at or
  * past offsets[nseq] are not written.
