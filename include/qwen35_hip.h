@@ -482,6 +482,96 @@ int qhip_launch_kv_attention(const qhip_kv_cache *cache, const qhip_kv_batch *ba
                              int causal, int window, void *d_out, long out_token_stride, long out_head_stride,
                              float *d_lse, void *d_work, long work_bytes, void *stream);
 
+/* ---- rows of heads --------------------------------------------------------------
+ * What the following three operators read and write: the elements of token t, head h
+ * lie side by side at `at` + t * token_stride + h * head_stride (strides in elements,
+ * not negative; any element's address will do).  Rows that are written must not share
+ * elements with each other (heads inside a token's row or tokens inside a head's),
+ * nor with anything else of the call but where it says so (hipErrorInvalidValue). */
+typedef struct qhip_rows {
+  void *at;
+  long token_stride;
+  long head_stride;
+} qhip_rows;
+
+/* Root-mean-square norm over the `dim` values of each row (heads = 1: whole hidden
+ * states; else heads), in front of the quantized products:
+ *   h = x + residual (nullable: h = x), which takes the residual's place
+ *   r = 1 / sqrt(mean(h^2) + eps), the mean and r in f64, r then rounded to f32
+ *   y = (h * r) * weight (f32 [dim], nullable), and with a gate (nullable) times
+ *   gate / (1 + exp(-gate)); every other operation rounds to f32
+ *   out (nullable) = y in the rows' type; d_xq (nullable): the activation rows of
+ *   weight type `ttype` (qhip_act_row_bytes(ttype, heads * dim) bytes a token) that
+ *   qhip_launch_quantize_act makes of the f32 y
+ * x, residual, gate and out are of one type (QHIP_TT_F32, F16 or BF16); `out` may be x
+ * or the gate.  One of out and d_xq is needed.  d_xq wants heads * dim in whole blocks
+ * (32 or 256 values) and 2-byte (Q8_0) or 4-byte (Q8_K) alignment; where a block spans
+ * several heads, dim must be a power of two (else QHIP_DECLINE).  With weight 1 /
+ * sqrt(dim) and eps / dim it is the L2 norm x / sqrt(sum(x^2) + eps). */
+int qhip_launch_rms_norm(int type, const qhip_rows *x, const qhip_rows *residual, const qhip_rows *gate,
+                         const float *d_weight, float eps, const qhip_rows *out, int ttype, void *d_xq,
+                         int tokens, int heads, int dim, void *stream);
+
+/* Rotary positions: pair i < rot_dim / 2 of a head is turned by position * f_i
+ * radians, f_i = base^(-2 i / rot_dim) or scaled for contexts beyond the trained one:
+ *   LINEAR  f_i / factor
+ *   NTK     base * factor^(rot_dim / (rot_dim - 2)) in base's place
+ *   YARN    f_i blended into f_i / factor from the pair that turns `fast` times over
+ *           `original` positions to the one that turns `slow` times, and turned
+ *           values times 1 + 0.1 ln(factor)
+ * qhip_rope_steps writes the frequencies (host memory, rot_dim / 2 of them) as
+ * fractions of 2^64 of a turn a position, and the factor on turned values;
+ * qhip_launch_rope takes them from device memory. */
+#define QHIP_ROPE_PLAIN 0
+#define QHIP_ROPE_LINEAR 1
+#define QHIP_ROPE_NTK 2
+#define QHIP_ROPE_YARN 3
+int qhip_rope_steps(int rot_dim, double base, int scaling, double factor, int original, double fast,
+                    double slow, unsigned long long *h_steps, float *h_gain);
+/* Turns the first rot_dim of the dim values of each query and key head (k_heads 0:
+ * no keys) by the token's d_positions[t] (any int; qhip_launch_kv_tables writes
+ * them) and copies the rest.  interleaved 0: a pair is values i and i + rot_dim / 2;
+ * 1: values 2 i and 2 i + 1.  q_out may be q, and k_out k (the values behind rot_dim
+ * then stay untouched).  At most 1024 values turn and 1024 stay (more: QHIP_DECLINE).
+ * Angles are exact to 2^-32 of a turn at any position; products are f32. */
+int qhip_launch_rope(int type, const qhip_rows *q, const qhip_rows *q_out, int q_heads, const qhip_rows *k,
+                     const qhip_rows *k_out, int k_heads, int dim, int rot_dim,
+                     const unsigned long long *d_steps, float gain, int interleaved,
+                     const int *d_positions, int tokens, void *stream);
+
+/* Linear attention with a decay for each head.  A sequence's value head h has a state
+ * S [key_dim][value_dim]; for each token in order, with q, k of key head h /
+ * (v_heads / k_heads) and a = exp(log_decay):
+ *   S <- a S;  u = beta (v - k S) (the delta rule; d_beta NULL: u = v)
+ *   S <- S + k^T u;  out = scale q S
+ * d_states: f32 [num_states][v_heads][key_dim][value_dim], 16-byte aligned.  Sequence i
+ * starts from state source[i] (-1: zeros; NULL: slots[i]) and leaves its last state in
+ * slots[i] (outside the pool: nowhere); without new tokens it copies.  Any other
+ * source outside the pool gives NaN.  A state that one sequence of a call writes may
+ * be read or written by no other of the call.
+ * d_log_decay and d_beta: f32, [token * stride + head]; log_decay is meant to be <= 0,
+ * -infinity forgets.  key_dim 64 or 128, value_dim 64, 128 or 256 (others:
+ * QHIP_DECLINE); at most 65535 sequences and value heads. */
+typedef struct qhip_linear_batch {
+  const int *offsets; /* [nseq + 1] packed tokens of sequence i: [offsets[i], offsets[i + 1]) */
+  const int *slots;   /* [nseq] */
+  const int *source;  /* [nseq], nullable */
+  int nseq;
+  int tokens;  /* packed tokens in all; rows of tokens at or past offsets[nseq] are not written */
+  int max_new; /* no sequence has more (those past it are left out) */
+  int num_states;
+  int k_heads;
+  int v_heads;
+  int key_dim;
+  int value_dim;
+} qhip_linear_batch;
+long qhip_linear_attention_work_bytes(const qhip_linear_batch *batch, int type, int delta);
+int qhip_launch_linear_attention(const qhip_linear_batch *batch, int type, const qhip_rows *q,
+                                 const qhip_rows *k, const qhip_rows *v, const float *d_log_decay,
+                                 long decay_stride, const float *d_beta, long beta_stride, float scale,
+                                 float *d_states, const qhip_rows *out, void *d_work, long work_bytes,
+                                 void *stream);
+
 /* ---- parity export -----------------------------------------------------------
  * Exact per-block integers through the same unit decode as the GEMV kernels:
  * ints[(t*rows + r)*nints + i], nints = cols/block_elems, except the formats

@@ -30,6 +30,19 @@ class QhipKvBatch(ctypes.Structure):
                 ("max_new", c_int), ("max_kv", c_int), ("table_width", c_int)]
 
 
+class QhipRows(ctypes.Structure):
+    _fields_ = [("at", c_void_p), ("token_stride", c_long), ("head_stride", c_long)]
+
+
+class QhipLinearBatch(ctypes.Structure):
+    _fields_ = [("offsets", c_void_p), ("slots", c_void_p), ("source", c_void_p), ("nseq", c_int), ("tokens", c_int),
+                ("max_new", c_int), ("num_states", c_int), ("k_heads", c_int), ("v_heads", c_int), ("key_dim", c_int),
+                ("value_dim", c_int)]
+
+
+c_rows = ctypes.POINTER(QhipRows)
+
+
 class QhipProfEntry(ctypes.Structure):
     _fields_ = [("slot", c_int), ("ttype", c_int), ("rows", c_int), ("cols", c_int), ("tokens", c_int),
                 ("calls", ctypes.c_longlong), ("device_us", ctypes.c_double), ("bytes", ctypes.c_double),
@@ -105,6 +118,16 @@ SIGNATURES = {
     "qhip_launch_kv_attention": (c_int, [ctypes.POINTER(QhipKvCache), ctypes.POINTER(QhipKvBatch), c_int, c_void_p,
                                          c_long, c_long, c_int, ctypes.c_float, c_int, c_int, c_void_p, c_long, c_long,
                                          c_void_p, c_void_p, c_long, c_void_p]),
+    "qhip_launch_rms_norm": (c_int, [c_int, c_rows, c_rows, c_rows, c_void_p, ctypes.c_float, c_rows, c_int, c_void_p,
+                                     c_int, c_int, c_int, c_void_p]),
+    "qhip_rope_steps": (c_int, [c_int, ctypes.c_double, c_int, ctypes.c_double, c_int, ctypes.c_double, ctypes.c_double,
+                                ctypes.POINTER(ctypes.c_ulonglong), ctypes.POINTER(ctypes.c_float)]),
+    "qhip_launch_rope": (c_int, [c_int, c_rows, c_rows, c_int, c_rows, c_rows, c_int, c_int, c_int, c_void_p,
+                                 ctypes.c_float, c_int, c_void_p, c_int, c_void_p]),
+    "qhip_linear_attention_work_bytes": (c_long, [ctypes.POINTER(QhipLinearBatch), c_int, c_int]),
+    "qhip_launch_linear_attention": (c_int, [ctypes.POINTER(QhipLinearBatch), c_int, c_rows, c_rows, c_rows, c_void_p,
+                                             c_long, c_void_p, c_long, ctypes.c_float, c_void_p, c_rows, c_void_p,
+                                             c_long, c_void_p]),
     "qhip_launch_block_ints": (c_int, [c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int,
                                        c_void_p]),
     "qhip_backend_create": (c_void_p, [c_int, c_int_p]),

@@ -186,6 +186,34 @@ __device__ __forceinline__ uint32_t quant_q8_0_lane4(const float* v, uint32_t& h
   return packed;
 }
 
+// Q8_0 with eight values per lane, the four lanes of a quad per block (lane 4 g +
+// i: values 8 i ..+7): the same bytes, packed (byte k of w[j] = value 8 i + 4 j + k).
+__device__ __forceinline__ void quant_q8_0_lane8(const float* v, uint32_t* w, uint32_t& hbits) {
+  // |v| with the reference's "if (a > amax)" NaN handling: NaN never wins
+  float a = 0.0f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    float e = v[i] < 0.0f ? -v[i] : v[i];
+    e = e > 0.0f ? e : 0.0f;
+    a = fmaxf(a, e);
+  }
+  a = fmaxf(a, dpp_f32<0xB1>(a));  // quad_perm [1, 0, 3, 2]
+  a = fmaxf(a, dpp_f32<0x4E>(a));  // quad_perm [2, 3, 0, 1]
+  const float scale = a > 0.0f ? a / 127.0f : 1.0f;
+  const float inv = a > 0.0f ? 1.0f / scale : 0.0f;
+  w[0] = w[1] = 0u;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float sv = v[i] * inv;
+    const float r = sv + (sv >= 0.0f ? 0.5f : -0.5f);
+    int q = trunc_i32_x86(r);
+    q = q > 127 ? 127 : q;
+    q = q < -128 ? -128 : q;
+    w[i >> 2] |= ((uint32_t)q & 0xFFu) << (8 * (i & 3));
+  }
+  hbits = f32_to_f16_bits(scale);
+}
+
 // Q8_K (src/kernels/x86/kernels256.c:865-896): lane l of a wave holds values
 // 4l..4l+3 of the 256-value block.  Returns them quantized and packed (byte i
 // = value 4l+i); `gsum` gets the sum of the lane's 16-value group (lanes 4g..4g+3
@@ -215,6 +243,35 @@ __device__ __forceinline__ uint32_t quant_q8_K_lane(const float* v, int& gsum, f
   }
   gsum = quad_sum(s);
   return packed;
+}
+
+// Q8_K with eight values per lane, a half of the wave per block (lane i of the half:
+// values 8 i ..+7): the same bytes, packed as above; `gsum` is the sum of the 16
+// values of lanes 2 j and 2 j + 1.
+__device__ __forceinline__ void quant_q8_K_lane8(const float* v, uint32_t* w, int& gsum, float& scale) {
+  float a = 0.0f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    float e = v[i] < 0.0f ? -v[i] : v[i];
+    e = e > 0.0f ? e : 0.0f;
+    a = fmaxf(a, e);
+  }
+  a = half_max(a);
+  scale = a > 0.0f ? a / 127.0f : 1.0f;
+  const float inv = a > 0.0f ? 1.0f / scale : 0.0f;
+  w[0] = w[1] = 0u;
+  int s = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    float r = roundf(v[i] * inv);
+    r = r < -127.0f ? -127.0f : r;
+    r = r > 127.0f ? 127.0f : r;
+    r = (r >= -127.0f) ? r : 127.0f;  // NaN
+    const int q = (int)r;
+    w[i >> 2] |= ((uint32_t)q & 0xFFu) << (8 * (i & 3));
+    s += q;
+  }
+  gsum = s + __builtin_amdgcn_update_dpp(0, s, 0xB1, 0xF, 0xF, false);  // quad_perm [1, 0, 3, 2]
 }
 
 // ---- wave reductions --------------------------------------------------------------

@@ -121,28 +121,8 @@ __global__ __launch_bounds__(256) void k_quantize_q8_0w(const float* __restrict_
   const float* xr = act_row<RAGGED>(x, src, off, nseq, t, x_stride) + 32 * b + 8 * pt;
   const qf32x4 v0 = load4f<RAGGED>(xr), v1 = load4f<RAGGED>(xr + 4);
   const float v[8] = {v0.x, v0.y, v0.z, v0.w, v1.x, v1.y, v1.z, v1.w};
-  // |v| with the reference's "if (a > amax)" NaN handling: NaN never wins
-  float a = 0.0f;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    float e = v[i] < 0.0f ? -v[i] : v[i];
-    e = e > 0.0f ? e : 0.0f;
-    a = fmaxf(a, e);
-  }
-  a = fmaxf(a, dpp_f32<0xB1>(a));  // quad_perm [1, 0, 3, 2]
-  a = fmaxf(a, dpp_f32<0x4E>(a));  // quad_perm [2, 3, 0, 1]
-  const float scale = a > 0.0f ? a / 127.0f : 1.0f;
-  const float inv = a > 0.0f ? 1.0f / scale : 0.0f;
-  uint32_t w[2] = {0u, 0u};
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float sv = v[i] * inv;
-    const float r = sv + (sv >= 0.0f ? 0.5f : -0.5f);
-    int q = trunc_i32_x86(r);
-    q = q > 127 ? 127 : q;
-    q = q < -128 ? -128 : q;
-    w[i >> 2] |= ((uint32_t)q & 0xFFu) << (8 * (i & 3));
-  }
+  uint32_t w[2], hbits;
+  quant_q8_0_lane8(v, w, hbits);
   if (g < total) {
     // the block is 2-byte aligned: four 16-bit stores
     uint16_t* ob = (uint16_t*)(out + (long)t * out_stride + 34L * b);
@@ -150,7 +130,7 @@ __global__ __launch_bounds__(256) void k_quantize_q8_0w(const float* __restrict_
     ob[2 + 4 * pt] = (uint16_t)(w[0] >> 16);
     ob[3 + 4 * pt] = (uint16_t)w[1];
     ob[4 + 4 * pt] = (uint16_t)(w[1] >> 16);
-    if (pt == 0) ob[0] = (uint16_t)f32_to_f16_bits(scale);
+    if (pt == 0) ob[0] = (uint16_t)hbits;
   }
 }
 

@@ -9,7 +9,7 @@ import ctypes
 
 import torch
 
-from ._lib import QhipKvBatch, QhipKvCache, QhipLinear, QhipProfEntry, check, load
+from ._lib import QhipKvBatch, QhipKvCache, QhipLinear, QhipLinearBatch, QhipProfEntry, QhipRows, check, load
 
 _GEOM = {8: (32, 34), 20: (32, 18), 12: (256, 144), 14: (256, 210), 13: (256, 176), 11: (256, 110),
          10: (256, 84), 23: (256, 136), 2: (32, 18), 3: (32, 20), 18: (256, 98), 21: (256, 110)}
@@ -493,6 +493,179 @@ def kv_attention(q: torch.Tensor, cache: KvCache, table: torch.Tensor, offsets: 
         cache.head_dim ** -0.5 if scale is None else scale, int(causal), window, out.data_ptr(), out.stride(0), out.stride(1),
         lse.data_ptr(), None if work is None else work.data_ptr(), 0 if work is None else work.numel(), _stream(dev)))
     return out, lse
+
+
+# ---- between a layer's products and its caches ------------------------------------------
+
+def _rows(name: str, t: torch.Tensor, device: int, like: torch.Tensor | None = None) -> QhipRows:
+    """Rows [tokens, dim] or [tokens, heads, dim] whose last dimension is contiguous, of the type (and shape) of `like`."""
+    if (t.dim() not in (2, 3) or (t.stride(-1) != 1 and t.shape[-1] != 1) or t.get_device() != device or t.dtype not in _KV_TYPES
+            or (like is not None and (t.dtype != like.dtype or t.shape != like.shape))):
+        kind = "a tensor [tokens, dim] or [tokens, heads, dim] of f32, f16 or bf16" if like is None else \
+            f"a tensor {list(like.shape)} of {like.dtype}"
+        raise ValueError(f"{name}: {kind} with a contiguous last dimension on the current GPU")
+    return QhipRows(t.data_ptr(), t.stride(0), t.stride(1) if t.dim() == 3 else 0)
+
+
+def _floats(name: str, t: torch.Tensor, shape: tuple, device: int) -> int:
+    if t.dtype != torch.float32 or t.shape != shape or t.get_device() != device or not t.is_contiguous():
+        raise ValueError(f"{name}: a contiguous f32 tensor {list(shape)} on the current GPU")
+    return t.data_ptr()
+
+
+def _rms_norm(x, weight, eps, residual, gate, out, ttype, xq):
+    dev = torch.cuda.current_device()
+    rows = _rows("x", x, dev)
+    more = [None if t is None else ctypes.byref(_rows(name, t, dev, x)) for name, t in (("residual", residual), ("gate", gate), ("out", out))]
+    tokens, heads, dim = x.shape[0], x.shape[1] if x.dim() == 3 else 1, x.shape[-1]
+    check("rms_norm", load().qhip_launch_rms_norm(
+        _KV_TYPES[x.dtype], ctypes.byref(rows), more[0], more[1], None if weight is None else _floats("weight", weight, (dim,), dev),
+        eps, more[2], ttype, xq, tokens, heads, dim, _stream(dev)))
+
+
+def rms_norm(x: torch.Tensor, weight: torch.Tensor | None, eps: float, residual: torch.Tensor | None = None,
+             gate: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """x / sqrt(mean(x^2) + eps) * weight over the last dimension of x [tokens, dim] or [tokens, heads, dim].
+
+    residual: x is added to it in place, and the sum is normalised.  gate: the result is multiplied by gate / (1 +
+    exp(-gate)).  weight: f32 [dim].  out may be x or gate."""
+    if out is None:
+        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    _rms_norm(x, weight, eps, residual, gate, out, 0, None)
+    return out
+
+
+def rms_norm_quantize(ttype: int, x: torch.Tensor, weight: torch.Tensor | None, eps: float, residual: torch.Tensor | None = None,
+                      gate: torch.Tensor | None = None, out: torch.Tensor | None = None,
+                      xq: torch.Tensor | None = None) -> torch.Tensor:
+    """rms_norm with its f32 result as the activation rows of weight type `ttype` (uint8 [tokens, act_row_bytes], the bytes
+    that quantize_act makes of it); out: the unquantized result as well."""
+    n = act_row_bytes(ttype, x.shape[-1] * (x.shape[1] if x.dim() == 3 else 1))
+    if xq is None:
+        xq = torch.empty((len(x), n), dtype=torch.uint8, device=x.device)
+    elif xq.dtype != torch.uint8 or xq.shape != (len(x), n) or not xq.is_contiguous() or xq.get_device() != torch.cuda.current_device():
+        raise ValueError(f"xq: a contiguous uint8 tensor [{len(x)}, {n}] on the current GPU")
+    _rms_norm(x, weight, eps, residual, gate, out, ttype, xq.data_ptr())
+    return xq
+
+
+class RopeTable:
+    """The frequencies of rotary positions: pair i of the first `rot_dim` values of a head turns by position * base^(-2 i /
+    rot_dim), scaled for contexts `factor` times the trained one: "linear", "ntk" or "yarn" (which blends between the pairs
+    that turn `fast` and `slow` times over `original` positions)."""
+
+    SCALINGS = {None: 0, "linear": 1, "ntk": 2, "yarn": 3}
+
+    def __init__(self, rot_dim: int, base: float = 10000.0, scaling: str | None = None, factor: float = 1.0, original: int = 0,
+                 fast: float = 32.0, slow: float = 1.0, device="cuda"):
+        if scaling not in self.SCALINGS:
+            raise ValueError(f"scaling: one of {list(self.SCALINGS)}")
+        _c_ints("rot_dim, original", rot_dim, original)
+        steps, gain = (ctypes.c_ulonglong * max(rot_dim // 2, 1))(), ctypes.c_float()
+        check("rope_steps", load().qhip_rope_steps(rot_dim, base, self.SCALINGS[scaling], factor, original, fast, slow, steps,
+                                                   ctypes.byref(gain)))
+        self.rot_dim, self.gain = rot_dim, gain.value
+        self.steps = torch.frombuffer(steps, dtype=torch.int64).to(device)
+
+
+def rope(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, table: RopeTable, interleaved: bool = False,
+         q_out: torch.Tensor | None = None, k_out: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor | None]:
+    """q [tokens, q_heads, dim] and k [tokens, k_heads, dim] (or None) with the first table.rot_dim values of every head
+    turned by their token's position (int32 [tokens], KvStep.positions).
+
+    Pairs are values i and i + rot_dim / 2, interleaved: 2 i and 2 i + 1.  q_out may be q, and k_out k."""
+    dev = torch.cuda.current_device()
+    tt, dim = _kv_rows("q", q, q.shape[-1], dev), q.shape[-1]
+    if q_out is None:
+        q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    k_heads, kr, ko = 0, None, None
+    if k is not None:
+        if _kv_rows("k", k, dim, dev) != tt or len(k) != len(q):
+            raise ValueError("k: [tokens, k_heads, dim] of q's type")
+        if k_out is None:
+            k_out = torch.empty(k.shape, dtype=k.dtype, device=k.device)
+        k_heads, kr, ko = k.shape[1], ctypes.byref(_rows("k", k, dev)), ctypes.byref(_rows("k_out", k_out, dev, k))
+    at = _ints("positions", positions, dev)
+    if len(positions) != len(q):
+        raise ValueError(f"positions: {len(q)} entries")
+    if table.steps.get_device() != dev:
+        raise ValueError("table: on the current GPU")
+    check("rope", load().qhip_launch_rope(
+        tt, ctypes.byref(_rows("q", q, dev)), ctypes.byref(_rows("q_out", q_out, dev, q)), q.shape[1], kr, ko, k_heads, dim,
+        table.rot_dim, table.steps.data_ptr(), table.gain, int(interleaved), at, len(q), _stream(dev)))
+    return q_out, k_out
+
+
+def _linear_states(states: torch.Tensor, device: int) -> None:
+    if states.dtype != torch.float32 or states.dim() != 4 or states.get_device() != device or not states.is_contiguous():
+        raise ValueError("states: a contiguous f32 tensor [states, v_heads, key_dim, value_dim] on the current GPU")
+
+
+def _linear_work(work: torch.Tensor, device: int) -> None:
+    if work.dtype != torch.uint8 or work.dim() != 1 or work.get_device() != device or not work.is_contiguous():
+        raise ValueError("work: a contiguous uint8 tensor on the current GPU (linear_attention_work)")
+
+
+def linear_attention_work(states: torch.Tensor, q: torch.Tensor, nseq: int, max_new: int, delta: bool = True,
+                          work: torch.Tensor | None = None) -> torch.Tensor | None:
+    """Workspace for linear_attention of q's tokens (None when none is needed), or `work` itself, an earlier one, if it is
+    large enough."""
+    dev = torch.cuda.current_device()
+    _linear_states(states, dev)
+    tt = _kv_rows("q", q, states.shape[2], dev)
+    _c_ints("nseq, max_new", nseq, max_new)
+    b = QhipLinearBatch(None, None, None, nseq, len(q), max_new, states.shape[0], q.shape[1], *states.shape[1:])
+    n = load().qhip_linear_attention_work_bytes(ctypes.byref(b), tt, int(delta))
+    if n < 0:
+        raise ValueError(f"bad (states {list(states.shape)}, q {list(q.shape)}, {nseq} sequences)")
+    if work is not None:
+        _linear_work(work, dev)
+        if work.numel() >= n:
+            return work
+    return torch.empty(n, dtype=torch.uint8, device=states.device) if n > 0 else None
+
+
+def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay: torch.Tensor, states: torch.Tensor,
+                     slots: torch.Tensor, offsets: torch.Tensor, max_new: int, beta: torch.Tensor | None = None,
+                     source: torch.Tensor | None = None, scale: float | None = None, work: torch.Tensor | None = None,
+                     out: torch.Tensor | None = None) -> torch.Tensor:
+    """Linear attention of packed tokens over states [n, v_heads, key_dim, value_dim] (f32): with a = exp(log_decay),
+    S <- a S + k^T u and out = scale q S, where u = v, or with `beta` (the delta rule) beta (v - k a S).
+
+    q, k [tokens, k_heads, key_dim], v [tokens, v_heads, value_dim]; log_decay, beta: f32 [tokens, v_heads].  Sequence i has
+    tokens offsets[i] .. offsets[i + 1], at most max_new, starts from state source[i] (-1: zeros; by default slots[i]) and
+    leaves its last state in slots[i] (-1: nowhere); no state that a sequence writes may be another's in the same call.
+    scale: 1 / sqrt(key_dim) by default.  Rows at or past offsets[-1] are not written."""
+    dev = torch.cuda.current_device()
+    _linear_states(states, dev)
+    n, v_heads, dk, dv = states.shape
+    tt, tokens, nseq = _kv_rows("q", q, dk, dev), len(q), len(slots)
+    if _kv_rows("k", k, dk, dev) != tt or k.shape != q.shape:
+        raise ValueError("k: as q")
+    if _kv_rows("v", v, dv, dev) != tt or v.shape != (tokens, v_heads, dv):
+        raise ValueError(f"v: [{tokens}, {v_heads}, {dv}] of q's type")
+    numbers = []
+    for name, t in (("log_decay", log_decay), ("beta", beta)):
+        if t is None:
+            numbers += [None, 0]
+            continue
+        if t.dtype != torch.float32 or t.shape != (tokens, v_heads) or t.get_device() != dev or (t.stride(1) != 1 and v_heads > 1):
+            raise ValueError(f"{name}: f32 [{tokens}, {v_heads}] with a contiguous last dimension on the current GPU")
+        numbers += [t.data_ptr(), t.stride(0)]
+    if len(offsets) != nseq + 1 or (source is not None and len(source) != nseq):
+        raise ValueError(f"offsets: {nseq + 1} entries, source: {nseq}")
+    if out is None:
+        out = torch.empty(v.shape, dtype=v.dtype, device=v.device)
+    if work is not None:
+        _linear_work(work, dev)
+    _c_ints("max_new", max_new)
+    b = QhipLinearBatch(_ints("offsets", offsets, dev), _ints("slots", slots, dev), None if source is None else _ints("source", source, dev),
+                        nseq, tokens, max_new, n, q.shape[1], v_heads, dk, dv)
+    check("linear_attention", load().qhip_launch_linear_attention(
+        ctypes.byref(b), tt, ctypes.byref(_rows("q", q, dev)), ctypes.byref(_rows("k", k, dev)), ctypes.byref(_rows("v", v, dev)),
+        *numbers, dk ** -0.5 if scale is None else scale, states.data_ptr(), ctypes.byref(_rows("out", out, dev, v)),
+        None if work is None else work.data_ptr(), 0 if work is None else work.numel(), _stream(dev)))
+    return out
 
 
 class Backend:
