@@ -497,30 +497,49 @@ def kv_attention(q: torch.Tensor, cache: KvCache, table: torch.Tensor, offsets: 
 
 # ---- between a layer's products and its caches ------------------------------------------
 
-def _rows(name: str, t: torch.Tensor, device: int, like: torch.Tensor | None = None) -> QhipRows:
-    """Rows [tokens, dim] or [tokens, heads, dim] whose last dimension is contiguous, of the type (and shape) of `like`."""
-    if (t.dim() not in (2, 3) or (t.stride(-1) != 1 and t.shape[-1] != 1) or t.get_device() != device or t.dtype not in _KV_TYPES
-            or (like is not None and (t.dtype != like.dtype or t.shape != like.shape))):
-        kind = "a tensor [tokens, dim] or [tokens, heads, dim] of f32, f16 or bf16" if like is None else \
-            f"a tensor {list(like.shape)} of {like.dtype}"
-        raise ValueError(f"{name}: {kind} with a contiguous last dimension on the current GPU")
-    return QhipRows(t.data_ptr(), t.stride(0), t.stride(1) if t.dim() == 3 else 0)
+# (each attribute of a tensor costs 0.1 to 0.3 us, and a call has up to twenty: shapes and strides are asked for once)
+def _rows(name: str, t: torch.Tensor, device: int, shape: torch.Size, dtype: torch.dtype) -> QhipRows:
+    """Rows of `shape` [tokens, dim] or [tokens, heads, dim] whose last dimension is contiguous."""
+    stride = t.stride()
+    if (t.dtype != dtype or t.shape != shape or t.get_device() != device or len(stride) not in (2, 3) or dtype not in _KV_TYPES
+            or (stride[-1] != 1 and shape[-1] != 1)):
+        raise ValueError(f"{name}: {list(shape)} of {dtype} (rows or heads of f32, f16 or bf16) with a contiguous last dimension on "
+                         "the current GPU")
+    return QhipRows(t.data_ptr(), stride[0], stride[1] if len(stride) == 3 else 0)
 
 
-def _floats(name: str, t: torch.Tensor, shape: tuple, device: int) -> int:
-    if t.dtype != torch.float32 or t.shape != shape or t.get_device() != device or not t.is_contiguous():
-        raise ValueError(f"{name}: a contiguous f32 tensor {list(shape)} on the current GPU")
-    return t.data_ptr()
+def _new_rows(shape: torch.Size, like: torch.Tensor) -> tuple[torch.Tensor, QhipRows]:
+    t = torch.empty_like(like)  # (torch.empty with a type and a device takes three times as long)
+    if t.shape != shape:
+        t = like.new_empty(shape)
+    stride = t.stride()
+    return t, QhipRows(t.data_ptr(), stride[0], stride[1] if len(stride) == 3 else 0)
 
 
 def _rms_norm(x, weight, eps, residual, gate, out, ttype, xq):
-    dev = torch.cuda.current_device()
-    rows = _rows("x", x, dev)
-    more = [None if t is None else ctypes.byref(_rows(name, t, dev, x)) for name, t in (("residual", residual), ("gate", gate), ("out", out))]
-    tokens, heads, dim = x.shape[0], x.shape[1] if x.dim() == 3 else 1, x.shape[-1]
+    dev, shape, dtype = torch.cuda.current_device(), x.shape, x.dtype
+    rows = _rows("x", x, dev, shape, dtype)
+    if ttype is None and out is None:
+        out, o = _new_rows(shape, x)
+    else:
+        o = None if out is None else _rows("out", out, dev, shape, dtype)
+    r = None if residual is None else _rows("residual", residual, dev, shape, dtype)
+    g = None if gate is None else _rows("gate", gate, dev, shape, dtype)
+    heads, dim, w = shape[1] if len(shape) == 3 else 1, shape[-1], None
+    if weight is not None:
+        if weight.dtype != torch.float32 or weight.shape != (dim,) or weight.get_device() != dev or not weight.is_contiguous():
+            raise ValueError(f"weight: a contiguous f32 tensor [{dim}] on the current GPU")
+        w = weight.data_ptr()
+    if ttype is not None:
+        n = act_row_bytes(ttype, heads * dim)
+        if xq is None:
+            xq = torch.empty((shape[0], n), dtype=torch.uint8, device=x.device)
+        elif xq.dtype != torch.uint8 or xq.shape != (shape[0], n) or not xq.is_contiguous() or xq.get_device() != dev:
+            raise ValueError(f"xq: a contiguous uint8 tensor [{shape[0]}, {n}] on the current GPU")
     check("rms_norm", load().qhip_launch_rms_norm(
-        _KV_TYPES[x.dtype], ctypes.byref(rows), more[0], more[1], None if weight is None else _floats("weight", weight, (dim,), dev),
-        eps, more[2], ttype, xq, tokens, heads, dim, _stream(dev)))
+        _KV_TYPES[dtype], rows, r, g, w, eps, o, ttype or 0, None if xq is None else xq.data_ptr(), shape[0], heads, dim,
+        _stream(dev)))
+    return out if ttype is None else xq
 
 
 def rms_norm(x: torch.Tensor, weight: torch.Tensor | None, eps: float, residual: torch.Tensor | None = None,
@@ -529,10 +548,7 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor | None, eps: float, residual:
 
     residual: x is added to it in place, and the sum is normalised.  gate: the result is multiplied by gate / (1 +
     exp(-gate)).  weight: f32 [dim].  out may be x or gate."""
-    if out is None:
-        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    _rms_norm(x, weight, eps, residual, gate, out, 0, None)
-    return out
+    return _rms_norm(x, weight, eps, residual, gate, out, None, None)
 
 
 def rms_norm_quantize(ttype: int, x: torch.Tensor, weight: torch.Tensor | None, eps: float, residual: torch.Tensor | None = None,
@@ -540,13 +556,7 @@ def rms_norm_quantize(ttype: int, x: torch.Tensor, weight: torch.Tensor | None, 
                       xq: torch.Tensor | None = None) -> torch.Tensor:
     """rms_norm with its f32 result as the activation rows of weight type `ttype` (uint8 [tokens, act_row_bytes], the bytes
     that quantize_act makes of it); out: the unquantized result as well."""
-    n = act_row_bytes(ttype, x.shape[-1] * (x.shape[1] if x.dim() == 3 else 1))
-    if xq is None:
-        xq = torch.empty((len(x), n), dtype=torch.uint8, device=x.device)
-    elif xq.dtype != torch.uint8 or xq.shape != (len(x), n) or not xq.is_contiguous() or xq.get_device() != torch.cuda.current_device():
-        raise ValueError(f"xq: a contiguous uint8 tensor [{len(x)}, {n}] on the current GPU")
-    _rms_norm(x, weight, eps, residual, gate, out, ttype, xq.data_ptr())
-    return xq
+    return _rms_norm(x, weight, eps, residual, gate, out, ttype, xq)
 
 
 class RopeTable:
@@ -566,6 +576,7 @@ class RopeTable:
                                                    ctypes.byref(gain)))
         self.rot_dim, self.gain = rot_dim, gain.value
         self.steps = torch.frombuffer(steps, dtype=torch.int64).to(device)
+        self.device, self.at = self.steps.get_device(), self.steps.data_ptr()
 
 
 def rope(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, table: RopeTable, interleaved: bool = False,
@@ -574,36 +585,45 @@ def rope(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, table
     turned by their token's position (int32 [tokens], KvStep.positions).
 
     Pairs are values i and i + rot_dim / 2, interleaved: 2 i and 2 i + 1.  q_out may be q, and k_out k."""
-    dev = torch.cuda.current_device()
-    tt, dim = _kv_rows("q", q, q.shape[-1], dev), q.shape[-1]
+    dev, shape, dtype = torch.cuda.current_device(), q.shape, q.dtype
+    if len(shape) != 3:
+        raise ValueError("q: [tokens, q_heads, dim]")
+    tokens, q_heads, dim = shape
+    qr, kr, ko, k_heads = _rows("q", q, dev, shape, dtype), None, None, 0
     if q_out is None:
-        q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    k_heads, kr, ko = 0, None, None
+        q_out, qo = _new_rows(shape, q)
+    else:
+        qo = _rows("q_out", q_out, dev, shape, dtype)
     if k is not None:
-        if _kv_rows("k", k, dim, dev) != tt or len(k) != len(q):
-            raise ValueError("k: [tokens, k_heads, dim] of q's type")
+        k_shape = k.shape
+        if len(k_shape) != 3 or k_shape[0] != tokens or k_shape[2] != dim:
+            raise ValueError(f"k: [{tokens}, k_heads, {dim}]")
+        k_heads, kr = k_shape[1], _rows("k", k, dev, k_shape, dtype)
         if k_out is None:
-            k_out = torch.empty(k.shape, dtype=k.dtype, device=k.device)
-        k_heads, kr, ko = k.shape[1], ctypes.byref(_rows("k", k, dev)), ctypes.byref(_rows("k_out", k_out, dev, k))
-    at = _ints("positions", positions, dev)
-    if len(positions) != len(q):
-        raise ValueError(f"positions: {len(q)} entries")
-    if table.steps.get_device() != dev:
+            k_out, ko = _new_rows(k_shape, k)
+        else:
+            ko = _rows("k_out", k_out, dev, k_shape, dtype)
+    if positions.shape != (tokens,):
+        raise ValueError(f"positions: {tokens} entries")
+    if table.device != dev:
         raise ValueError("table: on the current GPU")
     check("rope", load().qhip_launch_rope(
-        tt, ctypes.byref(_rows("q", q, dev)), ctypes.byref(_rows("q_out", q_out, dev, q)), q.shape[1], kr, ko, k_heads, dim,
-        table.rot_dim, table.steps.data_ptr(), table.gain, int(interleaved), at, len(q), _stream(dev)))
+        _KV_TYPES[dtype], qr, qo, q_heads, kr, ko, k_heads, dim, table.rot_dim, table.at, table.gain, int(interleaved),
+        _ints("positions", positions, dev), tokens, _stream(dev)))
     return q_out, k_out
 
 
-def _linear_states(states: torch.Tensor, device: int) -> None:
-    if states.dtype != torch.float32 or states.dim() != 4 or states.get_device() != device or not states.is_contiguous():
+def _linear_states(states: torch.Tensor, device: int) -> torch.Size:
+    shape = states.shape
+    if states.dtype != torch.float32 or len(shape) != 4 or states.get_device() != device or not states.is_contiguous():
         raise ValueError("states: a contiguous f32 tensor [states, v_heads, key_dim, value_dim] on the current GPU")
+    return shape
 
 
-def _linear_work(work: torch.Tensor, device: int) -> None:
+def _linear_work(work: torch.Tensor, device: int) -> int:
     if work.dtype != torch.uint8 or work.dim() != 1 or work.get_device() != device or not work.is_contiguous():
         raise ValueError("work: a contiguous uint8 tensor on the current GPU (linear_attention_work)")
+    return work.numel()
 
 
 def linear_attention_work(states: torch.Tensor, q: torch.Tensor, nseq: int, max_new: int, delta: bool = True,
@@ -611,17 +631,15 @@ def linear_attention_work(states: torch.Tensor, q: torch.Tensor, nseq: int, max_
     """Workspace for linear_attention of q's tokens (None when none is needed), or `work` itself, an earlier one, if it is
     large enough."""
     dev = torch.cuda.current_device()
-    _linear_states(states, dev)
-    tt = _kv_rows("q", q, states.shape[2], dev)
+    shape = _linear_states(states, dev)
+    tt = _kv_rows("q", q, shape[2], dev)
     _c_ints("nseq, max_new", nseq, max_new)
-    b = QhipLinearBatch(None, None, None, nseq, len(q), max_new, states.shape[0], q.shape[1], *states.shape[1:])
-    n = load().qhip_linear_attention_work_bytes(ctypes.byref(b), tt, int(delta))
+    b = QhipLinearBatch(None, None, None, nseq, q.shape[0], max_new, shape[0], q.shape[1], *shape[1:])
+    n = load().qhip_linear_attention_work_bytes(b, tt, int(delta))
     if n < 0:
-        raise ValueError(f"bad (states {list(states.shape)}, q {list(q.shape)}, {nseq} sequences)")
-    if work is not None:
-        _linear_work(work, dev)
-        if work.numel() >= n:
-            return work
+        raise ValueError(f"bad (states {list(shape)}, q {list(q.shape)}, {nseq} sequences)")
+    if work is not None and _linear_work(work, dev) >= n:
+        return work
     return torch.empty(n, dtype=torch.uint8, device=states.device) if n > 0 else None
 
 
@@ -636,35 +654,36 @@ def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_deca
     tokens offsets[i] .. offsets[i + 1], at most max_new, starts from state source[i] (-1: zeros; by default slots[i]) and
     leaves its last state in slots[i] (-1: nowhere); no state that a sequence writes may be another's in the same call.
     scale: 1 / sqrt(key_dim) by default.  Rows at or past offsets[-1] are not written."""
-    dev = torch.cuda.current_device()
-    _linear_states(states, dev)
-    n, v_heads, dk, dv = states.shape
-    tt, tokens, nseq = _kv_rows("q", q, dk, dev), len(q), len(slots)
-    if _kv_rows("k", k, dk, dev) != tt or k.shape != q.shape:
-        raise ValueError("k: as q")
-    if _kv_rows("v", v, dv, dev) != tt or v.shape != (tokens, v_heads, dv):
-        raise ValueError(f"v: [{tokens}, {v_heads}, {dv}] of q's type")
+    dev, q_shape, dtype = torch.cuda.current_device(), q.shape, q.dtype
+    n, v_heads, dk, dv = _linear_states(states, dev)
+    if len(q_shape) != 3 or q_shape[2] != dk:
+        raise ValueError(f"q: [tokens, k_heads, {dk}]")
+    tokens, k_heads, _ = q_shape
+    v_shape = torch.Size((tokens, v_heads, dv))
+    qr, kr, vr = _rows("q", q, dev, q_shape, dtype), _rows("k", k, dev, q_shape, dtype), _rows("v", v, dev, v_shape, dtype)
+    if out is None:
+        out, o = _new_rows(v_shape, v)
+    else:
+        o = _rows("out", out, dev, v_shape, dtype)
     numbers = []
     for name, t in (("log_decay", log_decay), ("beta", beta)):
         if t is None:
             numbers += [None, 0]
             continue
-        if t.dtype != torch.float32 or t.shape != (tokens, v_heads) or t.get_device() != dev or (t.stride(1) != 1 and v_heads > 1):
+        stride = t.stride()
+        if t.dtype != torch.float32 or t.shape != v_shape[:2] or t.get_device() != dev or (stride[1] != 1 and v_heads > 1):
             raise ValueError(f"{name}: f32 [{tokens}, {v_heads}] with a contiguous last dimension on the current GPU")
-        numbers += [t.data_ptr(), t.stride(0)]
-    if len(offsets) != nseq + 1 or (source is not None and len(source) != nseq):
-        raise ValueError(f"offsets: {nseq + 1} entries, source: {nseq}")
-    if out is None:
-        out = torch.empty(v.shape, dtype=v.dtype, device=v.device)
-    if work is not None:
-        _linear_work(work, dev)
+        numbers += [t.data_ptr(), stride[0]]
+    nseq = slots.shape[0] if slots.dim() == 1 else -1
+    if offsets.shape != (nseq + 1,) or (source is not None and source.shape != (nseq,)):
+        raise ValueError("slots [n], offsets [n + 1], source [n]")
     _c_ints("max_new", max_new)
     b = QhipLinearBatch(_ints("offsets", offsets, dev), _ints("slots", slots, dev), None if source is None else _ints("source", source, dev),
-                        nseq, tokens, max_new, n, q.shape[1], v_heads, dk, dv)
+                        nseq, tokens, max_new, n, k_heads, v_heads, dk, dv)
+    at, size = (None, 0) if work is None else (work.data_ptr(), _linear_work(work, dev))
     check("linear_attention", load().qhip_launch_linear_attention(
-        ctypes.byref(b), tt, ctypes.byref(_rows("q", q, dev)), ctypes.byref(_rows("k", k, dev)), ctypes.byref(_rows("v", v, dev)),
-        *numbers, dk ** -0.5 if scale is None else scale, states.data_ptr(), ctypes.byref(_rows("out", out, dev, v)),
-        None if work is None else work.data_ptr(), 0 if work is None else work.numel(), _stream(dev)))
+        b, _KV_TYPES[dtype], qr, kr, vr, *numbers, dk ** -0.5 if scale is None else scale, states.data_ptr(), o, at, size,
+        _stream(dev)))
     return out
 
 
