@@ -28,9 +28,9 @@ FLAGS = [
 ]
 
 
-# Per-file additions.  The MMQ files: keep MFMA accumulators in ordinary VGPRs, so
+# Per-file additions.  The MMQ files and the chunked linear attention: keep MFMA accumulators in ordinary VGPRs, so
 # the per-element scaling reads them without v_accvgpr_read copies.
-FILE_FLAGS = {f: ["-mllvm", "-amdgpu-mfma-vgpr-form"] for f in ("mmq.hip", "mmq_planes.hip")}
+FILE_FLAGS = {f: ["-mllvm", "-amdgpu-mfma-vgpr-form"] for f in ("mmq.hip", "mmq_planes.hip", "linear_attention.hip")}
 
 
 def _compile(src: Path) -> Path:

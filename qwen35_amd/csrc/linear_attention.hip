@@ -194,10 +194,13 @@ constexpr int kSome = sizeof(T) == 4 ? 3 : 2;  // of states read, weights inside
 // N planes of eight values (the last of two rounds to nearest, else bits are cut off:
 // no plane overflows)
 template <int N>
-__device__ __forceinline__ void split8(const float* x, u32x4* out) {
+__device__ __forceinline__ void split8(f32x4 x, f32x4 y, u32x4* out) {
   float rest[8];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) rest[i] = x[i];
+  for (int i = 0; i < 4; ++i) {
+    rest[i] = x[i];
+    rest[4 + i] = y[i];
+  }
 #pragma unroll
   for (int p = 0; p < N; ++p) {
     if (p == N - 1 && N < 3) {
@@ -209,8 +212,10 @@ __device__ __forceinline__ void split8(const float* x, u32x4* out) {
 #pragma unroll
       for (int i = 0; i < 4; ++i)
         out[p][i] = __builtin_amdgcn_perm(__float_as_uint(rest[2 * i + 1]), __float_as_uint(rest[2 * i]), 0x07060302u);
+      if (p + 1 < N) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) rest[i] -= __uint_as_float(__float_as_uint(rest[i]) & 0xFFFF0000u);
+        for (int i = 0; i < 8; ++i) rest[i] -= __uint_as_float(__float_as_uint(rest[i]) & 0xFFFF0000u);
+      }
     }
   }
 }
@@ -243,13 +248,14 @@ __device__ __forceinline__ f32x4 mfma_planes(const u32x4* a, const u32x4* b, f32
   return c;
 }
 
-// What prepare leaves for a chunk and value head: matrix operands, a plane of 16 rows
-// in 1 KB (lane l: row l mod 16, columns 4 (l / 16) ..+3 and 16 more), then exp(G),
+// What prepare leaves for a chunk and value head, as matrix operands (lane l: row l mod
+// 16, columns 4 (l / 16) ..+3): T's tiles (0, 0), (1, 0) and (1, 1) in f32; A's the
+// same way for f32 rows, else its two rows of tiles in two planes; then exp(G),
 // exp(G_31 - G) and exp(G_31).
 template <typename T, bool DELTA>
 struct ChunkWork {
-  static constexpr int solve = 0, inside = DELTA ? 2 * 3 * 1024 : 0, numbers = inside + 2 * kSome<T> * 1024,
-                       bytes = numbers + 512;
+  static constexpr bool whole = sizeof(T) == 4;
+  static constexpr int solve = 0, inside = DELTA ? 3 * 1024 : 0, numbers = inside + (whole ? 3 : 4) * 1024, bytes = numbers + 512;
 };
 
 // The chunk slot of a sequence's first: no two sequences' slots meet, and there are at
@@ -267,15 +273,18 @@ __device__ __forceinline__ void wave_sync() {
 template <typename T, int DK>
 struct RowTiles {
   u32x4 v[sizeof(T) == 4 ? DK / 16 : DK / 32];
-  __device__ __forceinline__ void load(const T* row, bool in) {
+  __device__ __forceinline__ void load(const T* row, bool in) {  // (the row of !in is there, but not this chunk's)
     const int g = (threadIdx.x & 63) >> 4;
     typedef uint32_t piece __attribute__((ext_vector_type(4), aligned(2)));
     constexpr int W = 16 / sizeof(T);  // elements of a piece
 #pragma unroll
     for (int s = 0; s < (int)(sizeof(v) / 16); ++s) {
-      v[s] = u32x4{0, 0, 0, 0};
-      if (in) v[s] = *(const piece*)(row + (4 * s + g) * W);
+      v[s] = *(const piece*)(row + (4 * s + g) * W);
     }
+#pragma unroll
+    for (int s = 0; s < (int)(sizeof(v) / 16); ++s)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[s][i] = in ? v[s][i] : 0u;
   }
 };
 template <typename T, int DK>
@@ -298,16 +307,24 @@ __device__ __forceinline__ f32x4 row_product(const RowTiles<T, DK>& a, const Row
 
 constexpr int kRowPad = 36;  // floats of a row of a 32 x 32 matrix in LDS
 
-// A wave takes a chunk of one key head and all of its value heads.
+__device__ __forceinline__ f32x4 mfma4(f32x4 a, f32x4 b, f32x4 c) {  // 16 columns of a against 16 rows of b
+#pragma unroll
+  for (int j = 0; j < 4; ++j) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[j], b[j], c, 0, 0, 0);
+  return c;
+}
+
+// A wave takes a chunk of two value heads, a half of its lanes for each where the work
+// goes by tokens or columns.
 template <typename T, int DK, bool DELTA>
 __global__ __launch_bounds__(256) void k_linear_prepare(LinearArgs a) {
   typedef ChunkWork<T, DELTA> W;
-  __shared__ __attribute__((aligned(16))) float s_mat[4][32 * kRowPad];
-  __shared__ double s_sum[4][32];
-  __shared__ __attribute__((aligned(16))) float s_beta[4][32];
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, g = lane >> 4, m = lane & 15;
-  const int slot = blockIdx.x, kh = blockIdx.y * 4 + wave;
-  if (kh >= a.k_heads) return;  // (waves do not wait for each other)
+  __shared__ __attribute__((aligned(16))) float s_mat[4][2][32 * kRowPad];
+  __shared__ double s_sum[4][2][32];
+  __shared__ __attribute__((aligned(16))) float s_beta[4][2][32];
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, g = lane >> 4, m = lane & 15, half = lane >> 5, token = lane & 31;
+  const int slot = blockIdx.x, head0 = __builtin_amdgcn_readfirstlane((blockIdx.y * 4 + wave) * 2);
+  if (head0 >= a.v_heads) return;  // (waves do not wait for each other)
+  const int heads = min(2, a.v_heads - head0);
   // the slot's sequence: the last whose first slot is not behind it
   int seq = -1;
   for (int i0 = 0; i0 < a.nseq; i0 += 64) {
@@ -324,376 +341,480 @@ __global__ __launch_bounds__(256) void k_linear_prepare(LinearArgs a) {
   if (chunk < 0 || n <= 0 || s.n <= a.few) return;
   const long t0 = s.first + (long)chunk * kChunk;
 
-  RowTiles<T, DK> k0, k1, q0, q1;
+  // G (times log2 e) in f64; a decay of exp(-200) is 0 in f32, and sums of -infinity
+  // have no differences
+  uint8_t* out = a.work + ((long)slot * a.v_heads + head0) * W::bytes;
   {
-    const T* k = (const T*)a.k + t0 * a.k_token + kh * a.k_head;
-    const T* q = (const T*)a.q + t0 * a.q_token + kh * a.q_head;
-    k0.load(k + m * a.k_token, m < n);
-    k1.load(k + (m + 16) * a.k_token, m + 16 < n);
-    q0.load(q + m * a.q_token, m < n);
-    q1.load(q + (m + 16) * a.q_token, m + 16 < n);
-  }
-  // tiles (0, 0), (1, 0), (1, 1): rows 16 i + 4 g + r, column 16 j + m
-  f32x4 kk[3], qk[3];
-  if constexpr (DELTA) {
-    kk[0] = row_product(k0, k0);
-    kk[1] = row_product(k1, k0);
-    kk[2] = row_product(k1, k1);
-  }
-  qk[0] = row_product(q0, k0);
-  qk[1] = row_product(q1, k0);
-  qk[2] = row_product(q1, k1);
-
-  float* mat = s_mat[wave];
-  for (int h = kh * a.group; h < (kh + 1) * a.group; ++h) {
-    uint8_t* out = a.work + ((long)slot * a.v_heads + h) * W::bytes;
-    // G in f64; a decay of exp(-200) is 0 in f32, and sums of -infinity have no differences
-    double sum = 0.0;
-    float beta = 0.0f;
-    if (lane < 32 && lane < n) {
-      const float x = a.log_decay[(t0 + lane) * a.decay_token + h];
-      sum = x < -200.0f ? -200.0 : (double)x;
-      if (DELTA) beta = a.beta[(t0 + lane) * a.beta_token + h];
-    }
+    const int h = head0 + min(half, heads - 1);
+    const long t = t0 + min(token, n - 1);
+    const float x = a.log_decay[t * a.decay_token + h];
+    const float beta = DELTA ? a.beta[t * a.beta_token + h] : 0.0f;
+    double sum = token < n ? (x < -200.0f ? -200.0 : (double)x) * 1.4426950408889634 : 0.0;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
       const double up = __shfl_up(sum, d, 64);
-      if ((lane & 31) >= d) sum += up;
+      if (token >= d) sum += up;
     }
+    s_sum[wave][half][token] = sum;
+    s_beta[wave][half][token] = token < n ? beta : 0.0f;
     wave_sync();
-    if (lane < 32) {
-      s_sum[wave][lane] = sum;
-      s_beta[wave][lane] = beta;
+    const double last = s_sum[wave][half][31];
+    if (half < heads) {
+      float* numbers = (float*)(out + half * W::bytes + W::numbers);
+      numbers[token] = __builtin_amdgcn_exp2f((float)sum);
+      numbers[32 + token] = __builtin_amdgcn_exp2f((float)(last - sum));
+      if (token == 0) numbers[64] = __builtin_amdgcn_exp2f((float)last);
     }
-    wave_sync();
-    const double last = s_sum[wave][31];
-    if (lane < 32) {
-      float* numbers = (float*)(out + W::numbers);
-      numbers[lane] = expf((float)sum);
-      numbers[32 + lane] = expf((float)(last - sum));
-      if (lane == 0) numbers[64] = expf((float)last);
+  }
+
+  // tiles (0, 0), (1, 0), (1, 1): rows 16 i + 4 g + r, column 16 j + m
+  f32x4 kk[3], qk[3], in[2][3];
+#pragma unroll
+  for (int x = 0; x < 2; ++x) {
+    if (x >= heads) break;
+    const int kh = (head0 + x) / a.group;
+    if (x == 0 || kh != (head0 + x - 1) / a.group) {
+      RowTiles<T, DK> k0, k1, q0, q1;
+      const T* k = (const T*)a.k + t0 * a.k_token + kh * a.k_head;
+      const T* q = (const T*)a.q + t0 * a.q_token + kh * a.q_head;
+      k0.load(k + min(m, n - 1) * a.k_token, m < n);
+      k1.load(k + min(m + 16, n - 1) * a.k_token, m + 16 < n);
+      q0.load(q + min(m, n - 1) * a.q_token, m < n);
+      q1.load(q + min(m + 16, n - 1) * a.q_token, m + 16 < n);
+      if constexpr (DELTA) {
+        kk[0] = row_product(k0, k0);
+        kk[1] = row_product(k1, k0);
+        kk[2] = row_product(k1, k1);
+      }
+      qk[0] = row_product(q0, k0);
+      qk[1] = row_product(q1, k0);
+      qk[2] = row_product(q1, k1);
     }
-    f32x4 in[3];
+    float* mat = s_mat[wave][x];
 #pragma unroll
     for (int t = 0; t < 3; ++t) {
       const int i0 = t > 0 ? 16 : 0, j = (t == 2 ? 16 : 0) + m;
-      const double gj = s_sum[wave][j];
+      const double gj = s_sum[wave][x][j];
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         const int i = i0 + 4 * g + r;
-        const float d = expf((float)(s_sum[wave][i] - gj));
-        in[t][r] = i >= j && i < n ? a.scale * qk[t][r] * d : 0.0f;
-        if constexpr (DELTA) mat[i * kRowPad + j] = i > j ? s_beta[wave][i] * kk[t][r] * d : 0.0f;
+        const float d = __builtin_amdgcn_exp2f((float)(s_sum[wave][x][i] - gj));
+        in[x][t][r] = i >= j && i < n ? a.scale * qk[t][r] * d : 0.0f;
+        if constexpr (DELTA) mat[i * kRowPad + j] = i > j ? s_beta[wave][x][i] * kk[t][r] * d : 0.0f;
       }
     }
-    wave_sync();
-    if constexpr (DELTA) {
-      // the two blocks of 16 on the diagonal by substitution, a column a lane
-      const int b = (lane & 16), c = m;
+  }
+  wave_sync();
+  if constexpr (DELTA) {
+    // (1 + L)^-1: the two blocks of 16 on the diagonal by substitution, a column a lane
+    {
+      float* mat = s_mat[wave][half];
+      const int b = lane & 16;
       float x[16];
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
-        float y = i == c ? 1.0f : 0.0f;
+        float y = i == m ? 1.0f : 0.0f;
 #pragma unroll
         for (int l = 0; l < i; ++l) y = __builtin_fmaf(-mat[(b + i) * kRowPad + b + l], x[l], y);
-        x[i] = i < c ? 0.0f : y;
-      }
-      // the block below: -X22 L21 X11, on the matrix cores (column 4 g + j of one is row 4 g + j of the other)
-      const f32x4 low = *(const f32x4*)(mat + (16 + m) * kRowPad + 4 * g);
-      wave_sync();
-      if (lane < 32) {
-#pragma unroll
-        for (int i = 0; i < 16; ++i) mat[(b + i) * kRowPad + b + c] = x[i];
+        x[i] = i < m ? 0.0f : y;
       }
       wave_sync();
-      f32x4 p = {0.0f, 0.0f, 0.0f, 0.0f}, y = p;
+      if (half < heads) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) p = __builtin_amdgcn_mfma_f32_16x16x4f32(low[j], mat[(4 * g + j) * kRowPad + m], p, 0, 0, 0);
-      const f32x4 diag = *(const f32x4*)(mat + (16 + m) * kRowPad + 16 + 4 * g);
+        for (int i = 0; i < 16; ++i) mat[(b + i) * kRowPad + b + m] = x[i];
+      }
+      wave_sync();
+    }
 #pragma unroll
-      for (int j = 0; j < 4; ++j) y = __builtin_amdgcn_mfma_f32_16x16x4f32(-diag[j], p[j], y, 0, 0, 0);
+    for (int x = 0; x < 2; ++x) {
+      if (x >= heads) break;
+      // the block below them: -X22 L21 X11 (a result's rows 4 g + r are an operand's)
+      float* mat = s_mat[wave][x];
+      const float* row = mat + m * kRowPad + 4 * g;
+      f32x4 top, low = *(const f32x4*)(row + 16 * kRowPad), diag = *(const f32x4*)(row + 16 * kRowPad + 16);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) top[j] = mat[(4 * g + j) * kRowPad + m];
+      const f32x4 none = {0.0f, 0.0f, 0.0f, 0.0f};
+      const f32x4 y = mfma4(-diag, mfma4(low, top, none), none);
+      wave_sync();
 #pragma unroll
       for (int r = 0; r < 4; ++r) mat[(16 + 4 * g + r) * kRowPad + m] = y[r];
       wave_sync();
-    }
-    // rows in the order of a matrix operand, split into planes
-    auto leave = [&](int at, auto planes, bool with_beta) {
-      constexpr int N = decltype(planes)::value;
+      // T = X diag(beta)
+      const f32x4 b0 = *(const f32x4*)(s_beta[wave][x] + 4 * g), b1 = *(const f32x4*)(s_beta[wave][x] + 16 + 4 * g);
+      f32x4 t00 = *(const f32x4*)row, t10 = *(const f32x4*)(row + 16 * kRowPad) * b0;
 #pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        float v[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const int j = (e & 4) * 4 + 4 * g + (e & 3);
-          v[e] = t == 0 && e >= 4 ? 0.0f : mat[(16 * t + m) * kRowPad + j];
-          if (with_beta) v[e] = j <= 16 * t + m ? v[e] * s_beta[wave][j] : 0.0f;
-        }
-        u32x4 planes_of[N];
-        split8<N>(v, planes_of);
-#pragma unroll
-        for (int q = 0; q < N; ++q) *(u32x4*)(out + at + (t * N + q) * 1024 + lane * 16) = planes_of[q];
+      for (int j = 0; j < 4; ++j) {  // (nothing above the diagonal, whatever beta holds)
+        t00[j] = 4 * g + j <= m ? t00[j] * b0[j] : 0.0f;
+        diag[j] = 4 * g + j <= m ? diag[j] * b1[j] : 0.0f;
       }
-    };
-    if constexpr (DELTA) {
-      leave(W::solve, std::integral_constant<int, 3>{}, true);
-      wave_sync();
+      f32x4* to = (f32x4*)(out + x * W::bytes + W::solve) + lane;
+      to[0] = t00;
+      to[64] = t10;
+      to[128] = diag;
     }
+    wave_sync();
+  }
+#pragma unroll
+  for (int x = 0; x < 2; ++x) {
+    if (x >= heads) break;
+    float* mat = s_mat[wave][x];
 #pragma unroll
     for (int t = 0; t < 3; ++t) {
       const int i0 = t > 0 ? 16 : 0, j = (t == 2 ? 16 : 0) + m;
 #pragma unroll
-      for (int r = 0; r < 4; ++r) mat[(i0 + 4 * g + r) * kRowPad + j] = in[t][r];
+      for (int r = 0; r < 4; ++r) mat[(i0 + 4 * g + r) * kRowPad + j] = in[x][t][r];
     }
-    wave_sync();
-    leave(W::inside, std::integral_constant<int, kSome<T>>{}, false);
+  }
+  wave_sync();
+#pragma unroll
+  for (int x = 0; x < 2; ++x) {
+    if (x >= heads) break;
+    const float* row = s_mat[wave][x] + m * kRowPad + 4 * g;
+    const f32x4 none = {0.0f, 0.0f, 0.0f, 0.0f};
+    const f32x4 t00 = *(const f32x4*)row, t10 = *(const f32x4*)(row + 16 * kRowPad), t11 = *(const f32x4*)(row + 16 * kRowPad + 16);
+    u32x4* to = (u32x4*)(out + x * W::bytes + W::inside) + lane;
+    if constexpr (W::whole) {
+      to[0] = __builtin_bit_cast(u32x4, t00);
+      to[64] = __builtin_bit_cast(u32x4, t10);
+      to[128] = __builtin_bit_cast(u32x4, t11);
+    } else {
+      u32x4 planes[2];
+      split8<2>(t00, none, planes);
+      to[0] = planes[0];
+      to[64] = planes[1];
+      split8<2>(t10, t11, planes);
+      to[128] = planes[0];
+      to[192] = planes[1];
+    }
   }
 }
 
-// A workgroup's four waves have 16 columns each and share the chunk's keys and queries
-// in LDS, as matrix operands: rows of 16 tokens (for products with the state), and of
-// 16 dimensions (for its update).
-template <typename T, int DK>
-struct ScanLds {
-  static constexpr int P = kPlanes<T>;
-  // a plane of 16 rows: 1 KB and a little, so that the stores of a row's pieces and
-  // of a column's fall on all banks
-  static constexpr int group = 272, tile = 4 * group, across = 1040;
-  static constexpr int keys = 0, queries = P * (DK / 16) * tile, turned = 2 * queries, buffer = turned + P * (DK / 16) * across;
-};
-
+// DK / 32 waves have the same 16 columns, 32 rows of the state each: they share the
+// products with the state out between them, hand their parts round in LDS (one
+// barrier a chunk), and go on with the sums by themselves.
 template <typename T, int DK, bool DELTA>
 __global__ __launch_bounds__(256) void k_linear_scan(LinearArgs a) {
   typedef ChunkWork<T, DELTA> W;
-  typedef ScanLds<T, DK> L;
-  constexpr int P = L::P, TILES = DK / 16, STEPS = DK / 32, SOME = kSome<T>;
-  __shared__ __attribute__((aligned(16))) uint8_t lds[2 * L::buffer];
-  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, g = lane >> 4, m = lane & 15;
-  const int seq = blockIdx.z, head = blockIdx.y, col = blockIdx.x * 64 + wave * 16 + m;
+  constexpr bool F32 = sizeof(T) == 4;       // f32 rows: f32 products throughout
+  constexpr int P = F32 ? 1 : kPlanes<T>;    // planes of keys and queries
+  constexpr int PARTS = DK / 32, SETS = 4 / PARTS, COLS = 16 * SETS;
+  // the keys of a chunk, turned: operands of 16 dimensions and 32 tokens.  A tile is 1 KB
+  // (f32: two, of 16 tokens) and 16 bytes, so that a thread's stores fall on all banks.
+  constexpr int TURNED = F32 ? 2 * 1024 + 16 : 1024 + 16, KEYS = P * (DK / 16) * TURNED;
+  __shared__ __attribute__((aligned(16))) uint8_t s_keys[2 * KEYS];
+  __shared__ f32x4 s_part[2][SETS][4][PARTS][64];
+  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, g = lane >> 4, m = lane & 15;
+  const int set = wave / PARTS, part = wave % PARTS;
+  // the workgroups of a sequence's head follow each other on one XCD
+  const int blocks = a.value_dim / COLS, id = (int)blockIdx.x;
+  const int pair = id / (8 * blocks) * 8 + (id & 7), seq = pair / a.v_heads, head = pair - seq * a.v_heads;
+  if (seq >= a.nseq) return;
+  const int col = (id >> 3) % blocks * COLS + set * 16 + m;
   const LinearSeq s = linear_seq(a, seq, head, DK);
   if (s.n <= a.few) return;
-  const int kh = head / a.group, chunks = (s.n + kChunk - 1) / kChunk;
-  const uint8_t* work = a.work + (first_slot(s, seq) * a.v_heads + head) * W::bytes;
-  const long work_step = (long)a.v_heads * W::bytes;
-  const T* k = (const T*)a.k + s.first * a.k_token + kh * a.k_head;
-  const T* q = (const T*)a.q + s.first * a.q_token + kh * a.q_head;
-  const T* v = (const T*)a.v + s.first * a.v_token + head * a.v_head + col;
-  T* out = (T*)a.out + s.first * a.out_token + head * a.out_head + col;
+  const int kh = head / a.group, chunks = (s.n + kChunk - 1) / kChunk, tail = s.n - (chunks - 1) * kChunk;
 
-  // state: tile i has rows 16 i + 4 g + r of the wave's columns
-  f32x4 st[TILES];
+  // state: tile i has rows 16 i + 4 g + r of the wave's 32, and the wave's columns
+  f32x4 st[2];
+  const long state_at = (long)(32 * part + 4 * g) * a.value_dim + col;
 #pragma unroll
-  for (int i = 0; i < TILES; ++i)
+  for (int i = 0; i < 2; ++i)
 #pragma unroll
     for (int r = 0; r < 4; ++r)
-      st[i][r] = s.from ? s.from[(long)(16 * i + 4 * g + r) * a.value_dim + col] : s.bad ? __builtin_nanf("") : 0.0f;
+      st[i][r] = s.from ? s.from[state_at + (16 * i + r) * a.value_dim] : s.bad ? __builtin_nanf("") : 0.0f;
 
-  // four tokens x four dimensions of keys or queries a thread
-  constexpr int BLOCKS = 8 * (DK / 4), EACH = BLOCKS / 128;  // of one of them; of both a thread
-  typedef T Four __attribute__((ext_vector_type(4)));
-  struct FourRows {
-    Four row[4];
-  } held[EACH];
-  auto block_of = [&](int e, bool& keys, int& tq, int& dq) {
-    const int b = EACH == 2 ? tid : tid & 127;
-    keys = EACH == 2 ? e == 0 : tid < 128;
-    dq = b & (DK / 4 - 1);
-    tq = b / (DK / 4);
+  // Everything of a chunk is loaded for the next one when the present one is done with
+  // it, without branches: uniform bases that go on by 32 tokens, offsets of 32 bits, and
+  // the last token's in the place of those behind it.
+  const char* k_at = (const char*)((const T*)a.k + s.first * a.k_token + kh * a.k_head);
+  const char* q_at = (const char*)((const T*)a.q + s.first * a.q_token + kh * a.q_head);
+  const char* v_at = (const char*)((const T*)a.v + s.first * a.v_token + head * a.v_head);
+  char* out_at = (char*)((T*)a.out + s.first * a.out_token + head * a.out_head);
+  // (global memory by name: through a flat address, a load would count as one of LDS too)
+  typedef const __attribute__((address_space(1))) uint8_t* Work;
+  Work work = (Work)a.work + (first_slot(s, seq) * a.v_heads + head) * W::bytes;
+  const long k_step = kChunk * a.k_token * (long)sizeof(T), q_step = kChunk * a.q_token * (long)sizeof(T),
+             v_step = kChunk * a.v_token * (long)sizeof(T), out_step = kChunk * a.out_token * (long)sizeof(T),
+             work_step = (long)a.v_heads * W::bytes;
+
+  typedef typename std::conditional<F32, u32x4, u32x2>::type Four;  // elements
+  typedef typename std::conditional<F32, uint32_t, uint16_t>::type Word;
+  typedef uint32_t four __attribute__((ext_vector_type(sizeof(Four) / 4), aligned(sizeof(Word))));
+  // rows 16 t + m: dimensions 4 g ..+3 of the wave's 32 and 16 more
+  Four kr[2][2], qr[2][2];
+  // four tokens x four dimensions a thread, to be turned (DK = 64: every second wave)
+  const int dq = tid & (DK / 4 - 1), tq = tid / (DK / 4) & 7;
+  const bool turns = tid < 2 * DK;
+  Four held[4];
+  T val[8];
+  uint32_t k_off[2], q_off[2], held_off[4], v_off[8];
+  auto place = [&](int rows) {  // of a chunk with that many tokens
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      k_off[t] = (uint32_t)(min(16 * t + m, rows - 1) * (int)a.k_token + 32 * part + 4 * g) * (uint32_t)sizeof(T);
+      q_off[t] = (uint32_t)(min(16 * t + m, rows - 1) * (int)a.q_token + 32 * part + 4 * g) * (uint32_t)sizeof(T);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) held_off[i] = (uint32_t)(min(4 * tq + i, rows - 1) * (int)a.k_token + 4 * dq) * (uint32_t)sizeof(T);
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      v_off[e] = (uint32_t)(min((e & 4) * 4 + 4 * g + (e & 3), rows - 1) * (int)a.v_token + col) * (uint32_t)sizeof(T);
   };
-  auto fetch = [&](int c) {
+  auto fetch_rows = [&](const char* k, const char* q) {
 #pragma unroll
-    for (int e = 0; e < EACH; ++e) {
-      bool keys;
-      int tq, dq;
-      block_of(e, keys, tq, dq);
-      const long stride = keys ? a.k_token : a.q_token;
-      const T* from = (keys ? k : q) + 4 * dq;
+    for (int t = 0; t < 2; ++t)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int t = c * kChunk + 4 * tq + i;
-        typedef T four __attribute__((ext_vector_type(4), aligned(sizeof(T))));
-        held[e].row[i] = Four{(T)0.0f, (T)0.0f, (T)0.0f, (T)0.0f};
-        if (t < s.n) held[e].row[i] = *(const four*)(from + t * stride);
+      for (int h = 0; h < 2; ++h) {
+        if (DELTA) kr[t][h] = *(const four*)(k + k_off[t] + 16 * h * sizeof(T));
+        qr[t][h] = *(const four*)(q + q_off[t] + 16 * h * sizeof(T));
       }
+  };
+  auto fetch_held = [&](const char* k) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) held[i] = *(const four*)(k + held_off[i]);
+  };
+  auto fetch_values = [&](const char* v) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) val[e] = *(const T*)(v + v_off[e]);
+  };
+  typedef const __attribute__((address_space(1))) f32x4* GlobalF4;
+  f32x4 solve[3], since[2], left[2];
+  f32x4 inside[3];  // f32 rows: the three tiles; else two planes of the wave's output tile
+  float total;
+  const int out_tile = part & 1;  // of the chunk's two, and of its rows 4 g + r those from out_row on
+  constexpr int OUT_ROWS = PARTS == 4 ? 2 : 4;
+  const int out_row = PARTS == 4 ? part & 2 : 0;
+  auto fetch_solve = [&](Work w) {
+    if constexpr (DELTA) {
+#pragma unroll
+      for (int i = 0; i < 3; ++i) solve[i] = *(GlobalF4)(w + W::solve + i * 1024 + lane * 16);
+#pragma unroll
+      for (int t = 0; t < 2; ++t) since[t] = *(GlobalF4)(w + W::numbers + (16 * t + 4 * g) * 4);
     }
   };
-  auto put = [&](int buffer) {
-    uint8_t* to = lds + buffer * L::buffer;
+  auto fetch_left = [&](Work w) {
 #pragma unroll
-    for (int e = 0; e < EACH; ++e) {
-      bool keys;
-      int tq, dq;
-      block_of(e, keys, tq, dq);
-      float x[4][4];
+    for (int t = 0; t < 2; ++t) left[t] = *(GlobalF4)(w + W::numbers + (32 + 16 * t + 4 * g) * 4);
+    total = *(const __attribute__((address_space(1))) float*)(w + W::numbers + 256);
+  };
+  f32x4 out_since;
+  auto fetch_inside = [&](Work w) {
+#pragma unroll
+    for (int i = 0; i < (F32 ? 3 : 2); ++i) inside[i] = *(GlobalF4)(w + W::inside + (F32 ? i : 2 * out_tile + i) * 1024 + lane * 16);
+    out_since = *(GlobalF4)(w + W::numbers + (16 * out_tile + 4 * g) * 4);
+  };
+  // the held keys into LDS, turned; `rows` of the chunk are there
+  uint8_t* const to_turned = s_keys + (dq >> 2) * TURNED + (dq & 3) * 64 +
+                             (F32 ? (tq >> 2) * 1024 + (tq & 3) * 256 : (tq & 3) * 256 + (tq >> 2) * 8);
+  auto turn = [&](int buffer, int rows) {
+    if (rows < kChunk) {
 #pragma unroll
       for (int i = 0; i < 4; ++i)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) x[i][j] = (float)held[e].row[i][j];
+        for (int j = 0; j < (int)(sizeof(Four) / 4); ++j) held[i][j] = 4 * tq + i < rows ? held[i][j] : 0u;
+    }
+    if constexpr (F32) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) *(u32x4*)(to_turned + buffer + j * 16) = u32x4{held[0][j], held[1][j], held[2][j], held[3][j]};
+    } else {
+      u32x2 planes[4][P];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        u32x2 planes[P];
-        split4<P>(x[i], planes);
-        const int t = 4 * tq + i;
-#pragma unroll
-        for (int p = 0; p < P; ++p)
-          *(u32x2*)(to + (keys ? L::keys : L::queries) + ((p * 2 + (t >> 4)) * STEPS + (dq >> 3)) * L::tile + (dq & 3) * L::group +
-                    (t & 15) * 16 + ((dq >> 2) & 1) * 8) = planes[p];
+        if constexpr (P == 1) {
+          planes[i][0] = held[i];
+        } else {
+          typedef T Four_t __attribute__((ext_vector_type(4)));
+          const Four_t x = __builtin_bit_cast(Four_t, held[i]);
+          const float y[4] = {(float)x[0], (float)x[1], (float)x[2], (float)x[3]};
+          split4<P>(y, planes[i]);
+        }
       }
-      if (keys) {
+#pragma unroll
+      for (int p = 0; p < P; ++p)
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const float y[4] = {x[0][j], x[1][j], x[2][j], x[3][j]};
-          u32x2 planes[P];
-          split4<P>(y, planes);
-#pragma unroll
-          for (int p = 0; p < P; ++p)
-            *(u32x2*)(to + L::turned + (p * TILES + (dq >> 2)) * L::across + (tq & 3) * 256 + (4 * (dq & 3) + j) * 16 + (tq >> 2) * 8) =
-                planes[p];
+          const uint32_t pick = j & 1 ? 0x07060302u : 0x05040100u;
+          *(u32x2*)(to_turned + buffer + p * (DK / 16) * TURNED + j * 16) =
+              u32x2{__builtin_amdgcn_perm(planes[1][p][j >> 1], planes[0][p][j >> 1], pick),
+                    __builtin_amdgcn_perm(planes[3][p][j >> 1], planes[2][p][j >> 1], pick)};
         }
-      }
     }
   };
-  // a chunk's operands from prepare, and its values: rows 16 t + 4 g + r
-  u32x4 solve[2][3], inside[2][SOME];
-  f32x4 since[2], left[2];
-  float total, val[8];
-  auto fetch_work = [&](int c) {
-    const uint8_t* w = work + c * work_step;
+  // a part of 16 rows' product with the state
+  u32x4 sp[2];
+  auto with_state = [&](const Four(&row)[2]) {
+    f32x4 c = {0.0f, 0.0f, 0.0f, 0.0f};
+    if constexpr (F32) {
+      c = mfma4(__builtin_bit_cast(f32x4, row[0]), st[0], c);
+      return mfma4(__builtin_bit_cast(f32x4, row[1]), st[1], c);
+    } else if constexpr (P == 1) {
+      const u32x4 x[1] = {u32x4{row[0][0], row[0][1], row[1][0], row[1][1]}};
+      return mfma_planes<1, 2>(x, sp, c);
+    } else {
+      typedef T Four_t __attribute__((ext_vector_type(4)));
+      f32x4 y[2];
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      if constexpr (DELTA) {
-#pragma unroll
-        for (int p = 0; p < 3; ++p) solve[t][p] = *(const u32x4*)(w + W::solve + (t * 3 + p) * 1024 + lane * 16);
+      for (int h = 0; h < 2; ++h) {
+        const Four_t z = __builtin_bit_cast(Four_t, row[h]);
+        y[h] = f32x4{(float)z[0], (float)z[1], (float)z[2], (float)z[3]};
       }
-#pragma unroll
-      for (int p = 0; p < SOME; ++p) inside[t][p] = *(const u32x4*)(w + W::inside + (t * SOME + p) * 1024 + lane * 16);
-      since[t] = *(const f32x4*)(w + W::numbers + (16 * t + 4 * g) * 4);
-      left[t] = *(const f32x4*)(w + W::numbers + (32 + 16 * t + 4 * g) * 4);
+      u32x4 x[P];
+      split8<P>(y[0], y[1], x);
+      return mfma_planes<P, 2>(x, sp, c);
     }
-    total = *(const float*)(w + W::numbers + 256);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const int t = c * kChunk + (e & 4) * 4 + 4 * g + (e & 3);
-      val[e] = t < s.n ? (float)v[t * a.v_token] : 0.0f;
-    }
-  };
-  auto operand = [&](int at, u32x4(&x)[P], int plane_bytes) {
-#pragma unroll
-    for (int p = 0; p < P; ++p) x[p] = *(const u32x4*)(lds + at + p * plane_bytes);
   };
 
-  fetch(0);
-  put(0);
-  __syncthreads();
+  place(chunks > 1 ? kChunk : tail);
+  fetch_rows(k_at, q_at);
+  fetch_held(k_at);
+  fetch_values(v_at);
+  fetch_solve(work);
+  fetch_left(work);
+  fetch_inside(work);
   for (int c = 0; c < chunks; ++c) {
-    fetch_work(c);
-    if (c + 1 < chunks) fetch(c + 1);
-    const int base = (c & 1) * L::buffer;
-    // Q S and K S
-    f32x4 qs[2] = {}, ks[2] = {};
-#pragma unroll
-    for (int step = 0; step < STEPS; ++step) {
-      float x[8];
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        x[r] = st[2 * step][r];
-        x[4 + r] = st[2 * step + 1][r];
-      }
-      u32x4 sp[SOME];
-      split8<SOME>(x, sp);
-#pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        const int at = base + (t * STEPS + step) * L::tile + g * L::group + m * 16;
-        u32x4 x[P];
-        if constexpr (DELTA) {
-          operand(at + L::keys, x, 2 * STEPS * L::tile);
-          ks[t] = mfma_planes<P, SOME>(x, sp, ks[t]);
-        }
-        operand(at + L::queries, x, 2 * STEPS * L::tile);
-        qs[t] = mfma_planes<P, SOME>(x, sp, qs[t]);
-      }
+    const bool more = c + 1 < chunks;
+    const int rows = more ? kChunk : tail, buffer = (c & 1) * KEYS;
+    if (more) {
+      work += work_step;
+      v_at += v_step;
+      k_at += k_step;
+      q_at += q_step;
+      if (c + 2 == chunks && tail < kChunk) place(tail);
     }
-    // U
-    float u[8];
+    // this wave's part of K S and Q S
+    if constexpr (!F32) split8<2>(st[0], st[1], sp);
+    f32x4(*parts)[PARTS][64] = s_part[c & 1][set];
+    if (turns) turn(buffer, rows);
+    fetch_held(k_at);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) u[e] = DELTA ? val[e] - since[e >> 2][e & 3] * ks[e >> 2][e & 3] : val[e];
+    for (int t = 0; t < 2; ++t) {
+      if (DELTA) parts[t][part][lane] = with_state(kr[t]);
+      parts[2 + t][part][lane] = with_state(qr[t]);
+    }
+    fetch_rows(k_at, q_at);
+    __syncthreads();  // (the buffers after next are written behind the next chunk's barrier)
+    // what U is made of, then U
+    f32x4 u[2];
+    float sum = 0.0f;
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+#pragma unroll
+      for (int r = 0; r < 4; ++r) u[t][r] = (float)val[4 * t + r];
+      if (rows < kChunk) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) u[t][r] = 16 * t + 4 * g + r < rows ? u[t][r] : 0.0f;
+      }
+      if constexpr (DELTA) {
+        f32x4 ks = parts[t][0][lane];
+#pragma unroll
+        for (int i = 1; i < PARTS; ++i) ks += parts[t][i][lane];
+        // (rows behind the sequence's end have the last row's keys: their T is 0)
+        u[t] -= since[t] * ks;
+      }
+#pragma unroll
+      for (int r = 0; r < 4; ++r) sum = __builtin_fmaf(u[t][r], 0.0f, sum);
+    }
+    fetch_values(v_at);
     // a value that is not finite spoils its column from its token on; in a product it
     // would spoil the tokens before as well (0 * NaN), so it stays out of them
+    const bool any = __ballot(sum != 0.0f) != 0;
     int spoilt = kChunk;  // the column's first such token
-#pragma unroll
-    for (int e = 7; e >= 0; --e)
-      if (!(__builtin_fabsf(u[e]) < INFINITY)) spoilt = (e & 4) * 4 + 4 * g + (e & 3);
-    const bool any = __ballot(spoilt < kChunk) != 0;
     auto clear = [&]() {
 #pragma unroll
       for (int e = 0; e < 8; ++e)
-        if ((e & 4) * 4 + 4 * g + (e & 3) >= spoilt) u[e] = 0.0f;
+        if ((e & 4) * 4 + 4 * g + (e & 3) >= spoilt) u[e >> 2][e & 3] = 0.0f;
     };
     if (any) {
+#pragma unroll
+      for (int e = 7; e >= 0; --e)
+        if (!(__builtin_fabsf(u[e >> 2][e & 3]) < INFINITY)) spoilt = (e & 4) * 4 + 4 * g + (e & 3);
       spoilt = min(spoilt, __shfl_xor(spoilt, 16, 64));
       spoilt = min(spoilt, __shfl_xor(spoilt, 32, 64));
       clear();
     }
+    const f32x4 none = {0.0f, 0.0f, 0.0f, 0.0f};
     if constexpr (DELTA) {
-      u32x4 planes[3];
-      split8<3>(u, planes);
-      const f32x4 none = {0.0f, 0.0f, 0.0f, 0.0f};
+      f32x4 y0 = none, y1 = none;
 #pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        const f32x4 y = mfma_planes<3, 3>(solve[t], planes, none);
-#pragma unroll
-        for (int r = 0; r < 4; ++r) u[4 * t + r] = y[r];
+      for (int j = 0; j < 4; ++j) {  // (side by side: each waits for the one before it)
+        y1 = __builtin_amdgcn_mfma_f32_16x16x4f32(solve[1][j], u[0][j], y1, 0, 0, 0);
+        y0 = __builtin_amdgcn_mfma_f32_16x16x4f32(solve[0][j], u[0][j], y0, 0, 0, 0);
       }
+      u[1] = mfma4(solve[2], u[1], y1);
+      u[0] = y0;
+      fetch_solve(work);
       if (any) clear();
     }
-    // the state, then the outputs
-    float w[8];
+    // the state
+    const uint8_t* turned = s_keys + buffer + 2 * part * TURNED + lane * 16;
+    if constexpr (F32) {
+      const f32x4 w0 = left[0] * u[0], w1 = left[1] * u[1];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) w[e] = left[e >> 2][e & 3] * u[e];
-    u32x4 planes[3];
-    split8<3>(w, planes);
+      for (int i = 0; i < 2; ++i) {
+        st[i] = mfma4(*(const f32x4*)(turned + i * TURNED), w0, st[i] * total);
+        st[i] = mfma4(*(const f32x4*)(turned + i * TURNED + 1024), w1, st[i]);
+      }
+    } else {
+      u32x4 planes[3];
+      split8<3>(left[0] * u[0], left[1] * u[1], planes);
 #pragma unroll
-    for (int i = 0; i < TILES; ++i) {
-      u32x4 x[P];
-      operand(base + L::turned + i * L::across + lane * 16, x, TILES * L::across);
-      st[i] = mfma_planes<P, 3>(x, planes, st[i] * total);
+      for (int i = 0; i < 2; ++i) {
+        u32x4 x[P];
+#pragma unroll
+        for (int p = 0; p < P; ++p) x[p] = *(const u32x4*)(turned + (p * (DK / 16) + i) * TURNED);
+        st[i] = mfma_planes<P, 3>(x, planes, st[i] * total);
+      }
     }
+    fetch_left(work);
     if (any && spoilt < kChunk) {
 #pragma unroll
-      for (int i = 0; i < TILES; ++i)
+      for (int i = 0; i < 2; ++i)
 #pragma unroll
         for (int r = 0; r < 4; ++r) st[i][r] = __builtin_nanf("");
     }
-    split8<SOME>(u, planes);
+    // the wave's rows of the output
+    f32x4 o = parts[2 + out_tile][0][lane];
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      f32x4 o;
-#pragma unroll
-      for (int r = 0; r < 4; ++r) o[r] = a.scale * since[t][r] * qs[t][r];
-      o = mfma_planes<SOME, SOME>(inside[t], planes, o);
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int i = 16 * t + 4 * g + r, at = c * kChunk + i;
-        if (any && i >= spoilt) o[r] = __builtin_nanf("");
-        if (at < s.n) out[at * a.out_token] = (T)o[r];
-      }
+    for (int i = 1; i < PARTS; ++i) o += parts[2 + out_tile][i][lane];
+    o *= a.scale * out_since;
+    if constexpr (F32) {
+      o = mfma4(out_tile ? inside[1] : inside[0], u[0], o);
+      if (out_tile) o = mfma4(inside[2], u[1], o);
+    } else {
+      u32x4 planes[2];
+      split8<2>(u[0], u[1], planes);
+      const u32x4 x[2] = {__builtin_bit_cast(u32x4, inside[0]), __builtin_bit_cast(u32x4, inside[1])};
+      o = mfma_planes<2, 2>(x, planes, o);
     }
-    if (c + 1 < chunks) put((c + 1) & 1);
-    __syncthreads();
+    fetch_inside(work);
+    float left_rows[OUT_ROWS];
+#pragma unroll
+    for (int r = 0; r < OUT_ROWS; ++r) {
+      left_rows[r] = PARTS == 4 && out_row ? o[2 + (r & 1)] : o[r];
+      if (any && 16 * out_tile + 4 * g + out_row + r >= spoilt) left_rows[r] = __builtin_nanf("");
+    }
+    const int out0 = 16 * out_tile + 4 * g + out_row;
+#pragma unroll
+    for (int r = 0; r < OUT_ROWS; ++r)
+      if (rows == kChunk || out0 + r < rows)
+        *(T*)(out_at + (uint32_t)((out0 + r) * (int)a.out_token + col) * (uint32_t)sizeof(T)) = (T)left_rows[r];
+    out_at += out_step;
   }
   if (s.to) {
 #pragma unroll
-    for (int i = 0; i < TILES; ++i)
+    for (int i = 0; i < 2; ++i)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) s.to[(long)(16 * i + 4 * g + r) * a.value_dim + col] = st[i][r];
+      for (int r = 0; r < 4; ++r) s.to[state_at + (16 * i + r) * a.value_dim] = st[i][r];
   }
 }
 
 template <typename T, int DK, bool DELTA>
 static void launch_chunks(const LinearArgs& a, hipStream_t s) {
-  hipLaunchKernelGGL((k_linear_prepare<T, DK, DELTA>), dim3((unsigned)(a.tokens / kChunk + a.nseq), (unsigned)((a.k_heads + 3) / 4)),
+  hipLaunchKernelGGL((k_linear_prepare<T, DK, DELTA>), dim3((unsigned)(a.tokens / kChunk + a.nseq), (unsigned)((a.v_heads + 7) / 8)),
                      dim3(256), 0, s, a);
-  hipLaunchKernelGGL((k_linear_scan<T, DK, DELTA>), dim3((unsigned)(a.value_dim / 64), (unsigned)a.v_heads, (unsigned)a.nseq),
-                     dim3(256), 0, s, a);
+  const long pairs = ((long)a.nseq * a.v_heads + 7) / 8 * 8;
+  hipLaunchKernelGGL((k_linear_scan<T, DK, DELTA>), dim3((unsigned)(pairs * (a.value_dim / (2048 / DK)))), dim3(256), 0, s, a);
 }
 
 template <typename T>
@@ -755,7 +876,10 @@ extern "C" int qhip_launch_linear_attention(const qhip_linear_batch* batch, int 
   if (rc) return rc;
   if (nseq == 0) return 0;
   if (tokens > 0) {
-    if (!rows_ok(q, size) || !rows_ok(k, size) || !rows_ok(v, size) || !rows_ok(out, size) || !d_log_decay ||
+    const qhip_rows* all[] = {q, k, v, out};
+    for (const qhip_rows* r : all)  // (a chunk's offsets are 32 bits)
+      if (!rows_ok(r, size) || r->token_stride > 1 << 23) return (int)hipErrorInvalidValue;
+    if (!d_log_decay ||
         ((uintptr_t)d_log_decay & 3u) || decay_stride < 0 || ((uintptr_t)d_beta & 3u) || beta_stride < 0)
       return (int)hipErrorInvalidValue;
     const long state_bytes = 4L * batch->num_states * batch->v_heads * batch->key_dim * batch->value_dim;
