@@ -158,84 +158,70 @@ static void launch_steps(const LinearArgs& a, int key_dim, hipStream_t s) {
   else hipLaunchKernelGGL((k_linear_steps<T, 128>), grid, dim3(256), 0, s, a);
 }
 
-// ---- chunks of 32 tokens ---------------------------------------------------------------
+// ---- chunks of 64 tokens ---------------------------------------------------------------
 //
 // Inside a chunk with G_i = log_decay_0 + .. + log_decay_i, S the state before it and
 // D_ij = exp(G_i - G_j):
 //
 //   L_ij = beta_i (k_i . k_j) D_ij  (j < i),   T = (1 + L)^-1 diag(beta)
 //   A_ij = scale (q_i . k_j) D_ij   (j <= i)
-//   U = T (V - diag(exp(G)) K S)    (U = V without the delta rule)
+//   R = V - diag(exp(G)) K S,   U = T R    (U = V without the delta rule)
 //   O = scale diag(exp(G)) Q S + A U
-//   S <- exp(G_31) S + (diag(exp(G_31 - G)) K)^T U
+//   S <- exp(G_63) S + K^T (diag(exp(G_63 - G)) U)
 //
 // k_linear_prepare makes T, A and the exponentials of every chunk side by side;
-// k_linear_scan then walks a sequence's chunks with 16 columns of a state in a wave's
-// registers.  All differences G_i - G_j are taken in f64: G is a long sum where the
-// decay between near tokens is small.
+// k_linear_scan then walks a sequence's chunks with 16 columns of a state in the
+// registers of a workgroup.  All differences G_i - G_j are taken in f64: G is a long sum
+// where the decay between near tokens is small.
 //
-// Products run on bf16 matrix tiles.  An f32 value goes in as a sum of planes of 8
-// bits: three hold it whole, and of their products those up to 2^-16 are summed, so a
-// product is good to f32; 16-bit inputs need one plane (bf16) or two (f16).
-constexpr int kChunk = 32;
+// f32 rows take f32 matrix tiles throughout.  16-bit rows take bf16 ones, for which an f32
+// value goes in as a sum of planes of 8 bits: what enters the state in three, which hold
+// it whole (of products of planes those down to 2^-16 are summed, so they are good to
+// f32), the state as it is read and the weights inside a chunk in two (2^-17); keys and
+// queries need one plane (bf16) or two (f16).
+constexpr int kChunk = 64, kTiles = kChunk / 16;
 
 typedef __bf16 b16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 h16x8 __attribute__((ext_vector_type(8)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
-template <typename T>
-constexpr int kPlanes = sizeof(T) == 4 ? 3 : 1;  // that hold an element whole
-template <>
-constexpr int kPlanes<f16_t> = 2;
-template <typename T>
-constexpr int kSome = sizeof(T) == 4 ? 3 : 2;  // of states read, weights inside a chunk
-
-// N planes of eight values (the last of two rounds to nearest, else bits are cut off:
-// no plane overflows)
+// N planes of four values, two dwords a plane: all but the last cut off (no plane
+// overflows), the last rounded to nearest.  (The third of three is exact.)
 template <int N>
-__device__ __forceinline__ void split8(f32x4 x, f32x4 y, u32x4* out) {
-  float rest[8];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    rest[i] = x[i];
-    rest[4 + i] = y[i];
-  }
+__device__ __forceinline__ void split4(f32x4 x, u32x2* out) {
 #pragma unroll
   for (int p = 0; p < N; ++p) {
-    if (p == N - 1 && N < 3) {
-      b16x8 b;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) b[i] = (__bf16)rest[i];
-      out[p] = __builtin_bit_cast(u32x4, b);
+    if (p == N - 1) {
+      typedef __bf16 b16x4 __attribute__((ext_vector_type(4)));
+      out[p] = __builtin_bit_cast(u32x2, b16x4{(__bf16)x[0], (__bf16)x[1], (__bf16)x[2], (__bf16)x[3]});
     } else {
+      out[p] = u32x2{__builtin_amdgcn_perm(__float_as_uint(x[1]), __float_as_uint(x[0]), 0x07060302u),
+                     __builtin_amdgcn_perm(__float_as_uint(x[3]), __float_as_uint(x[2]), 0x07060302u)};
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        out[p][i] = __builtin_amdgcn_perm(__float_as_uint(rest[2 * i + 1]), __float_as_uint(rest[2 * i]), 0x07060302u);
-      if (p + 1 < N) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) rest[i] -= __uint_as_float(__float_as_uint(rest[i]) & 0xFFFF0000u);
-      }
+      for (int i = 0; i < 4; ++i) x[i] -= __uint_as_float(__float_as_uint(x[i]) & 0xFFFF0000u);
     }
   }
 }
-// the same of four values, two dwords a plane
 template <int N>
-__device__ __forceinline__ void split4(const float* x, u32x2* out) {
-  float rest[4];
+__device__ __forceinline__ void split8(f32x4 x, f32x4 y, u32x4* out) {
+  u32x2 a[N], b[N];
+  split4<N>(x, a);
+  split4<N>(y, b);
 #pragma unroll
-  for (int i = 0; i < 4; ++i) rest[i] = x[i];
-#pragma unroll
-  for (int p = 0; p < N; ++p) {
-    out[p] = u32x2{__builtin_amdgcn_perm(__float_as_uint(rest[1]), __float_as_uint(rest[0]), 0x07060302u),
-                   __builtin_amdgcn_perm(__float_as_uint(rest[3]), __float_as_uint(rest[2]), 0x07060302u)};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) rest[i] -= __uint_as_float(__float_as_uint(rest[i]) & 0xFFFF0000u);
-  }
+  for (int p = 0; p < N; ++p) out[p] = u32x4{a[p][0], a[p][1], b[p][0], b[p][1]};
 }
 
-__device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
+// Products of 16 x 16 results.  Lane l = 16 g + m holds row m of the left operand, column
+// m of the right one and rows 4 g ..+3 of column m of the result: a result is a right
+// operand for the products that follow, with 4 g ..+3 as its rows.
+__device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {  // 32 of bf16: 4 g ..+3 and 16 + 4 g ..+3
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b16x8, a), __builtin_bit_cast(b16x8, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x4 mfma4(f32x4 a, f32x4 b, f32x4 c) {  // 16 of f32: 4 g ..+3
+#pragma unroll
+  for (int j = 0; j < 4; ++j) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[j], b[j], c, 0, 0, 0);
+  return c;
 }
 // the product of planes, smallest terms first
 template <int NA, int NB>
@@ -248,18 +234,23 @@ __device__ __forceinline__ f32x4 mfma_planes(const u32x4* a, const u32x4* b, f32
   return c;
 }
 
-// What prepare leaves for a chunk and value head, as matrix operands (lane l: row l mod
-// 16, columns 4 (l / 16) ..+3): T's tiles (0, 0), (1, 0) and (1, 1) in f32; A's the
-// same way for f32 rows, else its two rows of tiles in two planes; then exp(G),
-// exp(G_31 - G) and exp(G_31).
+// What prepare leaves for a chunk and value head, as left operands of 1 KB: T's tiles (i,
+// j), j <= i, in f32; A's the same way for f32 rows, else its rows of tiles in steps of two
+// tiles and two planes; then exp(G), exp(G_63 - G) and exp(G_63).
 template <typename T, bool DELTA>
 struct ChunkWork {
   static constexpr bool whole = sizeof(T) == 4;
-  static constexpr int solve = 0, inside = DELTA ? 3 * 1024 : 0, numbers = inside + (whole ? 3 : 4) * 1024, bytes = numbers + 512;
+  static constexpr int tiles = kTiles * (kTiles + 1) / 2 * 1024;
+  static constexpr int solve = 0, inside = DELTA ? tiles : 0, numbers = inside + (whole ? tiles : 12 * 1024), bytes = numbers + 576;
+  __host__ __device__ static constexpr int solve_tile(int i, int j) { return solve + (i * (i + 1) / 2 + j) * 1024; }
+  // of row i: its first tile (f32), or its first step's first plane
+  __host__ __device__ static constexpr int inside_row(int i) {
+    return inside + (whole ? i * (i + 1) / 2 : i < 2 ? 2 * i : 4 * i - 4) * 1024;
+  }
 };
 
 // The chunk slot of a sequence's first: no two sequences' slots meet, and there are at
-// most tokens / 32 + nseq.
+// most tokens / 64 + nseq.
 __device__ __forceinline__ long first_slot(const LinearSeq& s, int i) { return s.first / kChunk + i; }
 
 // (LDS between the lanes of a wave: in order in the hardware, kept in order here)
@@ -271,60 +262,50 @@ __device__ __forceinline__ void wave_sync() {
 // Sixteen rows of DK elements, a row to the lanes of equal l mod 16: either operand of
 // row_product, which gives the 16 x 16 products of two of them.
 template <typename T, int DK>
-struct RowTiles {
+struct RowTile {
   u32x4 v[sizeof(T) == 4 ? DK / 16 : DK / 32];
-  __device__ __forceinline__ void load(const T* row, bool in) {  // (the row of !in is there, but not this chunk's)
-    const int g = (threadIdx.x & 63) >> 4;
+  // rows from row0 on, of which n are there (n > 0; the others are 0)
+  __device__ __forceinline__ void load(const T* base, long stride, int row0, int n) {
+    const int lane = threadIdx.x & 63, g = lane >> 4, row = row0 + (lane & 15);
     typedef uint32_t piece __attribute__((ext_vector_type(4), aligned(2)));
     constexpr int W = 16 / sizeof(T);  // elements of a piece
+    const T* at = base + min(row, n - 1) * stride + g * W;
 #pragma unroll
-    for (int s = 0; s < (int)(sizeof(v) / 16); ++s) {
-      v[s] = *(const piece*)(row + (4 * s + g) * W);
-    }
+    for (int s = 0; s < (int)(sizeof(v) / 16); ++s) v[s] = *(const piece*)(at + 4 * s * W);
 #pragma unroll
     for (int s = 0; s < (int)(sizeof(v) / 16); ++s)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) v[s][i] = in ? v[s][i] : 0u;
+      for (int i = 0; i < 4; ++i) v[s][i] = row < n ? v[s][i] : 0u;
   }
 };
 template <typename T, int DK>
-__device__ __forceinline__ f32x4 row_product(const RowTiles<T, DK>& a, const RowTiles<T, DK>& b) {
+__device__ __forceinline__ f32x4 row_product(const RowTile<T, DK>& a, const RowTile<T, DK>& b) {
   f32x4 c = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
   for (int s = 0; s < (int)(sizeof(a.v) / 16); ++s) {
-    if constexpr (sizeof(T) == 4) {
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        c = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(a.v[s][j]), __uint_as_float(b.v[s][j]), c, 0, 0, 0);
-    } else if constexpr (std::is_same<T, f16_t>::value) {
+    if constexpr (sizeof(T) == 4)
+      c = mfma4(__builtin_bit_cast(f32x4, a.v[s]), __builtin_bit_cast(f32x4, b.v[s]), c);
+    else if constexpr (std::is_same<T, f16_t>::value)
       c = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h16x8, a.v[s]), __builtin_bit_cast(h16x8, b.v[s]), c, 0, 0, 0);
-    } else {
+    else
       c = mfma(a.v[s], b.v[s], c);
-    }
   }
   return c;
 }
 
-constexpr int kRowPad = 36;  // floats of a row of a 32 x 32 matrix in LDS
-
-__device__ __forceinline__ f32x4 mfma4(f32x4 a, f32x4 b, f32x4 c) {  // 16 columns of a against 16 rows of b
-#pragma unroll
-  for (int j = 0; j < 4; ++j) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[j], b[j], c, 0, 0, 0);
-  return c;
-}
-
-// A wave takes a chunk of two value heads, a half of its lanes for each where the work
-// goes by tokens or columns.
+// A workgroup takes a chunk of one value head.  The ten tiles of K K^T are two waves', those
+// of Q K^T the others'.  (1 + L)^-1 goes by blocks of 16: those on the diagonal by
+// substitution, a column a lane; then each column of blocks downwards, X_ij = -X_ii sum of
+// L_ik X_kj, a wave a column.
 template <typename T, int DK, bool DELTA>
 __global__ __launch_bounds__(256) void k_linear_prepare(LinearArgs a) {
   typedef ChunkWork<T, DELTA> W;
-  __shared__ __attribute__((aligned(16))) float s_mat[4][2][32 * kRowPad];
-  __shared__ double s_sum[4][2][32];
-  __shared__ __attribute__((aligned(16))) float s_beta[4][2][32];
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, g = lane >> 4, m = lane & 15, half = lane >> 5, token = lane & 31;
-  const int slot = blockIdx.x, head0 = __builtin_amdgcn_readfirstlane((blockIdx.y * 4 + wave) * 2);
-  if (head0 >= a.v_heads) return;  // (waves do not wait for each other)
-  const int heads = min(2, a.v_heads - head0);
+  constexpr int ROW = kChunk + 4;  // floats of a row in LDS
+  __shared__ __attribute__((aligned(16))) float s_mat[2][kChunk * ROW];  // L, then its inverse; A
+  __shared__ double s_sum[kChunk];
+  __shared__ __attribute__((aligned(16))) float s_beta[kChunk];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, g = lane >> 4, m = lane & 15;
+  const int slot = blockIdx.x, head = blockIdx.y;
   // the slot's sequence: the last whose first slot is not behind it
   int seq = -1;
   for (int i0 = 0; i0 < a.nseq; i0 += 64) {
@@ -340,170 +321,171 @@ __global__ __launch_bounds__(256) void k_linear_prepare(LinearArgs a) {
   const int chunk = (int)(slot - first_slot(s, seq)), n = s.n - chunk * kChunk;  // tokens from the chunk's first on
   if (chunk < 0 || n <= 0 || s.n <= a.few) return;
   const long t0 = s.first + (long)chunk * kChunk;
+  uint8_t* out = a.work + ((long)slot * a.v_heads + head) * W::bytes;
 
-  // G (times log2 e) in f64; a decay of exp(-200) is 0 in f32, and sums of -infinity
-  // have no differences
-  uint8_t* out = a.work + ((long)slot * a.v_heads + head0) * W::bytes;
-  {
-    const int h = head0 + min(half, heads - 1);
-    const long t = t0 + min(token, n - 1);
-    const float x = a.log_decay[t * a.decay_token + h];
-    const float beta = DELTA ? a.beta[t * a.beta_token + h] : 0.0f;
-    double sum = token < n ? (x < -200.0f ? -200.0 : (double)x) * 1.4426950408889634 : 0.0;
+  const int kh = head / a.group;
+  const T* k = (const T*)a.k + t0 * a.k_token + kh * a.k_head;
+  const T* q = (const T*)a.q + t0 * a.q_token + kh * a.q_head;
+  // rows of tiles 3 and 0, or 1 and 2, of K K^T or Q K^T: five tiles each
+  const bool keys = wave < 2, outer = (wave & 1) == 0;
+  f32x4 tile[5];
+  if (DELTA || !keys) {
+    const T* rows = keys ? k : q;
+    const long stride = keys ? a.k_token : a.q_token;
+    RowTile<T, DK> x, y;
+    if (outer) {
+      x.load(rows, stride, 48, n);
 #pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-      const double up = __shfl_up(sum, d, 64);
-      if (token >= d) sum += up;
-    }
-    s_sum[wave][half][token] = sum;
-    s_beta[wave][half][token] = token < n ? beta : 0.0f;
-    wave_sync();
-    const double last = s_sum[wave][half][31];
-    if (half < heads) {
-      float* numbers = (float*)(out + half * W::bytes + W::numbers);
-      numbers[token] = __builtin_amdgcn_exp2f((float)sum);
-      numbers[32 + token] = __builtin_amdgcn_exp2f((float)(last - sum));
-      if (token == 0) numbers[64] = __builtin_amdgcn_exp2f((float)last);
+      for (int j = 0; j < 4; ++j) {
+        y.load(k, a.k_token, 16 * j, n);
+        tile[j] = row_product(x, y);
+      }
+      x.load(rows, stride, 0, n);
+      y.load(k, a.k_token, 0, n);
+      tile[4] = row_product(x, y);
+    } else {
+      RowTile<T, DK> z;
+      x.load(rows, stride, 16, n);
+      z.load(rows, stride, 32, n);
+#pragma unroll
+      for (int j = 0; j < 3; ++j) {
+        y.load(k, a.k_token, 16 * j, n);
+        if (j < 2) tile[j] = row_product(x, y);
+        tile[2 + j] = row_product(z, y);
+      }
     }
   }
+  // tile e of the wave: row and column of tiles
+  auto tile_row = [&](int e) { return outer ? (e < 4 ? 3 : 0) : e < 2 ? 1 : 2; };
+  auto tile_col = [&](int e) { return outer ? (e < 4 ? e : 0) : e < 2 ? e : e - 2; };
 
-  // tiles (0, 0), (1, 0), (1, 1): rows 16 i + 4 g + r, column 16 j + m
-  f32x4 kk[3], qk[3], in[2][3];
+  if (wave == 0) {
+    // G (times log2 e) in f64; a decay of exp(-200) is 0 in f32, and sums of -infinity
+    // have no differences
+    const long t = t0 + min(lane, n - 1);
+    const float x = a.log_decay[t * a.decay_token + head];
+    const float beta = DELTA ? a.beta[t * a.beta_token + head] : 0.0f;
+    double sum = lane < n ? (x < -200.0f ? -200.0 : (double)x) * 1.4426950408889634 : 0.0;
 #pragma unroll
-  for (int x = 0; x < 2; ++x) {
-    if (x >= heads) break;
-    const int kh = (head0 + x) / a.group;
-    if (x == 0 || kh != (head0 + x - 1) / a.group) {
-      RowTiles<T, DK> k0, k1, q0, q1;
-      const T* k = (const T*)a.k + t0 * a.k_token + kh * a.k_head;
-      const T* q = (const T*)a.q + t0 * a.q_token + kh * a.q_head;
-      k0.load(k + min(m, n - 1) * a.k_token, m < n);
-      k1.load(k + min(m + 16, n - 1) * a.k_token, m + 16 < n);
-      q0.load(q + min(m, n - 1) * a.q_token, m < n);
-      q1.load(q + min(m + 16, n - 1) * a.q_token, m + 16 < n);
-      if constexpr (DELTA) {
-        kk[0] = row_product(k0, k0);
-        kk[1] = row_product(k1, k0);
-        kk[2] = row_product(k1, k1);
-      }
-      qk[0] = row_product(q0, k0);
-      qk[1] = row_product(q1, k0);
-      qk[2] = row_product(q1, k1);
+    for (int d = 1; d < 64; d <<= 1) {
+      const double up = __shfl_up(sum, d, 64);
+      if (lane >= d) sum += up;
     }
-    float* mat = s_mat[wave][x];
+    s_sum[lane] = sum;
+    s_beta[lane] = lane < n ? beta : 0.0f;
+  }
+  __syncthreads();
+  if (DELTA || !keys) {
+    float* mat = s_mat[keys ? 0 : 1];
 #pragma unroll
-    for (int t = 0; t < 3; ++t) {
-      const int i0 = t > 0 ? 16 : 0, j = (t == 2 ? 16 : 0) + m;
-      const double gj = s_sum[wave][x][j];
+    for (int e = 0; e < 5; ++e) {
+      const int i0 = 16 * tile_row(e) + 4 * g, j = 16 * tile_col(e) + m;
+      const double gj = s_sum[j];
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        const int i = i0 + 4 * g + r;
-        const float d = __builtin_amdgcn_exp2f((float)(s_sum[wave][x][i] - gj));
-        in[x][t][r] = i >= j && i < n ? a.scale * qk[t][r] * d : 0.0f;
-        if constexpr (DELTA) mat[i * kRowPad + j] = i > j ? s_beta[wave][x][i] * kk[t][r] * d : 0.0f;
+        const int i = i0 + r;
+        const float d = __builtin_amdgcn_exp2f((float)(s_sum[i] - gj)) * (keys ? s_beta[i] : a.scale);
+        mat[i * ROW + j] = (keys ? i > j : i >= j && i < n) ? tile[e][r] * d : 0.0f;
       }
     }
   }
-  wave_sync();
-  if constexpr (DELTA) {
-    // (1 + L)^-1: the two blocks of 16 on the diagonal by substitution, a column a lane
-    {
-      float* mat = s_mat[wave][half];
-      const int b = lane & 16;
-      float x[16];
+  __syncthreads();
+  if (DELTA && wave == 0) {
+    float* mat = s_mat[0];
+    const int b = lane & 48;
+    float x[16];
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        float y = i == m ? 1.0f : 0.0f;
+    for (int i = 0; i < 16; ++i) {
+      float y = i == m ? 1.0f : 0.0f;
 #pragma unroll
-        for (int l = 0; l < i; ++l) y = __builtin_fmaf(-mat[(b + i) * kRowPad + b + l], x[l], y);
-        x[i] = i < m ? 0.0f : y;
-      }
-      wave_sync();
-      if (half < heads) {
-#pragma unroll
-        for (int i = 0; i < 16; ++i) mat[(b + i) * kRowPad + b + m] = x[i];
-      }
-      wave_sync();
-    }
-#pragma unroll
-    for (int x = 0; x < 2; ++x) {
-      if (x >= heads) break;
-      // the block below them: -X22 L21 X11 (a result's rows 4 g + r are an operand's)
-      float* mat = s_mat[wave][x];
-      const float* row = mat + m * kRowPad + 4 * g;
-      f32x4 top, low = *(const f32x4*)(row + 16 * kRowPad), diag = *(const f32x4*)(row + 16 * kRowPad + 16);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) top[j] = mat[(4 * g + j) * kRowPad + m];
-      const f32x4 none = {0.0f, 0.0f, 0.0f, 0.0f};
-      const f32x4 y = mfma4(-diag, mfma4(low, top, none), none);
-      wave_sync();
-#pragma unroll
-      for (int r = 0; r < 4; ++r) mat[(16 + 4 * g + r) * kRowPad + m] = y[r];
-      wave_sync();
-      // T = X diag(beta)
-      const f32x4 b0 = *(const f32x4*)(s_beta[wave][x] + 4 * g), b1 = *(const f32x4*)(s_beta[wave][x] + 16 + 4 * g);
-      f32x4 t00 = *(const f32x4*)row, t10 = *(const f32x4*)(row + 16 * kRowPad) * b0;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {  // (nothing above the diagonal, whatever beta holds)
-        t00[j] = 4 * g + j <= m ? t00[j] * b0[j] : 0.0f;
-        diag[j] = 4 * g + j <= m ? diag[j] * b1[j] : 0.0f;
-      }
-      f32x4* to = (f32x4*)(out + x * W::bytes + W::solve) + lane;
-      to[0] = t00;
-      to[64] = t10;
-      to[128] = diag;
+      for (int l = 0; l < i; ++l) y = __builtin_fmaf(-mat[(b + i) * ROW + b + l], x[l], y);
+      x[i] = i < m ? 0.0f : y;
     }
     wave_sync();
-  }
 #pragma unroll
-  for (int x = 0; x < 2; ++x) {
-    if (x >= heads) break;
-    float* mat = s_mat[wave][x];
-#pragma unroll
-    for (int t = 0; t < 3; ++t) {
-      const int i0 = t > 0 ? 16 : 0, j = (t == 2 ? 16 : 0) + m;
-#pragma unroll
-      for (int r = 0; r < 4; ++r) mat[(i0 + 4 * g + r) * kRowPad + j] = in[x][t][r];
+    for (int i = 0; i < 16; ++i) mat[(b + i) * ROW + b + m] = x[i];
+  } else {
+    // A, its rows of tiles in turn
+    for (int i = DELTA ? wave - 1 : wave; i < kTiles; i += DELTA ? 3 : 4) {
+      const float* row = s_mat[1] + (16 * i + m) * ROW + 4 * g;
+      u32x4* to = (u32x4*)(out + W::inside_row(i)) + lane;
+      for (int j = 0; j <= i; j += W::whole ? 1 : 2) {
+        const f32x4 x = *(const f32x4*)(row + 16 * j);
+        if constexpr (W::whole) {
+          to[j * 64] = __builtin_bit_cast(u32x4, x);
+        } else {
+          const f32x4 none = {0.0f, 0.0f, 0.0f, 0.0f}, y = *(const f32x4*)(row + 16 * j + 16);
+          u32x4 planes[2];
+          split8<2>(x, j < i ? y : none, planes);
+          to[j * 64] = planes[0];
+          to[j * 64 + 64] = planes[1];
+        }
+      }
+    }
+    if (wave == 3) {
+      const double last = s_sum[63];
+      float* numbers = (float*)(out + W::numbers);
+      numbers[lane] = __builtin_amdgcn_exp2f((float)s_sum[lane]);
+      numbers[64 + lane] = __builtin_amdgcn_exp2f((float)(last - s_sum[lane]));
+      if (lane == 0) numbers[128] = __builtin_amdgcn_exp2f((float)last);
     }
   }
-  wave_sync();
+  if constexpr (DELTA) {
+    __syncthreads();
+    float* mat = s_mat[0];
+    auto block = [&](int i, int j) { return mat + (16 * i + m) * ROW + 16 * j + 4 * g; };  // as a left operand
+    // T = X diag(beta) (nothing above the diagonal, whatever beta holds)
+    auto leave = [&](int i, int j, f32x4 x) {
+      const f32x4 b = *(const f32x4*)(s_beta + 16 * j + 4 * g);
 #pragma unroll
-  for (int x = 0; x < 2; ++x) {
-    if (x >= heads) break;
-    const float* row = s_mat[wave][x] + m * kRowPad + 4 * g;
+      for (int e = 0; e < 4; ++e) x[e] = i > j || 4 * g + e <= m ? x[e] * b[e] : 0.0f;
+      *((f32x4*)(out + W::solve_tile(i, j)) + lane) = x;
+    };
     const f32x4 none = {0.0f, 0.0f, 0.0f, 0.0f};
-    const f32x4 t00 = *(const f32x4*)row, t10 = *(const f32x4*)(row + 16 * kRowPad), t11 = *(const f32x4*)(row + 16 * kRowPad + 16);
-    u32x4* to = (u32x4*)(out + x * W::bytes + W::inside) + lane;
-    if constexpr (W::whole) {
-      to[0] = __builtin_bit_cast(u32x4, t00);
-      to[64] = __builtin_bit_cast(u32x4, t10);
-      to[128] = __builtin_bit_cast(u32x4, t11);
+    if (wave == 3) {
+#pragma unroll
+      for (int i = 0; i < kTiles; ++i) leave(i, i, *(const f32x4*)block(i, i));
     } else {
-      u32x4 planes[2];
-      split8<2>(t00, none, planes);
-      to[0] = planes[0];
-      to[64] = planes[1];
-      split8<2>(t10, t11, planes);
-      to[128] = planes[0];
-      to[192] = planes[1];
+      const int j = wave;
+      f32x4 x[kTiles];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) x[0][r] = mat[(16 * j + 4 * g + r) * ROW + 16 * j + m];
+#pragma unroll
+      for (int d = 1; d < kTiles; ++d) {  // x[d] is X_{j + d, j}
+        if (j + d >= kTiles) break;
+        f32x4 sum = none;
+#pragma unroll
+        for (int e = 0; e < d; ++e) sum = mfma4(*(const f32x4*)block(j + d, j + e), x[e], sum);
+        x[d] = mfma4(-*(const f32x4*)block(j + d, j + d), sum, none);
+        // turned by way of the blocks above the diagonal, which nothing reads
+        wave_sync();
+#pragma unroll
+        for (int r = 0; r < 4; ++r) mat[(16 * j + 4 * g + r) * ROW + 16 * (j + d) + m] = x[d][r];
+        wave_sync();
+        leave(j + d, j, *(const f32x4*)block(j, j + d));
+      }
     }
   }
 }
 
-// DK / 32 waves have the same 16 columns, 32 rows of the state each: they share the
-// products with the state out between them, hand their parts round in LDS (one
-// barrier a chunk), and go on with the sums by themselves.
+// DK / 32 waves have the same 16 columns, 32 rows of the state each, and share the chunk's
+// tiles of 16 tokens out between them.  Three exchanges in LDS a chunk: the parts of the
+// products with the state; R; U (in planes).
 template <typename T, int DK, bool DELTA>
 __global__ __launch_bounds__(256) void k_linear_scan(LinearArgs a) {
   typedef ChunkWork<T, DELTA> W;
-  constexpr bool F32 = sizeof(T) == 4;       // f32 rows: f32 products throughout
-  constexpr int P = F32 ? 1 : kPlanes<T>;    // planes of keys and queries
-  constexpr int PARTS = DK / 32, SETS = 4 / PARTS, COLS = 16 * SETS;
-  // the keys of a chunk, turned: operands of 16 dimensions and 32 tokens.  A tile is 1 KB
-  // (f32: two, of 16 tokens) and 16 bytes, so that a thread's stores fall on all banks.
-  constexpr int TURNED = F32 ? 2 * 1024 + 16 : 1024 + 16, KEYS = P * (DK / 16) * TURNED;
-  __shared__ __attribute__((aligned(16))) uint8_t s_keys[2 * KEYS];
-  __shared__ f32x4 s_part[2][SETS][4][PARTS][64];
+  constexpr bool F32 = sizeof(T) == 4;
+  constexpr int P = std::is_same<T, f16_t>::value ? 2 : 1;  // planes of keys and queries
+  constexpr int PARTS = DK / 32, SETS = 4 / PARTS, COLS = 16 * SETS, OWN = kTiles / PARTS;
+  // the keys of a chunk, turned: left operands of 16 dimensions and its tokens, and 16
+  // bytes, so that a thread's stores fall on all banks
+  constexpr int TURNED = (F32 ? 4 : 2) * 1024 + 16;
+  __shared__ __attribute__((aligned(16))) uint8_t s_keys[P * (DK / 16) * TURNED];
+  __shared__ f32x4 s_part[SETS][DELTA ? 2 * kTiles : kTiles][PARTS][64];
+  __shared__ f32x4 s_rest[DELTA ? SETS : 1][kTiles][64];
+  __shared__ __attribute__((aligned(16))) int s_spoilt[SETS][16][kTiles];
+  __shared__ u32x4 s_new[SETS][F32 ? 2 : 3][kTiles / (F32 ? 1 : 2)][64];  // U as it enters the state; f32: and as it is
+  __shared__ u32x4 s_old[SETS][F32 ? 1 : 2][F32 ? 1 : kTiles / 2][64];    // U for the outputs
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, g = lane >> 4, m = lane & 15;
   const int set = wave / PARTS, part = wave % PARTS;
   // the workgroups of a sequence's head follow each other on one XCD
@@ -514,6 +496,9 @@ __global__ __launch_bounds__(256) void k_linear_scan(LinearArgs a) {
   const LinearSeq s = linear_seq(a, seq, head, DK);
   if (s.n <= a.few) return;
   const int kh = head / a.group, chunks = (s.n + kChunk - 1) / kChunk, tail = s.n - (chunks - 1) * kChunk;
+  // the wave's tiles of tokens (of two the first and last, or those between: T has 1 to 4
+  // tiles in a row)
+  auto own = [&](int o) { return o == 0 ? part : 3 - part; };
 
   // state: tile i has rows 16 i + 4 g + r of the wave's 32, and the wave's columns
   f32x4 st[2];
@@ -525,7 +510,7 @@ __global__ __launch_bounds__(256) void k_linear_scan(LinearArgs a) {
       st[i][r] = s.from ? s.from[state_at + (16 * i + r) * a.value_dim] : s.bad ? __builtin_nanf("") : 0.0f;
 
   // Everything of a chunk is loaded for the next one when the present one is done with
-  // it, without branches: uniform bases that go on by 32 tokens, offsets of 32 bits, and
+  // it, without branches: uniform bases that go on by 64 tokens, offsets of 32 bits, and
   // the last token's in the place of those behind it.
   const char* k_at = (const char*)((const T*)a.k + s.first * a.k_token + kh * a.k_head);
   const char* q_at = (const char*)((const T*)a.q + s.first * a.q_token + kh * a.q_head);
@@ -533,6 +518,7 @@ __global__ __launch_bounds__(256) void k_linear_scan(LinearArgs a) {
   char* out_at = (char*)((T*)a.out + s.first * a.out_token + head * a.out_head);
   // (global memory by name: through a flat address, a load would count as one of LDS too)
   typedef const __attribute__((address_space(1))) uint8_t* Work;
+  typedef const __attribute__((address_space(1))) f32x4* GlobalF4;
   Work work = (Work)a.work + (first_slot(s, seq) * a.v_heads + head) * W::bytes;
   const long k_step = kChunk * a.k_token * (long)sizeof(T), q_step = kChunk * a.q_token * (long)sizeof(T),
              v_step = kChunk * a.v_token * (long)sizeof(T), out_step = kChunk * a.out_token * (long)sizeof(T),
@@ -542,106 +528,119 @@ __global__ __launch_bounds__(256) void k_linear_scan(LinearArgs a) {
   typedef typename std::conditional<F32, uint32_t, uint16_t>::type Word;
   typedef uint32_t four __attribute__((ext_vector_type(sizeof(Four) / 4), aligned(sizeof(Word))));
   // rows 16 t + m: dimensions 4 g ..+3 of the wave's 32 and 16 more
-  Four kr[2][2], qr[2][2];
-  // four tokens x four dimensions a thread, to be turned (DK = 64: every second wave)
-  const int dq = tid & (DK / 4 - 1), tq = tid / (DK / 4) & 7;
-  const bool turns = tid < 2 * DK;
-  Four held[4];
-  T val[8];
-  uint32_t k_off[2], q_off[2], held_off[4], v_off[8];
+  Four kr[kTiles][2], qr[kTiles][2];
+  // four tokens x four dimensions a thread (twice with 128 dimensions), to be turned
+  constexpr int TURNS = DK / 64;
+  const int dq = tid & (DK / 4 - 1), tq = tid / (DK / 4);
+  Four held[TURNS][4];
+  T val[OWN][4];
+  uint32_t k_off[kTiles], q_off[kTiles], held_off[TURNS][4], v_off[OWN][4];
   auto place = [&](int rows) {  // of a chunk with that many tokens
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      k_off[t] = (uint32_t)(min(16 * t + m, rows - 1) * (int)a.k_token + 32 * part + 4 * g) * (uint32_t)sizeof(T);
-      q_off[t] = (uint32_t)(min(16 * t + m, rows - 1) * (int)a.q_token + 32 * part + 4 * g) * (uint32_t)sizeof(T);
+    for (int t = 0; t < kTiles; ++t) {
+      const int row = min(16 * t + m, rows - 1);
+      k_off[t] = (uint32_t)(row * (int)a.k_token + 32 * part + 4 * g) * (uint32_t)sizeof(T);
+      q_off[t] = (uint32_t)(row * (int)a.q_token + 32 * part + 4 * g) * (uint32_t)sizeof(T);
     }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) held_off[i] = (uint32_t)(min(4 * tq + i, rows - 1) * (int)a.k_token + 4 * dq) * (uint32_t)sizeof(T);
-#pragma unroll
-    for (int e = 0; e < 8; ++e)
-      v_off[e] = (uint32_t)(min((e & 4) * 4 + 4 * g + (e & 3), rows - 1) * (int)a.v_token + col) * (uint32_t)sizeof(T);
-  };
-  auto fetch_rows = [&](const char* k, const char* q) {
-#pragma unroll
-    for (int t = 0; t < 2; ++t)
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        if (DELTA) kr[t][h] = *(const four*)(k + k_off[t] + 16 * h * sizeof(T));
-        qr[t][h] = *(const four*)(q + q_off[t] + 16 * h * sizeof(T));
-      }
-  };
-  auto fetch_held = [&](const char* k) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) held[i] = *(const four*)(k + held_off[i]);
-  };
-  auto fetch_values = [&](const char* v) {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) val[e] = *(const T*)(v + v_off[e]);
-  };
-  typedef const __attribute__((address_space(1))) f32x4* GlobalF4;
-  f32x4 solve[3], since[2], left[2];
-  f32x4 inside[3];  // f32 rows: the three tiles; else two planes of the wave's output tile
-  float total;
-  const int out_tile = part & 1;  // of the chunk's two, and of its rows 4 g + r those from out_row on
-  constexpr int OUT_ROWS = PARTS == 4 ? 2 : 4;
-  const int out_row = PARTS == 4 ? part & 2 : 0;
-  auto fetch_solve = [&](Work w) {
-    if constexpr (DELTA) {
-#pragma unroll
-      for (int i = 0; i < 3; ++i) solve[i] = *(GlobalF4)(w + W::solve + i * 1024 + lane * 16);
-#pragma unroll
-      for (int t = 0; t < 2; ++t) since[t] = *(GlobalF4)(w + W::numbers + (16 * t + 4 * g) * 4);
-    }
-  };
-  auto fetch_left = [&](Work w) {
-#pragma unroll
-    for (int t = 0; t < 2; ++t) left[t] = *(GlobalF4)(w + W::numbers + (32 + 16 * t + 4 * g) * 4);
-    total = *(const __attribute__((address_space(1))) float*)(w + W::numbers + 256);
-  };
-  f32x4 out_since;
-  auto fetch_inside = [&](Work w) {
-#pragma unroll
-    for (int i = 0; i < (F32 ? 3 : 2); ++i) inside[i] = *(GlobalF4)(w + W::inside + (F32 ? i : 2 * out_tile + i) * 1024 + lane * 16);
-    out_since = *(GlobalF4)(w + W::numbers + (16 * out_tile + 4 * g) * 4);
-  };
-  // the held keys into LDS, turned; `rows` of the chunk are there
-  uint8_t* const to_turned = s_keys + (dq >> 2) * TURNED + (dq & 3) * 64 +
-                             (F32 ? (tq >> 2) * 1024 + (tq & 3) * 256 : (tq & 3) * 256 + (tq >> 2) * 8);
-  auto turn = [&](int buffer, int rows) {
-    if (rows < kChunk) {
+    for (int e = 0; e < TURNS; ++e)
 #pragma unroll
       for (int i = 0; i < 4; ++i)
+        held_off[e][i] = (uint32_t)(min(32 * e + 4 * tq + i, rows - 1) * (int)a.k_token + 4 * dq) * (uint32_t)sizeof(T);
 #pragma unroll
-        for (int j = 0; j < (int)(sizeof(Four) / 4); ++j) held[i][j] = 4 * tq + i < rows ? held[i][j] : 0u;
-    }
-    if constexpr (F32) {
+    for (int o = 0; o < OWN; ++o)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) *(u32x4*)(to_turned + buffer + j * 16) = u32x4{held[0][j], held[1][j], held[2][j], held[3][j]};
-    } else {
-      u32x2 planes[4][P];
+      for (int r = 0; r < 4; ++r)
+        v_off[o][r] = (uint32_t)(min(16 * own(o) + 4 * g + r, rows - 1) * (int)a.v_token + col) * (uint32_t)sizeof(T);
+  };
+  auto fetch_rows = [&]() {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if constexpr (P == 1) {
-          planes[i][0] = held[i];
-        } else {
-          typedef T Four_t __attribute__((ext_vector_type(4)));
-          const Four_t x = __builtin_bit_cast(Four_t, held[i]);
-          const float y[4] = {(float)x[0], (float)x[1], (float)x[2], (float)x[3]};
-          split4<P>(y, planes[i]);
-        }
+    for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        if (DELTA) kr[t][h] = *(const four*)(k_at + k_off[t] + 16 * h * sizeof(T));
+        qr[t][h] = *(const four*)(q_at + q_off[t] + 16 * h * sizeof(T));
       }
+  };
+  auto fetch_held = [&]() {
 #pragma unroll
-      for (int p = 0; p < P; ++p)
+    for (int e = 0; e < TURNS; ++e)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const uint32_t pick = j & 1 ? 0x07060302u : 0x05040100u;
-          *(u32x2*)(to_turned + buffer + p * (DK / 16) * TURNED + j * 16) =
-              u32x2{__builtin_amdgcn_perm(planes[1][p][j >> 1], planes[0][p][j >> 1], pick),
-                    __builtin_amdgcn_perm(planes[3][p][j >> 1], planes[2][p][j >> 1], pick)};
-        }
+      for (int i = 0; i < 4; ++i) held[e][i] = *(const four*)(k_at + held_off[e][i]);
+  };
+  auto fetch_values = [&]() {
+#pragma unroll
+    for (int o = 0; o < OWN; ++o)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) val[o][r] = *(const T*)(v_at + v_off[o][r]);
+  };
+  // (a row's tiles behind the diagonal are loaded too, from where there is something: the
+  // loads are not in branches)
+  f32x4 solve[OWN][kTiles], since[OWN], left[OWN], inside[OWN][kTiles];
+  float total;
+  auto fetch_solve = [&]() {
+#pragma unroll
+    for (int o = 0; o < OWN; ++o) {
+      if constexpr (DELTA) {
+#pragma unroll
+        for (int j = 0; j < kTiles; ++j) solve[o][j] = *(GlobalF4)(work + W::solve_tile(own(o), min(j, own(o))) + lane * 16);
+      }
+      since[o] = *(GlobalF4)(work + W::numbers + (16 * own(o) + 4 * g) * 4);
     }
   };
-  // a part of 16 rows' product with the state
+  auto fetch_left = [&]() {
+#pragma unroll
+    for (int o = 0; o < OWN; ++o) left[o] = *(GlobalF4)(work + W::numbers + (64 + 16 * own(o) + 4 * g) * 4);
+    total = *(const __attribute__((address_space(1))) float*)(work + W::numbers + 512);
+  };
+  auto fetch_inside = [&]() {
+#pragma unroll
+    for (int o = 0; o < OWN; ++o)
+#pragma unroll
+      for (int j = 0; j < kTiles; ++j)
+        inside[o][j] = *(GlobalF4)(work + W::inside_row(own(o)) + (F32 ? min(j, own(o)) : min(j >> 1, own(o) >> 1) * 2 + (j & 1)) * 1024 + lane * 16);
+  };
+  auto floats = [&](Four x) {
+    typedef T Elements __attribute__((ext_vector_type(4)));
+    const Elements y = __builtin_bit_cast(Elements, x);
+    return f32x4{(float)y[0], (float)y[1], (float)y[2], (float)y[3]};
+  };
+  // the held keys into LDS, turned; `rows` of the chunk are there
+  uint8_t* const to_turned = s_keys + (dq >> 2) * TURNED + (dq & 3) * 64 + (tq & 3) * 256;
+  auto turn = [&](int rows) {
+#pragma unroll
+    for (int e = 0; e < TURNS; ++e) {
+      const int quad = 8 * e + tq;  // of tokens
+      uint8_t* to = to_turned + (F32 ? (quad >> 2) * 1024 : (quad >> 3) * 1024 + ((quad >> 2) & 1) * 8);
+      if (rows < kChunk) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int j = 0; j < (int)(sizeof(Four) / 4); ++j) held[e][i][j] = 4 * quad + i < rows ? held[e][i][j] : 0u;
+      }
+      if constexpr (F32) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) *(u32x4*)(to + j * 16) = u32x4{held[e][0][j], held[e][1][j], held[e][2][j], held[e][3][j]};
+      } else {
+        u32x2 planes[4][P];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          if constexpr (P == 1) planes[i][0] = held[e][i];
+          else split4<P>(floats(held[e][i]), planes[i]);
+        }
+#pragma unroll
+        for (int p = 0; p < P; ++p)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const uint32_t pick = j & 1 ? 0x07060302u : 0x05040100u;
+            *(u32x2*)(to + p * (DK / 16) * TURNED + j * 16) =
+                u32x2{__builtin_amdgcn_perm(planes[1][p][j >> 1], planes[0][p][j >> 1], pick),
+                      __builtin_amdgcn_perm(planes[3][p][j >> 1], planes[2][p][j >> 1], pick)};
+          }
+      }
+    }
+  };
+  // this wave's part of 16 rows' product with the state
   u32x4 sp[2];
   auto with_state = [&](const Four(&row)[2]) {
     f32x4 c = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -652,29 +651,22 @@ __global__ __launch_bounds__(256) void k_linear_scan(LinearArgs a) {
       const u32x4 x[1] = {u32x4{row[0][0], row[0][1], row[1][0], row[1][1]}};
       return mfma_planes<1, 2>(x, sp, c);
     } else {
-      typedef T Four_t __attribute__((ext_vector_type(4)));
-      f32x4 y[2];
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const Four_t z = __builtin_bit_cast(Four_t, row[h]);
-        y[h] = f32x4{(float)z[0], (float)z[1], (float)z[2], (float)z[3]};
-      }
       u32x4 x[P];
-      split8<P>(y[0], y[1], x);
+      split8<P>(floats(row[0]), floats(row[1]), x);
       return mfma_planes<P, 2>(x, sp, c);
     }
   };
 
   place(chunks > 1 ? kChunk : tail);
-  fetch_rows(k_at, q_at);
-  fetch_held(k_at);
-  fetch_values(v_at);
-  fetch_solve(work);
-  fetch_left(work);
-  fetch_inside(work);
+  fetch_rows();
+  fetch_held();
+  fetch_values();
+  fetch_solve();
+  fetch_left();
+  fetch_inside();
   for (int c = 0; c < chunks; ++c) {
     const bool more = c + 1 < chunks;
-    const int rows = more ? kChunk : tail, buffer = (c & 1) * KEYS;
+    const int rows = more ? kChunk : tail;
     if (more) {
       work += work_step;
       v_at += v_step;
@@ -682,123 +674,180 @@ __global__ __launch_bounds__(256) void k_linear_scan(LinearArgs a) {
       q_at += q_step;
       if (c + 2 == chunks && tail < kChunk) place(tail);
     }
-    // this wave's part of K S and Q S
     if constexpr (!F32) split8<2>(st[0], st[1], sp);
-    f32x4(*parts)[PARTS][64] = s_part[c & 1][set];
-    if (turns) turn(buffer, rows);
-    fetch_held(k_at);
+    f32x4(*parts)[PARTS][64] = s_part[set];
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      if (DELTA) parts[t][part][lane] = with_state(kr[t]);
-      parts[2 + t][part][lane] = with_state(qr[t]);
+    for (int t = 0; t < kTiles; ++t) {
+      if constexpr (DELTA) parts[kTiles + t][part][lane] = with_state(kr[t]);
+      parts[t][part][lane] = with_state(qr[t]);
     }
-    fetch_rows(k_at, q_at);
-    __syncthreads();  // (the buffers after next are written behind the next chunk's barrier)
-    // what U is made of, then U
-    f32x4 u[2];
-    float sum = 0.0f;
+    fetch_rows();
+    __syncthreads();
+    turn(rows);  // (the last chunk's have been read: every wave has passed the barrier)
+    fetch_held();
+    // Q S and R of the wave's tiles
+    f32x4 u[OWN], o[OWN];
+    int spoilt = kChunk;  // the column's first token whose R is not finite
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
+    for (int w = 0; w < OWN; ++w) {
+      const int t = own(w);
+      o[w] = parts[t][0][lane];
 #pragma unroll
-      for (int r = 0; r < 4; ++r) u[t][r] = (float)val[4 * t + r];
+      for (int i = 1; i < PARTS; ++i) o[w] += parts[t][i][lane];
+      o[w] *= a.scale * since[w];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) u[w][r] = (float)val[w][r];
       if (rows < kChunk) {
 #pragma unroll
-        for (int r = 0; r < 4; ++r) u[t][r] = 16 * t + 4 * g + r < rows ? u[t][r] : 0.0f;
+        for (int r = 0; r < 4; ++r) u[w][r] = 16 * t + 4 * g + r < rows ? u[w][r] : 0.0f;
       }
       if constexpr (DELTA) {
-        f32x4 ks = parts[t][0][lane];
+        f32x4 ks = parts[kTiles + t][0][lane];
 #pragma unroll
-        for (int i = 1; i < PARTS; ++i) ks += parts[t][i][lane];
+        for (int i = 1; i < PARTS; ++i) ks += parts[kTiles + t][i][lane];
         // (rows behind the sequence's end have the last row's keys: their T is 0)
-        u[t] -= since[t] * ks;
+        u[w] -= since[w] * ks;
       }
+      // Such a value spoils its column from its token on; in a product it would spoil the
+      // tokens before as well (0 * NaN), so it stays out of them.
+      float sum = 0.0f;
 #pragma unroll
-      for (int r = 0; r < 4; ++r) sum = __builtin_fmaf(u[t][r], 0.0f, sum);
+      for (int r = 0; r < 4; ++r) sum = __builtin_fmaf(u[w][r], 0.0f, sum);
+      int first = kChunk;
+      if (__ballot(sum != 0.0f)) {
+#pragma unroll
+        for (int r = 3; r >= 0; --r)
+          if (!(__builtin_fabsf(u[w][r]) < INFINITY)) {
+            first = 16 * t + 4 * g + r;
+            u[w][r] = 0.0f;
+          }
+        first = min(first, __shfl_xor(first, 16, 64));
+        first = min(first, __shfl_xor(first, 32, 64));
+      }
+      if (lane < 16) s_spoilt[set][m][t] = first;
+      if constexpr (DELTA) s_rest[set][t][lane] = u[w];
     }
-    fetch_values(v_at);
-    // a value that is not finite spoils its column from its token on; in a product it
-    // would spoil the tokens before as well (0 * NaN), so it stays out of them
-    const bool any = __ballot(sum != 0.0f) != 0;
-    int spoilt = kChunk;  // the column's first such token
-    auto clear = [&]() {
-#pragma unroll
-      for (int e = 0; e < 8; ++e)
-        if ((e & 4) * 4 + 4 * g + (e & 3) >= spoilt) u[e >> 2][e & 3] = 0.0f;
-    };
-    if (any) {
-#pragma unroll
-      for (int e = 7; e >= 0; --e)
-        if (!(__builtin_fabsf(u[e >> 2][e & 3]) < INFINITY)) spoilt = (e & 4) * 4 + 4 * g + (e & 3);
-      spoilt = min(spoilt, __shfl_xor(spoilt, 16, 64));
-      spoilt = min(spoilt, __shfl_xor(spoilt, 32, 64));
-      clear();
-    }
-    const f32x4 none = {0.0f, 0.0f, 0.0f, 0.0f};
+    fetch_values();
     if constexpr (DELTA) {
-      f32x4 y0 = none, y1 = none;
+      __syncthreads();
+      f32x4 rest[kTiles];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {  // (side by side: each waits for the one before it)
-        y1 = __builtin_amdgcn_mfma_f32_16x16x4f32(solve[1][j], u[0][j], y1, 0, 0, 0);
-        y0 = __builtin_amdgcn_mfma_f32_16x16x4f32(solve[0][j], u[0][j], y0, 0, 0, 0);
+      for (int j = 0; j < kTiles; ++j) rest[j] = s_rest[set][j][lane];
+#pragma unroll
+      for (int w = 0; w < OWN; ++w) {
+        const int t = own(w);
+        f32x4 x = {0.0f, 0.0f, 0.0f, 0.0f}, y = x;  // (two sums side by side: each product waits for the one before it)
+#pragma unroll
+        for (int j = 0; j < kTiles; ++j)
+          if (j <= t) {
+            if (j & 1) y = mfma4(solve[w][j], rest[j], y);
+            else x = mfma4(solve[w][j], rest[j], x);
+          }
+        u[w] = x + y;
       }
-      u[1] = mfma4(solve[2], u[1], y1);
-      u[0] = y0;
-      fetch_solve(work);
-      if (any) clear();
     }
-    // the state
-    const uint8_t* turned = s_keys + buffer + 2 * part * TURNED + lane * 16;
-    if constexpr (F32) {
-      const f32x4 w0 = left[0] * u[0], w1 = left[1] * u[1];
+    if constexpr (DELTA) {
+      const u32x4 all = *(const u32x4*)s_spoilt[set][m];
+      spoilt = min(min((int)all[0], (int)all[1]), min((int)all[2], (int)all[3]));
+    }
+    const f32x4 scales[2] = {left[0], left[OWN - 1]};
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        st[i] = mfma4(*(const f32x4*)(turned + i * TURNED), w0, st[i] * total);
-        st[i] = mfma4(*(const f32x4*)(turned + i * TURNED + 1024), w1, st[i]);
+    for (int w = 0; w < OWN; ++w) {
+      const int t = own(w);
+      if (DELTA && __ballot(spoilt < kChunk)) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          if (16 * t + 4 * g + r >= spoilt) u[w][r] = 0.0f;
+      }
+      const f32x4 in = scales[w] * u[w];
+      if constexpr (F32) {
+        s_new[set][0][t][lane] = __builtin_bit_cast(u32x4, in);
+        s_new[set][1][t][lane] = __builtin_bit_cast(u32x4, u[w]);
+      } else {
+        u32x2 planes[3];
+        split4<3>(in, planes);
+#pragma unroll
+        for (int p = 0; p < 3; ++p) ((u32x2*)&s_new[set][p][t >> 1][lane])[t & 1] = planes[p];
+        split4<2>(u[w], planes);
+#pragma unroll
+        for (int p = 0; p < 2; ++p) ((u32x2*)&s_old[set][p][t >> 1][lane])[t & 1] = planes[p];
+      }
+    }
+    const float keep = total;
+    fetch_solve();
+    fetch_left();
+    __syncthreads();
+    if constexpr (!DELTA) {
+      const u32x4 all = *(const u32x4*)s_spoilt[set][m];
+      spoilt = min(min((int)all[0], (int)all[1]), min((int)all[2], (int)all[3]));
+    }
+    const bool any = __ballot(spoilt < kChunk) != 0;
+    // the state
+    const uint8_t* turned = s_keys + 2 * part * TURNED + lane * 16;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) st[i] *= keep;
+    if constexpr (F32) {
+#pragma unroll
+      for (int j = 0; j < kTiles; ++j) {
+        const f32x4 x = __builtin_bit_cast(f32x4, s_new[set][0][j][lane]);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) st[i] = mfma4(*(const f32x4*)(turned + i * TURNED + j * 1024), x, st[i]);
       }
     } else {
-      u32x4 planes[3];
-      split8<3>(left[0] * u[0], left[1] * u[1], planes);
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        u32x4 x[P];
+      for (int j = 0; j < kTiles / 2; ++j) {
+        const u32x4 x[3] = {s_new[set][0][j][lane], s_new[set][1][j][lane], s_new[set][2][j][lane]};
 #pragma unroll
-        for (int p = 0; p < P; ++p) x[p] = *(const u32x4*)(turned + (p * (DK / 16) + i) * TURNED);
-        st[i] = mfma_planes<P, 3>(x, planes, st[i] * total);
+        for (int i = 0; i < 2; ++i) {
+          u32x4 y[P];
+#pragma unroll
+          for (int p = 0; p < P; ++p) y[p] = *(const u32x4*)(turned + (p * (DK / 16) + i) * TURNED + j * 1024);
+          st[i] = mfma_planes<P, 3>(y, x, st[i]);
+        }
       }
     }
-    fetch_left(work);
     if (any && spoilt < kChunk) {
 #pragma unroll
       for (int i = 0; i < 2; ++i)
 #pragma unroll
         for (int r = 0; r < 4; ++r) st[i][r] = __builtin_nanf("");
     }
-    // the wave's rows of the output
-    f32x4 o = parts[2 + out_tile][0][lane];
+    // the outputs of the wave's tiles
 #pragma unroll
-    for (int i = 1; i < PARTS; ++i) o += parts[2 + out_tile][i][lane];
-    o *= a.scale * out_since;
-    if constexpr (F32) {
-      o = mfma4(out_tile ? inside[1] : inside[0], u[0], o);
-      if (out_tile) o = mfma4(inside[2], u[1], o);
-    } else {
-      u32x4 planes[2];
-      split8<2>(u[0], u[1], planes);
-      const u32x4 x[2] = {__builtin_bit_cast(u32x4, inside[0]), __builtin_bit_cast(u32x4, inside[1])};
-      o = mfma_planes<2, 2>(x, planes, o);
+    for (int w = 0; w < OWN; ++w) {
+      const int t = own(w);
+#pragma unroll
+      for (int j = 0; j < kTiles; ++j) {
+        if constexpr (F32) {
+          if (j <= t) o[w] = mfma4(inside[w][j], __builtin_bit_cast(f32x4, s_new[set][1][j][lane]), o[w]);
+        } else if ((j & 1) == 0 && j <= t) {
+          const u32x4 x[2] = {__builtin_bit_cast(u32x4, inside[w][j]), __builtin_bit_cast(u32x4, inside[w][j + 1])};
+          const u32x4 y[2] = {s_old[set][0][j >> 1][lane], s_old[set][1][j >> 1][lane]};
+          o[w] = mfma_planes<2, 2>(x, y, o[w]);
+        }
+      }
     }
-    fetch_inside(work);
-    float left_rows[OUT_ROWS];
+    fetch_inside();
 #pragma unroll
-    for (int r = 0; r < OUT_ROWS; ++r) {
-      left_rows[r] = PARTS == 4 && out_row ? o[2 + (r & 1)] : o[r];
-      if (any && 16 * out_tile + 4 * g + out_row + r >= spoilt) left_rows[r] = __builtin_nanf("");
+    for (int w = 0; w < OWN; ++w) {
+      const int row = 16 * own(w) + 4 * g;
+      if (any) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          if (row + r >= spoilt) o[w][r] = __builtin_nanf("");
+      }
+      auto store = [&](int r) {
+        *(T*)(out_at + (uint32_t)((row + r) * (int)a.out_token + col) * (uint32_t)sizeof(T)) = (T)o[w][r];
+      };
+      if (rows == kChunk) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) store(r);
+      } else {
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          if (row + r < rows) store(r);
+      }
     }
-    const int out0 = 16 * out_tile + 4 * g + out_row;
-#pragma unroll
-    for (int r = 0; r < OUT_ROWS; ++r)
-      if (rows == kChunk || out0 + r < rows)
-        *(T*)(out_at + (uint32_t)((out0 + r) * (int)a.out_token + col) * (uint32_t)sizeof(T)) = (T)left_rows[r];
     out_at += out_step;
   }
   if (s.to) {
@@ -811,7 +860,7 @@ __global__ __launch_bounds__(256) void k_linear_scan(LinearArgs a) {
 
 template <typename T, int DK, bool DELTA>
 static void launch_chunks(const LinearArgs& a, hipStream_t s) {
-  hipLaunchKernelGGL((k_linear_prepare<T, DK, DELTA>), dim3((unsigned)(a.tokens / kChunk + a.nseq), (unsigned)((a.v_heads + 7) / 8)),
+  hipLaunchKernelGGL((k_linear_prepare<T, DK, DELTA>), dim3((unsigned)(a.tokens / kChunk + a.nseq), (unsigned)a.v_heads),
                      dim3(256), 0, s, a);
   const long pairs = ((long)a.nseq * a.v_heads + 7) / 8 * 8;
   hipLaunchKernelGGL((k_linear_scan<T, DK, DELTA>), dim3((unsigned)(pairs * (a.value_dim / (2048 / DK)))), dim3(256), 0, s, a);
