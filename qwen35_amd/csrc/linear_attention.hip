@@ -203,6 +203,12 @@ __device__ __forceinline__ void split4(f32x4 x, u32x2* out) {
     }
   }
 }
+// four f16 values
+__device__ __forceinline__ f32x4 floats(uint32_t x, uint32_t y) {
+  typedef _Float16 h16x4 __attribute__((ext_vector_type(4)));
+  const h16x4 z = __builtin_bit_cast(h16x4, u32x2{x, y});
+  return f32x4{(float)z[0], (float)z[1], (float)z[2], (float)z[3]};
+}
 template <int N>
 __device__ __forceinline__ void split8(f32x4 x, f32x4 y, u32x4* out) {
   u32x2 a[N], b[N];
@@ -237,6 +243,7 @@ __device__ __forceinline__ f32x4 mfma_planes(const u32x4* a, const u32x4* b, f32
 // What prepare leaves for a chunk and value head, as left operands of 1 KB: T's tiles (i,
 // j), j <= i, in f32; A's the same way for f32 rows, else its rows of tiles in steps of two
 // tiles and two planes; then exp(G), exp(G_63 - G) and exp(G_63).
+constexpr int kNumbers = 2 * kChunk + 1;
 template <typename T, bool DELTA>
 struct ChunkWork {
   static constexpr bool whole = sizeof(T) == 4;
@@ -468,26 +475,36 @@ __global__ __launch_bounds__(256) void k_linear_prepare(LinearArgs a) {
   }
 }
 
-// DK / 32 waves have the same 16 columns, 32 rows of the state each, and share the chunk's
-// tiles of 16 tokens out between them.  Three exchanges in LDS a chunk: the parts of the
-// products with the state; R; U (in planes).
+// Four waves carry the state and four others make the outputs, each pair on one SIMD.  DK /
+// 32 of either kind have the same 16 columns: of the first, each keeps 32 rows of the state
+// in registers, and all have their share of the chunk's four tiles of 16 tokens.  Between
+// three barriers a chunk:
+//
+//   the state, in planes, into LDS
+//   R of the own tokens        | Q S of the own tokens
+//   U of the own tokens        | the next chunk's keys into LDS, as rows and turned
+//   the state's update         | the outputs
 template <typename T, int DK, bool DELTA>
-__global__ __launch_bounds__(256) void k_linear_scan(LinearArgs a) {
+__global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) void k_linear_scan(LinearArgs a) {
   typedef ChunkWork<T, DELTA> W;
   constexpr bool F32 = sizeof(T) == 4;
   constexpr int P = std::is_same<T, f16_t>::value ? 2 : 1;  // planes of keys and queries
   constexpr int PARTS = DK / 32, SETS = 4 / PARTS, COLS = 16 * SETS, OWN = kTiles / PARTS;
-  // the keys of a chunk, turned: left operands of 16 dimensions and its tokens, and 16
-  // bytes, so that a thread's stores fall on all banks
-  constexpr int TURNED = (F32 ? 4 : 2) * 1024 + 16;
-  __shared__ __attribute__((aligned(16))) uint8_t s_keys[P * (DK / 16) * TURNED];
-  __shared__ f32x4 s_part[SETS][DELTA ? 2 * kTiles : kTiles][PARTS][64];
+  constexpr int PIECES = DK * sizeof(T) / 64;  // of 16 bytes of a row a lane
+  // Keys, as left operands of 16 tokens, and turned, as those of 16 dimensions: steps of 32
+  // tokens (f32: 16), a step's lanes of equal l / 16 272 bytes apart.  The strides are such
+  // that the lanes of a store, which hold other tokens, fall on all banks.
+  constexpr int GROUP = 272, STEP = F32 ? 4 * GROUP : 4 * GROUP + 64, TURNED = (F32 ? 4 : 2) * STEP, KEYS = P * (DK / 16) * TURNED;
+  __shared__ u32x4 s_rows[DELTA ? kTiles : 1][PIECES * 64 + 1];
+  __shared__ __attribute__((aligned(16))) uint8_t s_keys[2 * KEYS];
+  __shared__ __attribute__((aligned(16))) float s_numbers[2][kNumbers + 3];
+  __shared__ u32x4 s_state[SETS][PARTS][2][64];  // two planes, f32: two tiles
   __shared__ f32x4 s_rest[DELTA ? SETS : 1][kTiles][64];
   __shared__ __attribute__((aligned(16))) int s_spoilt[SETS][16][kTiles];
-  __shared__ u32x4 s_new[SETS][F32 ? 2 : 3][kTiles / (F32 ? 1 : 2)][64];  // U as it enters the state; f32: and as it is
-  __shared__ u32x4 s_old[SETS][F32 ? 1 : 2][F32 ? 1 : kTiles / 2][64];    // U for the outputs
-  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, g = lane >> 4, m = lane & 15;
-  const int set = wave / PARTS, part = wave % PARTS;
+  __shared__ u32x4 s_new[SETS][F32 ? 1 : 3][kTiles / (F32 ? 1 : 2)][64];  // U as it enters the state
+  __shared__ u32x4 s_old[SETS][F32 ? 1 : 2][kTiles / (F32 ? 1 : 2)][64];  // U for the outputs
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, g = lane >> 4, m = lane & 15;
+  const int set = (wave & 3) / PARTS, part = (wave & 3) % PARTS;
   // the workgroups of a sequence's head follow each other on one XCD
   const int blocks = a.value_dim / COLS, id = (int)blockIdx.x;
   const int pair = id / (8 * blocks) * 8 + (id & 7), seq = pair / a.v_heads, head = pair - seq * a.v_heads;
@@ -499,339 +516,360 @@ __global__ __launch_bounds__(256) void k_linear_scan(LinearArgs a) {
   // the wave's tiles of tokens (of two the first and last, or those between: T has 1 to 4
   // tiles in a row)
   auto own = [&](int o) { return o == 0 ? part : 3 - part; };
-
-  // state: tile i has rows 16 i + 4 g + r of the wave's 32, and the wave's columns
-  f32x4 st[2];
-  const long state_at = (long)(32 * part + 4 * g) * a.value_dim + col;
-#pragma unroll
-  for (int i = 0; i < 2; ++i)
-#pragma unroll
-    for (int r = 0; r < 4; ++r)
-      st[i][r] = s.from ? s.from[state_at + (16 * i + r) * a.value_dim] : s.bad ? __builtin_nanf("") : 0.0f;
+  auto rows_of = [&](int c) { return c + 1 < chunks ? kChunk : tail; };
 
   // Everything of a chunk is loaded for the next one when the present one is done with
   // it, without branches: uniform bases that go on by 64 tokens, offsets of 32 bits, and
   // the last token's in the place of those behind it.
-  const char* k_at = (const char*)((const T*)a.k + s.first * a.k_token + kh * a.k_head);
-  const char* q_at = (const char*)((const T*)a.q + s.first * a.q_token + kh * a.q_head);
-  const char* v_at = (const char*)((const T*)a.v + s.first * a.v_token + head * a.v_head);
-  char* out_at = (char*)((T*)a.out + s.first * a.out_token + head * a.out_head);
   // (global memory by name: through a flat address, a load would count as one of LDS too)
   typedef const __attribute__((address_space(1))) uint8_t* Work;
   typedef const __attribute__((address_space(1))) f32x4* GlobalF4;
   Work work = (Work)a.work + (first_slot(s, seq) * a.v_heads + head) * W::bytes;
-  const long k_step = kChunk * a.k_token * (long)sizeof(T), q_step = kChunk * a.q_token * (long)sizeof(T),
-             v_step = kChunk * a.v_token * (long)sizeof(T), out_step = kChunk * a.out_token * (long)sizeof(T),
-             work_step = (long)a.v_heads * W::bytes;
-
-  typedef typename std::conditional<F32, u32x4, u32x2>::type Four;  // elements
-  typedef typename std::conditional<F32, uint32_t, uint16_t>::type Word;
-  typedef uint32_t four __attribute__((ext_vector_type(sizeof(Four) / 4), aligned(sizeof(Word))));
-  // rows 16 t + m: dimensions 4 g ..+3 of the wave's 32 and 16 more
-  Four kr[kTiles][2], qr[kTiles][2];
-  // four tokens x four dimensions a thread (twice with 128 dimensions), to be turned
-  constexpr int TURNS = DK / 64;
-  const int dq = tid & (DK / 4 - 1), tq = tid / (DK / 4);
-  Four held[TURNS][4];
-  T val[OWN][4];
-  uint32_t k_off[kTiles], q_off[kTiles], held_off[TURNS][4], v_off[OWN][4];
-  auto place = [&](int rows) {  // of a chunk with that many tokens
+  const long work_step = (long)a.v_heads * W::bytes;
+  typedef uint32_t piece __attribute__((ext_vector_type(4), aligned(2)));
+  // exp(G) or (64) exp(G_63 - G) of tile t's rows 4 g ..+3
+  auto number = [&](int c, int at, int t) { return *(const f32x4*)&s_numbers[c & 1][at + 16 * t + 4 * g]; };
+  // sixteen rows' product with the state, in two sums side by side (each product waits
+  // for the one before it)
+  auto with_state = [&](auto row) {
+    f32x4 c[2] = {};
 #pragma unroll
-    for (int t = 0; t < kTiles; ++t) {
-      const int row = min(16 * t + m, rows - 1);
-      k_off[t] = (uint32_t)(row * (int)a.k_token + 32 * part + 4 * g) * (uint32_t)sizeof(T);
-      q_off[t] = (uint32_t)(row * (int)a.q_token + 32 * part + 4 * g) * (uint32_t)sizeof(T);
+    for (int i = 0; i < PARTS; ++i) {
+      const u32x4 sp[2] = {s_state[set][i][0][lane], s_state[set][i][1][lane]};
+      if constexpr (F32) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) c[h] = mfma4(__builtin_bit_cast(f32x4, row(2 * i + h)), __builtin_bit_cast(f32x4, sp[h]), c[h]);
+      } else {
+        const u32x4 y = row(i);
+        u32x4 x[P];
+        if constexpr (P == 1) x[0] = y;
+        else split8<P>(floats(y[0], y[1]), floats(y[2], y[3]), x);
+        c[i & 1] = mfma_planes<P, 2>(x, sp, c[i & 1]);
+      }
     }
+    return c[0] + c[1];
+  };
+  // a column's first token whose R is not finite
+  auto first_spoilt = [&]() {
+    const u32x4 all = *(const u32x4*)s_spoilt[set][m];
+    return min(min((int)all[0], (int)all[1]), min((int)all[2], (int)all[3]));
+  };
+
+  if (wave < 4) {
+    // state: row 4 g + r of tile i is dimension 8 g + 4 i + r of the wave's 32, so that the
+    // eight of a lane are side by side in a key (f32: tiles of 16 dimensions as they lie)
+    f32x4 st[2];
+    auto state_at = [&](int i, int r) { return (long)(32 * part + (F32 ? 16 * i + 4 * g : 8 * g + 4 * i) + r) * a.value_dim + col; };
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) st[i][r] = s.from ? s.from[state_at(i, r)] : s.bad ? __builtin_nanf("") : 0.0f;
+
+    const char* v_at = (const char*)((const T*)a.v + s.first * a.v_token + head * a.v_head);
+    const long v_step = kChunk * a.v_token * (long)sizeof(T);
+    T val[OWN][4];
+    uint32_t v_off[OWN][4];
+    auto place = [&](int rows) {  // of a chunk with that many tokens
+#pragma unroll
+      for (int o = 0; o < OWN; ++o)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          v_off[o][r] = (uint32_t)(min(16 * own(o) + 4 * g + r, rows - 1) * (int)a.v_token + col) * (uint32_t)sizeof(T);
+    };
+    auto fetch_values = [&]() {
+#pragma unroll
+      for (int o = 0; o < OWN; ++o)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) val[o][r] = *(const T*)(v_at + v_off[o][r]);
+    };
+    f32x4 solve[OWN][kTiles];
+    auto fetch_solve = [&]() {
+#pragma unroll
+      for (int o = 0; o < OWN; ++o) {
+        if constexpr (DELTA) {
+#pragma unroll
+          for (int j = 0; j < kTiles; ++j) solve[o][j] = *(GlobalF4)(work + W::solve_tile(own(o), min(j, own(o))) + lane * 16);
+        }
+      }
+    };
+    place(rows_of(0));
+    fetch_values();
+    fetch_solve();
+    __syncthreads();  // (the first chunk's keys)
+    // (the last chunk apart: with branches around them, loads are waited for in vain)
+    auto step = [&](int c, auto last) {
+      constexpr bool LAST = decltype(last)::value;
+      if constexpr (!LAST) {
+        work += work_step;
+        v_at += v_step;
+        if (c + 2 == chunks) place(tail);
+      }
+      if constexpr (F32) {
+        s_state[set][part][0][lane] = __builtin_bit_cast(u32x4, st[0]);
+        s_state[set][part][1][lane] = __builtin_bit_cast(u32x4, st[1]);
+      } else {
+        u32x4 sp[2];
+        split8<2>(st[0], st[1], sp);
+        s_state[set][part][0][lane] = sp[0];
+        s_state[set][part][1][lane] = sp[1];
+      }
+      __syncthreads();
+      f32x4 u[OWN];
+#pragma unroll
+      for (int w = 0; w < OWN; ++w) {
+        const int t = own(w);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) u[w][r] = (float)val[w][r];
+        if constexpr (LAST) {
+#pragma unroll
+          for (int r = 0; r < 4; ++r) u[w][r] = 16 * t + 4 * g + r < tail ? u[w][r] : 0.0f;
+        }
+        // (rows behind the sequence's end have the last row's keys: their T is 0)
+        if constexpr (DELTA) u[w] -= number(c, 0, t) * with_state([&](int i) { return s_rows[t][i * 64 + lane]; });
+        // What is not finite spoils its column from its token on; in a product it would spoil
+        // the tokens before as well (0 * NaN), so it stays out of them.
+        float sum = 0.0f;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) sum = __builtin_fmaf(u[w][r], 0.0f, sum);
+        int first = kChunk;
+        if (__ballot(sum != 0.0f)) {
+#pragma unroll
+          for (int r = 3; r >= 0; --r)
+            if (!(__builtin_fabsf(u[w][r]) < INFINITY)) {
+              first = 16 * t + 4 * g + r;
+              u[w][r] = 0.0f;
+            }
+          first = min(first, __shfl_xor(first, 16, 64));
+          first = min(first, __shfl_xor(first, 32, 64));
+        }
+        if (lane < 16) s_spoilt[set][m][t] = first;
+        if constexpr (DELTA) s_rest[set][t][lane] = u[w];
+      }
+      if constexpr (!LAST) fetch_values();
+      if constexpr (DELTA) {
+        __syncthreads();
+        f32x4 rest[kTiles];
+#pragma unroll
+        for (int j = 0; j < kTiles; ++j) rest[j] = s_rest[set][j][lane];
+        const int spoilt = first_spoilt();
+#pragma unroll
+        for (int w = 0; w < OWN; ++w) {
+          const int t = own(w);
+          f32x4 x = {0.0f, 0.0f, 0.0f, 0.0f}, y = x;
+#pragma unroll
+          for (int j = 0; j < kTiles; ++j)
+            if (j <= t) {
+              if (j & 1) y = mfma4(solve[w][j], rest[j], y);
+              else x = mfma4(solve[w][j], rest[j], x);
+            }
+          u[w] = x + y;
+          if (__ballot(spoilt < kChunk)) {
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+              if (16 * t + 4 * g + r >= spoilt) u[w][r] = 0.0f;
+          }
+        }
+      }
+#pragma unroll
+      for (int w = 0; w < OWN; ++w) {
+        const int t = own(w);
+        const f32x4 in = number(c, kChunk, t) * u[w];
+        if constexpr (F32) {
+          s_new[set][0][t][lane] = __builtin_bit_cast(u32x4, in);
+          s_old[set][0][t][lane] = __builtin_bit_cast(u32x4, u[w]);
+        } else {
+          u32x2 planes[3];
+          split4<3>(in, planes);
+#pragma unroll
+          for (int p = 0; p < 3; ++p) ((u32x2*)&s_new[set][p][t >> 1][lane])[t & 1] = planes[p];
+          split4<2>(u[w], planes);
+#pragma unroll
+          for (int p = 0; p < 2; ++p) ((u32x2*)&s_old[set][p][t >> 1][lane])[t & 1] = planes[p];
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i) st[i] *= s_numbers[c & 1][kNumbers - 1];
+      if constexpr (!LAST) fetch_solve();
+      __syncthreads();
+      const uint8_t* turned = s_keys + (c & 1) * KEYS + 2 * part * TURNED + g * GROUP + m * 16;
+      if constexpr (F32) {
+#pragma unroll
+        for (int j = 0; j < kTiles; ++j) {
+          const f32x4 x = __builtin_bit_cast(f32x4, s_new[set][0][j][lane]);
+#pragma unroll
+          for (int i = 0; i < 2; ++i) st[i] = mfma4(*(const f32x4*)(turned + i * TURNED + j * STEP), x, st[i]);
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < kTiles / 2; ++j) {
+          const u32x4 x[3] = {s_new[set][0][j][lane], s_new[set][1][j][lane], s_new[set][2][j][lane]};
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            u32x4 y[P];
+#pragma unroll
+            for (int p = 0; p < P; ++p) y[p] = *(const u32x4*)(turned + (p * (DK / 16) + i) * TURNED + j * STEP);
+            st[i] = mfma_planes<P, 3>(y, x, st[i]);
+          }
+        }
+      }
+      const int spoilt = first_spoilt();
+      if (__ballot(spoilt < kChunk)) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) st[i][r] = spoilt < kChunk ? __builtin_nanf("") : st[i][r];
+      }
+    };
+    for (int c = 0; c + 1 < chunks; ++c) step(c, std::false_type{});
+    step(chunks - 1, std::true_type{});
+    if (s.to) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) s.to[state_at(i, r)] = st[i][r];
+    }
+    return;
+  }
+
+  const int tid = threadIdx.x & 255;
+  const char* k_at = (const char*)((const T*)a.k + s.first * a.k_token + kh * a.k_head);
+  const char* q_at = (const char*)((const T*)a.q + s.first * a.q_token + kh * a.q_head);
+  char* out_at = (char*)((T*)a.out + s.first * a.out_token + head * a.out_head);
+  const long k_step = kChunk * a.k_token * (long)sizeof(T), q_step = kChunk * a.q_token * (long)sizeof(T),
+             out_step = kChunk * a.out_token * (long)sizeof(T);
+  // the wave's tokens' queries: row m, piece i has 16 bytes from byte 64 i + 16 g on
+  u32x4 qr[OWN][PIECES];
+  Work key_work = work;
+  // keys: four tokens x 16 bytes a thread (f32 of 128 dimensions twice)
+  constexpr int ACROSS = DK * sizeof(T) / 16, TURNS = 16 * ACROSS > 256 ? 16 * ACROSS / 256 : 1;
+  const int dq = tid / (16 / TURNS) % ACROSS, tq = tid % (16 / TURNS);
+  const bool turns = tid < 16 * ACROSS;
+  u32x4 held[TURNS][4];
+  float held_number;
+  uint32_t q_off[OWN], held_off[TURNS][4];
+  auto place_queries = [&](int rows) {  // of a chunk with that many tokens
+#pragma unroll
+    for (int o = 0; o < OWN; ++o)
+      q_off[o] = (uint32_t)(min(16 * own(o) + m, rows - 1) * (int)a.q_token) * (uint32_t)sizeof(T) + 16 * g;
+  };
+  auto place_keys = [&](int rows) {
 #pragma unroll
     for (int e = 0; e < TURNS; ++e)
 #pragma unroll
       for (int i = 0; i < 4; ++i)
-        held_off[e][i] = (uint32_t)(min(32 * e + 4 * tq + i, rows - 1) * (int)a.k_token + 4 * dq) * (uint32_t)sizeof(T);
+        held_off[e][i] = (uint32_t)(min(4 * tq + 64 / TURNS * e + i, rows - 1) * (int)a.k_token) * (uint32_t)sizeof(T) + 16 * dq;
+  };
+  auto fetch_queries = [&]() {
 #pragma unroll
     for (int o = 0; o < OWN; ++o)
 #pragma unroll
-      for (int r = 0; r < 4; ++r)
-        v_off[o][r] = (uint32_t)(min(16 * own(o) + 4 * g + r, rows - 1) * (int)a.v_token + col) * (uint32_t)sizeof(T);
+      for (int i = 0; i < PIECES; ++i) qr[o][i] = *(const piece*)(q_at + q_off[o] + 64 * i);
   };
-  auto fetch_rows = [&]() {
-#pragma unroll
-    for (int t = 0; t < kTiles; ++t)
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        if (DELTA) kr[t][h] = *(const four*)(k_at + k_off[t] + 16 * h * sizeof(T));
-        qr[t][h] = *(const four*)(q_at + q_off[t] + 16 * h * sizeof(T));
-      }
-  };
-  auto fetch_held = [&]() {
+  auto fetch_keys = [&]() {
 #pragma unroll
     for (int e = 0; e < TURNS; ++e)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) held[e][i] = *(const four*)(k_at + held_off[e][i]);
+      for (int i = 0; i < 4; ++i) held[e][i] = *(const piece*)(k_at + held_off[e][i]);
+    held_number = *(const __attribute__((address_space(1))) float*)(key_work + W::numbers + 4 * min(tid, kNumbers - 1));
   };
-  auto fetch_values = [&]() {
-#pragma unroll
-    for (int o = 0; o < OWN; ++o)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) val[o][r] = *(const T*)(v_at + v_off[o][r]);
-  };
-  // (a row's tiles behind the diagonal are loaded too, from where there is something: the
-  // loads are not in branches)
-  f32x4 solve[OWN][kTiles], since[OWN], left[OWN], inside[OWN][kTiles];
-  float total;
-  auto fetch_solve = [&]() {
-#pragma unroll
-    for (int o = 0; o < OWN; ++o) {
-      if constexpr (DELTA) {
-#pragma unroll
-        for (int j = 0; j < kTiles; ++j) solve[o][j] = *(GlobalF4)(work + W::solve_tile(own(o), min(j, own(o))) + lane * 16);
-      }
-      since[o] = *(GlobalF4)(work + W::numbers + (16 * own(o) + 4 * g) * 4);
-    }
-  };
-  auto fetch_left = [&]() {
-#pragma unroll
-    for (int o = 0; o < OWN; ++o) left[o] = *(GlobalF4)(work + W::numbers + (64 + 16 * own(o) + 4 * g) * 4);
-    total = *(const __attribute__((address_space(1))) float*)(work + W::numbers + 512);
-  };
+  f32x4 inside[OWN][kTiles];
   auto fetch_inside = [&]() {
 #pragma unroll
     for (int o = 0; o < OWN; ++o)
 #pragma unroll
       for (int j = 0; j < kTiles; ++j)
-        inside[o][j] = *(GlobalF4)(work + W::inside_row(own(o)) + (F32 ? min(j, own(o)) : min(j >> 1, own(o) >> 1) * 2 + (j & 1)) * 1024 + lane * 16);
+        inside[o][j] = *(GlobalF4)(work + W::inside_row(own(o)) + (F32 ? min(j, own(o)) : min(j, own(o) | 1)) * 1024 + lane * 16);
   };
-  auto floats = [&](Four x) {
-    typedef T Elements __attribute__((ext_vector_type(4)));
-    const Elements y = __builtin_bit_cast(Elements, x);
-    return f32x4{(float)y[0], (float)y[1], (float)y[2], (float)y[3]};
-  };
-  // the held keys into LDS, turned; `rows` of the chunk are there
-  uint8_t* const to_turned = s_keys + (dq >> 2) * TURNED + (dq & 3) * 64 + (tq & 3) * 256;
-  auto turn = [&](int rows) {
+  // the held keys and numbers into LDS (behind the sequence's end the last key: U is 0 there)
+  auto put_keys = [&](int buffer) {
+    if (tid < kNumbers) s_numbers[buffer][tid] = held_number;
+    if (!turns) return;
 #pragma unroll
     for (int e = 0; e < TURNS; ++e) {
-      const int quad = 8 * e + tq;  // of tokens
-      uint8_t* to = to_turned + (F32 ? (quad >> 2) * 1024 : (quad >> 3) * 1024 + ((quad >> 2) & 1) * 8);
-      if (rows < kChunk) {
+      const int quad = tq + 16 / TURNS * e;  // of tokens
+      if constexpr (DELTA) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-          for (int j = 0; j < (int)(sizeof(Four) / 4); ++j) held[e][i][j] = 4 * quad + i < rows ? held[e][i][j] : 0u;
+        for (int i = 0; i < 4; ++i) s_rows[quad >> 2][(dq >> 2) * 64 + (dq & 3) * 16 + (quad & 3) * 4 + i] = held[e][i];
       }
-      if constexpr (F32) {
+      uint8_t* to = s_keys + buffer * KEYS + (dq & 3) * 64 + (quad & 3) * GROUP;
+      if constexpr (F32) {  // dimensions 4 dq ..+3
+        to += (dq >> 2) * TURNED + (quad >> 2) * STEP;
 #pragma unroll
         for (int j = 0; j < 4; ++j) *(u32x4*)(to + j * 16) = u32x4{held[e][0][j], held[e][1][j], held[e][2][j], held[e][3][j]};
-      } else {
-        u32x2 planes[4][P];
+      } else {  // dimensions 8 dq ..+7: rows 4 (dq mod 4) ..+3 of two tiles
+        to += (dq >> 2) * 2 * TURNED + (quad >> 3) * STEP + ((quad >> 2) & 1) * 8;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          if constexpr (P == 1) planes[i][0] = held[e][i];
-          else split4<P>(floats(held[e][i]), planes[i]);
-        }
+        for (int h = 0; h < 2; ++h) {
+          u32x2 planes[4][P];
 #pragma unroll
-        for (int p = 0; p < P; ++p)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const uint32_t pick = j & 1 ? 0x07060302u : 0x05040100u;
-            *(u32x2*)(to + p * (DK / 16) * TURNED + j * 16) =
-                u32x2{__builtin_amdgcn_perm(planes[1][p][j >> 1], planes[0][p][j >> 1], pick),
-                      __builtin_amdgcn_perm(planes[3][p][j >> 1], planes[2][p][j >> 1], pick)};
+          for (int i = 0; i < 4; ++i) {
+            if constexpr (P == 1) planes[i][0] = u32x2{held[e][i][2 * h], held[e][i][2 * h + 1]};
+            else split4<P>(floats(held[e][i][2 * h], held[e][i][2 * h + 1]), planes[i]);
           }
+#pragma unroll
+          for (int p = 0; p < P; ++p)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const uint32_t pick = j & 1 ? 0x07060302u : 0x05040100u;
+              *(u32x2*)(to + (p * (DK / 16) + h) * TURNED + j * 16) =
+                  u32x2{__builtin_amdgcn_perm(planes[1][p][j >> 1], planes[0][p][j >> 1], pick),
+                        __builtin_amdgcn_perm(planes[3][p][j >> 1], planes[2][p][j >> 1], pick)};
+            }
+        }
       }
     }
   };
-  // this wave's part of 16 rows' product with the state
-  u32x4 sp[2];
-  auto with_state = [&](const Four(&row)[2]) {
-    f32x4 c = {0.0f, 0.0f, 0.0f, 0.0f};
-    if constexpr (F32) {
-      c = mfma4(__builtin_bit_cast(f32x4, row[0]), st[0], c);
-      return mfma4(__builtin_bit_cast(f32x4, row[1]), st[1], c);
-    } else if constexpr (P == 1) {
-      const u32x4 x[1] = {u32x4{row[0][0], row[0][1], row[1][0], row[1][1]}};
-      return mfma_planes<1, 2>(x, sp, c);
-    } else {
-      u32x4 x[P];
-      split8<P>(floats(row[0]), floats(row[1]), x);
-      return mfma_planes<P, 2>(x, sp, c);
-    }
-  };
-
-  place(chunks > 1 ? kChunk : tail);
-  fetch_rows();
-  fetch_held();
-  fetch_values();
-  fetch_solve();
-  fetch_left();
+  place_queries(rows_of(0));
+  place_keys(rows_of(0));
+  fetch_keys();
+  fetch_queries();
   fetch_inside();
-  for (int c = 0; c < chunks; ++c) {
-    const bool more = c + 1 < chunks;
-    const int rows = more ? kChunk : tail;
-    if (more) {
+  put_keys(0);
+  if (chunks > 1) {
+    k_at += k_step;
+    key_work += work_step;
+    if (chunks == 2) place_keys(tail);
+  }
+  fetch_keys();
+  __syncthreads();
+  auto step = [&](int c, auto last) {
+    constexpr bool LAST = decltype(last)::value;
+    if constexpr (!LAST) {
       work += work_step;
-      v_at += v_step;
-      k_at += k_step;
       q_at += q_step;
-      if (c + 2 == chunks && tail < kChunk) place(tail);
+      if (c + 2 == chunks) place_queries(tail);
     }
-    if constexpr (!F32) split8<2>(st[0], st[1], sp);
-    f32x4(*parts)[PARTS][64] = s_part[set];
-#pragma unroll
-    for (int t = 0; t < kTiles; ++t) {
-      if constexpr (DELTA) parts[kTiles + t][part][lane] = with_state(kr[t]);
-      parts[t][part][lane] = with_state(qr[t]);
-    }
-    fetch_rows();
     __syncthreads();
-    turn(rows);  // (the last chunk's have been read: every wave has passed the barrier)
-    fetch_held();
-    // Q S and R of the wave's tiles
-    f32x4 u[OWN], o[OWN];
-    int spoilt = kChunk;  // the column's first token whose R is not finite
+    f32x4 o[OWN];
 #pragma unroll
-    for (int w = 0; w < OWN; ++w) {
-      const int t = own(w);
-      o[w] = parts[t][0][lane];
-#pragma unroll
-      for (int i = 1; i < PARTS; ++i) o[w] += parts[t][i][lane];
-      o[w] *= a.scale * since[w];
-#pragma unroll
-      for (int r = 0; r < 4; ++r) u[w][r] = (float)val[w][r];
-      if (rows < kChunk) {
-#pragma unroll
-        for (int r = 0; r < 4; ++r) u[w][r] = 16 * t + 4 * g + r < rows ? u[w][r] : 0.0f;
+    for (int w = 0; w < OWN; ++w) o[w] = a.scale * number(c, 0, own(w)) * with_state([&](int i) { return qr[w][i]; });
+    if constexpr (!LAST) fetch_queries();
+    if constexpr (DELTA) __syncthreads();
+    if constexpr (!LAST) {
+      put_keys((c + 1) & 1);
+      if (c + 2 < chunks) {
+        k_at += k_step;
+        key_work += work_step;
+        if (c + 3 == chunks) place_keys(tail);
       }
-      if constexpr (DELTA) {
-        f32x4 ks = parts[kTiles + t][0][lane];
-#pragma unroll
-        for (int i = 1; i < PARTS; ++i) ks += parts[kTiles + t][i][lane];
-        // (rows behind the sequence's end have the last row's keys: their T is 0)
-        u[w] -= since[w] * ks;
-      }
-      // Such a value spoils its column from its token on; in a product it would spoil the
-      // tokens before as well (0 * NaN), so it stays out of them.
-      float sum = 0.0f;
-#pragma unroll
-      for (int r = 0; r < 4; ++r) sum = __builtin_fmaf(u[w][r], 0.0f, sum);
-      int first = kChunk;
-      if (__ballot(sum != 0.0f)) {
-#pragma unroll
-        for (int r = 3; r >= 0; --r)
-          if (!(__builtin_fabsf(u[w][r]) < INFINITY)) {
-            first = 16 * t + 4 * g + r;
-            u[w][r] = 0.0f;
-          }
-        first = min(first, __shfl_xor(first, 16, 64));
-        first = min(first, __shfl_xor(first, 32, 64));
-      }
-      if (lane < 16) s_spoilt[set][m][t] = first;
-      if constexpr (DELTA) s_rest[set][t][lane] = u[w];
+      fetch_keys();
     }
-    fetch_values();
-    if constexpr (DELTA) {
-      __syncthreads();
-      f32x4 rest[kTiles];
-#pragma unroll
-      for (int j = 0; j < kTiles; ++j) rest[j] = s_rest[set][j][lane];
-#pragma unroll
-      for (int w = 0; w < OWN; ++w) {
-        const int t = own(w);
-        f32x4 x = {0.0f, 0.0f, 0.0f, 0.0f}, y = x;  // (two sums side by side: each product waits for the one before it)
-#pragma unroll
-        for (int j = 0; j < kTiles; ++j)
-          if (j <= t) {
-            if (j & 1) y = mfma4(solve[w][j], rest[j], y);
-            else x = mfma4(solve[w][j], rest[j], x);
-          }
-        u[w] = x + y;
-      }
-    }
-    if constexpr (DELTA) {
-      const u32x4 all = *(const u32x4*)s_spoilt[set][m];
-      spoilt = min(min((int)all[0], (int)all[1]), min((int)all[2], (int)all[3]));
-    }
-    const f32x4 scales[2] = {left[0], left[OWN - 1]};
-#pragma unroll
-    for (int w = 0; w < OWN; ++w) {
-      const int t = own(w);
-      if (DELTA && __ballot(spoilt < kChunk)) {
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-          if (16 * t + 4 * g + r >= spoilt) u[w][r] = 0.0f;
-      }
-      const f32x4 in = scales[w] * u[w];
-      if constexpr (F32) {
-        s_new[set][0][t][lane] = __builtin_bit_cast(u32x4, in);
-        s_new[set][1][t][lane] = __builtin_bit_cast(u32x4, u[w]);
-      } else {
-        u32x2 planes[3];
-        split4<3>(in, planes);
-#pragma unroll
-        for (int p = 0; p < 3; ++p) ((u32x2*)&s_new[set][p][t >> 1][lane])[t & 1] = planes[p];
-        split4<2>(u[w], planes);
-#pragma unroll
-        for (int p = 0; p < 2; ++p) ((u32x2*)&s_old[set][p][t >> 1][lane])[t & 1] = planes[p];
-      }
-    }
-    const float keep = total;
-    fetch_solve();
-    fetch_left();
     __syncthreads();
-    if constexpr (!DELTA) {
-      const u32x4 all = *(const u32x4*)s_spoilt[set][m];
-      spoilt = min(min((int)all[0], (int)all[1]), min((int)all[2], (int)all[3]));
-    }
-    const bool any = __ballot(spoilt < kChunk) != 0;
-    // the state
-    const uint8_t* turned = s_keys + 2 * part * TURNED + lane * 16;
-#pragma unroll
-    for (int i = 0; i < 2; ++i) st[i] *= keep;
-    if constexpr (F32) {
-#pragma unroll
-      for (int j = 0; j < kTiles; ++j) {
-        const f32x4 x = __builtin_bit_cast(f32x4, s_new[set][0][j][lane]);
-#pragma unroll
-        for (int i = 0; i < 2; ++i) st[i] = mfma4(*(const f32x4*)(turned + i * TURNED + j * 1024), x, st[i]);
-      }
-    } else {
-#pragma unroll
-      for (int j = 0; j < kTiles / 2; ++j) {
-        const u32x4 x[3] = {s_new[set][0][j][lane], s_new[set][1][j][lane], s_new[set][2][j][lane]};
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          u32x4 y[P];
-#pragma unroll
-          for (int p = 0; p < P; ++p) y[p] = *(const u32x4*)(turned + (p * (DK / 16) + i) * TURNED + j * 1024);
-          st[i] = mfma_planes<P, 3>(y, x, st[i]);
-        }
-      }
-    }
-    if (any && spoilt < kChunk) {
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) st[i][r] = __builtin_nanf("");
-    }
-    // the outputs of the wave's tiles
+    const int spoilt = first_spoilt();
 #pragma unroll
     for (int w = 0; w < OWN; ++w) {
-      const int t = own(w);
+      const int t = own(w), row = 16 * t + 4 * g;
 #pragma unroll
       for (int j = 0; j < kTiles; ++j) {
         if constexpr (F32) {
-          if (j <= t) o[w] = mfma4(inside[w][j], __builtin_bit_cast(f32x4, s_new[set][1][j][lane]), o[w]);
+          if (j <= t) o[w] = mfma4(inside[w][j], __builtin_bit_cast(f32x4, s_old[set][0][j][lane]), o[w]);
         } else if ((j & 1) == 0 && j <= t) {
           const u32x4 x[2] = {__builtin_bit_cast(u32x4, inside[w][j]), __builtin_bit_cast(u32x4, inside[w][j + 1])};
           const u32x4 y[2] = {s_old[set][0][j >> 1][lane], s_old[set][1][j >> 1][lane]};
           o[w] = mfma_planes<2, 2>(x, y, o[w]);
         }
       }
-    }
-    fetch_inside();
-#pragma unroll
-    for (int w = 0; w < OWN; ++w) {
-      const int row = 16 * own(w) + 4 * g;
-      if (any) {
+      if (__ballot(spoilt < kChunk)) {
 #pragma unroll
         for (int r = 0; r < 4; ++r)
           if (row + r >= spoilt) o[w][r] = __builtin_nanf("");
@@ -839,23 +877,15 @@ __global__ __launch_bounds__(256) void k_linear_scan(LinearArgs a) {
       auto store = [&](int r) {
         *(T*)(out_at + (uint32_t)((row + r) * (int)a.out_token + col) * (uint32_t)sizeof(T)) = (T)o[w][r];
       };
-      if (rows == kChunk) {
 #pragma unroll
-        for (int r = 0; r < 4; ++r) store(r);
-      } else {
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-          if (row + r < rows) store(r);
-      }
+      for (int r = 0; r < 4; ++r)
+        if (!LAST || row + r < tail) store(r);
     }
+    if constexpr (!LAST) fetch_inside();
     out_at += out_step;
-  }
-  if (s.to) {
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) s.to[state_at + (16 * i + r) * a.value_dim] = st[i][r];
-  }
+  };
+  for (int c = 0; c + 1 < chunks; ++c) step(c, std::false_type{});
+  step(chunks - 1, std::true_type{});
 }
 
 template <typename T, int DK, bool DELTA>
@@ -863,7 +893,7 @@ static void launch_chunks(const LinearArgs& a, hipStream_t s) {
   hipLaunchKernelGGL((k_linear_prepare<T, DK, DELTA>), dim3((unsigned)(a.tokens / kChunk + a.nseq), (unsigned)a.v_heads),
                      dim3(256), 0, s, a);
   const long pairs = ((long)a.nseq * a.v_heads + 7) / 8 * 8;
-  hipLaunchKernelGGL((k_linear_scan<T, DK, DELTA>), dim3((unsigned)(pairs * (a.value_dim / (2048 / DK)))), dim3(256), 0, s, a);
+  hipLaunchKernelGGL((k_linear_scan<T, DK, DELTA>), dim3((unsigned)(pairs * (a.value_dim / (2048 / DK)))), dim3(512), 0, s, a);
 }
 
 template <typename T>
