@@ -171,8 +171,8 @@ static void launch_steps(const LinearArgs& a, int key_dim, hipStream_t s) {
 //
 // k_linear_prepare makes T, A and the exponentials of every chunk side by side;
 // k_linear_scan then walks a sequence's chunks with 16 columns of a state in the
-// registers of a workgroup.  All differences G_i - G_j are taken in f64: G is a long sum
-// where the decay between near tokens is small.
+// registers of a workgroup.  G is summed in f64 and kept in two f32 parts, of which
+// differences are taken: it is a long sum where the decay between near tokens is small.
 //
 // f32 rows take f32 matrix tiles throughout.  16-bit rows take bf16 ones, for which an f32
 // value goes in as a sum of planes of 8 bits: what enters the state in three, which hold
@@ -271,7 +271,7 @@ __device__ __forceinline__ void wave_sync() {
 template <typename T, int DK>
 struct RowTile {
   u32x4 v[sizeof(T) == 4 ? DK / 16 : DK / 32];
-  // rows from row0 on, of which n are there (n > 0; the others are 0)
+  // rows from row0 on, of n > 0 (behind them, the last again)
   __device__ __forceinline__ void load(const T* base, long stride, int row0, int n) {
     const int lane = threadIdx.x & 63, g = lane >> 4, row = row0 + (lane & 15);
     typedef uint32_t piece __attribute__((ext_vector_type(4), aligned(2)));
@@ -279,10 +279,6 @@ struct RowTile {
     const T* at = base + min(row, n - 1) * stride + g * W;
 #pragma unroll
     for (int s = 0; s < (int)(sizeof(v) / 16); ++s) v[s] = *(const piece*)(at + 4 * s * W);
-#pragma unroll
-    for (int s = 0; s < (int)(sizeof(v) / 16); ++s)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) v[s][i] = row < n ? v[s][i] : 0u;
   }
 };
 template <typename T, int DK>
@@ -301,145 +297,154 @@ __device__ __forceinline__ f32x4 row_product(const RowTile<T, DK>& a, const RowT
 }
 
 // A workgroup takes a chunk of one value head.  The ten tiles of K K^T are two waves', those
-// of Q K^T the others'.  (1 + L)^-1 goes by blocks of 16: those on the diagonal by
-// substitution, a column a lane; then each column of blocks downwards, X_ij = -X_ii sum of
-// L_ik X_kj, a wave a column.
+// of K Q^T the others': with the keys on the left, a result has row m, columns 4 g ..+3 of L
+// or A, as they go into LDS and out.  (1 + L)^-1 goes by blocks of 16: those on the diagonal
+// by substitution, a column a lane; then each column of blocks downwards, X_ij = -X_ii sum
+// of L_ik X_kj, a wave a column.
 template <typename T, int DK, bool DELTA>
-__global__ __launch_bounds__(256) void k_linear_prepare(LinearArgs a) {
+__global__ __launch_bounds__(256, 2) void k_linear_prepare(LinearArgs a) {
   typedef ChunkWork<T, DELTA> W;
   constexpr int ROW = kChunk + 4;  // floats of a row in LDS
-  __shared__ __attribute__((aligned(16))) float s_mat[2][kChunk * ROW];  // L, then its inverse; A
-  __shared__ double s_sum[kChunk];
+  __shared__ __attribute__((aligned(16))) float s_mat[DELTA ? kChunk * ROW : 4];  // L, then its inverse
+  __shared__ __attribute__((aligned(16))) float s_sum[2][kChunk];  // G in two parts
   __shared__ __attribute__((aligned(16))) float s_beta[kChunk];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, g = lane >> 4, m = lane & 15;
-  const int slot = blockIdx.x, head = blockIdx.y;
+  // (heads side by side: a head's rows, a token's stride apart, lie in few memory channels)
+  const int slot = blockIdx.x / a.v_heads, head = blockIdx.x - slot * a.v_heads;
   // the slot's sequence: the last whose first slot is not behind it
-  int seq = -1;
+  int seq = -1, first = 0, end = 0;
   for (int i0 = 0; i0 < a.nseq; i0 += 64) {
-    const int i = i0 + lane;
-    const uint64_t before = __ballot(i < a.nseq && a.offsets[min(i, a.nseq - 1)] / kChunk + i <= slot);
-    seq += __builtin_popcountll(before);
-    if (before != ~0ull) break;
+    const int i = min(i0 + lane, a.nseq - 1), from = a.offsets[i], to = a.offsets[i + 1];
+    const uint64_t before = __ballot(i0 + lane < a.nseq && from / kChunk + i <= slot);
+    const int count = __builtin_popcountll(before);
+    if (count == 0) break;
+    seq = i0 + count - 1;
+    first = __builtin_amdgcn_readlane(from, count - 1);
+    end = __builtin_amdgcn_readlane(to, count - 1);
+    if (count < 64) break;
   }
   if (seq < 0) return;
-  LinearSeq s{a.offsets[seq], 0, nullptr, nullptr, false};
-  const int end = min(a.offsets[seq + 1], a.tokens);
-  if (s.first >= 0 && end > s.first) s.n = min(end - s.first, a.max_new);
+  LinearSeq s{first, 0, nullptr, nullptr, false};
+  end = min(end, a.tokens);
+  if (first >= 0 && end > first) s.n = min(end - first, a.max_new);
   const int chunk = (int)(slot - first_slot(s, seq)), n = s.n - chunk * kChunk;  // tokens from the chunk's first on
   if (chunk < 0 || n <= 0 || s.n <= a.few) return;
-  const long t0 = s.first + (long)chunk * kChunk;
+  const long t0 = first + (long)chunk * kChunk;
   uint8_t* out = a.work + ((long)slot * a.v_heads + head) * W::bytes;
+  float decay = 0.0f, beta = 0.0f;
+  if (wave == 0) {
+    const long t = t0 + min(lane, n - 1);
+    decay = a.log_decay[t * a.decay_token + head];
+    if (DELTA) beta = a.beta[t * a.beta_token + head];
+  }
 
   const int kh = head / a.group;
   const T* k = (const T*)a.k + t0 * a.k_token + kh * a.k_head;
   const T* q = (const T*)a.q + t0 * a.q_token + kh * a.q_head;
-  // rows of tiles 3 and 0, or 1 and 2, of K K^T or Q K^T: five tiles each
+  // rows of tiles 3 and 0, or 1 and 2, of L or A: five tiles each
   const bool keys = wave < 2, outer = (wave & 1) == 0;
   f32x4 tile[5];
   if (DELTA || !keys) {
     const T* rows = keys ? k : q;
     const long stride = keys ? a.k_token : a.q_token;
-    RowTile<T, DK> x, y;
+    RowTile<T, DK> x[2], y[4];  // (all loads before the first product)
+    x[0].load(rows, stride, outer ? 48 : 16, n);
+#pragma unroll
+    for (int j = 0; j < 3; ++j) y[j].load(k, a.k_token, 16 * j, n);
+    if (outer) y[3].load(k, a.k_token, 48, n);
+    x[1].load(rows, stride, outer ? 0 : 32, n);
     if (outer) {
-      x.load(rows, stride, 48, n);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        y.load(k, a.k_token, 16 * j, n);
-        tile[j] = row_product(x, y);
-      }
-      x.load(rows, stride, 0, n);
-      y.load(k, a.k_token, 0, n);
-      tile[4] = row_product(x, y);
+      for (int j = 0; j < 4; ++j) tile[j] = row_product(y[j], x[0]);
+      tile[4] = row_product(y[0], x[1]);
     } else {
-      RowTile<T, DK> z;
-      x.load(rows, stride, 16, n);
-      z.load(rows, stride, 32, n);
+      tile[0] = row_product(y[0], x[0]);
+      tile[1] = row_product(y[1], x[0]);
 #pragma unroll
-      for (int j = 0; j < 3; ++j) {
-        y.load(k, a.k_token, 16 * j, n);
-        if (j < 2) tile[j] = row_product(x, y);
-        tile[2 + j] = row_product(z, y);
-      }
+      for (int j = 0; j < 3; ++j) tile[2 + j] = row_product(y[j], x[1]);
     }
   }
-  // tile e of the wave: row and column of tiles
-  auto tile_row = [&](int e) { return outer ? (e < 4 ? 3 : 0) : e < 2 ? 1 : 2; };
-  auto tile_col = [&](int e) { return outer ? (e < 4 ? e : 0) : e < 2 ? e : e - 2; };
-
   if (wave == 0) {
     // G (times log2 e) in f64; a decay of exp(-200) is 0 in f32, and sums of -infinity
     // have no differences
-    const long t = t0 + min(lane, n - 1);
-    const float x = a.log_decay[t * a.decay_token + head];
-    const float beta = DELTA ? a.beta[t * a.beta_token + head] : 0.0f;
-    double sum = lane < n ? (x < -200.0f ? -200.0 : (double)x) * 1.4426950408889634 : 0.0;
+    double sum = lane < n ? (decay < -200.0f ? -200.0 : (double)decay) * 1.4426950408889634 : 0.0;
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) {
       const double up = __shfl_up(sum, d, 64);
       if (lane >= d) sum += up;
     }
-    s_sum[lane] = sum;
+    s_sum[0][lane] = (float)sum;
+    s_sum[1][lane] = (float)(sum - (float)sum);
     s_beta[lane] = lane < n ? beta : 0.0f;
   }
   __syncthreads();
+  // tile e of the wave: row and column of tiles
+  auto tile_row = [&](int e) { return outer ? (e < 4 ? 3 : 0) : e < 2 ? 1 : 2; };
+  auto tile_col = [&](int e) { return outer ? (e < 4 ? e : 0) : e < 2 ? e : e - 2; };
   if (DELTA || !keys) {
-    float* mat = s_mat[keys ? 0 : 1];
 #pragma unroll
     for (int e = 0; e < 5; ++e) {
-      const int i0 = 16 * tile_row(e) + 4 * g, j = 16 * tile_col(e) + m;
-      const double gj = s_sum[j];
+      const int i = 16 * tile_row(e) + m, j0 = 16 * tile_col(e) + 4 * g;
+      const f32x4 far = s_sum[0][i] - *(const f32x4*)&s_sum[0][j0], near = s_sum[1][i] - *(const f32x4*)&s_sum[1][j0];
+      const float scale = keys ? s_beta[i] : a.scale;
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        const int i = i0 + r;
-        const float d = __builtin_amdgcn_exp2f((float)(s_sum[i] - gj)) * (keys ? s_beta[i] : a.scale);
-        mat[i * ROW + j] = (keys ? i > j : i >= j && i < n) ? tile[e][r] * d : 0.0f;
+        const int j = j0 + r;
+        const float d = __builtin_amdgcn_exp2f(far[r] + near[r]) * scale;
+        tile[e][r] = (keys ? i > j : i >= j && i < n) ? tile[e][r] * d : 0.0f;
       }
+      if (DELTA && keys) *(f32x4*)&s_mat[i * ROW + j0] = tile[e];
     }
   }
-  __syncthreads();
-  if (DELTA && wave == 0) {
-    float* mat = s_mat[0];
-    const int b = lane & 48;
-    float x[16];
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      float y = i == m ? 1.0f : 0.0f;
-#pragma unroll
-      for (int l = 0; l < i; ++l) y = __builtin_fmaf(-mat[(b + i) * ROW + b + l], x[l], y);
-      x[i] = i < m ? 0.0f : y;
-    }
-    wave_sync();
-#pragma unroll
-    for (int i = 0; i < 16; ++i) mat[(b + i) * ROW + b + m] = x[i];
-  } else {
-    // A, its rows of tiles in turn
-    for (int i = DELTA ? wave - 1 : wave; i < kTiles; i += DELTA ? 3 : 4) {
-      const float* row = s_mat[1] + (16 * i + m) * ROW + 4 * g;
-      u32x4* to = (u32x4*)(out + W::inside_row(i)) + lane;
-      for (int j = 0; j <= i; j += W::whole ? 1 : 2) {
-        const f32x4 x = *(const f32x4*)(row + 16 * j);
-        if constexpr (W::whole) {
-          to[j * 64] = __builtin_bit_cast(u32x4, x);
-        } else {
-          const f32x4 none = {0.0f, 0.0f, 0.0f, 0.0f}, y = *(const f32x4*)(row + 16 * j + 16);
-          u32x4 planes[2];
-          split8<2>(x, j < i ? y : none, planes);
-          to[j * 64] = planes[0];
-          to[j * 64 + 64] = planes[1];
-        }
+  if (!keys) {  // A
+    const f32x4 none = {0.0f, 0.0f, 0.0f, 0.0f};
+    auto leave = [&](int i, int j, f32x4 x, f32x4 y) {
+      u32x4* to = (u32x4*)(out + W::inside_row(i) + j * 1024) + lane;
+      if constexpr (W::whole) {
+        to[0] = __builtin_bit_cast(u32x4, x);
+        if (j < i) to[64] = __builtin_bit_cast(u32x4, y);
+      } else {
+        u32x4 planes[2];
+        split8<2>(x, y, planes);
+        to[0] = planes[0];
+        to[64] = planes[1];
       }
+    };
+    if (outer) {
+      leave(3, 0, tile[0], tile[1]);
+      leave(3, 2, tile[2], tile[3]);
+      leave(0, 0, tile[4], none);
+    } else {
+      leave(1, 0, tile[0], tile[1]);
+      leave(2, 0, tile[2], tile[3]);
+      leave(2, 2, tile[4], none);
     }
-    if (wave == 3) {
-      const double last = s_sum[63];
-      float* numbers = (float*)(out + W::numbers);
-      numbers[lane] = __builtin_amdgcn_exp2f((float)s_sum[lane]);
-      numbers[64 + lane] = __builtin_amdgcn_exp2f((float)(last - s_sum[lane]));
-      if (lane == 0) numbers[128] = __builtin_amdgcn_exp2f((float)last);
-    }
+  }
+  if (wave == 3) {
+    float* numbers = (float*)(out + W::numbers);
+    const float sum = s_sum[0][lane];
+    numbers[lane] = __builtin_amdgcn_exp2f(sum);
+    numbers[64 + lane] = __builtin_amdgcn_exp2f((s_sum[0][63] - sum) + (s_sum[1][63] - s_sum[1][lane]));
+    if (lane == 63) numbers[128] = __builtin_amdgcn_exp2f(sum);
   }
   if constexpr (DELTA) {
+    float* mat = s_mat;
     __syncthreads();
-    float* mat = s_mat[0];
+    if (wave == 0) {
+      const int b = lane & 48;
+      float x[16];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        float y = i == m ? 1.0f : 0.0f;
+#pragma unroll
+        for (int l = 0; l < i; ++l) y = __builtin_fmaf(-mat[(b + i) * ROW + b + l], x[l], y);
+        x[i] = i < m ? 0.0f : y;
+      }
+      wave_sync();
+#pragma unroll
+      for (int i = 0; i < 16; ++i) mat[(b + i) * ROW + b + m] = x[i];
+    }
+    __syncthreads();
     auto block = [&](int i, int j) { return mat + (16 * i + m) * ROW + 16 * j + 4 * g; };  // as a left operand
     // T = X diag(beta) (nothing above the diagonal, whatever beta holds)
     auto leave = [&](int i, int j, f32x4 x) {
@@ -460,10 +465,10 @@ __global__ __launch_bounds__(256) void k_linear_prepare(LinearArgs a) {
 #pragma unroll
       for (int d = 1; d < kTiles; ++d) {  // x[d] is X_{j + d, j}
         if (j + d >= kTiles) break;
-        f32x4 sum = none;
+        f32x4 sum[2] = {none, none};  // (side by side: each product waits for the one before it)
 #pragma unroll
-        for (int e = 0; e < d; ++e) sum = mfma4(*(const f32x4*)block(j + d, j + e), x[e], sum);
-        x[d] = mfma4(-*(const f32x4*)block(j + d, j + d), sum, none);
+        for (int e = 0; e < d; ++e) sum[e & 1] = mfma4(*(const f32x4*)block(j + d, j + e), x[e], sum[e & 1]);
+        x[d] = mfma4(-*(const f32x4*)block(j + d, j + d), sum[0] + sum[1], none);
         // turned by way of the blocks above the diagonal, which nothing reads
         wave_sync();
 #pragma unroll
@@ -890,8 +895,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
 
 template <typename T, int DK, bool DELTA>
 static void launch_chunks(const LinearArgs& a, hipStream_t s) {
-  hipLaunchKernelGGL((k_linear_prepare<T, DK, DELTA>), dim3((unsigned)(a.tokens / kChunk + a.nseq), (unsigned)a.v_heads),
-                     dim3(256), 0, s, a);
+  hipLaunchKernelGGL((k_linear_prepare<T, DK, DELTA>), dim3((unsigned)((a.tokens / kChunk + a.nseq) * a.v_heads)), dim3(256), 0, s, a);
   const long pairs = ((long)a.nseq * a.v_heads + 7) / 8 * 8;
   hipLaunchKernelGGL((k_linear_scan<T, DK, DELTA>), dim3((unsigned)(pairs * (a.value_dim / (2048 / DK)))), dim3(512), 0, s, a);
 }
