@@ -260,57 +260,47 @@ struct ChunkWork {
 // most tokens / 64 + nseq.
 __device__ __forceinline__ long first_slot(const LinearSeq& s, int i) { return s.first / kChunk + i; }
 
+// A value that the compiler takes as new here.
+__device__ __forceinline__ int fresh(int v) {
+  asm volatile("" : "+v"(v));
+  return v;
+}
+
 // (LDS between the lanes of a wave: in order in the hardware, kept in order here)
 __device__ __forceinline__ void wave_sync() {
   __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
   __builtin_amdgcn_wave_barrier();
 }
 
-// Sixteen rows of DK elements, a row to the lanes of equal l mod 16: either operand of
-// row_product, which gives the 16 x 16 products of two of them.
-template <typename T, int DK>
-struct RowTile {
-  u32x4 v[sizeof(T) == 4 ? DK / 16 : DK / 32];
-  // rows from row0 on, of n > 0 (behind them, the last again)
-  __device__ __forceinline__ void load(const T* base, long stride, int row0, int n) {
-    const int lane = threadIdx.x & 63, g = lane >> 4, row = row0 + (lane & 15);
-    typedef uint32_t piece __attribute__((ext_vector_type(4), aligned(2)));
-    constexpr int W = 16 / sizeof(T);  // elements of a piece
-    const T* at = base + min(row, n - 1) * stride + g * W;
-#pragma unroll
-    for (int s = 0; s < (int)(sizeof(v) / 16); ++s) v[s] = *(const piece*)(at + 4 * s * W);
-  }
-};
-template <typename T, int DK>
-__device__ __forceinline__ f32x4 row_product(const RowTile<T, DK>& a, const RowTile<T, DK>& b) {
-  f32x4 c = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-  for (int s = 0; s < (int)(sizeof(a.v) / 16); ++s) {
-    if constexpr (sizeof(T) == 4)
-      c = mfma4(__builtin_bit_cast(f32x4, a.v[s]), __builtin_bit_cast(f32x4, b.v[s]), c);
-    else if constexpr (std::is_same<T, f16_t>::value)
-      c = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h16x8, a.v[s]), __builtin_bit_cast(h16x8, b.v[s]), c, 0, 0, 0);
-    else
-      c = mfma(a.v[s], b.v[s], c);
-  }
-  return c;
+// One step of sixteen rows against sixteen others: 16 bytes of a row a lane.
+template <typename T>
+__device__ __forceinline__ f32x4 row_product(u32x4 a, u32x4 b, f32x4 c) {
+  if constexpr (sizeof(T) == 4) return mfma4(__builtin_bit_cast(f32x4, a), __builtin_bit_cast(f32x4, b), c);
+  else if constexpr (std::is_same<T, f16_t>::value)
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h16x8, a), __builtin_bit_cast(h16x8, b), c, 0, 0, 0);
+  else return mfma(a, b, c);
 }
 
-// A workgroup takes a chunk of one value head.  The ten tiles of K K^T are two waves', those
-// of K Q^T the others': with the keys on the left, a result has row m, columns 4 g ..+3 of L
-// or A, as they go into LDS and out.  (1 + L)^-1 goes by blocks of 16: those on the diagonal
-// by substitution, a column a lane; then each column of blocks downwards, X_ij = -X_ii sum
-// of L_ik X_kj, a wave a column.
+// A workgroup takes a chunk of one key head, and its value heads in turn.  The ten tiles of K
+// K^T are two waves', those of K Q^T the others': with the keys on the left, a result has row
+// m, columns 4 g ..+3 of L or A, as they go into LDS and out.  (1 + L)^-1 goes by blocks of
+// 16: those on the diagonal by substitution, a column a lane; then each column of blocks
+// downwards, X_ij = -X_ii sum of L_ik X_kj, a wave a column.
 template <typename T, int DK, bool DELTA>
-__global__ __launch_bounds__(256, 2) void k_linear_prepare(LinearArgs a) {
+__global__ __launch_bounds__(256) void k_linear_prepare(LinearArgs a) {
   typedef ChunkWork<T, DELTA> W;
   constexpr int ROW = kChunk + 4;  // floats of a row in LDS
-  __shared__ __attribute__((aligned(16))) float s_mat[DELTA ? kChunk * ROW : 4];  // L, then its inverse
+  constexpr int PIECES = DK * sizeof(T) / 64, TILE = PIECES * 64;  // 16-byte pieces of a row a lane, of 16 rows
+  __shared__ u32x4 s_rows[2][kTiles][TILE];  // keys and queries; then L and its inverse
   __shared__ __attribute__((aligned(16))) float s_sum[2][kChunk];  // G in two parts
   __shared__ __attribute__((aligned(16))) float s_beta[kChunk];
+  static_assert(sizeof(s_rows) >= kChunk * ROW * 4 || DK == 64, "L");
+  constexpr int MORE = sizeof(s_rows) >= kChunk * ROW * 4 ? 1 : kChunk * ROW;  // (16-bit rows of 64)
+  __shared__ __attribute__((aligned(16))) float s_more[MORE];
+  float* const mat = MORE > 1 ? s_more : (float*)s_rows;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, g = lane >> 4, m = lane & 15;
   // (heads side by side: a head's rows, a token's stride apart, lie in few memory channels)
-  const int slot = blockIdx.x / a.v_heads, head = blockIdx.x - slot * a.v_heads;
+  const int slot = blockIdx.x / a.k_heads, kh = blockIdx.x - slot * a.k_heads;
   // the slot's sequence: the last whose first slot is not behind it
   int seq = -1, first = 0, end = 0;
   for (int i0 = 0; i0 < a.nseq; i0 += 64) {
@@ -330,153 +320,178 @@ __global__ __launch_bounds__(256, 2) void k_linear_prepare(LinearArgs a) {
   const int chunk = (int)(slot - first_slot(s, seq)), n = s.n - chunk * kChunk;  // tokens from the chunk's first on
   if (chunk < 0 || n <= 0 || s.n <= a.few) return;
   const long t0 = first + (long)chunk * kChunk;
-  uint8_t* out = a.work + ((long)slot * a.v_heads + head) * W::bytes;
-  float decay = 0.0f, beta = 0.0f;
-  if (wave == 0) {
-    const long t = t0 + min(lane, n - 1);
-    decay = a.log_decay[t * a.decay_token + head];
-    if (DELTA) beta = a.beta[t * a.beta_token + head];
-  }
-
-  const int kh = head / a.group;
-  const T* k = (const T*)a.k + t0 * a.k_token + kh * a.k_head;
-  const T* q = (const T*)a.q + t0 * a.q_token + kh * a.q_head;
-  // rows of tiles 3 and 0, or 1 and 2, of L or A: five tiles each
-  const bool keys = wave < 2, outer = (wave & 1) == 0;
-  f32x4 tile[5];
-  if (DELTA || !keys) {
-    const T* rows = keys ? k : q;
-    const long stride = keys ? a.k_token : a.q_token;
-    RowTile<T, DK> x[2], y[4];  // (all loads before the first product)
-    x[0].load(rows, stride, outer ? 48 : 16, n);
+  {
+    const char* k = (const char*)((const T*)a.k + t0 * a.k_token + kh * a.k_head);
+    const char* q = (const char*)((const T*)a.q + t0 * a.q_token + kh * a.q_head);
+    typedef uint32_t piece __attribute__((ext_vector_type(4), aligned(2)));
+    constexpr int EACH = TILE / 256 ? TILE / 256 : 1;  // pieces of a tile a thread
+    const int tid = threadIdx.x, step = tid >> 6;
+    if (TILE >= 256 || tid < TILE) {
+      u32x4 x[2][kTiles][EACH];  // (rows behind the sequence's end: the last again)
 #pragma unroll
-    for (int j = 0; j < 3; ++j) y[j].load(k, a.k_token, 16 * j, n);
-    if (outer) y[3].load(k, a.k_token, 48, n);
-    x[1].load(rows, stride, outer ? 0 : 32, n);
-    if (outer) {
+      for (int t = 0; t < kTiles; ++t) {
+        const long row = min(16 * t + m, n - 1);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) tile[j] = row_product(y[j], x[0]);
-      tile[4] = row_product(y[0], x[1]);
-    } else {
-      tile[0] = row_product(y[0], x[0]);
-      tile[1] = row_product(y[1], x[0]);
+        for (int e = 0; e < EACH; ++e) {
+          const int at = 64 * (step + 4 * e) + 16 * g;
+          x[0][t][e] = *(const piece*)(k + row * a.k_token * (long)sizeof(T) + at);
+          x[1][t][e] = *(const piece*)(q + row * a.q_token * (long)sizeof(T) + at);
+        }
+      }
 #pragma unroll
-      for (int j = 0; j < 3; ++j) tile[2 + j] = row_product(y[j], x[1]);
+      for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+        for (int e = 0; e < EACH; ++e) {
+          s_rows[0][t][tid + 256 * e] = x[0][t][e];
+          s_rows[1][t][tid + 256 * e] = x[1][t][e];
+        }
     }
-  }
-  if (wave == 0) {
-    // G (times log2 e) in f64; a decay of exp(-200) is 0 in f32, and sums of -infinity
-    // have no differences
-    double sum = lane < n ? (decay < -200.0f ? -200.0 : (double)decay) * 1.4426950408889634 : 0.0;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-      const double up = __shfl_up(sum, d, 64);
-      if (lane >= d) sum += up;
-    }
-    s_sum[0][lane] = (float)sum;
-    s_sum[1][lane] = (float)(sum - (float)sum);
-    s_beta[lane] = lane < n ? beta : 0.0f;
   }
   __syncthreads();
-  // tile e of the wave: row and column of tiles
-  auto tile_row = [&](int e) { return outer ? (e < 4 ? 3 : 0) : e < 2 ? 1 : 2; };
-  auto tile_col = [&](int e) { return outer ? (e < 4 ? e : 0) : e < 2 ? e : e - 2; };
+  // rows of tiles 3 and 0, or 1 and 2, of L or A: five tiles each
+  const bool keys = wave < 2, outer = (wave & 1) == 0;
+  f32x4 product[5] = {};
   if (DELTA || !keys) {
+    const u32x4(*rows)[TILE] = s_rows[keys ? 0 : 1];
 #pragma unroll
-    for (int e = 0; e < 5; ++e) {
-      const int i = 16 * tile_row(e) + m, j0 = 16 * tile_col(e) + 4 * g;
-      const f32x4 far = s_sum[0][i] - *(const f32x4*)&s_sum[0][j0], near = s_sum[1][i] - *(const f32x4*)&s_sum[1][j0];
-      const float scale = keys ? s_beta[i] : a.scale;
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int j = j0 + r;
-        const float d = __builtin_amdgcn_exp2f(far[r] + near[r]) * scale;
-        tile[e][r] = (keys ? i > j : i >= j && i < n) ? tile[e][r] * d : 0.0f;
-      }
-      if (DELTA && keys) *(f32x4*)&s_mat[i * ROW + j0] = tile[e];
-    }
-  }
-  if (!keys) {  // A
-    const f32x4 none = {0.0f, 0.0f, 0.0f, 0.0f};
-    auto leave = [&](int i, int j, f32x4 x, f32x4 y) {
-      u32x4* to = (u32x4*)(out + W::inside_row(i) + j * 1024) + lane;
-      if constexpr (W::whole) {
-        to[0] = __builtin_bit_cast(u32x4, x);
-        if (j < i) to[64] = __builtin_bit_cast(u32x4, y);
+    for (int i = 0; i < PIECES; ++i) {
+      const int at = i * 64 + lane;
+      const u32x4 x0 = rows[outer ? 3 : 1][at], x1 = rows[outer ? 0 : 2][at];
+      const u32x4 y0 = s_rows[0][0][at], y1 = s_rows[0][1][at], y2 = s_rows[0][2][at];
+      product[0] = row_product<T>(y0, x0, product[0]);
+      product[1] = row_product<T>(y1, x0, product[1]);
+      if (outer) {
+        product[2] = row_product<T>(y2, x0, product[2]);
+        product[3] = row_product<T>(s_rows[0][3][at], x0, product[3]);
+        product[4] = row_product<T>(y0, x1, product[4]);
       } else {
-        u32x4 planes[2];
-        split8<2>(x, y, planes);
-        to[0] = planes[0];
-        to[64] = planes[1];
+        product[2] = row_product<T>(y0, x1, product[2]);
+        product[3] = row_product<T>(y1, x1, product[3]);
+        product[4] = row_product<T>(y2, x1, product[4]);
       }
-    };
-    if (outer) {
-      leave(3, 0, tile[0], tile[1]);
-      leave(3, 2, tile[2], tile[3]);
-      leave(0, 0, tile[4], none);
-    } else {
-      leave(1, 0, tile[0], tile[1]);
-      leave(2, 0, tile[2], tile[3]);
-      leave(2, 2, tile[4], none);
     }
   }
-  if (wave == 3) {
-    float* numbers = (float*)(out + W::numbers);
-    const float sum = s_sum[0][lane];
-    numbers[lane] = __builtin_amdgcn_exp2f(sum);
-    numbers[64 + lane] = __builtin_amdgcn_exp2f((s_sum[0][63] - sum) + (s_sum[1][63] - s_sum[1][lane]));
-    if (lane == 63) numbers[128] = __builtin_amdgcn_exp2f(sum);
-  }
-  if constexpr (DELTA) {
-    float* mat = s_mat;
-    __syncthreads();
+  for (int head = kh * a.group; head < (kh + 1) * a.group; ++head) {
+    // (lanes as something new in each pass: what follows from them would fill the registers)
+    const int lane = fresh(threadIdx.x & 63), g = lane >> 4, m = lane & 15;
+    uint8_t* out = a.work + ((long)slot * a.v_heads + head) * W::bytes;
     if (wave == 0) {
-      const int b = lane & 48;
-      float x[16];
+      // G (times log2 e) in f64; a decay of exp(-200) is 0 in f32, and sums of -infinity
+      // have no differences
+      const long t = t0 + min(lane, n - 1);
+      const float decay = a.log_decay[t * a.decay_token + head], beta = DELTA ? a.beta[t * a.beta_token + head] : 0.0f;
+      double sum = lane < n ? (decay < -200.0f ? -200.0 : (double)decay) * 1.4426950408889634 : 0.0;
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        float y = i == m ? 1.0f : 0.0f;
-#pragma unroll
-        for (int l = 0; l < i; ++l) y = __builtin_fmaf(-mat[(b + i) * ROW + b + l], x[l], y);
-        x[i] = i < m ? 0.0f : y;
+      for (int d = 1; d < 64; d <<= 1) {
+        const double up = __shfl_up(sum, d, 64);
+        if (lane >= d) sum += up;
       }
-      wave_sync();
-#pragma unroll
-      for (int i = 0; i < 16; ++i) mat[(b + i) * ROW + b + m] = x[i];
+      s_sum[0][lane] = (float)sum;
+      s_sum[1][lane] = (float)(sum - (float)sum);
+      s_beta[lane] = lane < n ? beta : 0.0f;
     }
     __syncthreads();
-    auto block = [&](int i, int j) { return mat + (16 * i + m) * ROW + 16 * j + 4 * g; };  // as a left operand
-    // T = X diag(beta) (nothing above the diagonal, whatever beta holds)
-    auto leave = [&](int i, int j, f32x4 x) {
-      const f32x4 b = *(const f32x4*)(s_beta + 16 * j + 4 * g);
+    f32x4 tile[5];
+    if (DELTA || !keys) {
+      // of tiles (3, 0) .. (3, 3), (0, 0), or (1, 0), (1, 1), (2, 0) .. (2, 2)
+      const float scales[2] = {keys ? s_beta[outer ? 48 + m : 16 + m] : a.scale, keys ? s_beta[outer ? m : 32 + m] : a.scale};
 #pragma unroll
-      for (int e = 0; e < 4; ++e) x[e] = i > j || 4 * g + e <= m ? x[e] * b[e] : 0.0f;
-      *((f32x4*)(out + W::solve_tile(i, j)) + lane) = x;
-    };
-    const f32x4 none = {0.0f, 0.0f, 0.0f, 0.0f};
-    if (wave == 3) {
+      for (int e = 0; e < 5; ++e) {
+        const int first_of = outer ? 4 : 2, second = e >= first_of;
+        const int i = (outer ? (second ? 0 : 48) : (second ? 32 : 16)) + m, j0 = 16 * (second ? e - first_of : e) + 4 * g;
+        const f32x4 far = s_sum[0][i] - *(const f32x4*)&s_sum[0][j0], near = s_sum[1][i] - *(const f32x4*)&s_sum[1][j0];
+        const float scale = second ? scales[1] : scales[0];
+        const int seen = i < n ? i + !keys - j0 : 0;  // columns of the four that the row has
 #pragma unroll
-      for (int i = 0; i < kTiles; ++i) leave(i, i, *(const f32x4*)block(i, i));
-    } else {
-      const int j = wave;
-      f32x4 x[kTiles];
-#pragma unroll
-      for (int r = 0; r < 4; ++r) x[0][r] = mat[(16 * j + 4 * g + r) * ROW + 16 * j + m];
-#pragma unroll
-      for (int d = 1; d < kTiles; ++d) {  // x[d] is X_{j + d, j}
-        if (j + d >= kTiles) break;
-        f32x4 sum[2] = {none, none};  // (side by side: each product waits for the one before it)
-#pragma unroll
-        for (int e = 0; e < d; ++e) sum[e & 1] = mfma4(*(const f32x4*)block(j + d, j + e), x[e], sum[e & 1]);
-        x[d] = mfma4(-*(const f32x4*)block(j + d, j + d), sum[0] + sum[1], none);
-        // turned by way of the blocks above the diagonal, which nothing reads
-        wave_sync();
-#pragma unroll
-        for (int r = 0; r < 4; ++r) mat[(16 * j + 4 * g + r) * ROW + 16 * (j + d) + m] = x[d][r];
-        wave_sync();
-        leave(j + d, j, *(const f32x4*)block(j, j + d));
+        for (int r = 0; r < 4; ++r) {
+          const float x = product[e][r] * (__builtin_amdgcn_exp2f(far[r] + near[r]) * scale);
+          tile[e][r] = r < seen ? x : 0.0f;
+        }
+        if (DELTA && keys) *(f32x4*)&mat[i * ROW + j0] = tile[e];
       }
     }
+    if (!keys) {  // A
+      const f32x4 none = {0.0f, 0.0f, 0.0f, 0.0f};
+      auto leave = [&](int i, int j, f32x4 x, f32x4 y) {
+        u32x4* to = (u32x4*)(out + W::inside_row(i) + j * 1024) + lane;
+        if constexpr (W::whole) {
+          to[0] = __builtin_bit_cast(u32x4, x);
+          if (j < i) to[64] = __builtin_bit_cast(u32x4, y);
+        } else {
+          u32x4 planes[2];
+          split8<2>(x, y, planes);
+          to[0] = planes[0];
+          to[64] = planes[1];
+        }
+      };
+      if (outer) {
+        leave(3, 0, tile[0], tile[1]);
+        leave(3, 2, tile[2], tile[3]);
+        leave(0, 0, tile[4], none);
+      } else {
+        leave(1, 0, tile[0], tile[1]);
+        leave(2, 0, tile[2], tile[3]);
+        leave(2, 2, tile[4], none);
+      }
+    }
+    if (wave == 3) {
+      float* numbers = (float*)(out + W::numbers);
+      const float sum = s_sum[0][lane];
+      numbers[lane] = __builtin_amdgcn_exp2f(sum);
+      numbers[64 + lane] = __builtin_amdgcn_exp2f((s_sum[0][63] - sum) + (s_sum[1][63] - s_sum[1][lane]));
+      if (lane == 63) numbers[128] = __builtin_amdgcn_exp2f(sum);
+    }
+    if constexpr (DELTA) {
+      __syncthreads();
+      if (wave == 0) {
+        const int b = lane & 48;
+        float x[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          float y = i == m ? 1.0f : 0.0f;
+#pragma unroll
+          for (int l = 0; l < i; ++l) y = __builtin_fmaf(-mat[(b + i) * ROW + b + l], x[l], y);
+          x[i] = i < m ? 0.0f : y;
+        }
+        wave_sync();
+#pragma unroll
+        for (int i = 0; i < 16; ++i) mat[(b + i) * ROW + b + m] = x[i];
+      }
+      __syncthreads();
+      auto block = [&](int i, int j) { return mat + (16 * i + m) * ROW + 16 * j + 4 * g; };  // as a left operand
+      // T = X diag(beta) (nothing above the diagonal, whatever beta holds)
+      auto leave = [&](int i, int j, f32x4 x) {
+        const f32x4 b = *(const f32x4*)(s_beta + 16 * j + 4 * g);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] = i > j || 4 * g + e <= m ? x[e] * b[e] : 0.0f;
+        *((f32x4*)(out + W::solve_tile(i, j)) + lane) = x;
+      };
+      const f32x4 none = {0.0f, 0.0f, 0.0f, 0.0f};
+      if (wave == 3) {
+#pragma unroll
+        for (int i = 0; i < kTiles; ++i) leave(i, i, *(const f32x4*)block(i, i));
+      } else {
+        const int j = wave;
+        f32x4 x[kTiles];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) x[0][r] = mat[(16 * j + 4 * g + r) * ROW + 16 * j + m];
+#pragma unroll
+        for (int d = 1; d < kTiles; ++d) {  // x[d] is X_{j + d, j}
+          if (j + d >= kTiles) break;
+          f32x4 sum[2] = {none, none};  // (side by side: each product waits for the one before it)
+#pragma unroll
+          for (int e = 0; e < d; ++e) sum[e & 1] = mfma4(*(const f32x4*)block(j + d, j + e), x[e], sum[e & 1]);
+          x[d] = mfma4(-*(const f32x4*)block(j + d, j + d), sum[0] + sum[1], none);
+          // turned by way of the blocks above the diagonal, which nothing reads
+          wave_sync();
+#pragma unroll
+          for (int r = 0; r < 4; ++r) mat[(16 * j + 4 * g + r) * ROW + 16 * (j + d) + m] = x[d][r];
+          wave_sync();
+          leave(j + d, j, *(const f32x4*)block(j, j + d));
+        }
+      }
+    }
+    if (head + 1 < (kh + 1) * a.group) __syncthreads();
   }
 }
 
@@ -895,7 +910,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
 
 template <typename T, int DK, bool DELTA>
 static void launch_chunks(const LinearArgs& a, hipStream_t s) {
-  hipLaunchKernelGGL((k_linear_prepare<T, DK, DELTA>), dim3((unsigned)((a.tokens / kChunk + a.nseq) * a.v_heads)), dim3(256), 0, s, a);
+  hipLaunchKernelGGL((k_linear_prepare<T, DK, DELTA>), dim3((unsigned)((a.tokens / kChunk + a.nseq) * a.k_heads)), dim3(256), 0, s, a);
   const long pairs = ((long)a.nseq * a.v_heads + 7) / 8 * 8;
   hipLaunchKernelGGL((k_linear_scan<T, DK, DELTA>), dim3((unsigned)(pairs * (a.value_dim / (2048 / DK)))), dim3(512), 0, s, a);
 }
