@@ -50,8 +50,14 @@ __device__ __forceinline__ LinearSeq linear_seq(const LinearArgs& a, int i, int 
   return s;
 }
 
-// Sequences of at most this many new tokens go token by token.
-constexpr int kFew = 12;
+// Beside sequences that go in chunks, those of at most this many new tokens go token by
+// token: a chunk takes one sequence of 16 heads 15 us, a token 0.8.
+constexpr int kFew = 16;
+// A batch whose sequences all have at most this many does without chunks.  Of sequences
+// that fill the card (256 workgroups of 64 columns) a chunk costs more tokens: 16 heads of
+// 128 x 128, token by token / in chunks: 1 sequence, 16 tokens 16.5 / 15 us, 32: 29 / 16; 64
+// sequences, 16 tokens 66 / 199 us, 32: 120 / 213.
+static int few_alone(const qhip_linear_batch* b) { return (long)b->nseq * b->v_heads * (b->value_dim / 64) < 256 ? kFew : 2 * kFew; }
 
 // sum over lanes l, l ^ 16, l ^ 32, l ^ 48
 __device__ __forceinline__ float sum_rows(float v) {
@@ -61,19 +67,35 @@ __device__ __forceinline__ float sum_rows(float v) {
   return __uint_as_float(x[0]) + __uint_as_float(x[1]);
 }
 
+// N elements side by side, from any element's address
+template <typename T, int N>
+struct Some {
+  T e[N];
+  __device__ __forceinline__ void load(const T* p) {
+    typedef uint32_t words __attribute__((ext_vector_type(N * sizeof(T) / 4 > 4 ? 4 : N * sizeof(T) / 4), aligned(2)));
+    struct Words {
+      words w[(N * sizeof(T) + 15) / 16];
+    } x;
+#pragma unroll
+    for (unsigned i = 0; i < sizeof(x.w) / sizeof(words); ++i) x.w[i] = ((const words*)p)[i];
+    *this = __builtin_bit_cast(Some, x);
+  }
+};
+
 // ---- token by token --------------------------------------------------------------------
 //
-// A workgroup holds 64 columns of a head's state in registers: lane l of a wave
-// columns 4 (l mod 16) ..+3 of DK / 16 rows.  A token's products k S and q S (of the
-// state before it) are summed over the rows together, so that one exchange between
-// the waves serves both:  out = scale (a q S + (q . k) u).
+// A workgroup holds 64 columns of a head's state in registers: a lane four of them, of DK /
+// 16 rows.  A token's products k S and q S (of the state before it) are summed over the rows
+// together, so that one exchange between the waves serves both:  out = scale (a q S + (q . k)
+// u).  (16 columns a workgroup: one token of one sequence of 16 heads 4.0 us instead of 4.2, of
+// eight 8.8 instead of 5.5.)
 template <typename T, int DK>
 __global__ __launch_bounds__(256) void k_linear_steps(LinearArgs a) {
-  constexpr int R = DK / 16;  // rows of a thread
-  __shared__ float s_part[2][4][2][64];
+  constexpr int COLS = 64, ACROSS = COLS / 4, R = DK * ACROSS / 256;  // lanes of a row, rows of a thread
+  __shared__ __attribute__((aligned(16))) float s_part[2][4][2][COLS];
   __shared__ float s_qk[2][4];
-  const int tid = threadIdx.x, wave = tid >> 6, col = (tid & 15) * 4, row0 = (tid >> 4) * R;
-  const int seq = blockIdx.z, head = blockIdx.y, d0 = blockIdx.x * 64 + col;
+  const int tid = threadIdx.x, wave = tid >> 6, col = (tid % ACROSS) * 4, row0 = tid / ACROSS * R;
+  const int seq = blockIdx.z, head = blockIdx.y, d0 = blockIdx.x * COLS + col;
   const LinearSeq s = linear_seq(a, seq, head, DK);
   if (s.n > a.few || (s.n == 0 && s.from == s.to)) return;
   f32x4 st[R];
@@ -90,26 +112,34 @@ __global__ __launch_bounds__(256) void k_linear_steps(LinearArgs a) {
   T* out = (T*)a.out + s.first * a.out_token + head * a.out_head + d0;
   const float* decay = a.log_decay + s.first * a.decay_token + head;
   const float* beta = a.beta ? a.beta + s.first * a.beta_token + head : nullptr;
+  Some<T, R> kr, qr;
+  Some<T, 4> vr;
+  float log_keep = 0.0f, b = 0.0f;
+  auto fetch = [&](int t) {
+    kr.load(k + t * a.k_token);
+    qr.load(q + t * a.q_token);
+    vr.load(v + t * a.v_token);
+    log_keep = decay[t * a.decay_token];
+    if (beta) b = beta[t * a.beta_token];
+  };
+  if (s.n > 0) fetch(0);
   for (int t = 0; t < s.n; ++t) {
-    float kr[R], qr[R], vc[4];
+    float kf[R], vc[4], ks[4] = {}, qs[4] = {}, qk = 0.0f;
+    const float keep = expf(log_keep), rate = b;
+#pragma unroll
+    for (int c = 0; c < 4; ++c) vc[c] = (float)vr.e[c];
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-      kr[r] = (float)k[t * a.k_token + r];
-      qr[r] = (float)q[t * a.q_token + r];
-    }
-#pragma unroll
-    for (int c = 0; c < 4; ++c) vc[c] = (float)v[t * a.v_token + c];
-    const float keep = expf(decay[t * a.decay_token]), b = beta ? beta[t * a.beta_token] : 0.0f;
-    float ks[4] = {}, qs[4] = {}, qk = 0.0f;
-#pragma unroll
-    for (int r = 0; r < R; ++r) {
-      qk = __builtin_fmaf(qr[r], kr[r], qk);
+      const float qf = (float)qr.e[r];
+      kf[r] = (float)kr.e[r];
+      qk = __builtin_fmaf(qf, kf[r], qk);
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
-        ks[c] = __builtin_fmaf(kr[r], st[r][c], ks[c]);
-        qs[c] = __builtin_fmaf(qr[r], st[r][c], qs[c]);
+        ks[c] = __builtin_fmaf(kf[r], st[r][c], ks[c]);
+        qs[c] = __builtin_fmaf(qf, st[r][c], qs[c]);
       }
     }
+    if (t + 1 < s.n) fetch(t + 1);
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
       ks[c] = sum_rows(ks[c]);
@@ -117,30 +147,30 @@ __global__ __launch_bounds__(256) void k_linear_steps(LinearArgs a) {
     }
     qk = sum_rows(qk);
     const int buf = t & 1;
-    if ((tid & 63) < 16) {
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        s_part[buf][wave][0][col + c] = ks[c];
-        s_part[buf][wave][1][col + c] = qs[c];
-      }
+    if ((tid & 63) < ACROSS) {
+      *(f32x4*)&s_part[buf][wave][0][col] = f32x4{ks[0], ks[1], ks[2], ks[3]};
+      *(f32x4*)&s_part[buf][wave][1][col] = f32x4{qs[0], qs[1], qs[2], qs[3]};
       if ((tid & 63) == 0) s_qk[buf][wave] = qk;
     }
     __syncthreads();  // (the buffer after next is written behind the next token's barrier)
     qk = (s_qk[buf][0] + s_qk[buf][1]) + (s_qk[buf][2] + s_qk[buf][3]);
+    f32x4 kc = {0.0f, 0.0f, 0.0f, 0.0f}, qc = kc;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      kc += *(const f32x4*)&s_part[buf][w][0][col];
+      qc += *(const f32x4*)&s_part[buf][w][1][col];
+    }
     float u[4], o[4];
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
-      const float(*p)[2][64] = s_part[buf];
-      const float kc = (p[0][0][col + c] + p[1][0][col + c]) + (p[2][0][col + c] + p[3][0][col + c]);
-      const float qc = (p[0][1][col + c] + p[1][1][col + c]) + (p[2][1][col + c] + p[3][1][col + c]);
-      u[c] = a.beta ? b * (vc[c] - keep * kc) : vc[c];
-      o[c] = a.scale * __builtin_fmaf(qk, u[c], keep * qc);
+      u[c] = beta ? rate * (vc[c] - keep * kc[c]) : vc[c];
+      o[c] = a.scale * __builtin_fmaf(qk, u[c], keep * qc[c]);
     }
 #pragma unroll
     for (int r = 0; r < R; ++r)
 #pragma unroll
-      for (int c = 0; c < 4; ++c) st[r][c] = __builtin_fmaf(kr[r], u[c], keep * st[r][c]);
-    if (tid < 16) {
+      for (int c = 0; c < 4; ++c) st[r][c] = __builtin_fmaf(kf[r], u[c], keep * st[r][c]);
+    if (tid < ACROSS) {
 #pragma unroll
       for (int c = 0; c < 4; ++c) out[t * a.out_token + c] = (T)o[c];
     }
@@ -532,6 +562,16 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   const int col = (id >> 3) % blocks * COLS + set * 16 + m;
   const LinearSeq s = linear_seq(a, seq, head, DK);
   if (s.n <= a.few) return;
+  if (s.n == 0) {  // (where no other kernel is launched)
+    const int block = (id >> 3) % blocks * COLS;
+    const float none = s.bad ? __builtin_nanf("") : 0.0f;
+    if (s.to != s.from)
+      for (int e = threadIdx.x; e < DK * COLS; e += 512) {
+        const long at = (long)(e / COLS) * a.value_dim + block + e % COLS;
+        if (s.to) s.to[at] = s.from ? s.from[at] : none;
+      }
+    return;
+  }
   const int kh = head / a.group, chunks = (s.n + kChunk - 1) / kChunk, tail = s.n - (chunks - 1) * kChunk;
   // the wave's tiles of tokens (of two the first and last, or those between: T has 1 to 4
   // tiles in a row)
@@ -927,9 +967,12 @@ static long chunk_bytes(int type, bool delta) {
   if (type == QHIP_TT_F32) return delta ? ChunkWork<float, true>::bytes : ChunkWork<float, false>::bytes;
   return delta ? ChunkWork<f16_t, true>::bytes : ChunkWork<f16_t, false>::bytes;
 }
+// 0: token by token (also where a grid would pass 2^32 threads)
 static long linear_work(const qhip_linear_batch* b, int type, bool delta) {
-  if (b->max_new <= kFew || b->nseq == 0 || b->tokens == 0) return 0;
-  return ((long)b->tokens / kChunk + b->nseq) * b->v_heads * chunk_bytes(type, delta);
+  if (b->max_new <= few_alone(b) || b->nseq == 0 || b->tokens == 0) return 0;
+  const long slots = (long)b->tokens / kChunk + b->nseq, pairs = (long)b->nseq * b->v_heads + 8;
+  if (slots * b->k_heads >= 1L << 24 || pairs * (b->value_dim / 16) >= 1L << 23) return 0;
+  return slots * b->v_heads * chunk_bytes(type, delta);
 }
 
 }  // namespace qhip
@@ -1024,13 +1067,13 @@ extern "C" int qhip_launch_linear_attention(const qhip_linear_batch* batch, int 
   a.value_dim = batch->value_dim;
   a.group = batch->v_heads / batch->k_heads;
   a.scale = scale;
-  // without a workspace every sequence goes token by token; where all have more than
-  // a few tokens the other kernel has nothing to do
+  // without a workspace every sequence goes token by token; where the tokens are as many
+  // as the longest would make, short ones are none or few, and all go in chunks
   const long need = linear_work(batch, type, d_beta != nullptr);
   const bool chunks = need > 0 && d_work;
   if (chunks && (work_bytes < need || !aligned16(d_work))) return (int)hipErrorInvalidValue;
   const bool steps = !chunks || (long)nseq * batch->max_new != tokens;
-  a.few = chunks ? kFew : 0x7FFFFFFF;
+  a.few = !chunks ? 0x7FFFFFFF : steps ? kFew : -1;
   a.work = (uint8_t*)d_work;
   hipStream_t st = (hipStream_t)stream;
   if (type == QHIP_TT_F32) launch_linear<float>(a, batch->key_dim, steps, chunks, st);
