@@ -621,15 +621,16 @@ def _linear_states(states: torch.Tensor, device: int) -> torch.Size:
 
 
 def _linear_work(work: torch.Tensor, device: int) -> int:
-    if work.dtype != torch.uint8 or work.dim() != 1 or work.get_device() != device or not work.is_contiguous():
-        raise ValueError("work: a contiguous uint8 tensor on the current GPU (linear_attention_work)")
+    if work.dtype != torch.uint8 or work.dim() != 1 or work.get_device() != device or not work.is_contiguous() or not work.numel():
+        raise ValueError("work: a contiguous uint8 tensor on the current GPU, not empty (linear_attention_work)")
     return work.numel()
 
 
 def linear_attention_work(states: torch.Tensor, q: torch.Tensor, nseq: int, max_new: int, delta: bool = True,
                           work: torch.Tensor | None = None) -> torch.Tensor | None:
-    """Workspace for linear_attention of q's tokens (None when none is needed), or `work` itself, an earlier one, if it is
-    large enough."""
+    """Workspace for linear_attention of q's tokens, or `work` itself, an earlier one, if it is large enough; None where the
+    call needs none (few new tokens a sequence).  What it holds is of no use behind the call, and it need not be cleared;
+    calls that may run at once, captured ones too, each take their own."""
     dev = torch.cuda.current_device()
     shape = _linear_states(states, dev)
     tt = _kv_rows("q", q, shape[2], dev)
@@ -653,7 +654,9 @@ def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_deca
     q, k [tokens, k_heads, key_dim], v [tokens, v_heads, value_dim]; log_decay, beta: f32 [tokens, v_heads].  Sequence i has
     tokens offsets[i] .. offsets[i + 1], at most max_new, starts from state source[i] (-1: zeros; by default slots[i]) and
     leaves its last state in slots[i] (-1: nowhere); no state that a sequence writes may be another's in the same call.
-    scale: 1 / sqrt(key_dim) by default.  Rows at or past offsets[-1] are not written."""
+    scale: 1 / sqrt(key_dim) by default.  Rows at or past offsets[-1] are not written.
+    work: linear_attention_work's; with it sequences of more than a few tokens go in chunks of 64, several times as fast,
+    without it (None) token by token."""
     dev, q_shape, dtype = torch.cuda.current_device(), q.shape, q.dtype
     n, v_heads, dk, dv = _linear_states(states, dev)
     if len(q_shape) != 3 or q_shape[2] != dk:

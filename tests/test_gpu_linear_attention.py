@@ -263,3 +263,83 @@ def test_in_a_graph_on_another_stream(gpu):
             graph.replay()
             torch.cuda.synchronize()
             assert torch.equal(out, want.run()) and torch.equal(b.states, want.states)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("delta", [True, False])
+@pytest.mark.parametrize("lengths", [[70, 3, 0, 40], [64, 0, 64, 0], [0, 0, 5, 90], [33, 1, 16, 17]])
+def test_rows_of_a_padded_batch(gpu, dtype, delta, lengths):
+    """As many rows as sequences of the longest length would have; short sequences and those without tokens, which copy."""
+    longest = max(lengths)
+    b = Batch(lengths, 2, 2, 128, 128, dtype, delta, pool=9, pad=longest * len(lengths) - sum(lengths))
+    b.slots, b.source = [4, 0, 7, 2], [-1, 5, 8, 2]
+    b.check()
+    b = Batch(lengths, 1, 2, 64, 256, dtype, delta, pool=9, pad=longest * len(lengths) - sum(lengths))
+    b.slots, b.source = [4, 0, 7, -1], [4, 0, 8, 2]
+    b.check()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_many_sequences_of_all_lengths(gpu, dtype):
+    """More sequences than a wave has lanes, those without tokens between, in chunks and token by token."""
+    lengths = [(0, 1, 70, 3, 0, 0, 129, 16, 17, 64, 65, 2)[i % 12] for i in range(150)]
+    Batch(lengths, 1, 2, 64, 128, dtype, pad=1).check()
+    Batch([0] * 130 + [90] + [0] * 67 + [1, 200], 1, 2, 64, 64, dtype).check()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_a_workspace_used_again_and_none(gpu, dtype):
+    """What a workspace holds is not read; without one every token goes by itself."""
+    got, bound = [], 8 * math.sqrt(300 + 128) * 2.0 ** -24
+    for work in ("nan", "larger", None):
+        b = Batch([300, 20, 1], 2, 4, 128, 128, dtype)
+        w = b.work()
+        if work == "nan":
+            w.view(torch.float32).fill_(torch.nan)
+        elif work == "larger":
+            w = torch.full((2 * w.numel(),), 255, dtype=torch.uint8, device="cuda")
+            assert ops.linear_attention_work(b.states, b.q, 3, 300, work=w) is w
+        got.append((b.run(work=None if work is None else w), b.states[b.slots]))
+    assert torch.equal(got[0][0], got[1][0]) and torch.equal(got[0][1], got[1][1])
+    own = torch.finfo(dtype).eps if dtype != torch.float32 else 0.0  # two roundings
+    for x, y, more in ((got[0][0], got[2][0], own), (got[0][1], got[2][1], 0.0)):
+        assert float((x.double() - y.double()).norm() / y.double().norm()) <= bound + more
+
+
+def test_workspaces_that_do_not_fit(gpu):
+    b = Batch([300, 20], 1, 2, 64, 64, torch.float32)
+    w = b.work()
+    for bad in (w[:-1], torch.zeros(w.numel() + 4, dtype=torch.uint8, device="cuda")[4:], w[:0]):
+        with pytest.raises((RuntimeError, ValueError)):
+            b.run(work=bad)
+    assert Batch([16] * 3, 1, 2, 64, 64, torch.float32).work() is None
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
+def test_states_past_32_bits(gpu, dtype):
+    """A pool of more than 2^32 values, tokens further apart than 2^32 bytes in all."""
+    pool = torch.empty((2 ** 32 // (4 * 128 * 128) + 3, 4, 128, 128), device="cuda")
+    b = Batch([2, 90, 1], 2, 4, 128, 128, dtype, pool=3)
+    small, n = b.states, len(pool)
+    far = [n - 1, 0, n - 3]
+    want, after = b.want()
+    for i, s in enumerate(b.slots):
+        pool[far[i]] = small[s]
+    rows = torch.empty((len(b.v), 1 << 23), device="cuda", dtype=dtype)
+    for name, heads in (("q", 2), ("k", 2), ("v", 4)):
+        x = getattr(b, name)
+        at = {"q": 0, "k": 1000, "v": 2 ** 23 - 512}[name]
+        wide = rows[:, at:at + heads * 128].view(-1, heads, 128)
+        wide.copy_(x)
+        setattr(b, name, wide)
+    old, b.slots, b.states = b.slots, far, pool
+    got = b.run()
+    bound = 4 * math.sqrt(90 + 128) * 2.0 ** -24
+    own = torch.finfo(dtype).eps / 2 if dtype != torch.float32 else 0.0
+    assert float((got.double() - want).norm() / want.norm()) <= bound + own
+    assert float((pool[far].double() - after[old]).norm() / after[old].norm()) <= bound
+    further = torch.empty((3, (1 << 23) + 8), device="cuda", dtype=dtype)[:, :256].view(3, 2, 128)
+    c = Batch([3], 2, 4, 128, 128, dtype)
+    c.q = further
+    with pytest.raises(RuntimeError):
+        c.run()

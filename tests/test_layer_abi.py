@@ -105,3 +105,22 @@ def test_linear_attention(lib):
     for bad in (dict(key_dim=32), dict(key_dim=256), dict(value_dim=96), dict(value_dim=512)):
         assert call(batch(**bad)) == DECLINE, bad
     assert lib.qhip_linear_attention_work_bytes(batch(), 0, 1) >= 0
+
+
+def test_linear_attention_work(lib):
+    def need(type=0, delta=1, **kw):
+        f = dict(offsets=P, slots=P, source=P, nseq=2, tokens=700, max_new=400, num_states=5, k_heads=2, v_heads=4, key_dim=64, value_dim=64)
+        return lib.qhip_linear_attention_work_bytes(ctypes.byref(QhipLinearBatch(**{**f, **kw})), type, delta)
+
+    full = need()
+    assert full > 0 and full % 16 == 0 and 0 < need(delta=0) < full and need(type=1) > 0
+    assert need(nseq=0) == need(tokens=0) == need(max_new=16) == 0
+    assert need(max_new=17) > 0 and need(max_new=17, nseq=64) == need(max_new=32, nseq=64) == 0 < need(max_new=33, nseq=64)
+    # grids of 2^32 threads: token by token
+    assert need(nseq=65535, v_heads=64, k_heads=64) == 0 == need(tokens=2 ** 30, k_heads=1, v_heads=1)
+    batch = QhipLinearBatch(P, P, None, 2, 700, 400, 5, 2, 4, 64, 64)
+    for work, size in ((P, full - 1), (P + 8, full), (P, 0)):
+        assert lib.qhip_launch_linear_attention(ctypes.byref(batch), 0, rows(FAR[0]), rows(FAR[1]), rows(FAR[2]), FAR[3], 4, FAR[4], 4, 1.0,
+                                                FAR[5], rows(FAR[6]), work, size, None) == INVALID
+    assert lib.qhip_launch_linear_attention(ctypes.byref(batch), 0, rows(FAR[0], 2 ** 23 + 1), rows(FAR[1]), rows(FAR[2]), FAR[3], 4, FAR[4], 4,
+                                            1.0, FAR[5], rows(FAR[6]), None, 0, None) == INVALID
