@@ -205,10 +205,11 @@ static void launch_steps(const LinearArgs& a, int key_dim, hipStream_t s) {
 // differences are taken: it is a long sum where the decay between near tokens is small.
 //
 // f32 rows take f32 matrix tiles throughout.  16-bit rows take bf16 ones, for which an f32
-// value goes in as a sum of planes of 8 bits: what enters the state in three, which hold
-// it whole (of products of planes those down to 2^-16 are summed, so they are good to
-// f32), the state as it is read and the weights inside a chunk in two (2^-17); keys and
-// queries need one plane (bf16) or two (f16).
+// value goes in as a sum of planes of 8 bits: what enters the state, so with the delta rule
+// the state as it is read too, in three, which hold it whole (of products of planes those
+// down to 2^-16 are summed, so they are good to f32: states of 4000 tokens are 2e-7 off;
+// with the state read in two 1.5e-6, and 3% faster), what goes to outputs alone in two
+// (2^-17); keys and queries need one plane (bf16) or two (f16).
 constexpr int kChunk = 64, kTiles = kChunk / 16;
 
 typedef __bf16 b16x8 __attribute__((ext_vector_type(8)));
@@ -548,7 +549,8 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   __shared__ u32x4 s_rows[DELTA ? kTiles : 1][PIECES * 64 + 1];
   __shared__ __attribute__((aligned(16))) uint8_t s_keys[2 * KEYS];
   __shared__ __attribute__((aligned(16))) float s_numbers[2][kNumbers + 3];
-  __shared__ u32x4 s_state[SETS][PARTS][2][64];  // two planes, f32: two tiles
+  constexpr int READ = DELTA && !F32 ? 3 : 2;       // planes of the state, f32: tiles
+  __shared__ u32x4 s_state[SETS][PARTS][READ][64];
   __shared__ f32x4 s_rest[DELTA ? SETS : 1][kTiles][64];
   __shared__ __attribute__((aligned(16))) int s_spoilt[SETS][16][kTiles];
   __shared__ u32x4 s_new[SETS][F32 ? 1 : 3][kTiles / (F32 ? 1 : 2)][64];  // U as it enters the state
@@ -595,7 +597,9 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     f32x4 c[2] = {};
 #pragma unroll
     for (int i = 0; i < PARTS; ++i) {
-      const u32x4 sp[2] = {s_state[set][i][0][lane], s_state[set][i][1][lane]};
+      u32x4 sp[READ];
+#pragma unroll
+      for (int p = 0; p < READ; ++p) sp[p] = s_state[set][i][p][lane];
       if constexpr (F32) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) c[h] = mfma4(__builtin_bit_cast(f32x4, row(2 * i + h)), __builtin_bit_cast(f32x4, sp[h]), c[h]);
@@ -604,7 +608,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
         u32x4 x[P];
         if constexpr (P == 1) x[0] = y;
         else split8<P>(floats(y[0], y[1]), floats(y[2], y[3]), x);
-        c[i & 1] = mfma_planes<P, 2>(x, sp, c[i & 1]);
+        c[i & 1] = mfma_planes<P, READ>(x, sp, c[i & 1]);
       }
     }
     return c[0] + c[1];
@@ -668,10 +672,10 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
         s_state[set][part][0][lane] = __builtin_bit_cast(u32x4, st[0]);
         s_state[set][part][1][lane] = __builtin_bit_cast(u32x4, st[1]);
       } else {
-        u32x4 sp[2];
-        split8<2>(st[0], st[1], sp);
-        s_state[set][part][0][lane] = sp[0];
-        s_state[set][part][1][lane] = sp[1];
+        u32x4 sp[READ];
+        split8<READ>(st[0], st[1], sp);
+#pragma unroll
+        for (int p = 0; p < READ; ++p) s_state[set][part][p][lane] = sp[p];
       }
       __syncthreads();
       f32x4 u[OWN];
