@@ -13,6 +13,8 @@
 #include "qhip_internal.hpp"
 #include "rows_internal.hpp"
 
+#include <algorithm>
+
 namespace qhip {
 
 struct NormArgs {
@@ -22,6 +24,7 @@ struct NormArgs {
   const float* weight;
   uint8_t* xq;
   long groups;  // tokens * heads
+  long first;   // row of this launch
   int heads, dim, lanes;
   int act;  // 32: Q8_0 rows, 256: Q8_K rows
   float eps;
@@ -90,7 +93,7 @@ template <typename T, int NT, int P>
 __global__ __launch_bounds__(NT) void k_norm_row(NormArgs a) {
   __shared__ double s_sum[NT / 64];
   const int tid = threadIdx.x;
-  const long g = blockIdx.x, token = a.heads == 1 ? g : (unsigned)g / (unsigned)a.heads, head = g - token * a.heads;
+  const long g = a.first + blockIdx.x, token = a.heads == 1 ? g : (unsigned)g / (unsigned)a.heads, head = g - token * a.heads;
   const T* x = (const T*)a.x + token * a.x_token + head * a.x_head;
   T* res = a.residual ? (T*)a.residual + token * a.res_token + head * a.res_head : nullptr;
   const T* gate = a.gate ? (const T*)a.gate + token * a.gate_token + head * a.gate_head : nullptr;
@@ -171,7 +174,7 @@ __global__ __launch_bounds__(NT) void k_norm_row(NormArgs a) {
 template <typename T>
 __global__ __launch_bounds__(256) void k_norm_heads(NormArgs a) {
   const int lane = threadIdx.x & (a.lanes - 1), d = lane * 8, n = a.dim - d;
-  const long g = (long)blockIdx.x * (256 / a.lanes) + threadIdx.x / a.lanes;
+  const long g = a.first + (long)blockIdx.x * (256 / a.lanes) + threadIdx.x / a.lanes;
   const bool in = g < a.groups && n > 0;
   const long token = (unsigned)g / (unsigned)a.heads, head = g - token * a.heads;
   float h[8] = {}, t[8], w[8];
@@ -205,18 +208,25 @@ __global__ __launch_bounds__(256) void k_norm_heads(NormArgs a) {
 constexpr int kHeadMost = 512;  // values of a row that a wave's lanes hold
 
 template <typename T>
-static void launch_norm(const NormArgs& a, hipStream_t s) {
+static void launch_norm_part(const NormArgs& a, long count, hipStream_t s) {
   if (a.dim <= kHeadMost) {
     const long rows = 256 / a.lanes;
-    hipLaunchKernelGGL(k_norm_heads<T>, dim3((unsigned)((a.groups + rows - 1) / rows)), dim3(256), 0, s, a);
+    hipLaunchKernelGGL(k_norm_heads<T>, dim3((unsigned)((count + rows - 1) / rows)), dim3(256), 0, s, a);
     return;
   }
-  const dim3 grid((unsigned)a.groups);
+  const dim3 grid((unsigned)count);
   if (a.dim <= 2048) hipLaunchKernelGGL((k_norm_row<T, 256, 1>), grid, dim3(256), 0, s, a);
   else if (a.dim <= 4096) hipLaunchKernelGGL((k_norm_row<T, 256, 2>), grid, dim3(256), 0, s, a);
   else if (a.dim <= 8192) hipLaunchKernelGGL((k_norm_row<T, 256, 4>), grid, dim3(256), 0, s, a);
   else if (a.dim <= 16384) hipLaunchKernelGGL((k_norm_row<T, 512, 4>), grid, dim3(512), 0, s, a);
   else hipLaunchKernelGGL((k_norm_row<T, 1024, 0>), grid, dim3(1024), 0, s, a);
+}
+
+template <typename T>
+static void launch_norm(NormArgs a, hipStream_t s) {
+  constexpr long most = 1 << 21;  // workgroups of a launch (2^32 threads are too many)
+  const long rows = a.dim <= kHeadMost ? 256 / a.lanes : 1;
+  for (; a.first < a.groups; a.first += most * rows) launch_norm_part<T>(a, std::min(a.groups - a.first, most * rows), s);
 }
 
 }  // namespace qhip

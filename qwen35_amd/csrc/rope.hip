@@ -11,6 +11,7 @@
 #include "qhip_internal.hpp"
 #include "rows_internal.hpp"
 
+#include <algorithm>
 #include <cmath>
 
 namespace qhip {
@@ -28,6 +29,7 @@ struct RopeArgs {
   int tokens, q_heads, heads, dim, rot, interleaved;
   int lanes, pieces;  // lanes of a head (a power of two), pieces of eight pairs or values that they hold
   int each;           // heads of a lane
+  int first;          // token of this launch
 };
 
 // cos and sin of `turn` / 2^32 turns: the nearest quarter by its top bits, then the
@@ -57,7 +59,7 @@ template <typename T, bool PAIRS>
 __global__ __launch_bounds__(256) void k_rope(RopeArgs a) {
   constexpr int N = PAIRS ? 4 : 8;  // pairs of a piece
   const int piece = threadIdx.x & (a.lanes - 1);
-  const int t = blockIdx.x * (256 / a.lanes) + threadIdx.x / a.lanes;
+  const int t = a.first + (int)blockIdx.x * (256 / a.lanes) + threadIdx.x / a.lanes;
   if (t >= a.tokens || piece >= a.pieces) return;
   const int half = a.rot >> 1, turned = (half + N - 1) / N;
   const int h0 = blockIdx.y * a.each, h1 = min(a.heads, h0 + a.each);
@@ -119,9 +121,15 @@ __global__ __launch_bounds__(256) void k_rope(RopeArgs a) {
 }
 
 template <typename T>
-static void launch_rope(const RopeArgs& a, dim3 grid, hipStream_t s) {
-  if (a.interleaved) hipLaunchKernelGGL((k_rope<T, true>), grid, dim3(256), 0, s, a);
-  else hipLaunchKernelGGL((k_rope<T, false>), grid, dim3(256), 0, s, a);
+static void launch_rope(RopeArgs a, unsigned slices, hipStream_t s) {
+  constexpr long most = 1 << 23;  // workgroups of a launch (2^32 threads are too many)
+  const int rows = 256 / a.lanes;
+  for (long at = 0; at < a.tokens; at += most * rows) {
+    a.first = (int)at;
+    const dim3 grid((unsigned)((std::min(a.tokens - at, most * rows) + rows - 1) / rows), slices);
+    if (a.interleaved) hipLaunchKernelGGL((k_rope<T, true>), grid, dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((k_rope<T, false>), grid, dim3(256), 0, s, a);
+  }
 }
 
 }  // namespace qhip
@@ -226,13 +234,13 @@ extern "C" int qhip_launch_rope(int type, const qhip_rows* q, const qhip_rows* q
   a.lanes = 1;
   while (a.lanes < a.pieces) a.lanes *= 2;
   const long blocks = ((long)tokens * a.lanes + 255) / 256;
-  // heads of a lane: as many as leave four workgroups a CU
-  a.each = (int)((long)a.heads * blocks / 1024);
+  // heads of a lane: as many as leave eight workgroups a CU (4097 tokens of 10 heads of 256,
+  // 8192 of 40 of 128, with four 20.1 and 33.2 us, eight 18.5 and 29.9, sixteen 20.6 and 31.5)
+  a.each = (int)((long)a.heads * blocks / 2048);
   a.each = a.each < 1 ? 1 : a.each > a.heads ? a.heads : a.each;
-  const dim3 grid((unsigned)blocks, (unsigned)((a.heads + a.each - 1) / a.each));
-  if (grid.y > 65535u) return (int)hipErrorInvalidValue;
-  if (type == QHIP_TT_F32) launch_rope<float>(a, grid, (hipStream_t)stream);
-  else if (type == QHIP_TT_F16) launch_rope<f16_t>(a, grid, (hipStream_t)stream);
-  else launch_rope<bf16_t>(a, grid, (hipStream_t)stream);
+  const unsigned slices = (unsigned)((a.heads + a.each - 1) / a.each);  // fewer than 4096
+  if (type == QHIP_TT_F32) launch_rope<float>(a, slices, (hipStream_t)stream);
+  else if (type == QHIP_TT_F16) launch_rope<f16_t>(a, slices, (hipStream_t)stream);
+  else launch_rope<bf16_t>(a, slices, (hipStream_t)stream);
   return (int)hipGetLastError();
 }

@@ -152,3 +152,17 @@ def test_in_a_graph_on_another_stream(gpu):
         torch.cuda.synchronize()
         want = ops.rms_norm_quantize(8, x, w, EPS, residual=r0.clone())
         assert torch.equal(xq, want) and torch.equal(r, r0 + x)
+
+
+@pytest.mark.parametrize("dim", [257, 513])
+def test_more_rows_than_a_launch_takes(gpu, dim):
+    """A grid holds fewer than 2^32 threads: rows before, at and behind the place where the next launch begins."""
+    tokens = 2 ** 21 * (4 if dim <= 512 else 1) + 7  # (four rows a workgroup of 256, and one)
+    gen = torch.Generator(device="cuda").manual_seed(dim)
+    x = torch.zeros((tokens, dim), device="cuda", dtype=torch.bfloat16)
+    some = torch.tensor([0, 1, 5000, tokens - 12, tokens - 8, tokens - 7, tokens - 6, tokens - 1], device="cuda")
+    x[some] = rows(gen, torch.bfloat16, len(some), dim)
+    w = 1 + rows(gen, torch.float32, dim, loud=1.0) / 5
+    out = ops.rms_norm(x, w, EPS, out=torch.full_like(x, 7.0))
+    near(out[some], ref.rms_norm(x[some], w, EPS)[0], 3)
+    assert int((out == 0).all(-1).sum()) == tokens - len(some)

@@ -141,3 +141,14 @@ def test_in_a_graph_on_another_stream(gpu):
         torch.cuda.synchronize()
         a, b = ops.rope(q, k, at, table)
         assert torch.equal(a, qo) and torch.equal(b, ko)
+
+
+def test_more_tokens_than_a_launch_takes(gpu):
+    """A grid holds fewer than 2^32 threads: one head of 2048 values a workgroup of 256, all tokens of one row."""
+    tokens = 2 ** 23 + 5
+    x = torch.randn((1, 1, 2048), device="cuda", generator=torch.Generator(device="cuda").manual_seed(1)).bfloat16().expand(tokens, 1, 2048)
+    at = torch.arange(tokens, device="cuda", dtype=torch.int32)
+    out, _ = ops.rope(x, None, at, ops.RopeTable(1024), interleaved=True)
+    some = torch.tensor([0, 1, 70000, 2 ** 23 - 1, 2 ** 23, 2 ** 23 + 4], device="cuda")
+    freq, gain = ref.frequencies(1024, 10000.0)
+    near(out[some], x[some], at[some], freq, gain, True)
