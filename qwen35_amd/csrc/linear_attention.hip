@@ -554,8 +554,8 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   __shared__ u32x4 s_rows[DELTA ? kTiles : 1][PIECES * 64 + 1];
   __shared__ __attribute__((aligned(16))) uint8_t s_keys[2 * KEYS];
   __shared__ __attribute__((aligned(16))) float s_numbers[2][kNumbers + 3];
-  constexpr int READ = DELTA && !F32 ? 3 : 2;       // planes of the state, f32: tiles
-  __shared__ u32x4 s_state[SETS][PARTS][READ][64];
+  __shared__ u32x4 s_state[SETS][PARTS][2][64];  // two planes, f32: two tiles
+  __shared__ f32x4 s_part[DELTA ? SETS : 1][PARTS][kTiles][64];  // K S over the dimensions of a wave
   __shared__ f32x4 s_rest[DELTA ? SETS : 1][kTiles][64];
   __shared__ __attribute__((aligned(16))) int s_spoilt[SETS][16][kTiles];
   __shared__ u32x4 s_new[SETS][F32 ? 1 : 3][kTiles / (F32 ? 1 : 2)][64];  // U as it enters the state
@@ -581,8 +581,8 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   }
   const int kh = head / a.group, chunks = (s.n + kChunk - 1) / kChunk, tail = s.n - (chunks - 1) * kChunk;
   // the wave's tiles of tokens (of two the first and last, or those between: T has 1 to 4
-  // tiles in a row)
-  auto own = [&](int o) { return o == 0 ? part : 3 - part; };
+  // tiles in a row, and so has A, which a SIMD's other wave takes the other way round)
+  auto own = [&](int o) { return (o == 0) == (wave < 4) ? part : 3 - part; };
   auto rows_of = [&](int c) { return c + 1 < chunks ? kChunk : tail; };
 
   // Everything of a chunk is loaded for the next one when the present one is done with
@@ -602,9 +602,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     f32x4 c[2] = {};
 #pragma unroll
     for (int i = 0; i < PARTS; ++i) {
-      u32x4 sp[READ];
-#pragma unroll
-      for (int p = 0; p < READ; ++p) sp[p] = s_state[set][i][p][lane];
+      const u32x4 sp[2] = {s_state[set][i][0][lane], s_state[set][i][1][lane]};
       if constexpr (F32) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) c[h] = mfma4(__builtin_bit_cast(f32x4, row(2 * i + h)), __builtin_bit_cast(f32x4, sp[h]), c[h]);
@@ -613,7 +611,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
         u32x4 x[P];
         if constexpr (P == 1) x[0] = y;
         else split8<P>(floats(y[0], y[1]), floats(y[2], y[3]), x);
-        c[i & 1] = mfma_planes<P, READ>(x, sp, c[i & 1]);
+        c[i & 1] = mfma_planes<P, 2>(x, sp, c[i & 1]);
       }
     }
     return c[0] + c[1];
@@ -677,10 +675,30 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
         s_state[set][part][0][lane] = __builtin_bit_cast(u32x4, st[0]);
         s_state[set][part][1][lane] = __builtin_bit_cast(u32x4, st[1]);
       } else {
-        u32x4 sp[READ];
-        split8<READ>(st[0], st[1], sp);
+        u32x4 sp[DELTA ? 3 : 2];
+        split8<DELTA ? 3 : 2>(st[0], st[1], sp);
+        s_state[set][part][0][lane] = sp[0];
+        s_state[set][part][1][lane] = sp[1];
+        if constexpr (DELTA) {
 #pragma unroll
-        for (int p = 0; p < READ; ++p) s_state[set][part][p][lane] = sp[p];
+          for (int t = 0; t < kTiles; ++t) {
+            const u32x4 y = s_rows[t][part * 64 + lane];
+            u32x4 x[P];
+            if constexpr (P == 1) x[0] = y;
+            else split8<P>(floats(y[0], y[1]), floats(y[2], y[3]), x);
+            s_part[set][part][t][lane] = mfma_planes<P, 3>(x, sp, f32x4{0.0f, 0.0f, 0.0f, 0.0f});
+          }
+        }
+      }
+      if constexpr (DELTA && F32) {
+#pragma unroll
+        for (int t = 0; t < kTiles; ++t) {
+          f32x4 x[2];
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+            x[h] = mfma4(__builtin_bit_cast(f32x4, s_rows[t][(2 * part + h) * 64 + lane]), st[h], f32x4{0.0f, 0.0f, 0.0f, 0.0f});
+          s_part[set][part][t][lane] = x[0] + x[1];
+        }
       }
       __syncthreads();
       f32x4 u[OWN];
@@ -694,7 +712,12 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
           for (int r = 0; r < 4; ++r) u[w][r] = 16 * t + 4 * g + r < tail ? u[w][r] : 0.0f;
         }
         // (rows behind the sequence's end have the last row's keys: their T is 0)
-        if constexpr (DELTA) u[w] -= number(c, 0, t) * with_state([&](int i) { return s_rows[t][i * 64 + lane]; });
+        if constexpr (DELTA) {
+          f32x4 ks = s_part[set][0][t][lane];
+#pragma unroll
+          for (int p = 1; p < PARTS; ++p) ks += s_part[set][p][t][lane];
+          u[w] -= number(c, 0, t) * ks;
+        }
         // What is not finite spoils its column from its token on; in a product it would spoil
         // the tokens before as well (0 * NaN), so it stays out of them.
         float sum = 0.0f;
