@@ -56,7 +56,7 @@ constexpr int kFew = 16;
 // A batch whose sequences all have at most this many does without chunks.  Of sequences
 // that fill the card (256 workgroups of 64 columns) a chunk costs more tokens: 16 heads of
 // 128 x 128, token by token / in chunks: 1 sequence, 16 tokens 16.5 / 15 us, 32: 29 / 16; 64
-// sequences, 16 tokens 66 / 199 us, 32: 120 / 213.
+// sequences, 16 tokens 71 / 199 us, 32: 117 / 213.
 static int few_alone(const qhip_linear_batch* b) { return (long)b->nseq * b->v_heads * (b->value_dim / 64) < 256 ? kFew : 2 * kFew; }
 
 // sum over lanes l, l ^ 16, l ^ 32, l ^ 48
@@ -536,10 +536,18 @@ __global__ __launch_bounds__(256) void k_linear_prepare(LinearArgs a) {
 // in registers, and all have their share of the chunk's four tiles of 16 tokens.  Between
 // three barriers a chunk:
 //
-//   the state, in planes, into LDS
+//   the state, in planes, into LDS, and all tokens' K S over the own rows
 //   R of the own tokens        | Q S of the own tokens
 //   U of the own tokens        | the next chunk's keys into LDS, as rows and turned
 //   the state's update         | the outputs
+//
+// A chunk waits for the one before it, so its chain bounds a sequence: 1.7 us for bf16 rows of
+// 128, of which products fill a quarter and vector instructions another, the rest being LDS,
+// barriers and waits for each other (loads a chunk ahead do not show); 2.8 us for f32 rows,
+// 4096 cycles of f32 products on each SIMD among them.  8192 bf16 tokens of 16 heads: 223 us, beside 42 of prepare; eight f32
+// prompts of up to 256 tokens 57 and 14.5.  (K S of the own tokens over all rows of the
+// state, read by every wave from LDS: 229 us.  T in three planes of bf16, so that its product
+// takes a third of the cycles: 263, for the splits and the larger loads.)
 template <typename T, int DK, bool DELTA>
 __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) void k_linear_scan(LinearArgs a) {
   typedef ChunkWork<T, DELTA> W;

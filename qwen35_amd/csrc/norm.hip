@@ -9,6 +9,12 @@
 // rounded once to f32; all else is single f32 operations.  So a row's bits do not
 // depend on how its sum is cut over lanes, and the codes are those of the
 // quantizers applied to the f32 y.
+//
+// Memory bounds it: each value is read once, held in registers over the sum and written
+// once.  4096 bf16 rows of 5120 with the residual 33 us (5.0 TB/s of the 5.1 of a copy), 131,056
+// heads of 128 in f32 with gates 35 us (5.7), 1673 f32 rows of 5120 with the residual to Q8_0
+// codes 27 us (4.2: one uneven round of workgroups); one row of 2560 4.3 us, a chain of loads,
+// two sums and stores.
 #include "qhip_device.hpp"
 #include "qhip_internal.hpp"
 #include "rows_internal.hpp"
@@ -87,7 +93,8 @@ __device__ __forceinline__ void put_codes(const NormArgs& a, const float (&y)[8]
   }
 }
 
-// A row a workgroup of NT threads, P pieces of eight values a thread in
+// A row a workgroup of NT threads (a wave's lanes would hold 40 values of 2560 each, and one
+// row would wait for one wave), P pieces of eight values a thread in
 // registers; P = 0: rows of any length, read a second time (from L2).
 template <typename T, int NT, int P>
 __global__ __launch_bounds__(NT) void k_norm_row(NormArgs a) {
