@@ -278,8 +278,9 @@ __device__ __forceinline__ f32x4 mfma_planes(const u32x4* a, const u32x4* b, f32
 
 // What prepare leaves for a chunk and value head, as left operands of 1 KB: T's tiles (i,
 // j), j <= i, in f32; A's the same way for f32 rows, else its rows of tiles in steps of two
-// tiles and two planes; then exp(G), exp(G_63 - G) and exp(G_63).
-constexpr int kNumbers = 2 * kChunk + 1;
+// tiles and two planes; then exp(G), exp(G_63 - G), exp(G_63) and the
+// first token whose row of L, or beta, is not finite (64: none).
+constexpr int kWhole = 2 * kChunk, kSound = kWhole + 1, kNumbers = kWhole + 2;
 template <typename T, bool DELTA>
 struct ChunkWork {
   static constexpr bool whole = sizeof(T) == 4;
@@ -330,6 +331,7 @@ __global__ __launch_bounds__(256) void k_linear_prepare(LinearArgs a) {
   __shared__ u32x4 s_rows[2][kTiles][TILE];  // keys and queries; then L and its inverse
   __shared__ __attribute__((aligned(16))) float s_sum[2][kChunk];  // G in two parts
   __shared__ __attribute__((aligned(16))) float s_beta[kChunk];
+  __shared__ int s_sound[3];  // the first token that is not finite: beta, L's rows of either wave
   static_assert(sizeof(s_rows) >= kChunk * ROW * 4 || DK == 64, "L");
   constexpr int MORE = sizeof(s_rows) >= kChunk * ROW * 4 ? 1 : kChunk * ROW;  // (16-bit rows of 64)
   __shared__ __attribute__((aligned(16))) float s_more[MORE];
@@ -425,6 +427,8 @@ __global__ __launch_bounds__(256) void k_linear_prepare(LinearArgs a) {
       s_sum[0][lane] = (float)sum;
       s_sum[1][lane] = (float)(sum - (float)sum);
       s_beta[lane] = lane < n ? beta : 0.0f;
+      const uint64_t bad = __ballot(lane < n && !(__builtin_fabsf(beta) < INFINITY));
+      if (lane == 0) s_sound[2] = bad ? __builtin_ctzll(bad) : kChunk;
     }
     __syncthreads();
     f32x4 tile[5];
@@ -444,6 +448,20 @@ __global__ __launch_bounds__(256) void k_linear_prepare(LinearArgs a) {
           tile[e][r] = r < seen ? x : 0.0f;
         }
         if (DELTA && keys) *(f32x4*)&mat[i * ROW + j0] = tile[e];
+      }
+      if (DELTA && keys) {
+        const int second_of = outer ? 4 : 2;  // (rows of two tiles, as above)
+        int bad = kChunk;
+#pragma unroll
+        for (int e = 0; e < 5; ++e) {
+          const f32x4 none = tile[e] * 0.0f;
+          if ((none[0] + none[1]) + (none[2] + none[3]) != 0.0f) bad = min(bad, (outer ? (e >= second_of ? 0 : 48) : (e >= second_of ? 32 : 16)) + m);
+        }
+        if (__ballot(bad < kChunk)) {
+#pragma unroll
+          for (int d = 1; d < 64; d <<= 1) bad = min(bad, __shfl_xor(bad, d, 64));
+        }
+        if (lane == 0) s_sound[outer] = bad;
       }
     }
     if (!keys) {  // A
@@ -475,10 +493,18 @@ __global__ __launch_bounds__(256) void k_linear_prepare(LinearArgs a) {
       const float sum = s_sum[0][lane];
       numbers[lane] = __builtin_amdgcn_exp2f(sum);
       numbers[64 + lane] = __builtin_amdgcn_exp2f((s_sum[0][63] - sum) + (s_sum[1][63] - s_sum[1][lane]));
-      if (lane == 63) numbers[128] = __builtin_amdgcn_exp2f(sum);
+      if (lane == 63) numbers[kWhole] = __builtin_amdgcn_exp2f(sum);
     }
     if constexpr (DELTA) {
       __syncthreads();
+      // Rows of the inverse from the first that is not finite on are left out (0): in the
+      // products below they would spoil the rows before, with 0 * NaN.
+      const int sound = min(min(s_sound[0], s_sound[1]), s_sound[2]);
+      if (sound < kChunk) {
+        for (int e = threadIdx.x; e < (kChunk - sound) * ROW; e += 256) mat[sound * ROW + e] = 0.0f;
+        __syncthreads();
+      }
+      if (wave == 3 && lane == 0) ((float*)(out + W::numbers))[kSound] = (float)sound;
       if (wave == 0) {
         const int b = lane & 48;
         float x[16];
@@ -499,7 +525,7 @@ __global__ __launch_bounds__(256) void k_linear_prepare(LinearArgs a) {
       auto leave = [&](int i, int j, f32x4 x) {
         const f32x4 b = *(const f32x4*)(s_beta + 16 * j + 4 * g);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) x[e] = i > j || 4 * g + e <= m ? x[e] * b[e] : 0.0f;
+        for (int e = 0; e < 4; ++e) x[e] = 16 * i + m < sound && (i > j || 4 * g + e <= m) ? x[e] * b[e] : 0.0f;
         *((f32x4*)(out + W::solve_tile(i, j)) + lane) = x;
       };
       const f32x4 none = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -561,7 +587,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   constexpr int GROUP = 272, STEP = F32 ? 4 * GROUP : 4 * GROUP + 64, TURNED = (F32 ? 4 : 2) * STEP, KEYS = P * (DK / 16) * TURNED;
   __shared__ u32x4 s_rows[DELTA ? kTiles : 1][PIECES * 64 + 1];
   __shared__ __attribute__((aligned(16))) uint8_t s_keys[2 * KEYS];
-  __shared__ __attribute__((aligned(16))) float s_numbers[2][kNumbers + 3];
+  __shared__ __attribute__((aligned(16))) float s_numbers[2][kNumbers + 2];
   __shared__ u32x4 s_state[SETS][PARTS][2][64];  // two planes, f32: two tiles
   __shared__ f32x4 s_part[DELTA ? SETS : 1][PARTS][kTiles][64];  // K S over the dimensions of a wave
   __shared__ f32x4 s_rest[DELTA ? SETS : 1][kTiles][64];
@@ -731,12 +757,12 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
         float sum = 0.0f;
 #pragma unroll
         for (int r = 0; r < 4; ++r) sum = __builtin_fmaf(u[w][r], 0.0f, sum);
-        int first = kChunk;
+        int first = DELTA ? (int)s_numbers[c & 1][kSound] : kChunk;
         if (__ballot(sum != 0.0f)) {
 #pragma unroll
           for (int r = 3; r >= 0; --r)
             if (!(__builtin_fabsf(u[w][r]) < INFINITY)) {
-              first = 16 * t + 4 * g + r;
+              first = min(first, 16 * t + 4 * g + r);
               u[w][r] = 0.0f;
             }
           first = min(first, __shfl_xor(first, 16, 64));
@@ -788,7 +814,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
         }
       }
 #pragma unroll
-      for (int i = 0; i < 2; ++i) st[i] *= s_numbers[c & 1][kNumbers - 1];
+      for (int i = 0; i < 2; ++i) st[i] *= s_numbers[c & 1][kWhole];
       if constexpr (!LAST) fetch_solve();
       __syncthreads();
       const uint8_t* turned = s_keys + (c & 1) * KEYS + 2 * part * TURNED + g * GROUP + m * 16;

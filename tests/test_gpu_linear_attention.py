@@ -343,3 +343,44 @@ def test_states_past_32_bits(gpu, dtype):
     c.q = further
     with pytest.raises(RuntimeError):
         c.run()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("delta", [True, False])
+@pytest.mark.parametrize("dk", [64, 128])
+@pytest.mark.parametrize("token", [0, 1, 16, 37, 63, 64, 101, 149])
+@pytest.mark.parametrize("name", ["q", "k", "v", "log_decay", "beta"])
+def test_what_is_not_finite_stays_behind_its_token(gpu, name, token, dk, delta, dtype):
+    """One NaN or infinity in the middle of a chunk, of a block of the triangular system and of neither: the tokens before
+    are as without it, those after it and the state are lost, other heads and sequences are not."""
+    if name == "beta" and not delta:
+        pytest.skip("no beta")
+    for value in (torch.nan, torch.inf):
+        clean, b = (Batch([150, 30], 2, 2, dk, 64, dtype, delta, seed=token) for _ in range(2))
+        x = getattr(b, name)
+        if x.dim() == 3:
+            x[token, 1, 5] = value
+        else:
+            x[token, 1] = value
+        want, got = clean.run(), b.run()
+        same = torch.ones(got.shape, dtype=torch.bool, device="cuda")
+        if name == "q":
+            same[token, 1] = False
+        elif name == "v":
+            same[token:150, 1, 5] = False
+        else:
+            same[token:150, 1] = False
+        assert bool(torch.isfinite(got[same]).all())
+        bound = 4 * math.sqrt(150 + dk) * 2.0 ** -24 + torch.finfo(dtype).eps
+        assert float((got - want)[same].float().norm() / want[same].float().norm()) <= bound
+        assert not bool(torch.isfinite(got[~same]).any())
+        states, state = clean.states, b.states[b.slots[0], 1]
+        assert torch.equal(b.states[b.slots[1]], states[b.slots[1]]) and torch.equal(b.states[b.slots[0], 0], states[b.slots[0], 0])
+        if name == "q":
+            assert torch.equal(b.states, states)
+        elif name == "v":
+            assert not bool(torch.isfinite(state[:, 5]).any()) and torch.equal(state[:, :5], states[b.slots[0], 1][:, :5])
+        elif name == "k" and not delta:
+            assert not bool(torch.isfinite(state[5]).any())  # the key's row
+        else:
+            assert not bool(torch.isfinite(state).any())
