@@ -1085,7 +1085,7 @@ extern "C" int qhip_launch_linear_attention(const qhip_linear_batch* batch, int 
   if (tokens > 0) {
     const qhip_rows* all[] = {q, k, v, out};
     for (const qhip_rows* r : all)  // (a chunk's offsets are 32 bits)
-      if (!rows_ok(r, size) || r->token_stride > 1 << 23) return (int)hipErrorInvalidValue;
+      if (!rows_ok(r, size) || (tokens > 1 && r->token_stride > 1 << 23)) return (int)hipErrorInvalidValue;
     if (!d_log_decay ||
         ((uintptr_t)d_log_decay & 3u) || decay_stride < 0 || ((uintptr_t)d_beta & 3u) || beta_stride < 0)
       return (int)hipErrorInvalidValue;

@@ -27,8 +27,8 @@ inline bool rows_apart(const qhip_rows* r, int tokens, int heads, int dim) {
 inline bool rows_same(const qhip_rows* a, const qhip_rows* b) {
   return a->at == b->at && a->token_stride == b->token_stride && a->head_stride == b->head_stride;
 }
-// Whether two sets of rows may share memory.  Columns of one wider array (equal
-// token strides, heads inside them) do not, though their ranges meet.
+// Whether two sets of rows may share memory.  Columns of one wider array (equal token
+// strides, heads inside them) do not, though their ranges meet.
 inline bool rows_overlap(const qhip_rows* a, int a_heads, int a_dim, const qhip_rows* b, int b_heads, int b_dim, int tokens,
                          int size) {
   const char *pa = (const char*)a->at, *pb = (const char*)b->at;
@@ -38,6 +38,13 @@ inline bool rows_overlap(const qhip_rows* a, int a_heads, int a_dim, const qhip_
     const long wa = ((a_heads - 1) * a->head_stride + a_dim) * size, wb = ((b_heads - 1) * b->head_stride + b_dim) * size;
     const long off = (((pb - pa) % row) + row) % row;  // of b's columns in a's row
     if (wa <= row && wb <= row && off >= wa && off + wb <= row) return false;
+  }
+  // nor do parts of one array's heads
+  const long head = a->head_stride * size;
+  if (head > 0 && a->head_stride == b->head_stride &&
+      (tokens == 1 || (a->token_stride == b->token_stride && a->token_stride % a->head_stride == 0))) {
+    const long off = (((pb - pa) % head) + head) % head;
+    if (off >= (long)a_dim * size && off + (long)b_dim * size <= head) return false;
   }
   return true;
 }

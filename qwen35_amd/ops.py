@@ -502,7 +502,7 @@ def _rows(name: str, t: torch.Tensor, device: int, shape: torch.Size, dtype: tor
     """Rows of `shape` [tokens, dim] or [tokens, heads, dim] whose last dimension is contiguous."""
     stride = t.stride()
     if (t.dtype != dtype or t.shape != shape or t.get_device() != device or len(stride) not in (2, 3) or dtype not in _KV_TYPES
-            or (stride[-1] != 1 and shape[-1] != 1)):
+            or (stride[-1] != 1 and shape[-1] != 1) or (t.numel() > 0x7FFFFFFF and max(shape) > 0x7FFFFFFF)):
         raise ValueError(f"{name}: {list(shape)} of {dtype} (rows or heads of f32, f16 or bf16) with a contiguous last dimension on "
                          "the current GPU")
     return QhipRows(t.data_ptr(), stride[0], stride[1] if len(stride) == 3 else 0)

@@ -166,3 +166,19 @@ def test_more_rows_than_a_launch_takes(gpu, dim):
     out = ops.rms_norm(x, w, EPS, out=torch.full_like(x, 7.0))
     near(out[some], ref.rms_norm(x[some], w, EPS)[0], 3)
     assert int((out == 0).all(-1).sum()) == tokens - len(some)
+
+
+@pytest.mark.parametrize("tokens", [1, 5])
+def test_parts_of_one_array_s_heads(gpu, tokens):
+    """Values and gates side by side in each head: the norm in the values' place."""
+    gen = torch.Generator(device="cuda").manual_seed(tokens)
+    both = rows(gen, torch.float32, tokens, 4, 2, 64)
+    w, x, g = torch.ones(64, device="cuda"), both[:, :, 0], both[:, :, 1]
+    want, gates = ref.rms_norm(x, w, EPS, None, g)[0], g.clone()
+    near(ops.rms_norm(x, w, EPS, gate=g, out=x), want, 11)
+    assert torch.equal(g, gates)
+    with pytest.raises(RuntimeError):  # one value into the gates
+        ops.rms_norm(x, w, EPS, gate=g, out=both.view(tokens, 4, 128)[:, :, 1:65])
+    k = rows(gen, torch.float32, tokens + 3, 4, 64)[:tokens]
+    with pytest.raises(ValueError):
+        ops.rms_norm(k[:1, :1, :1].expand(2 ** 31, 1, 1), None, EPS, out=k)
