@@ -210,11 +210,12 @@ static void launch_steps(const LinearArgs& a, int key_dim, hipStream_t s) {
 // differences are taken: it is a long sum where the decay between near tokens is small.
 //
 // f32 rows take f32 matrix tiles throughout.  16-bit rows take bf16 ones, for which an f32
-// value goes in as a sum of planes of 8 bits: what enters the state, so with the delta rule
-// the state as it is read too, in three, which hold it whole (of products of planes those
-// down to 2^-16 are summed, so they are good to f32: states of 4000 tokens are 2e-7 off;
-// with the state read in two 1.5e-6, and 3% faster), what goes to outputs alone in two
-// (2^-17); keys and queries need one plane (bf16) or two (f16).
+// value goes in as a sum of three planes of 8 bits, which hold it whole; of products of planes
+// those down to 2^-16 are summed, so all sums are good to f32, and an output is rounded once,
+// to its type.  (With the state, U and A in two planes for the outputs, 2^-16 off, 0.6% of
+// bf16 outputs and 3% of f16 ones were rounded otherwise than the f64 results, instead of
+// 0.02% and 0.09%: 253 us for 8192 tokens, now 264.)  Keys and queries need one plane (bf16)
+// or two (f16).
 constexpr int kChunk = 64, kTiles = kChunk / 16;
 
 typedef __bf16 b16x8 __attribute__((ext_vector_type(8)));
@@ -277,19 +278,21 @@ __device__ __forceinline__ f32x4 mfma_planes(const u32x4* a, const u32x4* b, f32
 }
 
 // What prepare leaves for a chunk and value head, as left operands of 1 KB: T's tiles (i,
-// j), j <= i, in f32; A's the same way for f32 rows, else its rows of tiles in steps of two
-// tiles and two planes; then exp(G), exp(G_63 - G), exp(G_63) and the
+// j), j <= i, in f32; A's the same way, but for 16-bit rows without the delta rule as rows of
+// tiles in steps of two tiles and three planes (with it, the outputs' waves split A while they
+// wait for U: 264 us for 8192 bf16 tokens instead of 272; without it they wait for nothing: a
+// mixed f16 batch 71 us, from planes 65); then exp(G), exp(G_63 - G), exp(G_63) and the
 // first token whose row of L, or beta, is not finite (64: none).
 constexpr int kWhole = 2 * kChunk, kSound = kWhole + 1, kNumbers = kWhole + 2;
 template <typename T, bool DELTA>
 struct ChunkWork {
-  static constexpr bool whole = sizeof(T) == 4;
+  static constexpr bool whole = DELTA || sizeof(T) == 4;
   static constexpr int tiles = kTiles * (kTiles + 1) / 2 * 1024;
-  static constexpr int solve = 0, inside = DELTA ? tiles : 0, numbers = inside + (whole ? tiles : 12 * 1024), bytes = numbers + 576;
+  static constexpr int solve = 0, inside = DELTA ? tiles : 0, numbers = inside + (whole ? tiles : 18 * 1024), bytes = numbers + 576;
   __host__ __device__ static constexpr int solve_tile(int i, int j) { return solve + (i * (i + 1) / 2 + j) * 1024; }
-  // of row i: its first tile (f32), or its first step's first plane
+  // of row i: its first tile (whole), or its first step's first plane
   __host__ __device__ static constexpr int inside_row(int i) {
-    return inside + (whole ? i * (i + 1) / 2 : i < 2 ? 2 * i : 4 * i - 4) * 1024;
+    return inside + (whole ? i * (i + 1) / 2 : i < 2 ? 3 * i : 6 * i - 6) * 1024;
   }
 };
 
@@ -467,15 +470,15 @@ __global__ __launch_bounds__(256) void k_linear_prepare(LinearArgs a) {
     if (!keys) {  // A
       const f32x4 none = {0.0f, 0.0f, 0.0f, 0.0f};
       auto leave = [&](int i, int j, f32x4 x, f32x4 y) {
-        u32x4* to = (u32x4*)(out + W::inside_row(i) + j * 1024) + lane;
+        u32x4* to = (u32x4*)(out + W::inside_row(i) + (W::whole ? j : j / 2 * 3) * 1024) + lane;
         if constexpr (W::whole) {
           to[0] = __builtin_bit_cast(u32x4, x);
           if (j < i) to[64] = __builtin_bit_cast(u32x4, y);
         } else {
-          u32x4 planes[2];
-          split8<2>(x, y, planes);
-          to[0] = planes[0];
-          to[64] = planes[1];
+          u32x4 planes[3];
+          split8<3>(x, y, planes);
+#pragma unroll
+          for (int p = 0; p < 3; ++p) to[64 * p] = planes[p];
         }
       };
       if (outer) {
@@ -588,12 +591,13 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   __shared__ u32x4 s_rows[DELTA ? kTiles : 1][PIECES * 64 + 1];
   __shared__ __attribute__((aligned(16))) uint8_t s_keys[2 * KEYS];
   __shared__ __attribute__((aligned(16))) float s_numbers[2][kNumbers + 2];
-  __shared__ u32x4 s_state[SETS][PARTS][2][64];  // two planes, f32: two tiles
+  constexpr int SP = F32 ? 2 : 3;
+  __shared__ u32x4 s_state[SETS][PARTS][SP][64];  // three planes, f32: two tiles
   __shared__ f32x4 s_part[DELTA ? SETS : 1][PARTS][kTiles][64];  // K S over the dimensions of a wave
   __shared__ f32x4 s_rest[DELTA ? SETS : 1][kTiles][64];
   __shared__ __attribute__((aligned(16))) int s_spoilt[SETS][16][kTiles];
   __shared__ u32x4 s_new[SETS][F32 ? 1 : 3][kTiles / (F32 ? 1 : 2)][64];  // U as it enters the state
-  __shared__ u32x4 s_old[SETS][F32 ? 1 : 2][kTiles / (F32 ? 1 : 2)][64];  // U for the outputs
+  __shared__ u32x4 s_old[SETS][F32 ? 1 : 3][kTiles / (F32 ? 1 : 2)][64];  // U for the outputs
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, g = lane >> 4, m = lane & 15;
   const int set = (wave & 3) / PARTS, part = (wave & 3) % PARTS;
   // the workgroups of a sequence's head follow each other on one XCD
@@ -636,7 +640,9 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     f32x4 c[2] = {};
 #pragma unroll
     for (int i = 0; i < PARTS; ++i) {
-      const u32x4 sp[2] = {s_state[set][i][0][lane], s_state[set][i][1][lane]};
+      u32x4 sp[SP];
+#pragma unroll
+      for (int p = 0; p < SP; ++p) sp[p] = s_state[set][i][p][lane];
       if constexpr (F32) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) c[h] = mfma4(__builtin_bit_cast(f32x4, row(2 * i + h)), __builtin_bit_cast(f32x4, sp[h]), c[h]);
@@ -645,7 +651,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
         u32x4 x[P];
         if constexpr (P == 1) x[0] = y;
         else split8<P>(floats(y[0], y[1]), floats(y[2], y[3]), x);
-        c[i & 1] = mfma_planes<P, 2>(x, sp, c[i & 1]);
+        c[i & 1] = mfma_planes<P, 3>(x, sp, c[i & 1]);
       }
     }
     return c[0] + c[1];
@@ -709,10 +715,10 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
         s_state[set][part][0][lane] = __builtin_bit_cast(u32x4, st[0]);
         s_state[set][part][1][lane] = __builtin_bit_cast(u32x4, st[1]);
       } else {
-        u32x4 sp[DELTA ? 3 : 2];
-        split8<DELTA ? 3 : 2>(st[0], st[1], sp);
-        s_state[set][part][0][lane] = sp[0];
-        s_state[set][part][1][lane] = sp[1];
+        u32x4 sp[3];
+        split8<3>(st[0], st[1], sp);
+#pragma unroll
+        for (int p = 0; p < 3; ++p) s_state[set][part][p][lane] = sp[p];
         if constexpr (DELTA) {
 #pragma unroll
           for (int t = 0; t < kTiles; ++t) {
@@ -808,9 +814,9 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
           split4<3>(in, planes);
 #pragma unroll
           for (int p = 0; p < 3; ++p) ((u32x2*)&s_new[set][p][t >> 1][lane])[t & 1] = planes[p];
-          split4<2>(u[w], planes);
+          split4<3>(u[w], planes);
 #pragma unroll
-          for (int p = 0; p < 2; ++p) ((u32x2*)&s_old[set][p][t >> 1][lane])[t & 1] = planes[p];
+          for (int p = 0; p < 3; ++p) ((u32x2*)&s_old[set][p][t >> 1][lane])[t & 1] = planes[p];
         }
       }
 #pragma unroll
@@ -898,13 +904,14 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
       for (int i = 0; i < 4; ++i) held[e][i] = *(const piece*)(k_at + held_off[e][i]);
     held_number = *(const __attribute__((address_space(1))) float*)(key_work + W::numbers + 4 * min(tid, kNumbers - 1));
   };
-  f32x4 inside[OWN][kTiles];
+  constexpr int PIECES_A = W::whole ? kTiles : kTiles / 2 * 3;
+  f32x4 inside[OWN][PIECES_A];
   auto fetch_inside = [&]() {
 #pragma unroll
     for (int o = 0; o < OWN; ++o)
 #pragma unroll
-      for (int j = 0; j < kTiles; ++j)
-        inside[o][j] = *(GlobalF4)(work + W::inside_row(own(o)) + (F32 ? min(j, own(o)) : min(j, own(o) | 1)) * 1024 + lane * 16);
+      for (int j = 0; j < PIECES_A; ++j)
+        inside[o][j] = *(GlobalF4)(work + W::inside_row(own(o)) + (W::whole ? min(j, own(o)) : own(o) < 2 ? j % 3 : j) * 1024 + lane * 16);
   };
   // the held keys and numbers into LDS (behind the sequence's end the last key: U is 0 there)
   auto put_keys = [&](int buffer) {
@@ -980,21 +987,37 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
       }
       fetch_keys();
     }
+    u32x4 weights[OWN][F32 ? 1 : kTiles / 2][3];
+    if constexpr (!F32) {
+#pragma unroll
+      for (int w = 0; w < OWN; ++w)
+#pragma unroll
+        for (int j = 0; j < kTiles; j += 2) {
+          if constexpr (W::whole) {
+            if (j <= own(w)) split8<3>(inside[w][j], j < own(w) ? inside[w][j + 1] : f32x4{0.0f, 0.0f, 0.0f, 0.0f}, weights[w][j / 2]);
+          } else {
+#pragma unroll
+            for (int p = 0; p < 3; ++p) weights[w][j / 2][p] = __builtin_bit_cast(u32x4, inside[w][j / 2 * 3 + p]);
+          }
+        }
+    }
     __syncthreads();
     const int spoilt = first_spoilt();
 #pragma unroll
     for (int w = 0; w < OWN; ++w) {
       const int t = own(w), row = 16 * t + 4 * g;
+      f32x4 more = {0.0f, 0.0f, 0.0f, 0.0f};  // a second sum beside o[w], as above
 #pragma unroll
       for (int j = 0; j < kTiles; ++j) {
         if constexpr (F32) {
           if (j <= t) o[w] = mfma4(inside[w][j], __builtin_bit_cast(f32x4, s_old[set][0][j][lane]), o[w]);
         } else if ((j & 1) == 0 && j <= t) {
-          const u32x4 x[2] = {__builtin_bit_cast(u32x4, inside[w][j]), __builtin_bit_cast(u32x4, inside[w][j + 1])};
-          const u32x4 y[2] = {s_old[set][0][j >> 1][lane], s_old[set][1][j >> 1][lane]};
-          o[w] = mfma_planes<2, 2>(x, y, o[w]);
+          const u32x4 y[3] = {s_old[set][0][j >> 1][lane], s_old[set][1][j >> 1][lane], s_old[set][2][j >> 1][lane]};
+          f32x4& sum = DELTA && j ? more : o[w];
+          sum = mfma_planes<3, 3>(weights[w][j >> 1], y, sum);
         }
       }
+      if constexpr (DELTA && !F32) o[w] += more;
       if (__ballot(spoilt < kChunk)) {
 #pragma unroll
         for (int r = 0; r < 4; ++r)
