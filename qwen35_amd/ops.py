@@ -562,7 +562,8 @@ def rms_norm_quantize(ttype: int, x: torch.Tensor, weight: torch.Tensor | None, 
 class RopeTable:
     """The frequencies of rotary positions: pair i of the first `rot_dim` values of a head turns by position * base^(-2 i /
     rot_dim), scaled for contexts `factor` times the trained one: "linear", "ntk" or "yarn" (which blends between the pairs
-    that turn `fast` and `slow` times over `original` positions)."""
+    that turn `fast` and `slow` times over `original` positions).  steps: an int64 tensor [rot_dim / 2], which another may
+    replace (rope checks it and takes its address at each call); rot_dim is fixed."""
 
     SCALINGS = {None: 0, "linear": 1, "ntk": 2, "yarn": 3}
 
@@ -574,9 +575,18 @@ class RopeTable:
         steps, gain = (ctypes.c_ulonglong * max(rot_dim // 2, 1))(), ctypes.c_float()
         check("rope_steps", load().qhip_rope_steps(rot_dim, base, self.SCALINGS[scaling], factor, original, fast, slow, steps,
                                                    ctypes.byref(gain)))
-        self.rot_dim, self.gain = rot_dim, gain.value
+        self.__dict__.update(rot_dim=rot_dim)
+        self.gain = gain.value
         self.steps = torch.frombuffer(steps, dtype=torch.int64).to(device)
-        self.device, self.at = self.steps.get_device(), self.steps.data_ptr()
+
+    def __setattr__(self, name, value):
+        if name == "rot_dim":
+            raise AttributeError("rot_dim: fixed (another RopeTable has another)")
+        super().__setattr__(name, value)
+
+    @property
+    def device(self) -> int:
+        return self.steps.get_device()
 
 
 def rope(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, table: RopeTable, interleaved: bool = False,
@@ -605,10 +615,11 @@ def rope(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, table
             ko = _rows("k_out", k_out, dev, k_shape, dtype)
     if positions.shape != (tokens,):
         raise ValueError(f"positions: {tokens} entries")
-    if table.device != dev:
-        raise ValueError("table: on the current GPU")
+    steps, rot_dim = table.steps, table.rot_dim
+    if steps.dtype != torch.int64 or steps.shape != (rot_dim // 2,) or steps.get_device() != dev or not steps.is_contiguous():
+        raise ValueError(f"table: steps, a contiguous int64 tensor [{rot_dim // 2}] on the current GPU")
     check("rope", load().qhip_launch_rope(
-        _KV_TYPES[dtype], qr, qo, q_heads, kr, ko, k_heads, dim, table.rot_dim, table.at, table.gain, int(interleaved),
+        _KV_TYPES[dtype], qr, qo, q_heads, kr, ko, k_heads, dim, rot_dim, steps.data_ptr(), table.gain, int(interleaved),
         _ints("positions", positions, dev), tokens, _stream(dev)))
     return q_out, k_out
 
