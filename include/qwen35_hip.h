@@ -503,11 +503,12 @@ typedef struct qhip_rows {
  *   out (nullable) = y in the rows' type; d_xq (nullable): the activation rows of
  *   weight type `ttype` (qhip_act_row_bytes(ttype, heads * dim) bytes a token) that
  *   qhip_launch_quantize_act makes of the f32 y
- * x, residual, gate and out are of one type (QHIP_TT_F32, F16 or BF16); `out` may be x
- * or the gate.  One of out and d_xq is needed.  d_xq wants heads * dim in whole blocks
- * (32 or 256 values) and 2-byte (Q8_0) or 4-byte (Q8_K) alignment; where a block spans
- * several heads, dim must be a power of two (else QHIP_DECLINE).  With weight 1 /
- * sqrt(dim) and eps / dim it is the L2 norm x / sqrt(sum(x^2) + eps). */
+ * x, residual, gate and out are of one type (QHIP_TT_F32, F16 or BF16), heads * dim below
+ * 2^31 and dim at most 2^31 - 8193; `out` may be x or the gate.  One of out and d_xq is
+ * needed.  d_xq wants heads * dim in whole blocks (32 or 256 values) and 2-byte (Q8_0) or
+ * 4-byte (Q8_K) alignment; where a block spans several heads, dim must be a power of two
+ * (else QHIP_DECLINE).  With weight 1 / sqrt(dim) and eps / dim it is the L2 norm x /
+ * sqrt(sum(x^2) + eps). */
 int qhip_launch_rms_norm(int type, const qhip_rows *x, const qhip_rows *residual, const qhip_rows *gate,
                          const float *d_weight, float eps, const qhip_rows *out, int ttype, void *d_xq,
                          int tokens, int heads, int dim, void *stream);

@@ -213,6 +213,8 @@ __global__ __launch_bounds__(256) void k_norm_heads(NormArgs a) {
 }
 
 constexpr int kHeadMost = 512;  // values of a row that a wave's lanes hold
+// values of a row at most: 1024 lanes of eight step past its end within an int
+constexpr int kRowMost = 0x7FFFFFFF - 8192;
 
 template <typename T>
 static void launch_norm_part(const NormArgs& a, long count, hipStream_t s) {
@@ -244,7 +246,8 @@ extern "C" int qhip_launch_rms_norm(int type, const qhip_rows* x, const qhip_row
                                     const float* d_weight, float eps, const qhip_rows* out, int ttype, void* d_xq,
                                     int tokens, int heads, int dim, void* stream) {
   const int size = kv_type_size(type);
-  if (!size || tokens < 0 || heads <= 0 || dim <= 0 || !(eps >= 0.0f) || (long)heads * dim > 0x7FFFFFFFL)
+  if (!size || tokens < 0 || heads <= 0 || dim <= 0 || dim > kRowMost || !(eps >= 0.0f) ||
+      (long)heads * dim > 0x7FFFFFFFL)
     return (int)hipErrorInvalidValue;
   NormArgs a{};
   if (d_xq) {
