@@ -607,16 +607,6 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   const int col = (id >> 3) % blocks * COLS + set * 16 + m;
   const LinearSeq s = linear_seq(a, seq, head, DK);
   if (s.n <= a.few) return;
-  if (s.n == 0) {  // (where no other kernel is launched)
-    const int block = (id >> 3) % blocks * COLS;
-    const float none = s.bad ? __builtin_nanf("") : 0.0f;
-    if (s.to != s.from)
-      for (int e = threadIdx.x; e < DK * COLS; e += 512) {
-        const long at = (long)(e / COLS) * a.value_dim + block + e % COLS;
-        if (s.to) s.to[at] = s.from ? s.from[at] : none;
-      }
-    return;
-  }
   const int kh = head / a.group, chunks = (s.n + kChunk - 1) / kChunk, tail = s.n - (chunks - 1) * kChunk;
   // the wave's tiles of tokens (of two the first and last, or those between: T has 1 to 4
   // tiles in a row, and so has A, which a SIMD's other wave takes the other way round)
@@ -1045,8 +1035,8 @@ static void launch_chunks(const LinearArgs& a, hipStream_t s) {
 }
 
 template <typename T>
-static void launch_linear(const LinearArgs& a, int key_dim, bool steps, bool chunks, hipStream_t s) {
-  if (steps) launch_steps<T>(a, key_dim, s);
+static void launch_linear(const LinearArgs& a, int key_dim, bool chunks, hipStream_t s) {
+  launch_steps<T>(a, key_dim, s);
   if (!chunks) return;
   if (key_dim == 64) a.beta ? launch_chunks<T, 64, true>(a, s) : launch_chunks<T, 64, false>(a, s);
   else a.beta ? launch_chunks<T, 128, true>(a, s) : launch_chunks<T, 128, false>(a, s);
@@ -1156,17 +1146,18 @@ extern "C" int qhip_launch_linear_attention(const qhip_linear_batch* batch, int 
   a.value_dim = batch->value_dim;
   a.group = batch->v_heads / batch->k_heads;
   a.scale = scale;
-  // without a workspace every sequence goes token by token; where the tokens are as many
-  // as the longest would make, short ones are none or few, and all go in chunks
+  // Without a workspace every sequence goes token by token.  Beside chunks short sequences do:
+  // how many new tokens each has stands on the device, so both forms are launched always
+  // (without a short one the first is idle, 1 to 4 us of launch; rows for max_new tokens of
+  // every sequence say nothing, a captured step has them whatever comes).
   const long need = linear_work(batch, type, d_beta != nullptr);
   const bool chunks = need > 0 && d_work;
   if (chunks && (work_bytes < need || !aligned16(d_work))) return (int)hipErrorInvalidValue;
-  const bool steps = !chunks || (long)nseq * batch->max_new != tokens;
-  a.few = !chunks ? 0x7FFFFFFF : steps ? kFew : -1;
+  a.few = chunks ? kFew : 0x7FFFFFFF;
   a.work = (uint8_t*)d_work;
   hipStream_t st = (hipStream_t)stream;
-  if (type == QHIP_TT_F32) launch_linear<float>(a, batch->key_dim, steps, chunks, st);
-  else if (type == QHIP_TT_F16) launch_linear<f16_t>(a, batch->key_dim, steps, chunks, st);
-  else launch_linear<bf16_t>(a, batch->key_dim, steps, chunks, st);
+  if (type == QHIP_TT_F32) launch_linear<float>(a, batch->key_dim, chunks, st);
+  else if (type == QHIP_TT_F16) launch_linear<f16_t>(a, batch->key_dim, chunks, st);
+  else launch_linear<bf16_t>(a, batch->key_dim, chunks, st);
   return (int)hipGetLastError();
 }
