@@ -546,7 +546,17 @@ __global__ __launch_bounds__(256) void k_linear_prepare(LinearArgs a) {
           f32x4 sum[2] = {none, none};  // (side by side: each product waits for the one before it)
 #pragma unroll
           for (int e = 0; e < d; ++e) sum[e & 1] = mfma4(*(const f32x4*)block(j + d, j + e), x[e], sum[e & 1]);
-          x[d] = mfma4(-*(const f32x4*)block(j + d, j + d), sum[0] + sum[1], none);
+          sum[0] += sum[1];
+          // a sum that overflowed would, by the zeros of X_ii, spoil the rows before its own:
+          // it stays out of the product, and its row of X is NaN
+          const f32x4 over = sum[0] * 0.0f;
+          const bool some = __ballot((over[0] + over[1]) + (over[2] + over[3]) != 0.0f);
+          if (some) {
+#pragma unroll
+            for (int r = 0; r < 4; ++r) sum[0][r] = over[r] == 0.0f ? sum[0][r] : 0.0f;
+          }
+          x[d] = mfma4(-*(const f32x4*)block(j + d, j + d), sum[0], none);
+          if (some) x[d] += over;
           // turned by way of the blocks above the diagonal, which nothing reads
           wave_sync();
 #pragma unroll
@@ -595,7 +605,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   __shared__ u32x4 s_state[SETS][PARTS][SP][64];  // three planes, f32: two tiles
   __shared__ f32x4 s_part[DELTA ? SETS : 1][PARTS][kTiles][64];  // K S over the dimensions of a wave
   __shared__ f32x4 s_rest[DELTA ? SETS : 1][kTiles][64];
-  __shared__ __attribute__((aligned(16))) int s_spoilt[SETS][16][kTiles];
+  __shared__ __attribute__((aligned(16))) int s_spoilt[DELTA ? 2 : 1][SETS][16][kTiles];  // by R; by U too
   __shared__ u32x4 s_new[SETS][F32 ? 1 : 3][kTiles / (F32 ? 1 : 2)][64];  // U as it enters the state
   __shared__ u32x4 s_old[SETS][F32 ? 1 : 3][kTiles / (F32 ? 1 : 2)][64];  // U for the outputs
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, g = lane >> 4, m = lane & 15;
@@ -646,9 +656,9 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     }
     return c[0] + c[1];
   };
-  // a column's first token whose R is not finite
-  auto first_spoilt = [&]() {
-    const u32x4 all = *(const u32x4*)s_spoilt[set][m];
+  // a column's first token whose R (or U) is not finite
+  auto first_spoilt = [&](int by) {
+    const u32x4 all = *(const u32x4*)s_spoilt[by][set][m];
     return min(min((int)all[0], (int)all[1]), min((int)all[2], (int)all[3]));
   };
 
@@ -688,6 +698,24 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
           for (int j = 0; j < kTiles; ++j) solve[o][j] = *(GlobalF4)(work + W::solve_tile(own(o), min(j, own(o))) + lane * 16);
         }
       }
+    };
+    // What is not finite spoils its column from its token on; in a product it would spoil
+    // the tokens before as well (0 * NaN), so it stays out of them.
+    auto leave_out = [&](f32x4& x, int t, int first, int by) {
+      float sum = 0.0f;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) sum = __builtin_fmaf(x[r], 0.0f, sum);
+      if (__ballot(sum != 0.0f)) {
+#pragma unroll
+        for (int r = 3; r >= 0; --r)
+          if (!(__builtin_fabsf(x[r]) < INFINITY)) {
+            first = min(first, 16 * t + 4 * g + r);
+            x[r] = 0.0f;
+          }
+        first = min(first, __shfl_xor(first, 16, 64));
+        first = min(first, __shfl_xor(first, 32, 64));
+      }
+      if (lane < 16) s_spoilt[by][set][m][t] = first;
     };
     place(rows_of(0));
     fetch_values();
@@ -748,23 +776,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
           for (int p = 1; p < PARTS; ++p) ks += s_part[set][p][t][lane];
           u[w] -= number(c, 0, t) * ks;
         }
-        // What is not finite spoils its column from its token on; in a product it would spoil
-        // the tokens before as well (0 * NaN), so it stays out of them.
-        float sum = 0.0f;
-#pragma unroll
-        for (int r = 0; r < 4; ++r) sum = __builtin_fmaf(u[w][r], 0.0f, sum);
-        int first = DELTA ? (int)s_numbers[c & 1][kSound] : kChunk;
-        if (__ballot(sum != 0.0f)) {
-#pragma unroll
-          for (int r = 3; r >= 0; --r)
-            if (!(__builtin_fabsf(u[w][r]) < INFINITY)) {
-              first = min(first, 16 * t + 4 * g + r);
-              u[w][r] = 0.0f;
-            }
-          first = min(first, __shfl_xor(first, 16, 64));
-          first = min(first, __shfl_xor(first, 32, 64));
-        }
-        if (lane < 16) s_spoilt[set][m][t] = first;
+        leave_out(u[w], t, DELTA ? (int)s_numbers[c & 1][kSound] : kChunk, 0);
         if constexpr (DELTA) s_rest[set][t][lane] = u[w];
       }
       if constexpr (!LAST) fetch_values();
@@ -773,7 +785,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
         f32x4 rest[kTiles];
 #pragma unroll
         for (int j = 0; j < kTiles; ++j) rest[j] = s_rest[set][j][lane];
-        const int spoilt = first_spoilt();
+        const int spoilt = first_spoilt(0);
 #pragma unroll
         for (int w = 0; w < OWN; ++w) {
           const int t = own(w);
@@ -790,6 +802,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
             for (int r = 0; r < 4; ++r)
               if (16 * t + 4 * g + r >= spoilt) u[w][r] = 0.0f;
           }
+          leave_out(u[w], t, spoilt, 1);  // (T or the product may have overflowed)
         }
       }
 #pragma unroll
@@ -834,7 +847,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
           }
         }
       }
-      const int spoilt = first_spoilt();
+      const int spoilt = first_spoilt(DELTA);
       if (__ballot(spoilt < kChunk)) {
 #pragma unroll
         for (int i = 0; i < 2; ++i)
@@ -992,7 +1005,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
         }
     }
     __syncthreads();
-    const int spoilt = first_spoilt();
+    const int spoilt = first_spoilt(DELTA);
 #pragma unroll
     for (int w = 0; w < OWN; ++w) {
       const int t = own(w), row = 16 * t + 4 * g;
