@@ -209,13 +209,14 @@ static void launch_steps(const LinearArgs& a, int key_dim, hipStream_t s) {
 // registers of a workgroup.  G is summed in f64 and kept in two f32 parts, of which
 // differences are taken: it is a long sum where the decay between near tokens is small.
 //
-// f32 rows take f32 matrix tiles throughout.  16-bit rows take bf16 ones, for which an f32
-// value goes in as a sum of three planes of 8 bits, which hold it whole; of products of planes
-// those down to 2^-16 are summed, so all sums are good to f32, and an output is rounded once,
-// to its type.  (With the state, U and A in two planes for the outputs, 2^-16 off, 0.6% of
-// bf16 outputs and 3% of f16 ones were rounded otherwise than the f64 results, instead of
-// 0.02% and 0.09%: 253 us for 8192 tokens, now 264.)  Keys and queries need one plane (bf16)
-// or two (f16).
+// f32 rows take f32 matrix tiles throughout.  16-bit rows take bf16 ones for products with
+// keys and queries, for which an f32 value goes in as a sum of three planes of 8 bits, which
+// hold it whole; of products of planes those down to 2^-16 are summed.  So all sums are good
+// to f32, and an output is rounded once, to its type.  (With the state, U and A in two planes
+// for the outputs, 2^-16 off, 0.6% of bf16 outputs and 3% of f16 ones were rounded otherwise
+// than the f64 results, instead of 0.02% and 0.09%: 253 us for 8192 tokens instead of 264.)
+// Keys and queries need one plane (bf16) or two (f16).  T R and A U take f32 tiles for all
+// types (A U in planes: as fast, with three times the registers or half as much again to read).
 constexpr int kChunk = 64, kTiles = kChunk / 16;
 
 typedef __bf16 b16x8 __attribute__((ext_vector_type(8)));
@@ -277,23 +278,15 @@ __device__ __forceinline__ f32x4 mfma_planes(const u32x4* a, const u32x4* b, f32
   return c;
 }
 
-// What prepare leaves for a chunk and value head, as left operands of 1 KB: T's tiles (i,
-// j), j <= i, in f32; A's the same way, but for 16-bit rows without the delta rule as rows of
-// tiles in steps of two tiles and three planes (with it, the outputs' waves split A while they
-// wait for U: 264 us for 8192 bf16 tokens instead of 272; without it they wait for nothing: a
-// mixed f16 batch 71 us, from planes 65); then exp(G), exp(G_63 - G), exp(G_63) and the
+// What prepare leaves for a chunk and value head, as left operands of 1 KB: T's and A's tiles
+// (i, j), j <= i, in f32; then exp(G), exp(G_63 - G), exp(G_63) and the
 // first token whose row of L, or beta, is not finite (64: none).
 constexpr int kWhole = 2 * kChunk, kSound = kWhole + 1, kNumbers = kWhole + 2;
-template <typename T, bool DELTA>
+template <bool DELTA>
 struct ChunkWork {
-  static constexpr bool whole = DELTA || sizeof(T) == 4;
   static constexpr int tiles = kTiles * (kTiles + 1) / 2 * 1024;
-  static constexpr int solve = 0, inside = DELTA ? tiles : 0, numbers = inside + (whole ? tiles : 18 * 1024), bytes = numbers + 576;
-  __host__ __device__ static constexpr int solve_tile(int i, int j) { return solve + (i * (i + 1) / 2 + j) * 1024; }
-  // of row i: its first tile (whole), or its first step's first plane
-  __host__ __device__ static constexpr int inside_row(int i) {
-    return inside + (whole ? i * (i + 1) / 2 : i < 2 ? 3 * i : 6 * i - 6) * 1024;
-  }
+  static constexpr int solve = 0, inside = DELTA ? tiles : 0, numbers = inside + tiles, bytes = numbers + 576;
+  __host__ __device__ static constexpr int tile(int i, int j) { return (i * (i + 1) / 2 + j) * 1024; }
 };
 
 // The chunk slot of a sequence's first: no two sequences' slots meet, and there are at
@@ -328,7 +321,7 @@ __device__ __forceinline__ f32x4 row_product(u32x4 a, u32x4 b, f32x4 c) {
 // downwards, X_ij = -X_ii sum of L_ik X_kj, a wave a column.
 template <typename T, int DK, bool DELTA>
 __global__ __launch_bounds__(256) void k_linear_prepare(LinearArgs a) {
-  typedef ChunkWork<T, DELTA> W;
+  typedef ChunkWork<DELTA> W;
   constexpr int ROW = kChunk + 4;  // floats of a row in LDS
   constexpr int PIECES = DK * sizeof(T) / 64, TILE = PIECES * 64;  // 16-byte pieces of a row a lane, of 16 rows
   __shared__ u32x4 s_rows[2][kTiles][TILE];  // keys and queries; then L and its inverse
@@ -468,27 +461,10 @@ __global__ __launch_bounds__(256) void k_linear_prepare(LinearArgs a) {
       }
     }
     if (!keys) {  // A
-      const f32x4 none = {0.0f, 0.0f, 0.0f, 0.0f};
-      auto leave = [&](int i, int j, f32x4 x, f32x4 y) {
-        u32x4* to = (u32x4*)(out + W::inside_row(i) + (W::whole ? j : j / 2 * 3) * 1024) + lane;
-        if constexpr (W::whole) {
-          to[0] = __builtin_bit_cast(u32x4, x);
-          if (j < i) to[64] = __builtin_bit_cast(u32x4, y);
-        } else {
-          u32x4 planes[3];
-          split8<3>(x, y, planes);
 #pragma unroll
-          for (int p = 0; p < 3; ++p) to[64 * p] = planes[p];
-        }
-      };
-      if (outer) {
-        leave(3, 0, tile[0], tile[1]);
-        leave(3, 2, tile[2], tile[3]);
-        leave(0, 0, tile[4], none);
-      } else {
-        leave(1, 0, tile[0], tile[1]);
-        leave(2, 0, tile[2], tile[3]);
-        leave(2, 2, tile[4], none);
+      for (int e = 0; e < 5; ++e) {
+        const int at = outer ? (e < 4 ? W::tile(3, e) : W::tile(0, 0)) : e < 2 ? W::tile(1, e) : W::tile(2, e - 2);
+        *((f32x4*)(out + W::inside + at) + lane) = tile[e];
       }
     }
     if (wave == 3) {
@@ -529,7 +505,7 @@ __global__ __launch_bounds__(256) void k_linear_prepare(LinearArgs a) {
         const f32x4 b = *(const f32x4*)(s_beta + 16 * j + 4 * g);
 #pragma unroll
         for (int e = 0; e < 4; ++e) x[e] = 16 * i + m < sound && (i > j || 4 * g + e <= m) ? x[e] * b[e] : 0.0f;
-        *((f32x4*)(out + W::solve_tile(i, j)) + lane) = x;
+        *((f32x4*)(out + W::solve + W::tile(i, j)) + lane) = x;
       };
       const f32x4 none = {0.0f, 0.0f, 0.0f, 0.0f};
       if (wave == 3) {
@@ -589,7 +565,7 @@ __global__ __launch_bounds__(256) void k_linear_prepare(LinearArgs a) {
 // takes a third of the cycles: 263, for the splits and the larger loads.)
 template <typename T, int DK, bool DELTA>
 __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) void k_linear_scan(LinearArgs a) {
-  typedef ChunkWork<T, DELTA> W;
+  typedef ChunkWork<DELTA> W;
   constexpr bool F32 = sizeof(T) == 4;
   constexpr int P = std::is_same<T, f16_t>::value ? 2 : 1;  // planes of keys and queries
   constexpr int PARTS = DK / 32, SETS = 4 / PARTS, COLS = 16 * SETS, OWN = kTiles / PARTS;
@@ -607,7 +583,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   __shared__ f32x4 s_rest[DELTA ? SETS : 1][kTiles][64];
   __shared__ __attribute__((aligned(16))) int s_spoilt[DELTA ? 2 : 1][SETS][16][kTiles];  // by R; by U too
   __shared__ u32x4 s_new[SETS][F32 ? 1 : 3][kTiles / (F32 ? 1 : 2)][64];  // U as it enters the state
-  __shared__ u32x4 s_old[SETS][F32 ? 1 : 3][kTiles / (F32 ? 1 : 2)][64];  // U for the outputs
+  __shared__ f32x4 s_old[SETS][kTiles][64];  // U for the outputs
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, g = lane >> 4, m = lane & 15;
   const int set = (wave & 3) / PARTS, part = (wave & 3) % PARTS;
   // the workgroups of a sequence's head follow each other on one XCD
@@ -695,7 +671,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
       for (int o = 0; o < OWN; ++o) {
         if constexpr (DELTA) {
 #pragma unroll
-          for (int j = 0; j < kTiles; ++j) solve[o][j] = *(GlobalF4)(work + W::solve_tile(own(o), min(j, own(o))) + lane * 16);
+          for (int j = 0; j < kTiles; ++j) solve[o][j] = *(GlobalF4)(work + W::solve + W::tile(own(o), min(j, own(o))) + lane * 16);
         }
       }
     };
@@ -809,17 +785,14 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
       for (int w = 0; w < OWN; ++w) {
         const int t = own(w);
         const f32x4 in = number(c, kChunk, t) * u[w];
+        s_old[set][t][lane] = u[w];
         if constexpr (F32) {
           s_new[set][0][t][lane] = __builtin_bit_cast(u32x4, in);
-          s_old[set][0][t][lane] = __builtin_bit_cast(u32x4, u[w]);
         } else {
           u32x2 planes[3];
           split4<3>(in, planes);
 #pragma unroll
           for (int p = 0; p < 3; ++p) ((u32x2*)&s_new[set][p][t >> 1][lane])[t & 1] = planes[p];
-          split4<3>(u[w], planes);
-#pragma unroll
-          for (int p = 0; p < 3; ++p) ((u32x2*)&s_old[set][p][t >> 1][lane])[t & 1] = planes[p];
         }
       }
 #pragma unroll
@@ -907,14 +880,12 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
       for (int i = 0; i < 4; ++i) held[e][i] = *(const piece*)(k_at + held_off[e][i]);
     held_number = *(const __attribute__((address_space(1))) float*)(key_work + W::numbers + 4 * min(tid, kNumbers - 1));
   };
-  constexpr int PIECES_A = W::whole ? kTiles : kTiles / 2 * 3;
-  f32x4 inside[OWN][PIECES_A];
+  f32x4 inside[OWN][kTiles];
   auto fetch_inside = [&]() {
 #pragma unroll
     for (int o = 0; o < OWN; ++o)
 #pragma unroll
-      for (int j = 0; j < PIECES_A; ++j)
-        inside[o][j] = *(GlobalF4)(work + W::inside_row(own(o)) + (W::whole ? min(j, own(o)) : own(o) < 2 ? j % 3 : j) * 1024 + lane * 16);
+      for (int j = 0; j < kTiles; ++j) inside[o][j] = *(GlobalF4)(work + W::inside + W::tile(own(o), min(j, own(o))) + lane * 16);
   };
   // the held keys and numbers into LDS (behind the sequence's end the last key: U is 0 there)
   auto put_keys = [&](int buffer) {
@@ -990,20 +961,6 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
       }
       fetch_keys();
     }
-    u32x4 weights[OWN][F32 ? 1 : kTiles / 2][3];
-    if constexpr (!F32) {
-#pragma unroll
-      for (int w = 0; w < OWN; ++w)
-#pragma unroll
-        for (int j = 0; j < kTiles; j += 2) {
-          if constexpr (W::whole) {
-            if (j <= own(w)) split8<3>(inside[w][j], j < own(w) ? inside[w][j + 1] : f32x4{0.0f, 0.0f, 0.0f, 0.0f}, weights[w][j / 2]);
-          } else {
-#pragma unroll
-            for (int p = 0; p < 3; ++p) weights[w][j / 2][p] = __builtin_bit_cast(u32x4, inside[w][j / 2 * 3 + p]);
-          }
-        }
-    }
     __syncthreads();
     const int spoilt = first_spoilt(DELTA);
 #pragma unroll
@@ -1011,16 +968,12 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
       const int t = own(w), row = 16 * t + 4 * g;
       f32x4 more = {0.0f, 0.0f, 0.0f, 0.0f};  // a second sum beside o[w], as above
 #pragma unroll
-      for (int j = 0; j < kTiles; ++j) {
-        if constexpr (F32) {
-          if (j <= t) o[w] = mfma4(inside[w][j], __builtin_bit_cast(f32x4, s_old[set][0][j][lane]), o[w]);
-        } else if ((j & 1) == 0 && j <= t) {
-          const u32x4 y[3] = {s_old[set][0][j >> 1][lane], s_old[set][1][j >> 1][lane], s_old[set][2][j >> 1][lane]};
-          f32x4& sum = DELTA && j ? more : o[w];
-          sum = mfma_planes<3, 3>(weights[w][j >> 1], y, sum);
+      for (int j = 0; j < kTiles; ++j)
+        if (j <= t) {
+          f32x4& sum = j & 1 ? more : o[w];
+          sum = mfma4(inside[w][j], s_old[set][j][lane], sum);
         }
-      }
-      if constexpr (DELTA && !F32) o[w] += more;
+      o[w] += more;
       if (__ballot(spoilt < kChunk)) {
 #pragma unroll
         for (int r = 0; r < 4; ++r)
@@ -1055,16 +1008,12 @@ static void launch_linear(const LinearArgs& a, int key_dim, bool chunks, hipStre
   else a.beta ? launch_chunks<T, 128, true>(a, s) : launch_chunks<T, 128, false>(a, s);
 }
 
-static long chunk_bytes(int type, bool delta) {
-  if (type == QHIP_TT_F32) return delta ? ChunkWork<float, true>::bytes : ChunkWork<float, false>::bytes;
-  return delta ? ChunkWork<f16_t, true>::bytes : ChunkWork<f16_t, false>::bytes;
-}
 // 0: token by token (also where a grid would pass 2^32 threads)
-static long linear_work(const qhip_linear_batch* b, int type, bool delta) {
+static long linear_work(const qhip_linear_batch* b, bool delta) {
   if (b->max_new <= few_alone(b) || b->nseq == 0 || b->tokens == 0) return 0;
   const long slots = (long)b->tokens / kChunk + b->nseq, pairs = (long)b->nseq * b->v_heads + 8;
   if (slots * b->k_heads >= 1L << 24 || pairs * (b->value_dim / 16) >= 1L << 23) return 0;
-  return slots * b->v_heads * chunk_bytes(type, delta);
+  return slots * b->v_heads * (delta ? ChunkWork<true>::bytes : ChunkWork<false>::bytes);
 }
 
 }  // namespace qhip
@@ -1092,7 +1041,7 @@ static int check_linear(const qhip_linear_batch* b, int type) {
 
 extern "C" long qhip_linear_attention_work_bytes(const qhip_linear_batch* batch, int type, int delta) {
   if (check_linear(batch, type)) return -1;
-  return linear_work(batch, type, delta != 0);
+  return linear_work(batch, delta != 0);
 }
 
 extern "C" int qhip_launch_linear_attention(const qhip_linear_batch* batch, int type, const qhip_rows* q, const qhip_rows* k,
@@ -1163,7 +1112,7 @@ extern "C" int qhip_launch_linear_attention(const qhip_linear_batch* batch, int 
   // how many new tokens each has stands on the device, so both forms are launched always
   // (without a short one the first is idle, 1 to 4 us of launch; rows for max_new tokens of
   // every sequence say nothing, a captured step has them whatever comes).
-  const long need = linear_work(batch, type, d_beta != nullptr);
+  const long need = linear_work(batch, d_beta != nullptr);
   const bool chunks = need > 0 && d_work;
   if (chunks && (work_bytes < need || !aligned16(d_work))) return (int)hipErrorInvalidValue;
   a.few = chunks ? kFew : 0x7FFFFFFF;
