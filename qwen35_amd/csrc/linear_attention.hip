@@ -1028,6 +1028,14 @@ static bool numbers_meet(const qhip_rows* r, int heads, int dim, int tokens, int
   return rows_overlap(r, heads, dim, &n, 1, heads * (4 / size), tokens, size);
 }
 
+struct Bytes {
+  const void* at;
+  long n;
+};
+static bool bytes_meet(Bytes a, Bytes b) {
+  return a.n > 0 && b.n > 0 && (const char*)a.at < (const char*)b.at + b.n && (const char*)b.at < (const char*)a.at + a.n;
+}
+
 // 0, hipErrorInvalidValue or QHIP_DECLINE (dimensions without kernels)
 static int check_linear(const qhip_linear_batch* b, int type) {
   if (!b || !kv_type_size(type) || b->nseq < 0 || b->nseq > 65535 || b->tokens < 0 || b->tokens > kMaxCount || b->max_new < 0 ||
@@ -1057,6 +1065,16 @@ extern "C" int qhip_launch_linear_attention(const qhip_linear_batch* batch, int 
   if (batch->num_states > 0 && (!d_states || !aligned16(d_states))) return (int)hipErrorInvalidValue;
   if (rc) return rc;
   if (nseq == 0) return 0;
+  const long need = linear_work(batch, d_beta != nullptr);
+  const bool chunks = need > 0 && d_work;
+  if (chunks && (work_bytes < need || !aligned16(d_work))) return (int)hipErrorInvalidValue;
+  // the states and the workspace are written: nothing else of the call may lie in them
+  const long state_bytes = 4L * batch->num_states * batch->v_heads * batch->key_dim * batch->value_dim;
+  const Bytes states{d_states, state_bytes}, work{d_work, chunks ? need : 0};
+  const Bytes lists[] = {{batch->offsets, 4L * (nseq + 1)}, {batch->slots, 4L * nseq}, {batch->source, batch->source ? 4L * nseq : 0}};
+  if (bytes_meet(states, work)) return (int)hipErrorInvalidValue;
+  for (const Bytes& list : lists)
+    if (bytes_meet(list, states) || bytes_meet(list, work)) return (int)hipErrorInvalidValue;
   if (tokens > 0) {
     const qhip_rows* all[] = {q, k, v, out};
     for (const qhip_rows* r : all)  // (a chunk's offsets are 32 bits)
@@ -1064,15 +1082,21 @@ extern "C" int qhip_launch_linear_attention(const qhip_linear_batch* batch, int 
     if (!d_log_decay ||
         ((uintptr_t)d_log_decay & 3u) || decay_stride < 0 || ((uintptr_t)d_beta & 3u) || beta_stride < 0)
       return (int)hipErrorInvalidValue;
-    const long state_bytes = 4L * batch->num_states * batch->v_heads * batch->key_dim * batch->value_dim;
-    if (!rows_apart(out, tokens, batch->v_heads, batch->value_dim) ||
-        rows_meet(out, tokens, batch->v_heads, batch->value_dim, size, d_states, state_bytes))
+    const auto meets = [&](const qhip_rows* rows, int heads, int dim, Bytes b) { return rows_meet(rows, tokens, heads, dim, size, b.at, b.n); };
+    if (!rows_apart(out, tokens, batch->v_heads, batch->value_dim) || meets(out, batch->v_heads, batch->value_dim, states) ||
+        meets(out, batch->v_heads, batch->value_dim, work))
       return (int)hipErrorInvalidValue;
+    for (const Bytes& list : lists)
+      if (meets(out, batch->v_heads, batch->value_dim, list)) return (int)hipErrorInvalidValue;
+    const Bytes numbers[] = {{d_log_decay, 4 * ((tokens - 1) * decay_stride + batch->v_heads)},
+                             {d_beta, d_beta ? 4 * ((tokens - 1) * beta_stride + batch->v_heads) : 0}};
+    for (const Bytes& n : numbers)
+      if (bytes_meet(n, states) || bytes_meet(n, work)) return (int)hipErrorInvalidValue;
     const qhip_rows* read[] = {q, k, v};
     const int heads[] = {batch->k_heads, batch->k_heads, batch->v_heads}, dims[] = {batch->key_dim, batch->key_dim, batch->value_dim};
     for (int i = 0; i < 3; ++i)
       if (rows_overlap(out, batch->v_heads, batch->value_dim, read[i], heads[i], dims[i], tokens, size) ||
-          rows_meet(read[i], tokens, heads[i], dims[i], size, d_states, state_bytes))
+          meets(read[i], heads[i], dims[i], states) || meets(read[i], heads[i], dims[i], work))
         return (int)hipErrorInvalidValue;
     if (numbers_meet(out, batch->v_heads, batch->value_dim, tokens, size, d_log_decay, decay_stride) ||
         numbers_meet(out, batch->v_heads, batch->value_dim, tokens, size, d_beta, beta_stride))
@@ -1112,9 +1136,6 @@ extern "C" int qhip_launch_linear_attention(const qhip_linear_batch* batch, int 
   // how many new tokens each has stands on the device, so both forms are launched always
   // (without a short one the first is idle, 1 to 4 us of launch; rows for max_new tokens of
   // every sequence say nothing, a captured step has them whatever comes).
-  const long need = linear_work(batch, d_beta != nullptr);
-  const bool chunks = need > 0 && d_work;
-  if (chunks && (work_bytes < need || !aligned16(d_work))) return (int)hipErrorInvalidValue;
   a.few = chunks ? kFew : 0x7FFFFFFF;
   a.work = (uint8_t*)d_work;
   hipStream_t st = (hipStream_t)stream;
