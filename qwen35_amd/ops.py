@@ -510,9 +510,10 @@ def _rows(name: str, t: torch.Tensor, device: int, shape: torch.Size, dtype: tor
 
 def _new_rows(shape: torch.Size, like: torch.Tensor) -> tuple[torch.Tensor, QhipRows]:
     t = torch.empty_like(like)  # (torch.empty with a type and a device takes three times as long)
-    if t.shape != shape:
-        t = like.new_empty(shape)
     stride = t.stride()
+    if t.shape != shape or stride[-1] != 1:  # (overlapping windows, for one, have an order of their own there)
+        t = like.new_empty(shape)
+        stride = t.stride()
     return t, QhipRows(t.data_ptr(), stride[0], stride[1] if len(stride) == 3 else 0)
 
 
