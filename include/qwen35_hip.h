@@ -553,9 +553,9 @@ int qhip_launch_rope(int type, const qhip_rows *q, const qhip_rows *q_out, int q
  * d_log_decay and d_beta: f32, [token * stride + head]; log_decay is meant to be <= 0,
  * -infinity forgets.  key_dim 64 or 128, value_dim 64, 128 or 256 (others:
  * QHIP_DECLINE); at most 65535 sequences and value heads, rows' tokens at most 2^23
- * elements apart.  States, decays and sums are f32 or more whatever the rows' type;
- * values that are not finite stay in their head (those of v and the state in their
- * column) and behind their token.
+ * elements apart.  States, decays and sums are f32 or more whatever the rows' type, and an
+ * output is rounded once, to it; values that are not finite stay in their head (those of
+ * v and the state in their column) and behind their token.
  * d_work (qhip_linear_attention_work_bytes, 16-byte aligned; 0 bytes: none is needed):
  * scratch of one launch, in any state before it; launches that may run at once, those of
  * captured graphs too, each take their own.  With it sequences of more than a few new

@@ -51,12 +51,17 @@ __device__ __forceinline__ LinearSeq linear_seq(const LinearArgs& a, int i, int 
 }
 
 // Beside sequences that go in chunks, those of at most this many new tokens go token by
-// token: a chunk takes one sequence of 16 heads 15 us, a token 0.8.
+// token: a chunk takes one sequence of 16 heads 13 (bf16) to 18 us (f32), a token 0.8.
 constexpr int kFew = 16;
 // A batch whose sequences all have at most this many does without chunks.  Of sequences
-// that fill the card (256 workgroups of 64 columns) a chunk costs more tokens: 16 heads of
-// 128 x 128, token by token / in chunks: 1 sequence, 16 tokens 16.5 / 15 us, 32: 29 / 16; 64
-// sequences, 16 tokens 71 / 199 us, 32: 117 / 213.
+// that fill the card (256 workgroups of 64 columns) a chunk costs more tokens.  16 heads of
+// 128 x 128, us token by token / in chunks of f32 / of bf16:
+//    1 sequence   17 tokens  18 /  18 /  13   32:  30 /  18 /  14   64:  56 /  20 /  14
+//    8 sequences  33 tokens  35 /  37 /  28   48:  47 /  40 /  29   64:  60 /  42 /  30
+//   64 sequences  33 tokens 119 / 233 / 159   48: 170 / 247 / 167   64: 217 / 275 / 178
+//                 96 tokens 318 / 382 / 238  128: 418 / 401 / 246
+// So it is right where the card is empty or just filled.  For many times as many sequences
+// chunks pay from 48 (bf16) or 110 tokens (f32) on, and below that take up to twice as long.
 static int few_alone(const qhip_linear_batch* b) { return (long)b->nseq * b->v_heads * (b->value_dim / 64) < 256 ? kFew : 2 * kFew; }
 
 // sum over lanes l, l ^ 16, l ^ 32, l ^ 48
@@ -556,13 +561,18 @@ __global__ __launch_bounds__(256) void k_linear_prepare(LinearArgs a) {
 //   U of the own tokens        | the next chunk's keys into LDS, as rows and turned
 //   the state's update         | the outputs
 //
-// A chunk waits for the one before it, so its chain bounds a sequence: 1.7 us for bf16 rows of
-// 128, of which products fill a quarter and vector instructions another, the rest being LDS,
-// barriers and waits for each other (loads a chunk ahead do not show); 2.8 us for f32 rows,
-// 4096 cycles of f32 products on each SIMD among them.  8192 bf16 tokens of 16 heads: 223 us, beside 42 of prepare; eight f32
-// prompts of up to 256 tokens 57 and 14.5.  (K S of the own tokens over all rows of the
-// state, read by every wave from LDS: 229 us.  T in three planes of bf16, so that its product
-// takes a third of the cycles: 263, for the splits and the larger loads.)
+// A chunk waits for the one before it, so its chain bounds a sequence.  bf16 rows of 128 with
+// the delta rule: 2.0 us, of which products fill three tenths and vector instructions a quarter,
+// the rest being LDS, barriers and waits for each other (loads a chunk ahead do not show); 8192
+// tokens of 32 value heads, a workgroup on every CU, 252 to 262 us, beside 41 of prepare, and
+// of 16 heads, on half of the CUs, 236 and 27.  f32 rows: 3.4 us (16 heads), 3700 cycles of f32
+// products on each SIMD among them; eight prompts of up to 256 tokens of 16 heads, four rounds of
+// workgroups, 58 and 15.  (Of the bf16 prompt, before outputs took three planes, 223: with K S of
+// the own tokens over all rows of the state, read by every wave from LDS, 229; with T in three
+// planes of bf16, so that its product takes a third of the cycles, 263, for the splits and the
+// larger loads.)  A second workgroup on a CU has no room in LDS (with the delta rule 86 to 141
+// KB, f32 and f16 rows of 128 without it 87 and 98) or in registers (keys of 64: 146 to 162);
+// bf16 rows of 128 without it (61 KB, 110 registers) would fit, but for amdgpu_waves_per_eu.
 template <typename T, int DK, bool DELTA>
 __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) void k_linear_scan(LinearArgs a) {
   typedef ChunkWork<DELTA> W;
@@ -1134,8 +1144,9 @@ extern "C" int qhip_launch_linear_attention(const qhip_linear_batch* batch, int 
   a.scale = scale;
   // Without a workspace every sequence goes token by token.  Beside chunks short sequences do:
   // how many new tokens each has stands on the device, so both forms are launched always
-  // (without a short one the first is idle, 1 to 4 us of launch; rows for max_new tokens of
-  // every sequence say nothing, a captured step has them whatever comes).
+  // (without a short one the first is idle, 5 us; rows for max_new tokens of every sequence
+  // say nothing, a captured step has them whatever comes: 64 single tokens of 16 f32 heads in
+  // rows for 64 each 50 us, in chunks 201).
   a.few = chunks ? kFew : 0x7FFFFFFF;
   a.work = (uint8_t*)d_work;
   hipStream_t st = (hipStream_t)stream;

@@ -11,10 +11,12 @@
 // quantizers applied to the f32 y.
 //
 // Memory bounds it: each value is read once, held in registers over the sum and written
-// once.  4096 bf16 rows of 5120 with the residual 33 us (5.0 TB/s of the 5.1 of a copy), 131,056
-// heads of 128 in f32 with gates 35 us (5.7), 1673 f32 rows of 5120 with the residual to Q8_0
-// codes 27 us (4.2: one uneven round of workgroups); one row of 2560 4.3 us, a chain of loads,
-// two sums and stores.
+// once.  Inputs from memory, outputs into memory not used before (in brackets: into what the
+// call before wrote, which the last cache still holds): 4096 bf16 rows of 5120 with the residual
+// 37 us, 4.5 TB/s of the 5.1 of a copy (33); 131,056 heads of 128 in f32 with gates 40 us, 5.0
+// (40); 1673 f32 rows of 5120 with the residual to Q8_0 codes 29 us, 3.9 (27: one uneven round
+// of workgroups), to Q8_K 27.5 us; the heads with gates to Q8_0 codes 40.5 us, 3.8, to Q8_K 42;
+// one row of 2560 4.3 us, a chain of loads, two sums and stores.
 #include "qhip_device.hpp"
 #include "qhip_internal.hpp"
 #include "rows_internal.hpp"

@@ -9,8 +9,10 @@
 // position * steps[i] mod 2^64 is the place on the circle, exact to 2^-32 turns at
 // any position, without a floating reduction of a large angle.
 //
-// Memory bounds it: 4097 tokens of 10 heads of 256 in f32 18.2 us (4.6 TB/s), 8192 of 40 heads of
-// 128 in bf16 30 us (5.6); 64 tokens of 20 heads 5.8 us, a chain of loads and the angles.
+// Memory bounds it: 4097 tokens of 10 heads of 256 in f32 22 us (3.8 TB/s of the 5.1 of a copy),
+// 8192 of 40 heads of 128 in bf16 38 us (4.4), inputs from memory and outputs into memory not
+// used before; 18 and 30 us into what the call before wrote, which the last cache still holds.
+// 64 tokens of 20 heads 5.8 us, a chain of loads and the angles.
 #include "qhip_internal.hpp"
 #include "rows_internal.hpp"
 
@@ -238,7 +240,9 @@ extern "C" int qhip_launch_rope(int type, const qhip_rows* q, const qhip_rows* q
   while (a.lanes < a.pieces) a.lanes *= 2;
   const long blocks = ((long)tokens * a.lanes + 255) / 256;
   // heads of a lane: as many as leave eight workgroups a CU (4097 tokens of 10 heads of 256,
-  // 8192 of 40 of 128, with four 20.1 and 33.2 us, eight 18.5 and 29.9, sixteen 20.6 and 31.5)
+  // 8192 of 40 of 128, into new memory: with two 25.9 and 47.3 us, four 22.9 and 40.2, eight 22.2
+  // and 37.4, sixteen 23.0 and 38.7; into what the call before wrote 21.4 and 45.4, 19.8 and
+  // 33.1, 17.9 and 30.0, 20.4 and 31.2)
   a.each = (int)((long)a.heads * blocks / 2048);
   a.each = a.each < 1 ? 1 : a.each > a.heads ? a.heads : a.each;
   const unsigned slices = (unsigned)((a.heads + a.each - 1) / a.each);  // fewer than 4096

@@ -666,7 +666,8 @@ def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_deca
     q, k [tokens, k_heads, key_dim], v [tokens, v_heads, value_dim]; log_decay, beta: f32 [tokens, v_heads].  Sequence i has
     tokens offsets[i] .. offsets[i + 1], at most max_new, starts from state source[i] (-1: zeros; by default slots[i]) and
     leaves its last state in slots[i] (-1: nowhere); no state that a sequence writes may be another's in the same call.
-    scale: 1 / sqrt(key_dim) by default.  Rows at or past offsets[-1] are not written.
+    scale: 1 / sqrt(key_dim) by default.  Sums are f32 or more whatever the rows' type, and an output is rounded once, to it.
+    Rows at or past offsets[-1] are not written.
     work: linear_attention_work's; with it sequences of more than a few tokens go in chunks of 64, several times as fast,
     without it (None) token by token."""
     dev, q_shape, dtype = torch.cuda.current_device(), q.shape, q.dtype
